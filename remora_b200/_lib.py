@@ -1,4 +1,5 @@
-"""ctypes binding of libremora_b200.so (the C ABI in include/remora_b200.h).
+"""ctypes binding of libremora_b200.so (the C ABI in include/remora_b200.h and
+include/remora_b200_seq.h).
 
 Loading fails loudly: there is no CPU fallback.  Set REMORA_B200_LIB to use a
 library outside the package directory.
@@ -128,9 +129,34 @@ class RemoraFilterPred(ctypes.Structure):
     ]
 
 
+class RemoraNormSpec(ctypes.Structure):
+    _fields_ = [("eps", ctypes.c_float), ("group", ctypes.c_int32)]
+
+
+class RemoraCausalConvSpec(ctypes.Structure):
+    _fields_ = [("silu", ctypes.c_int32), ("reserved_", ctypes.c_int32)]
+
+
+class RemoraSelectiveScanSpec(ctypes.Structure):
+    _fields_ = [("softplus", ctypes.c_int32), ("reserved_", ctypes.c_int32)]
+
+
+class RemoraSelectiveScanIn(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("u", "delta", "a", "b", "c", "d", "z", "delta_bias", "h0", "lengths")]
+
+
+class RemoraSelectiveScanGrads(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("du", "ddelta", "da", "db", "dc", "dd", "dz", "ddelta_bias", "dh0")]
+
+
+class RemoraSelectiveStepIn(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("state", "u", "delta", "a", "b", "c", "d", "z", "delta_bias", "slots")]
+
+
 # ------------------------------------------------------------------ loading
 _VP = ctypes.c_void_p
 _I32 = ctypes.c_int32
+_I64 = ctypes.c_int64
 _SZ = ctypes.c_size_t
 _PROTOTYPES: dict[str, tuple] = {
     "remora_b200_init": (_I32, [ctypes.c_int, ctypes.POINTER(_VP)]),
@@ -173,6 +199,20 @@ _PROTOTYPES: dict[str, tuple] = {
     "remora_b200_replicate": (_I32, [_VP, _I32, _VP, _VP, _VP, _VP, _VP]),
     "remora_b200_rotate": (_I32, [_VP, _I32, ctypes.c_int64, _VP, _VP, _I32, _VP]),
     "remora_b200_append": (_I32, [_VP, _I32, _VP, _VP, _VP, _I32, _VP]),
+    "remora_b200_rms_norm_fwd": (_I32, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _I32, _VP]),
+    "remora_b200_rms_norm_quant": (_I32, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I32, _VP]),
+    "remora_b200_rms_norm_bwd_scratch": (_I32, [_VP, _I64, _I64, ctypes.POINTER(_SZ)]),
+    "remora_b200_rms_norm_bwd": (_I32, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I32, _VP, _SZ, _VP]),
+    "remora_b200_causal_conv_fwd": (_I32, [_VP] * 10),
+    "remora_b200_causal_conv_bwd_scratch": (_I32, [_VP, _I64, _I64, _I64, _I64, ctypes.POINTER(_SZ)]),
+    "remora_b200_causal_conv_bwd": (_I32, [_VP] * 14 + [_SZ, _VP]),
+    "remora_b200_causal_conv_step": (_I32, [_VP] * 10),
+    "remora_b200_selective_scan_saved": (_I32, [_I64, _I64, _I64, _I64, ctypes.POINTER(_SZ)]),
+    "remora_b200_selective_scan_fwd_scratch": (_I32, [_VP, _I64, _I64, _I64, _I64, _I64, ctypes.POINTER(_SZ)]),
+    "remora_b200_selective_scan_fwd": (_I32, [_VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP, _SZ, _VP]),
+    "remora_b200_selective_scan_bwd_scratch": (_I32, [_VP, _I64, _I64, _I64, _I64, _I64, ctypes.POINTER(_SZ)]),
+    "remora_b200_selective_scan_bwd": (_I32, [_VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP, _VP, _SZ, _VP]),
+    "remora_b200_selective_scan_step": (_I32, [_VP] * 6),
 }
 
 _lib: ctypes.CDLL | None = None

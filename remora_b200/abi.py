@@ -107,11 +107,14 @@ def contiguous_strides(shape: Sequence[int]) -> tuple[int, ...]:
 def tensor_descriptor(t) -> ctypes.Structure:
     """Descriptor of a torch tensor view: `aligned` is the storage base and the
     view's start lives in `offset` (the ABI's view rule, docs/ABI.md:32)."""
-    if t.dim() > MAX_RANK:
-        raise RemoraB200Error(f"rank {t.dim()} exceeds the ABI's {MAX_RANK}")
-    base = t.untyped_storage().data_ptr() if t.numel() else t.data_ptr()
-    off = t.storage_offset() if t.numel() else 0
-    return make_memref_descriptor(base, t.shape, t.stride(), None, off)
+    rank = t.dim()
+    if rank > MAX_RANK:
+        raise RemoraB200Error(f"rank {rank} exceeds the ABI's {MAX_RANK}")
+    if t.numel():
+        base, off = t.untyped_storage().data_ptr(), t.storage_offset()
+    else:
+        base, off = t.data_ptr(), 0
+    return DESCRIPTORS[rank](base, base, off, *t.shape, *t.stride())
 
 
 def numpy_descriptor(array: np.ndarray) -> ctypes.Structure:

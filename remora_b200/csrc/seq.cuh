@@ -1,0 +1,204 @@
+// seq.cuh — what the sequence operators (seq_norm.cu, seq_conv.cu,
+// seq_scan*.cu) share: host-side checks of descriptors, the device guard, and
+// a few device helpers.
+#pragma once
+
+#include <initializer_list>
+
+#include "../../include/remora_b200_seq.h"
+#include "common.cuh"
+
+namespace remora {
+namespace seq {
+
+// Makes the context's device current and puts the caller's back.  Entered
+// once the arguments are checked: a refused call makes no CUDA call.
+struct DeviceGuard {
+  int prev = -1;
+  bool moved = false;
+  int enter(RemoraB200Ctx *ctx) {
+    REMORA_CUDA_TRY(cudaGetDevice(&prev));
+    if (prev != ctx->device) {
+      REMORA_CUDA_TRY(cudaSetDevice(ctx->device));
+      moved = true;
+    }
+    return REMORA_OK;
+  }
+  ~DeviceGuard() {
+    if (moved) cudaSetDevice(prev);
+  }
+};
+
+inline int read_f32(const void *desc, int rank, DescView *out, const char *what) {
+  REMORA_TRY(read_desc(desc, rank, out, what));
+  if (reinterpret_cast<uintptr_t>(out->aligned) & 3)
+    return fail(REMORA_ERR_ARG, "%s: data pointer is not aligned to its 4-byte elements", what);
+  return REMORA_OK;
+}
+
+// As read_f32, and leaves *have false for a null descriptor.
+inline int read_optional(const void *desc, int rank, DescView *out, bool *have, const char *what) {
+  *have = desc != nullptr;
+  return *have ? read_f32(desc, rank, out, what) : REMORA_OK;
+}
+
+inline int want_shape(const DescView &v, std::initializer_list<int64_t> sizes, const char *what) {
+  int d = 0;
+  for (int64_t s : sizes) {
+    if (v.sizes[d] != s)
+      return fail(REMORA_ERR_SHAPE, "%s: axis %d has size %lld where the other operands give %lld", what, d,
+                  (long long)v.sizes[d], (long long)s);
+    ++d;
+  }
+  return REMORA_OK;
+}
+
+inline bool same_view(const DescView &a, const DescView &b) {
+  if (a.rank != b.rank || a.aligned + a.offset * 4 != b.aligned + b.offset * 4) return false;
+  for (int d = 0; d < a.rank; ++d)
+    if (a.sizes[d] != b.sizes[d] || (a.sizes[d] > 1 && a.strides[d] != b.strides[d])) return false;
+  return true;
+}
+
+// Byte range of a view's elements.
+inline void byte_range(const DescView &v, int esize, uintptr_t *lo, uintptr_t *hi) {
+  int64_t mn = 0, mx = 0;
+  for (int d = 0; d < v.rank; ++d) {
+    const int64_t span = (v.sizes[d] - 1) * v.strides[d];
+    (span < 0 ? mn : mx) += span;
+  }
+  const uintptr_t base = reinterpret_cast<uintptr_t>(v.aligned) + (uintptr_t)(v.offset * esize);
+  *lo = base + (uintptr_t)(mn * esize);
+  *hi = base + (uintptr_t)(mx * esize) + (uintptr_t)esize;
+}
+
+// Whether two views may share a byte.  Ranges that meet are still apart when
+// both views are columns of rows with one pitch (strides that are multiples
+// of it, but for a unit stride along the row) and their columns are apart.
+inline bool may_overlap(const DescView &a, int ea, const DescView &b, int eb) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  uintptr_t alo, ahi, blo, bhi;
+  byte_range(a, ea, &alo, &ahi);
+  byte_range(b, eb, &blo, &bhi);
+  if (ahi <= blo || bhi <= alo) return false;
+  int64_t pitch = 0;  // bytes: the largest common row pitch of the two
+  const DescView *vs[2] = {&a, &b};
+  const int es[2] = {ea, eb};
+  int64_t extent[2] = {ea, eb};
+  for (int k = 0; k < 2; ++k)
+    for (int d = 0; d < vs[k]->rank; ++d) {
+      if (vs[k]->sizes[d] <= 1) continue;
+      const int64_t st = vs[k]->strides[d] * es[k];
+      if (st == es[k]) {
+        extent[k] = vs[k]->sizes[d] * (int64_t)es[k];
+        continue;
+      }
+      if (st <= 0) return true;
+      int64_t x = pitch, y = st;  // gcd
+      while (y) {
+        const int64_t t = x % y;
+        x = y;
+        y = t;
+      }
+      pitch = x;
+    }
+  if (pitch == 0) return true;
+  // b's columns start `gap` bytes behind a's, in a's row or the next
+  int64_t gap = ((b.aligned + b.offset * eb) - (a.aligned + a.offset * ea)) % pitch;
+  if (gap < 0) gap += pitch;
+  return gap < extent[0] || gap + extent[1] > pitch;
+}
+
+// An output whose own elements share addresses (a stride of 0 over more than
+// one element) cannot hold a result.
+inline int want_own_elements(const DescView &v, const char *what) {
+  for (int d = 0; d < v.rank; ++d)
+    if (v.sizes[d] > 1 && v.strides[d] == 0)
+      return fail(REMORA_ERR_ARG, "%s: an output with stride 0 along axis %d", what, d);
+  return REMORA_OK;
+}
+
+struct Named {
+  const DescView *v;
+  const char *name;
+  int esize;
+};
+
+// Refuses outputs that overlap an input or another output.  An output listed
+// in `in_place` may be exactly that input.
+inline int want_apart(std::initializer_list<Named> outs, std::initializer_list<Named> ins,
+                      std::initializer_list<const DescView *> in_place = {}) {
+  for (const Named &o : outs) {
+    if (o.v == nullptr) continue;
+    REMORA_TRY(want_own_elements(*o.v, o.name));
+    for (const Named &i : ins) {
+      if (i.v == nullptr || !may_overlap(*o.v, o.esize, *i.v, i.esize)) continue;
+      bool allowed = false;
+      for (const DescView *p : in_place) allowed |= p == i.v && o.esize == i.esize && same_view(*o.v, *i.v);
+      if (!allowed) return fail(REMORA_ERR_ARG, "%s overlaps %s", o.name, i.name);
+    }
+    for (const Named &p : outs)
+      if (p.v != nullptr && p.v < o.v && may_overlap(*o.v, o.esize, *p.v, p.esize))
+        return fail(REMORA_ERR_ARG, "%s overlaps %s", o.name, p.name);
+  }
+  return REMORA_OK;
+}
+
+inline int want_scratch(const void *scratch, size_t have, size_t need, const char *what) {
+  if (need == 0) return REMORA_OK;
+  if (scratch == nullptr || have < need)
+    return fail(REMORA_ERR_LIMIT, "%s: needs %zu bytes of scratch, got %zu", what, need, scratch ? have : (size_t)0);
+  if (reinterpret_cast<uintptr_t>(scratch) & 15)
+    return fail(REMORA_ERR_ARG, "%s: scratch is not 16-byte aligned", what);
+  return REMORA_OK;
+}
+
+// Where reduce_rows puts column c: out[(c / inner) * outer_stride + (c % inner)
+// * inner_stride], or from column `split` on tail[(c - split) * tail_stride]
+// (columns whose target is null are left out).
+struct Columns {
+  float *out;
+  int64_t inner, outer_stride, inner_stride;
+  int64_t split;
+  float *tail;
+  int64_t tail_stride;
+};
+
+// The sum over the rows of part [rows, cols], in a fixed order.
+int reduce_rows(const float *part, int64_t rows, int64_t cols, const Columns &to, cudaStream_t stream);
+
+#ifdef __CUDACC__
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 1 / (1 + exp(-v)).  __expf is within 2 + 1.2 |v| units in the last place, so
+// the result is too; exp(-v) = inf gives 0.
+__device__ __forceinline__ float sigmoid(float v) { return __frcp_rn(1.0f + __expf(-v)); }
+
+// log(1 + exp(v)) = max(v, 0) + log1p(e), e = exp(-|v|) in (0, 1].  With
+// s = e / (2 + e) <= 1/3, log1p(e) = 2 atanh(s) = 2 s (1 + s^2/3 + s^4/5 + ..):
+// seven terms leave a relative remainder below 9^-7 / 15 = 1.4e-8.  *sig gets
+// the derivative 1 / (1 + exp(-v)).
+__device__ __forceinline__ float softplus(float v, float *sig) {
+  const float e = expf(-fabsf(v));
+  const float r = __frcp_rn(1.0f + e);
+  *sig = v >= 0.0f ? r : e * r;
+  const float s = __fdividef(e, 2.0f + e);
+  const float q = s * s;
+  float p = fmaf(q, 1.0f / 13, 1.0f / 11);
+  p = fmaf(q, p, 1.0f / 9);
+  p = fmaf(q, p, 1.0f / 7);
+  p = fmaf(q, p, 1.0f / 5);
+  p = fmaf(q, p, 1.0f / 3);
+  p = fmaf(q, p, 1.0f);
+  return fmaxf(v, 0.0f) + 2.0f * s * p;
+}
+#endif
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+}  // namespace seq
+}  // namespace remora

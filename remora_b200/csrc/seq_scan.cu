@@ -1,0 +1,515 @@
+// seq_scan.cu — selective state space scan: forward over prompts and training
+// sequences, and one step for single tokens.
+//
+//   s = f(delta + bias);  h[n] = exp(s a[n]) h[n] + s u b[n];  p = sum_n c[n] h[n] + d u;  y = p silu(z)
+//
+// Per position and channel: 16 bytes of HBM (u, delta, z, y), N exponentials
+// and about 6 N other operations.  At N = 16 the exponentials bound it: the
+// special function units give 16 per clock and SM.
+//
+// The recurrence is serial in time.  Where batch x channels give too few
+// threads, time is cut into pieces: a first pass gives each piece's end state
+// from a zero start and its sum of steps (its decay is exp(a sum s)), a small
+// kernel joins them, and the main pass starts each piece from its own state.
+// That doubles the exponentials, so pieces are as few as fill the device.
+#include <algorithm>
+
+#include "seq_scan.cuh"
+
+namespace remora {
+namespace seq {
+namespace {
+
+constexpr int kTile = 32;  // steps of b and c staged at a time
+
+// MAIN: writes y (and h_last, saved).  Otherwise the first pass of a cut time
+// axis: sum_h and sum_dt.  PADDED: N is not 4 NL; the states past N must stay
+// zero even where s u is not finite.
+template <int NL, bool PADDED, bool MAIN>
+__global__ void __launch_bounds__(kScanThreads) scan_fwd_kernel(const ScanArgs a) {
+  constexpr int NP = 4 * NL;
+  constexpr int GROUP = NL > 8 ? NL : 8;  // steps whose inputs are loaded together
+  constexpr int PF = GROUP / NL;          // of them, per lane
+  __shared__ __align__(16) float bs[2][kTile * NP];
+  __shared__ __align__(16) float cs[2][MAIN ? kTile * NP : 4];
+  const Place<NL> at(a);
+  const int64_t len = scan_length(a, at.b);
+  const int64_t t0 = at.chunk * a.chunk, t_end = min(t0 + a.chunk, len);
+  if (t0 >= len && t0 > 0) return;  // the first piece of an empty sequence hands h0 on
+  const int nv = a.states - 4 * at.q;  // of the four states, those below N
+  float A[4], h[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const bool on = at.live && k < nv;
+    A[k] = on ? a.a[at.d * a.a_d + (4 * at.q + k) * a.a_n] * kLog2e : 0.0f;
+    h[k] = 0.0f;
+    if (MAIN && on && a.chunks == 1 && a.h0.p)
+      h[k] = a.h0.p[at.b * a.h0.s0 + at.d * a.h0.s1 + (4 * at.q + k) * a.h0.s2];
+  }
+  if (MAIN && a.chunks > 1)
+    unpack(reinterpret_cast<const float4 *>(a.sum_h)[((at.b * a.chunks + at.chunk) * a.dim + at.d) * NL + at.q], h);
+  const float bias = a.bias ? a.bias[at.d * a.bias_s] : 0.0f;
+  const float skip = MAIN && a.d ? a.d[at.d * a.d_s] : 0.0f;
+  const float *up = a.u.p + at.b * a.u.s0 + at.d * a.u.s2;
+  const float *dp = a.delta.p + at.b * a.delta.s0 + at.d * a.delta.s2;
+  const float *zp = a.z.p + at.b * a.z.s0 + at.d * a.z.s2;
+  float *yp = a.y.p + at.b * a.y.s0 + at.d * a.y.s2;
+  float ru[PF], rd[PF], rz[PF], total = 0.0f;
+  auto fetch = [&](int64_t base) {
+#pragma unroll
+    for (int i = 0; i < PF; ++i) {
+      const int64_t t = base + i * NL + at.q;
+      const bool on = at.live && t < t_end;
+      ru[i] = on ? up[t * a.u.s1] : 0.0f;
+      rd[i] = on ? dp[t * a.delta.s1] : 0.0f;
+      if (MAIN && a.z.p) rz[i] = on ? zp[t * a.z.s1] : 0.0f;
+    }
+  };
+  auto stage = [&](int buf, int64_t t) {
+    stage_rows<NL, kTile>(bs[buf], a.b, a.vec_b, at.b, at.g, t, t_end, a.states);
+    if (MAIN) stage_rows<NL, kTile>(cs[buf], a.c, a.vec_c, at.b, at.g, t, t_end, a.states);
+    copy_commit();
+  };
+  if (t0 < t_end) {
+    stage(0, t0);
+    fetch(t0);
+  }
+  int buf = 0;
+  for (int64_t tile = t0; tile < t_end; tile += kTile, buf ^= 1) {
+    if (tile + kTile < t_end)
+      stage(buf ^ 1, tile + kTile);
+    else
+      copy_commit();  // an empty group, so that the wait below counts alike
+    copy_wait<1>();
+    __syncthreads();
+#pragma unroll 1
+    for (int off = 0; off < kTile && tile + off < t_end; off += GROUP) {
+      const int64_t base = tile + off;
+      float s[PF], su[PF], u[PF], z[PF];
+#pragma unroll
+      for (int i = 0; i < PF; ++i) {
+        const float raw = rd[i] + bias;
+        float sig;
+        s[i] = a.softplus ? softplus(raw, &sig) : raw;
+        u[i] = ru[i], z[i] = rz[i];
+        su[i] = s[i] * u[i];
+        if (!MAIN && base + i * NL + at.q < t_end) total += s[i];
+      }
+      if (base + GROUP < t_end) fetch(base + GROUP);
+      if (MAIN && a.saved && at.live && base % kSaveEvery == 0)
+        reinterpret_cast<float4 *>(
+            a.saved)[((at.b * ((a.length + kSaveEvery - 1) / kSaveEvery) + base / kSaveEvery) * a.dim + at.d) * NL +
+                     at.q] = make_float4(h[0], h[1], h[2], h[3]);
+      const bool full = base + GROUP <= t_end;
+#pragma unroll
+      for (int i = 0; i < PF; ++i) {
+        float part[NL];
+#pragma unroll
+        for (int j = 0; j < NL; ++j) {
+          part[j] = 0.0f;
+          const float sj = __shfl_sync(0xffffffffu, s[i], j, NL);
+          const float suj = __shfl_sync(0xffffffffu, su[i], j, NL);
+          if (full || base + i * NL + j < t_end) {
+            float b[4], c[4];
+            unpack(*reinterpret_cast<const float4 *>(&bs[buf][(off + i * NL + j) * NP + 4 * at.q]), b);
+            if (MAIN) unpack(*reinterpret_cast<const float4 *>(&cs[buf][(off + i * NL + j) * NP + 4 * at.q]), c);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float in = PADDED && k >= nv ? 0.0f : suj * b[k];
+              h[k] = fmaf(ex2(sj * A[k]), h[k], in);
+              if (MAIN) part[j] = fmaf(h[k], c[k], part[j]);
+            }
+          }
+        }
+        if (MAIN) {
+          transpose_sum<NL>(part, at.q);
+          const int64_t t = base + i * NL + at.q;
+          if (at.live && t < t_end) {
+            float y = fmaf(skip, u[i], part[0]);
+            if (a.z.p) y *= z[i] * sigmoid(z[i]);
+            yp[t * a.y.s1] = y;
+          }
+        }
+      }
+    }
+    __syncthreads();  // this buffer is filled again in the next turn
+  }
+  if (MAIN) {
+    if (a.h_last.p && at.live && t_end == len) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k < nv) a.h_last.p[at.b * a.h_last.s0 + at.d * a.h_last.s1 + (4 * at.q + k) * a.h_last.s2] = h[k];
+    }
+  } else {
+#pragma unroll
+    for (int o = 1; o < NL; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if (at.live) {
+      const int64_t i = (at.b * a.chunks + at.chunk) * a.dim + at.d;
+      reinterpret_cast<float4 *>(a.sum_h)[i * NL + at.q] = make_float4(h[0], h[1], h[2], h[3]);
+      if (at.q == 0) a.sum_dt[i] = total;
+    }
+  }
+}
+
+// Joins the pieces: sum_h of a piece becomes the state it starts from (in
+// reverse, the adjoint that reaches its end).
+__global__ void __launch_bounds__(256) scan_combine_kernel(const ScanArgs a, int np, int reverse) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.batch * a.dim * np) return;
+  const int n = (int)(i % np);
+  const int64_t d = i / np % a.dim, b = i / np / a.dim;
+  const int64_t len = scan_length(a, b);
+  const int64_t used = max((int64_t)1, (len + a.chunk - 1) / a.chunk);
+  const Op3 &first = reverse ? a.dh_last : a.h0;
+  const bool on = n < a.states;
+  const float A = on ? a.a[d * a.a_d + n * a.a_n] * kLog2e : 0.0f;
+  float h = on && first.p ? first.p[b * first.s0 + d * first.s1 + n * first.s2] : 0.0f;
+  for (int64_t k = 0; k < used; ++k) {
+    const int64_t j = (b * a.chunks + (reverse ? used - 1 - k : k)) * a.dim + d;
+    const float own = a.sum_h[j * np + n], dt = a.sum_dt[j];
+    a.sum_h[j * np + n] = h;
+    h = fmaf(ex2(dt * A), h, own);
+  }
+}
+
+struct TokenArgs {
+  Op3 state, state_out, b, c;  // b, c: [B, G, N]
+  const float *u, *delta, *z, *a, *d, *bias;
+  float *y;
+  int64_t u_b, u_d, delta_b, delta_d, z_b, z_d, y_b, y_d, a_d, a_n, d_s, bias_s;
+  const int *slots;
+  int64_t slots_s;
+  int64_t batch, rows, dim, per;
+  int states, softplus, vec;
+};
+
+// Four states of one channel and row per thread; bound by the states' bytes.
+template <int NL>
+__global__ void __launch_bounds__(kScanThreads) scan_step_kernel(const TokenArgs a) {
+  const int64_t i = blockIdx.y;
+  int64_t slot = i;
+  bool live = true;
+  if (a.slots != nullptr) {
+    slot = a.slots[i * a.slots_s];
+    bool again = false;
+    for (int64_t k = threadIdx.x; k < i; k += kScanThreads) again |= a.slots[k * a.slots_s] == slot;
+    live = !__syncthreads_or(again) && slot >= 0 && slot < a.rows;
+  }
+  const int q = threadIdx.x % NL;
+  const int64_t d = (int64_t)blockIdx.x * (kScanThreads / NL) + threadIdx.x / NL;
+  live = live && d < a.dim;
+  const int nv = live ? a.states - 4 * q : 0;
+  float sum = 0.0f, u = 0.0f;
+  if (live) {
+    const int64_t g = d / a.per;
+    const float *hp = a.state.p + slot * a.state.s0 + d * a.state.s1 + 4 * q * a.state.s2;
+    const float *ap = a.a + d * a.a_d + 4 * q * a.a_n;
+    const float *bp = a.b.p + i * a.b.s0 + g * a.b.s1 + 4 * q * a.b.s2;
+    const float *cp = a.c.p + i * a.c.s0 + g * a.c.s1 + 4 * q * a.c.s2;
+    float h[4], A[4], b[4], c[4];
+    if (a.vec) {
+      if (nv > 0) {
+        unpack(*reinterpret_cast<const float4 *>(hp), h);
+        unpack(*reinterpret_cast<const float4 *>(ap), A);
+        unpack(*reinterpret_cast<const float4 *>(bp), b);
+        unpack(*reinterpret_cast<const float4 *>(cp), c);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k < nv) h[k] = hp[k * a.state.s2], A[k] = ap[k * a.a_n], b[k] = bp[k * a.b.s2], c[k] = cp[k * a.c.s2];
+    }
+    u = a.u[i * a.u_b + d * a.u_d];
+    float s = a.delta[i * a.delta_b + d * a.delta_d] + (a.bias ? a.bias[d * a.bias_s] : 0.0f), sig;
+    if (a.softplus) s = softplus(s, &sig);
+    const float su = s * u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < nv) {
+        h[k] = fmaf(ex2(s * (A[k] * kLog2e)), h[k], su * b[k]);
+        sum = fmaf(h[k], c[k], sum);
+      }
+    float *ho = a.state_out.p + slot * a.state_out.s0 + d * a.state_out.s1 + 4 * q * a.state_out.s2;
+    if (a.vec) {
+      if (nv > 0) *reinterpret_cast<float4 *>(ho) = make_float4(h[0], h[1], h[2], h[3]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k < nv) ho[k * a.state_out.s2] = h[k];
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < NL; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (live && q == 0) {
+    float y = fmaf(a.d ? a.d[d * a.d_s] : 0.0f, u, sum);
+    if (a.z) {
+      const float z = a.z[i * a.z_b + d * a.z_d];
+      y *= z * sigmoid(z);
+    }
+    a.y[i * a.y_b + d * a.y_d] = y;
+  }
+}
+
+// ------------------------------------------------------------------ host --
+Op3 op3(const DescView &v) {
+  return {reinterpret_cast<float *>(v.data(4)), v.strides[0], v.strides[1], v.strides[2]};
+}
+
+Op4 op4(const DescView &v) {
+  return {reinterpret_cast<float *>(v.data(4)), v.strides[0], v.strides[1], v.strides[2], v.strides[3]};
+}
+
+// Rows that 16-byte copies can take: unit stride, a multiple of four states,
+// every row 16-byte aligned.
+bool vec_states(const DescView &v) {
+  const int last = v.rank - 1;
+  if (v.sizes[last] % 4 || v.strides[last] != 1 || (reinterpret_cast<uintptr_t>(v.data(4)) & 15)) return false;
+  for (int d = 0; d < last; ++d)
+    if (v.sizes[d] > 1 && (v.strides[d] & 3)) return false;
+  return true;
+}
+
+// Pieces of the time axis: one when the channels alone give the device enough
+// warps, else as many as do, of at least 64 steps each.
+void cut_time(int64_t batch, int64_t length, int64_t dim, int states, int groups, int64_t *chunks, int64_t *chunk) {
+  const int nl = lanes_for(states);
+  const int64_t per_block = kScanThreads / nl, per = dim / std::max(groups, 1);
+  const int64_t blocks = std::max<int64_t>(1, batch * groups * ((per + per_block - 1) / per_block));
+  int64_t n = 1;
+  if (blocks < 148 * 3) n = std::max<int64_t>(1, std::min<int64_t>(148 * 5 / blocks, length / 64));
+  *chunk = std::max<int64_t>(kTile, ((length + n - 1) / n + kTile - 1) / kTile * kTile);
+  *chunks = std::max<int64_t>(1, (length + *chunk - 1) / *chunk);
+}
+
+size_t scratch_for(int64_t batch, int64_t dim, int states, int64_t chunks) {
+  if (chunks <= 1) return 0;
+  return (size_t)(batch * chunks * dim) * (4 * lanes_for(states) + 4) * 4;
+}
+
+int check_sizes(int64_t batch, int64_t length, int64_t dim, int64_t states, int64_t groups, const char *what) {
+  if (batch < 0 || length < 0 || dim < 0) return fail(REMORA_ERR_ARG, "%s: negative size", what);
+  if (states < 1 || states > kMaxStates)
+    return fail(REMORA_ERR_UNSUPPORTED, "%s: %lld states (1..%d)", what, (long long)states, kMaxStates);
+  if (groups < 1 || dim % groups)
+    return fail(REMORA_ERR_SHAPE, "%s: %lld channels in %lld groups", what, (long long)dim, (long long)groups);
+  return REMORA_OK;
+}
+
+template <bool MAIN>
+int launch_fwd(const ScanArgs &a, int nl, cudaStream_t stream) {
+  const unsigned grid = (unsigned)(a.batch * a.chunks * a.groups * a.blocks_d);
+  const bool padded = a.states != 4 * nl;
+  note_launch();
+#define REMORA_SCAN_CASE(NL)                                                            \
+  case NL:                                                                              \
+    if (padded)                                                                         \
+      scan_fwd_kernel<NL, true, MAIN><<<grid, kScanThreads, 0, stream>>>(a);            \
+    else                                                                                \
+      scan_fwd_kernel<NL, false, MAIN><<<grid, kScanThreads, 0, stream>>>(a);           \
+    break;
+  switch (nl) {
+    REMORA_SCAN_CASE(1)
+    REMORA_SCAN_CASE(2)
+    REMORA_SCAN_CASE(4)
+    REMORA_SCAN_CASE(8)
+    REMORA_SCAN_CASE(16)
+  }
+#undef REMORA_SCAN_CASE
+  REMORA_CUDA_TRY(cudaGetLastError());
+  return REMORA_OK;
+}
+
+}  // namespace
+
+// Reads and checks the inputs; views: u, delta, a, b, c, d, z, delta_bias,
+// h0, lengths, those not given with a null data pointer and rank 0.
+int read_scan_in(const RemoraSelectiveScanSpec *spec, const RemoraSelectiveScanIn *in, ScanArgs *a, DescView views[10],
+                 const char *what) {
+  if (spec == nullptr || in == nullptr) return fail(REMORA_ERR_ARG, "%s: null spec or inputs", what);
+  bool have[10];
+  REMORA_TRY(read_f32(in->u, 3, &views[0], "selective_scan u"));
+  REMORA_TRY(read_f32(in->delta, 3, &views[1], "selective_scan delta"));
+  REMORA_TRY(read_f32(in->a, 2, &views[2], "selective_scan a"));
+  REMORA_TRY(read_f32(in->b, 4, &views[3], "selective_scan b"));
+  REMORA_TRY(read_f32(in->c, 4, &views[4], "selective_scan c"));
+  REMORA_TRY(read_optional(in->d, 1, &views[5], &have[5], "selective_scan d"));
+  REMORA_TRY(read_optional(in->z, 3, &views[6], &have[6], "selective_scan z"));
+  REMORA_TRY(read_optional(in->delta_bias, 1, &views[7], &have[7], "selective_scan delta_bias"));
+  REMORA_TRY(read_optional(in->h0, 3, &views[8], &have[8], "selective_scan h0"));
+  REMORA_TRY(read_optional(in->lengths, 1, &views[9], &have[9], "selective_scan lengths"));
+  const int64_t B = views[0].sizes[0], L = views[0].sizes[1], D = views[0].sizes[2];
+  const int64_t N = views[2].sizes[1], G = views[3].sizes[2];
+  REMORA_TRY(check_sizes(B, L, D, N, G, what));
+  REMORA_TRY(want_shape(views[1], {B, L, D}, "selective_scan delta"));
+  REMORA_TRY(want_shape(views[2], {D, N}, "selective_scan a"));
+  REMORA_TRY(want_shape(views[3], {B, L, G, N}, "selective_scan b"));
+  REMORA_TRY(want_shape(views[4], {B, L, G, N}, "selective_scan c"));
+  if (have[5]) REMORA_TRY(want_shape(views[5], {D}, "selective_scan d"));
+  if (have[6]) REMORA_TRY(want_shape(views[6], {B, L, D}, "selective_scan z"));
+  if (have[7]) REMORA_TRY(want_shape(views[7], {D}, "selective_scan delta_bias"));
+  if (have[8]) REMORA_TRY(want_shape(views[8], {B, D, N}, "selective_scan h0"));
+  if (have[9]) REMORA_TRY(want_shape(views[9], {B}, "selective_scan lengths"));
+  a->u = op3(views[0]), a->delta = op3(views[1]);
+  a->a = reinterpret_cast<const float *>(views[2].data(4)), a->a_d = views[2].strides[0], a->a_n = views[2].strides[1];
+  a->b = op4(views[3]), a->c = op4(views[4]);
+  a->vec_b = vec_states(views[3]), a->vec_c = vec_states(views[4]);
+  if (have[5]) a->d = reinterpret_cast<const float *>(views[5].data(4)), a->d_s = views[5].strides[0];
+  if (have[6]) a->z = op3(views[6]);
+  if (have[7]) a->bias = reinterpret_cast<const float *>(views[7].data(4)), a->bias_s = views[7].strides[0];
+  if (have[8]) a->h0 = op3(views[8]);
+  if (have[9]) a->lengths = reinterpret_cast<const int *>(views[9].data(4)), a->lengths_s = views[9].strides[0];
+  a->batch = B, a->length = L, a->dim = D, a->states = (int)N, a->groups = (int)G, a->softplus = spec->softplus != 0;
+  a->per = D / G;
+  const int64_t per_block = kScanThreads / lanes_for((int)N);
+  a->blocks_d = (a->per + per_block - 1) / per_block;
+  return REMORA_OK;
+}
+
+int combine_chunks(const ScanArgs &a, int nl, bool reverse, cudaStream_t stream) {
+  const int64_t n = a.batch * a.dim * 4 * nl;
+  note_launch();
+  scan_combine_kernel<<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(a, 4 * nl, reverse ? 1 : 0);
+  REMORA_CUDA_TRY(cudaGetLastError());
+  return REMORA_OK;
+}
+
+}  // namespace seq
+}  // namespace remora
+
+using namespace remora;
+using namespace remora::seq;
+
+extern "C" {
+
+int remora_b200_selective_scan_saved(int64_t batch, int64_t length, int64_t dim, int64_t states, size_t *bytes) {
+  if (bytes == nullptr) return fail(REMORA_ERR_ARG, "selective_scan_saved: null pointer");
+  REMORA_TRY(check_sizes(batch, length, dim, states, 1, "selective_scan_saved"));
+  *bytes = (size_t)(batch * ((length + kSaveEvery - 1) / kSaveEvery) * dim) * (size_t)(4 * lanes_for((int)states)) * 4;
+  return REMORA_OK;
+}
+
+int remora_b200_selective_scan_fwd_scratch(RemoraB200Ctx *ctx, int64_t batch, int64_t length, int64_t dim,
+                                           int64_t states, int64_t groups, size_t *bytes) {
+  if (ctx == nullptr || bytes == nullptr) return fail(REMORA_ERR_ARG, "selective_scan_fwd_scratch: null pointer");
+  REMORA_TRY(check_sizes(batch, length, dim, states, groups, "selective_scan_fwd_scratch"));
+  int64_t chunks, chunk;
+  cut_time(batch, length, dim, (int)states, (int)groups, &chunks, &chunk);
+  *bytes = scratch_for(batch, dim, (int)states, chunks);
+  return REMORA_OK;
+}
+
+int remora_b200_selective_scan_fwd(RemoraB200Ctx *ctx, const RemoraSelectiveScanSpec *spec,
+                                   const RemoraSelectiveScanIn *in, RemoraMemRef3 *y, RemoraMemRef3 *h_last,
+                                   void *saved, size_t saved_bytes, void *scratch, size_t scratch_bytes,
+                                   remora_stream_t stream_) {
+  if (ctx == nullptr) return fail(REMORA_ERR_ARG, "null context");
+  cudaStream_t stream = (cudaStream_t)stream_;
+  ScanArgs a = {};
+  DescView v[10], yv, hv;
+  bool has_h;
+  REMORA_TRY(read_scan_in(spec, in, &a, v, "selective_scan_fwd"));
+  REMORA_TRY(read_f32(y, 3, &yv, "selective_scan y"));
+  REMORA_TRY(read_optional(h_last, 3, &hv, &has_h, "selective_scan h_last"));
+  REMORA_TRY(want_shape(yv, {a.batch, a.length, a.dim}, "selective_scan y"));
+  if (has_h) REMORA_TRY(want_shape(hv, {a.batch, a.dim, a.states}, "selective_scan h_last"));
+  auto given = [&](int k) { return v[k].aligned != nullptr ? &v[k] : nullptr; };
+  REMORA_TRY(want_apart({{&yv, "y", 4}, {has_h ? &hv : nullptr, "h_last", 4}},
+                        {{given(0), "u", 4}, {given(1), "delta", 4}, {given(2), "a", 4}, {given(3), "b", 4},
+                         {given(4), "c", 4}, {given(5), "d", 4}, {given(6), "z", 4}, {given(7), "delta_bias", 4},
+                         {given(8), "h0", 4}, {given(9), "lengths", 4}}, {&v[8]}));
+  a.y = op3(yv);
+  if (has_h) a.h_last = op3(hv);
+  cut_time(a.batch, a.length, a.dim, a.states, a.groups, &a.chunks, &a.chunk);
+  const int nl = lanes_for(a.states);
+  if (saved != nullptr) {
+    size_t need = 0;
+    REMORA_TRY(remora_b200_selective_scan_saved(a.batch, a.length, a.dim, a.states, &need));
+    REMORA_TRY(want_scratch(saved, saved_bytes, need, "selective_scan_fwd (saved)"));
+    a.saved = static_cast<float *>(saved);
+  }
+  REMORA_TRY(want_scratch(scratch, scratch_bytes, scratch_for(a.batch, a.dim, a.states, a.chunks),
+                          "selective_scan_fwd"));
+  if (a.batch == 0 || a.dim == 0 || (a.length == 0 && !has_h)) return REMORA_OK;
+  if (a.batch * a.chunks * a.groups * a.blocks_d > 0x7fffffff || a.batch * a.dim * 4 * nl / 256 > 0x7ffffffe)
+    return fail(REMORA_ERR_LIMIT, "selective_scan_fwd: too many blocks");
+  DeviceGuard guard;
+  REMORA_TRY(guard.enter(ctx));
+  if (a.chunks > 1) {
+    a.sum_h = static_cast<float *>(scratch);
+    a.sum_dt = a.sum_h + a.batch * a.chunks * a.dim * 4 * nl;
+    REMORA_TRY(launch_fwd<false>(a, nl, stream));
+    REMORA_TRY(combine_chunks(a, nl, false, stream));
+  }
+  return launch_fwd<true>(a, nl, stream);
+}
+
+int remora_b200_selective_scan_step(RemoraB200Ctx *ctx, const RemoraSelectiveScanSpec *spec,
+                                    const RemoraSelectiveStepIn *in, RemoraMemRef2 *y, RemoraMemRef3 *state_out,
+                                    remora_stream_t stream) {
+  if (ctx == nullptr) return fail(REMORA_ERR_ARG, "null context");
+  if (spec == nullptr || in == nullptr) return fail(REMORA_ERR_ARG, "selective_scan_step: null spec or inputs");
+  DescView sv, uv, ev, av, bv, cv, dv, zv, iv, lv, yv, ov;
+  bool has_d, has_z, has_i, has_l;
+  REMORA_TRY(read_f32(in->state, 3, &sv, "selective_scan_step state"));
+  REMORA_TRY(read_f32(in->u, 2, &uv, "selective_scan_step u"));
+  REMORA_TRY(read_f32(in->delta, 2, &ev, "selective_scan_step delta"));
+  REMORA_TRY(read_f32(in->a, 2, &av, "selective_scan_step a"));
+  REMORA_TRY(read_f32(in->b, 3, &bv, "selective_scan_step b"));
+  REMORA_TRY(read_f32(in->c, 3, &cv, "selective_scan_step c"));
+  REMORA_TRY(read_optional(in->d, 1, &dv, &has_d, "selective_scan_step d"));
+  REMORA_TRY(read_optional(in->z, 2, &zv, &has_z, "selective_scan_step z"));
+  REMORA_TRY(read_optional(in->delta_bias, 1, &iv, &has_i, "selective_scan_step delta_bias"));
+  REMORA_TRY(read_optional(in->slots, 1, &lv, &has_l, "selective_scan_step slots"));
+  REMORA_TRY(read_f32(y, 2, &yv, "selective_scan_step y"));
+  REMORA_TRY(read_f32(state_out, 3, &ov, "selective_scan_step state_out"));
+  const int64_t B = uv.sizes[0], D = uv.sizes[1], N = av.sizes[1], G = bv.sizes[1], S = sv.sizes[0];
+  REMORA_TRY(check_sizes(B, 1, D, N, G, "selective_scan_step"));
+  REMORA_TRY(want_shape(ev, {B, D}, "selective_scan_step delta"));
+  REMORA_TRY(want_shape(av, {D, N}, "selective_scan_step a"));
+  REMORA_TRY(want_shape(bv, {B, G, N}, "selective_scan_step b"));
+  REMORA_TRY(want_shape(cv, {B, G, N}, "selective_scan_step c"));
+  REMORA_TRY(want_shape(sv, {S, D, N}, "selective_scan_step state"));
+  REMORA_TRY(want_shape(ov, {S, D, N}, "selective_scan_step state_out"));
+  REMORA_TRY(want_shape(yv, {B, D}, "selective_scan_step y"));
+  if (has_d) REMORA_TRY(want_shape(dv, {D}, "selective_scan_step d"));
+  if (has_z) REMORA_TRY(want_shape(zv, {B, D}, "selective_scan_step z"));
+  if (has_i) REMORA_TRY(want_shape(iv, {D}, "selective_scan_step delta_bias"));
+  if (has_l) REMORA_TRY(want_shape(lv, {B}, "selective_scan_step slots"));
+  if (!has_l && B > S)
+    return fail(REMORA_ERR_SHAPE, "selective_scan_step: %lld rows and %lld states", (long long)B, (long long)S);
+  if (B > 65535) return fail(REMORA_ERR_LIMIT, "selective_scan_step: more than 65535 rows");
+  REMORA_TRY(want_apart({{&yv, "y", 4}, {&ov, "state_out", 4}},
+                        {{&sv, "state", 4}, {&uv, "u", 4}, {&ev, "delta", 4}, {&av, "a", 4}, {&bv, "b", 4},
+                         {&cv, "c", 4}, {has_d ? &dv : nullptr, "d", 4}, {has_z ? &zv : nullptr, "z", 4},
+                         {has_i ? &iv : nullptr, "delta_bias", 4}, {has_l ? &lv : nullptr, "slots", 4}}, {&sv}));
+  if (B == 0 || D == 0) return REMORA_OK;
+  TokenArgs a = {};
+  a.state = op3(sv), a.state_out = op3(ov), a.b = op3(bv), a.c = op3(cv);
+  a.u = reinterpret_cast<const float *>(uv.data(4)), a.u_b = uv.strides[0], a.u_d = uv.strides[1];
+  a.delta = reinterpret_cast<const float *>(ev.data(4)), a.delta_b = ev.strides[0], a.delta_d = ev.strides[1];
+  a.a = reinterpret_cast<const float *>(av.data(4)), a.a_d = av.strides[0], a.a_n = av.strides[1];
+  if (has_d) a.d = reinterpret_cast<const float *>(dv.data(4)), a.d_s = dv.strides[0];
+  if (has_z) a.z = reinterpret_cast<const float *>(zv.data(4)), a.z_b = zv.strides[0], a.z_d = zv.strides[1];
+  if (has_i) a.bias = reinterpret_cast<const float *>(iv.data(4)), a.bias_s = iv.strides[0];
+  if (has_l) a.slots = reinterpret_cast<const int *>(lv.data(4)), a.slots_s = lv.strides[0];
+  a.y = reinterpret_cast<float *>(yv.data(4)), a.y_b = yv.strides[0], a.y_d = yv.strides[1];
+  a.batch = B, a.rows = S, a.dim = D, a.per = D / G, a.states = (int)N, a.softplus = spec->softplus != 0;
+  a.vec = vec_states(sv) && vec_states(ov) && vec_states(av) && vec_states(bv) && vec_states(cv);
+  const int nl = lanes_for(a.states);
+  const dim3 grid((unsigned)((D + kScanThreads / nl - 1) / (kScanThreads / nl)), (unsigned)B);
+  DeviceGuard guard;
+  REMORA_TRY(guard.enter(ctx));
+  cudaStream_t s = (cudaStream_t)stream;
+  note_launch();
+  switch (nl) {
+  case 1: scan_step_kernel<1><<<grid, kScanThreads, 0, s>>>(a); break;
+  case 2: scan_step_kernel<2><<<grid, kScanThreads, 0, s>>>(a); break;
+  case 4: scan_step_kernel<4><<<grid, kScanThreads, 0, s>>>(a); break;
+  case 8: scan_step_kernel<8><<<grid, kScanThreads, 0, s>>>(a); break;
+  default: scan_step_kernel<16><<<grid, kScanThreads, 0, s>>>(a); break;
+  }
+  REMORA_CUDA_TRY(cudaGetLastError());
+  return REMORA_OK;
+}
+
+}  // extern "C"

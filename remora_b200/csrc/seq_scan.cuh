@@ -1,0 +1,152 @@
+// seq_scan.cuh — what the forward (seq_scan.cu) and backward
+// (seq_scan_bwd.cu) selective scans share: the operands as the kernels see
+// them, the mapping of channels and states to threads, and the staging of b
+// and c in shared memory.
+//
+// Mapping.  A channel's N states are spread over NL neighbouring lanes of a
+// warp, four states each (NP = 4 NL >= N, the states past N are zero), so a
+// warp works on 32 / NL channels.  Time runs serially in a thread.  The
+// per-channel inputs are loaded by the lane that a step falls to (lane q of a
+// channel takes steps q, q + NL, ...) and broadcast by shuffle; sums over the
+// states go back to that lane by a transposed (reduce-scatter) shuffle, so
+// every per-channel value is loaded, transformed and stored once.
+#pragma once
+
+#include "seq.cuh"
+
+namespace remora {
+namespace seq {
+
+constexpr int kScanThreads = 128;
+constexpr int kSaveEvery = 16;  // steps between the states that the forward keeps
+constexpr int kMaxStates = 64;
+
+struct Op3 {  // [B, time, D], or [B, D, N]
+  float *p;
+  int64_t s0, s1, s2;
+};
+
+struct Op4 {  // [B, time, G, N]
+  float *p;
+  int64_t s0, s1, s2, s3;
+};
+
+struct ScanArgs {
+  Op3 u, delta, z, y, h0, h_last;
+  Op4 b, c;
+  const float *a, *d, *bias;
+  int64_t a_d, a_n, d_s, bias_s;
+  const int *lengths;
+  int64_t lengths_s;
+  int64_t batch, length, dim;
+  int states, groups, softplus;
+  int64_t per;       // channels per group
+  int64_t blocks_d;  // channel blocks per group
+  int64_t chunks;    // pieces of the time axis, each by blocks of its own
+  int64_t chunk;     // their length, a multiple of 32
+  int vec_b, vec_c;  // b, c rows can be copied 16 bytes at a time
+  float *saved;      // [B, ceil(L / kSaveEvery), D, NP]
+  float *sum_h;      // [B, chunks, D, NP]: a piece's own end state, then its start state
+  float *sum_dt;     // [B, chunks, D]: a piece's sum of steps
+  // backward
+  Op3 dy, dh_last, du, ddelta, dz, dh0;
+  Op4 db, dc;
+  float *part_bc;  // [blocks_d, 2, B, L, G, N]
+  float *part_a;   // [B * chunks, D, N]
+  float *part_d;   // [B * chunks, 2, D]
+};
+
+// Lanes per channel for N states.
+inline int lanes_for(int states) {
+  int nl = 1;
+  while (nl * 4 < states) nl *= 2;
+  return nl;
+}
+
+int read_scan_in(const RemoraSelectiveScanSpec *spec, const RemoraSelectiveScanIn *in, ScanArgs *a, DescView views[10],
+                 const char *what);
+int combine_chunks(const ScanArgs &a, int nl, bool reverse, cudaStream_t stream);
+
+#ifdef __CUDACC__
+__device__ __forceinline__ int64_t scan_length(const ScanArgs &a, int64_t b) {
+  if (a.lengths == nullptr) return a.length;
+  const int64_t n = a.lengths[b * a.lengths_s];
+  return n < 0 ? 0 : n > a.length ? a.length : n;
+}
+
+// The place of a thread: block = ((b * chunks + chunk) * groups + g) * blocks_d + bd.
+template <int NL>
+struct Place {
+  int64_t bd, g, chunk, b, d;
+  int q;
+  bool live;
+  __device__ __forceinline__ explicit Place(const ScanArgs &a) {
+    int64_t i = blockIdx.x;
+    bd = i % a.blocks_d, i /= a.blocks_d;
+    g = i % a.groups, i /= a.groups;
+    chunk = i % a.chunks, b = i / a.chunks;
+    q = threadIdx.x % NL;
+    const int64_t in_group = bd * (kScanThreads / NL) + threadIdx.x / NL;
+    live = in_group < a.per;
+    d = g * a.per + (live ? in_group : 0);
+  }
+};
+
+__device__ __forceinline__ void copy_async4(float *dst, const float *src, bool on) {
+  const uint32_t s = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(s), "l"(src), "r"(on ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_async16(float *dst, const float *src, bool on) {
+  const uint32_t s = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(s), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
+// Starts the copy of rows [t0, t0 + STEPS) of one group of b or c to dst
+// [STEPS][4 NL]; rows from t_end on and states from N on become zero (and
+// their address, that of row t0, is not read).
+template <int NL, int STEPS>
+__device__ __forceinline__ void stage_rows(float *dst, const Op4 &src, int vec, int64_t b, int64_t g, int64_t t0,
+                                           int64_t t_end, int states) {
+  constexpr int NP = 4 * NL;
+  const float *base = src.p + b * src.s0 + t0 * src.s1 + g * src.s2;
+  const int rows = (int)(t_end - t0 < STEPS ? t_end - t0 : STEPS);
+  if (vec) {
+    for (int i = threadIdx.x; i < STEPS * NL; i += kScanThreads) {
+      const int r = i / NL, n = (i % NL) * 4;
+      const bool on = r < rows && n < states;
+      copy_async16(dst + r * NP + n, on ? base + r * src.s1 + n : base, on);
+    }
+  } else {
+    for (int i = threadIdx.x; i < STEPS * NP; i += kScanThreads) {
+      const int r = i / NP, n = i % NP;
+      const bool on = r < rows && n < states;
+      copy_async4(dst + i, on ? base + r * src.s1 + n * src.s3 : base, on);
+    }
+  }
+}
+
+// v[k] of lane q becomes the sum over the NL lanes of v[q], in v[0].
+template <int NL>
+__device__ __forceinline__ void transpose_sum(float (&v)[NL], int q) {
+#pragma unroll
+  for (int o = NL / 2; o >= 1; o >>= 1) {
+    const bool up = q & o;
+#pragma unroll
+    for (int k = 0; k < o; ++k) {
+      const float send = up ? v[k] : v[k + o];
+      const float keep = up ? v[k + o] : v[k];
+      v[k] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+    }
+  }
+}
+
+__device__ __forceinline__ void unpack(const float4 &v, float (&o)[4]) { o[0] = v.x, o[1] = v.y, o[2] = v.z, o[3] = v.w; }
+#endif
+
+}  // namespace seq
+}  // namespace remora

@@ -15,7 +15,7 @@ from typing import Any, Sequence
 from remora_b200 import _lib as L
 from remora_b200.abi import tensor_descriptor
 from remora_b200.codegen import fold_spec, scan_spec
-from remora_b200.errors import RemoraB200Error, RemoraShapeError
+from remora_b200.errors import RemoraB200Error, RemoraShapeError, RemoraUnsupportedError
 from remora_b200.program import Expr, compile_program
 from remora_b200.runtime import context
 
@@ -376,4 +376,321 @@ def append(a, b, out=None):
     ad, bd, od = tensor_descriptor(a), tensor_descriptor(b), tensor_descriptor(out)
     L.check(L.lib().remora_b200_append(_ctx(out).ptr, dtype_of(a), ctypes.addressof(ad), ctypes.addressof(bd),
                                        ctypes.addressof(od), a.dim(), _stream(out)), "append")
+    return out
+
+
+# ------------------------------------------------------- sequence operators
+# Root-mean-square norm, depthwise causal convolution and selective state
+# space scan (include/remora_b200_seq.h).  f32 CUDA tensors with any strides;
+# nothing synchronises, and scratch comes from torch on the current stream, so
+# every call can be captured into a CUDA graph.  With `lengths`, rows behind a
+# sequence's end are never read; results made here are zero there, and those
+# rows of a given `out` stay as they were.
+def _operands(what: str, **named):
+    """Checks that the tensors given are f32 (int32: lengths, slots) on one
+    CUDA device; returns their descriptors by name (None for None)."""
+    torch = _torch()
+    device, descs = None, {}
+    for name, t in named.items():
+        if t is None:
+            descs[name] = None
+            continue
+        if not t.is_cuda:
+            raise RemoraB200Error("remora_b200 ops take CUDA tensors (there is no CPU path)")
+        want = torch.int32 if name in ("lengths", "slots") else torch.float8_e4m3fn if name == "q" else torch.float32
+        if t.dtype != want:
+            raise RemoraUnsupportedError(f"{what}: {name} is {t.dtype}, not {want}")
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise RemoraB200Error(f"{what}: {name} is on {t.device}, the others on {device}")
+        descs[name] = tensor_descriptor(t)
+    return descs
+
+
+def _rank(what: str, t, *ranks: int) -> None:
+    if t is not None and t.dim() not in ranks:
+        raise RemoraShapeError(f"{what} has rank {t.dim()}, not {' or '.join(f'{r}' for r in ranks)}")
+
+
+def _at(d):
+    return ctypes.addressof(d) if d is not None else None
+
+
+def _scratch(fn, what: str, device, *sizes):
+    """A byte tensor of the size that a _scratch entry point asks for."""
+    n = ctypes.c_size_t()
+    L.check(fn(*sizes, ctypes.byref(n)), what)
+    return _torch().empty((n.value,), dtype=_torch().uint8, device=device) if n.value else None
+
+
+def _ptr(t):
+    return (t.data_ptr(), t.numel() * t.element_size()) if t is not None else (None, 0)
+
+
+def _fresh(lengths):
+    """torch.zeros where some rows will not be written, else torch.empty."""
+    return _torch().zeros if lengths is not None else _torch().empty
+
+
+def rms_norm_fwd(x, w, *, residual=None, eps: float = 1e-6, out=None, sum_out=None):
+    """s = x + residual; y = s / sqrt(mean(s^2) + eps) * w over the last axis
+    (rank 1 to 4).  Returns y, and (y, s) with a residual.  `out` or `sum_out`
+    may be x or the residual itself."""
+    torch = _torch()
+    _rank("rms_norm_fwd: x", x, 1, 2, 3, 4)
+    _rank("rms_norm_fwd: w", w, 1)
+    y = out if out is not None else torch.empty(x.shape, dtype=torch.float32, device=x.device)
+    s = sum_out
+    if s is None and residual is not None:
+        s = torch.empty(x.shape, dtype=torch.float32, device=x.device)
+    for name, t in (("residual", residual), ("out", y), ("sum_out", s)):
+        _rank(f"rms_norm_fwd: {name}", t, x.dim())
+    d = _operands("rms_norm_fwd", x=x, w=w, residual=residual, out=y, sum_out=s)
+    spec = L.RemoraNormSpec(eps, 0)
+    L.check(L.lib().remora_b200_rms_norm_fwd(_ctx(x).ptr, ctypes.addressof(spec), _at(d["x"]), _at(d["residual"]),
+                                             _at(d["w"]), _at(d["out"]), _at(d["sum_out"]), x.dim(), _stream(x)),
+            "rms_norm_fwd")
+    return y if residual is None else (y, s)
+
+
+def rms_norm_quant(x, w, *, residual=None, eps: float = 1e-6, group: int = 0, out=None, scales=None, sum_out=None):
+    """rms_norm_fwd's y as e4m3 values with f32 scales, one per row (group 0)
+    or per `group` (32, 64 or 128) columns: y ~ q * scale with scale =
+    max(max|y| / 448, 2^-126).  Returns (q, scales), and (q, scales, s) with a
+    residual."""
+    torch = _torch()
+    _rank("rms_norm_quant: x", x, 1, 2, 3, 4)
+    _rank("rms_norm_quant: w", w, 1)
+    q = out if out is not None else torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    if scales is None:
+        scales = torch.empty((*x.shape[:-1], x.shape[-1] // group if group > 0 else 1), dtype=torch.float32,
+                             device=x.device)
+    s = sum_out
+    if s is None and residual is not None:
+        s = torch.empty(x.shape, dtype=torch.float32, device=x.device)
+    for name, t in (("residual", residual), ("out", q), ("scales", scales), ("sum_out", s)):
+        _rank(f"rms_norm_quant: {name}", t, x.dim())
+    d = _operands("rms_norm_quant", x=x, w=w, residual=residual, q=q, scales=scales, sum_out=s)
+    spec = L.RemoraNormSpec(eps, group)
+    L.check(L.lib().remora_b200_rms_norm_quant(_ctx(x).ptr, ctypes.addressof(spec), _at(d["x"]), _at(d["residual"]),
+                                               _at(d["w"]), _at(d["q"]), _at(d["scales"]), _at(d["sum_out"]), x.dim(),
+                                               _stream(x)), "rms_norm_quant")
+    return (q, scales) if residual is None else (q, scales, s)
+
+
+def rms_norm_bwd(s, w, dy, *, dsum=None, eps: float = 1e-6, out=None):
+    """Gradients of rms_norm_fwd from its s (x itself without a residual):
+    (dx, dw), dx being the gradient of x and of the residual alike; dsum is
+    the gradient that reaches s from its other readers.  `out` (dx) may be s,
+    dy or dsum itself."""
+    torch = _torch()
+    _rank("rms_norm_bwd: s", s, 1, 2, 3, 4)
+    _rank("rms_norm_bwd: w", w, 1)
+    dx = out if out is not None else torch.empty(s.shape, dtype=torch.float32, device=s.device)
+    dw = torch.empty(w.shape, dtype=torch.float32, device=s.device)
+    for name, t in (("dy", dy), ("dsum", dsum), ("out", dx)):
+        _rank(f"rms_norm_bwd: {name}", t, s.dim())
+    d = _operands("rms_norm_bwd", s=s, w=w, dy=dy, dsum=dsum, out=dx, dw=dw)
+    lib, ctx = L.lib(), _ctx(s).ptr
+    dim = s.shape[-1]
+    scratch = _scratch(lib.remora_b200_rms_norm_bwd_scratch, "rms_norm_bwd", s.device, ctx,
+                       s.numel() // dim if dim else 0, dim)
+    spec = L.RemoraNormSpec(eps, 0)
+    L.check(lib.remora_b200_rms_norm_bwd(ctx, ctypes.addressof(spec), _at(d["s"]), _at(d["w"]), _at(d["dy"]),
+                                         _at(d["dsum"]), _at(d["out"]), _at(d["dw"]), s.dim(), *_ptr(scratch),
+                                         _stream(s)), "rms_norm_bwd")
+    return dx, dw
+
+
+def causal_conv_fwd(x, w, bias=None, *, state=None, lengths=None, silu: bool = False, out=None, state_out=None,
+                    return_state: bool = False):
+    """Depthwise causal convolution of x [B, L, D] with w [D, W] (2 to 8 taps)
+    along time, with an optional bias [D] and SiLU.  The W - 1 rows ahead of a
+    sequence are `state` [B, W - 1, D] (zeros without one).  With
+    return_state (or state_out, which may be `state` itself) returns
+    (y, the state that continues the sequence), else y."""
+    torch = _torch()
+    _rank("causal_conv_fwd: x", x, 3)
+    _rank("causal_conv_fwd: w", w, 2)
+    if out is None:
+        out = _fresh(lengths)(x.shape, dtype=torch.float32, device=x.device)
+    if state_out is None and return_state:
+        state_out = torch.empty((x.shape[0], max(w.shape[1] - 1, 0), x.shape[2]), dtype=torch.float32, device=x.device)
+    for name, t, r in (("bias", bias, 1), ("state", state, 3), ("lengths", lengths, 1), ("out", out, 3),
+                       ("state_out", state_out, 3)):
+        _rank(f"causal_conv_fwd: {name}", t, r)
+    d = _operands("causal_conv_fwd", x=x, w=w, bias=bias, state=state, lengths=lengths, out=out, state_out=state_out)
+    spec = L.RemoraCausalConvSpec(int(bool(silu)), 0)
+    L.check(L.lib().remora_b200_causal_conv_fwd(_ctx(x).ptr, ctypes.addressof(spec), _at(d["x"]), _at(d["w"]),
+                                                _at(d["bias"]), _at(d["state"]), _at(d["lengths"]), _at(d["out"]),
+                                                _at(d["state_out"]), _stream(x)), "causal_conv_fwd")
+    return out if state_out is None else (out, state_out)
+
+
+def causal_conv_bwd(x, w, dy, bias=None, *, state=None, lengths=None, silu: bool = False, dstate_out=None, out=None):
+    """Gradients of causal_conv_fwd: (dx, dw, dbias, dstate), dbias and dstate
+    None where bias or state is.  dstate_out is the gradient that reaches the
+    returned state; `out` receives dx."""
+    torch = _torch()
+    _rank("causal_conv_bwd: x", x, 3)
+    _rank("causal_conv_bwd: w", w, 2)
+    B, T, D = x.shape
+    dx = out if out is not None else _fresh(lengths)(x.shape, dtype=torch.float32, device=x.device)
+    dw = torch.empty(w.shape, dtype=torch.float32, device=x.device)
+    dbias = torch.empty(bias.shape, dtype=torch.float32, device=x.device) if bias is not None else None
+    dstate = torch.empty(state.shape, dtype=torch.float32, device=x.device) if state is not None else None
+    for name, t, r in (("bias", bias, 1), ("state", state, 3), ("lengths", lengths, 1), ("dy", dy, 3), ("out", dx, 3),
+                       ("dstate_out", dstate_out, 3)):
+        _rank(f"causal_conv_bwd: {name}", t, r)
+    d = _operands("causal_conv_bwd", x=x, w=w, bias=bias, state=state, lengths=lengths, dy=dy, dstate_out=dstate_out,
+                  out=dx, dw=dw, dbias=dbias, dstate=dstate)
+    lib, ctx = L.lib(), _ctx(x).ptr
+    scratch = _scratch(lib.remora_b200_causal_conv_bwd_scratch, "causal_conv_bwd", x.device, ctx, B, T, D, w.shape[1])
+    spec = L.RemoraCausalConvSpec(int(bool(silu)), 0)
+    L.check(lib.remora_b200_causal_conv_bwd(ctx, ctypes.addressof(spec), _at(d["x"]), _at(d["w"]), _at(d["bias"]),
+                                            _at(d["state"]), _at(d["lengths"]), _at(d["dy"]), _at(d["dstate_out"]),
+                                            _at(d["out"]), _at(d["dw"]), _at(d["dbias"]), _at(d["dstate"]),
+                                            *_ptr(scratch), _stream(x)), "causal_conv_bwd")
+    return dx, dw, dbias, dstate
+
+
+def causal_conv_step(x, state, w, bias=None, *, silu: bool = False, slots=None, out=None, state_out=None):
+    """One token per row of x [B, D]: y, with the window state [S, W - 1, D]
+    moved on in place (or into state_out).  Row i uses state row slots[i], or
+    row i without slots; a row whose slot is -1 or was named by an earlier row
+    is left out (its y is zero, or as it was in a given `out`)."""
+    torch = _torch()
+    _rank("causal_conv_step: x", x, 2)
+    if out is None:
+        out = _fresh(slots)(x.shape, dtype=torch.float32, device=x.device)
+    if state_out is None:
+        state_out = state
+    for name, t, r in (("state", state, 3), ("w", w, 2), ("bias", bias, 1), ("slots", slots, 1), ("out", out, 2),
+                       ("state_out", state_out, 3)):
+        _rank(f"causal_conv_step: {name}", t, r)
+    d = _operands("causal_conv_step", x=x, state=state, w=w, bias=bias, slots=slots, out=out, state_out=state_out)
+    spec = L.RemoraCausalConvSpec(int(bool(silu)), 0)
+    L.check(L.lib().remora_b200_causal_conv_step(_ctx(x).ptr, ctypes.addressof(spec), _at(d["x"]), _at(d["state"]),
+                                                 _at(d["w"]), _at(d["bias"]), _at(d["slots"]), _at(d["out"]),
+                                                 _at(d["state_out"]), _stream(x)), "causal_conv_step")
+    return out
+
+
+def _scan_inputs(what: str, u, delta, A, B, C, D, z, delta_bias, h0, lengths):
+    for name, t, *ranks in (("u", u, 3), ("delta", delta, 3), ("A", A, 2), ("B", B, 3, 4), ("C", C, 3, 4), ("D", D, 1),
+                            ("z", z, 3), ("delta_bias", delta_bias, 1), ("h0", h0, 3), ("lengths", lengths, 1)):
+        _rank(f"{what}: {name}", t, *ranks)
+    if B.dim() != C.dim():
+        raise RemoraShapeError(f"{what}: B has rank {B.dim()} and C rank {C.dim()}")
+    return (B, C) if B.dim() == 4 else (B.unsqueeze(2), C.unsqueeze(2))
+
+
+def selective_scan_fwd(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, softplus: bool = False, h0=None,
+                       lengths=None, out=None, h_last=None, return_state: bool = False, save: bool = False):
+    """Selective state space scan of u [B, L, D] (see
+    remora_b200_selective_scan_fwd): with s = softplus(delta + delta_bias),
+    h_t = exp(s A) h_{t-1} + s u B_t per channel and state, y = C_t . h_t + D u,
+    times silu(z) with a gate z.  A is [D, N] (N up to 64), B and C are
+    [B, L, N] or, shared by groups of channels, [B, L, G, N].  Returns y, then
+    the state behind each sequence's end with return_state (or h_last, which
+    may be h0 itself), then with save what selective_scan_bwd needs."""
+    torch = _torch()
+    Bg, Cg = _scan_inputs("selective_scan_fwd", u, delta, A, B, C, D, z, delta_bias, h0, lengths)
+    if out is None:
+        out = _fresh(lengths)(u.shape, dtype=torch.float32, device=u.device)
+    batch, length, dim = u.shape
+    states = A.shape[1]
+    if h_last is None and return_state:
+        h_last = torch.empty((batch, dim, states), dtype=torch.float32, device=u.device)
+    _rank("selective_scan_fwd: out", out, 3)
+    _rank("selective_scan_fwd: h_last", h_last, 3)
+    d = _operands("selective_scan_fwd", u=u, delta=delta, A=A, B=Bg, C=Cg, D=D, z=z, delta_bias=delta_bias, h0=h0,
+                  lengths=lengths, out=out, h_last=h_last)
+    args = L.RemoraSelectiveScanIn(*(_at(d[k]) for k in ("u", "delta", "A", "B", "C", "D", "z", "delta_bias", "h0",
+                                                          "lengths")))
+    lib, ctx = L.lib(), _ctx(u).ptr
+    scratch = _scratch(lib.remora_b200_selective_scan_fwd_scratch, "selective_scan_fwd", u.device, ctx, batch, length,
+                       dim, states, Bg.shape[2])
+    saved = None
+    if save:
+        n = ctypes.c_size_t()
+        L.check(lib.remora_b200_selective_scan_saved(batch, length, dim, states, ctypes.byref(n)), "selective_scan_fwd")
+        saved = torch.empty((n.value // 4,), dtype=torch.float32, device=u.device)
+    spec = L.RemoraSelectiveScanSpec(int(bool(softplus)), 0)
+    L.check(lib.remora_b200_selective_scan_fwd(ctx, ctypes.addressof(spec), ctypes.addressof(args), _at(d["out"]),
+                                               _at(d["h_last"]), *_ptr(saved), *_ptr(scratch), _stream(u)),
+            "selective_scan_fwd")
+    results = (out,) + ((h_last,) if h_last is not None else ()) + ((saved,) if save else ())
+    return results if len(results) > 1 else out
+
+
+def selective_scan_bwd(u, delta, A, B, C, dy, saved, D=None, *, z=None, delta_bias=None, softplus: bool = False,
+                       h0=None, lengths=None, dh_last=None):
+    """Gradients of selective_scan_fwd on the same inputs, from dy and what the
+    forward returned with save=True: (du, ddelta, dA, dB, dC, dD, dz,
+    ddelta_bias, dh0), None where the input is None.  dh_last is the gradient
+    that reaches the returned state."""
+    torch = _torch()
+    Bg, Cg = _scan_inputs("selective_scan_bwd", u, delta, A, B, C, D, z, delta_bias, h0, lengths)
+    _rank("selective_scan_bwd: dy", dy, 3)
+    _rank("selective_scan_bwd: dh_last", dh_last, 3)
+    _rank("selective_scan_bwd: saved", saved, 1)
+
+    def like(t, fresh):
+        return fresh(t.shape, dtype=torch.float32, device=u.device) if t is not None else None
+
+    rows = _fresh(lengths)
+    grads = dict(du=like(u, rows), ddelta=like(delta, rows), dA=like(A, torch.empty), dB=like(Bg, rows),
+                 dC=like(Cg, rows), dD=like(D, torch.empty), dz=like(z, rows), ddelta_bias=like(delta_bias, torch.empty),
+                 dh0=like(h0, torch.empty))
+    d = _operands("selective_scan_bwd", u=u, delta=delta, A=A, B=Bg, C=Cg, D=D, z=z, delta_bias=delta_bias, h0=h0,
+                  lengths=lengths, dy=dy, dh_last=dh_last, saved=saved, **grads)
+    args = L.RemoraSelectiveScanIn(*(_at(d[k]) for k in ("u", "delta", "A", "B", "C", "D", "z", "delta_bias", "h0",
+                                                          "lengths")))
+    outs = L.RemoraSelectiveScanGrads(*(_at(d[k]) for k in grads))
+    if not saved.is_contiguous():
+        raise RemoraUnsupportedError("selective_scan_bwd: saved is not the forward's contiguous tensor")
+    lib, ctx = L.lib(), _ctx(u).ptr
+    batch, length, dim = u.shape
+    scratch = _scratch(lib.remora_b200_selective_scan_bwd_scratch, "selective_scan_bwd", u.device, ctx, batch, length,
+                       dim, A.shape[1], Bg.shape[2])
+    spec = L.RemoraSelectiveScanSpec(int(bool(softplus)), 0)
+    L.check(lib.remora_b200_selective_scan_bwd(ctx, ctypes.addressof(spec), ctypes.addressof(args), _at(d["dy"]),
+                                               _at(d["dh_last"]), *_ptr(saved), ctypes.addressof(outs), *_ptr(scratch),
+                                               _stream(u)), "selective_scan_bwd")
+    if B.dim() == 3:
+        grads["dB"], grads["dC"] = grads["dB"].squeeze(2), grads["dC"].squeeze(2)
+    return tuple(grads.values())
+
+
+def selective_scan_step(state, u, delta, A, B, C, D=None, *, z=None, delta_bias=None, softplus: bool = False,
+                        slots=None, out=None, state_out=None):
+    """One token per row of u [B, D] (B and C: [B, N] or [B, G, N]): y, with
+    the state [S, D, N] moved on in place (or into state_out).  Row i uses
+    state row slots[i], or row i without slots; a row whose slot is -1 or was
+    named by an earlier row is left out, as in causal_conv_step."""
+    torch = _torch()
+    for name, t, *ranks in (("state", state, 3), ("u", u, 2), ("delta", delta, 2), ("A", A, 2), ("B", B, 2, 3),
+                            ("C", C, 2, 3), ("D", D, 1), ("z", z, 2), ("delta_bias", delta_bias, 1),
+                            ("slots", slots, 1)):
+        _rank(f"selective_scan_step: {name}", t, *ranks)
+    if B.dim() != C.dim():
+        raise RemoraShapeError(f"selective_scan_step: B has rank {B.dim()} and C rank {C.dim()}")
+    if B.dim() == 2:
+        B, C = B.unsqueeze(1), C.unsqueeze(1)
+    if out is None:
+        out = _fresh(slots)(u.shape, dtype=torch.float32, device=u.device)
+    if state_out is None:
+        state_out = state
+    _rank("selective_scan_step: out", out, 2)
+    _rank("selective_scan_step: state_out", state_out, 3)
+    d = _operands("selective_scan_step", state=state, u=u, delta=delta, A=A, B=B, C=C, D=D, z=z,
+                  delta_bias=delta_bias, slots=slots, out=out, state_out=state_out)
+    args = L.RemoraSelectiveStepIn(*(_at(d[k]) for k in ("state", "u", "delta", "A", "B", "C", "D", "z", "delta_bias",
+                                                          "slots")))
+    spec = L.RemoraSelectiveScanSpec(int(bool(softplus)), 0)
+    L.check(L.lib().remora_b200_selective_scan_step(_ctx(u).ptr, ctypes.addressof(spec), ctypes.addressof(args),
+                                                    _at(d["out"]), _at(d["state_out"]), _stream(u)),
+            "selective_scan_step")
     return out
