@@ -10,6 +10,7 @@ computes on the host.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Any, Sequence
 
 from remora_b200 import _lib as L
@@ -386,71 +387,102 @@ def append(a, b, out=None):
 # every call can be captured into a CUDA graph.  With `lengths`, rows behind a
 # sequence's end are never read; results made here are zero there, and those
 # rows of a given `out` stay as they were.
-def _operands(what: str, **named):
-    """Checks that the tensors given are f32 (int32: lengths, slots) on one
-    CUDA device; returns their descriptors by name (None for None)."""
-    torch = _torch()
-    device, descs = None, {}
-    for name, t in named.items():
+#
+# A single-token call costs what the host does, so the operands of a call are
+# checked and laid out in one loop, as one buffer of descriptors, and results
+# are made by the cheapest torch call for each.
+_CALL_BUFFER = ctypes.c_char * 3072  # descriptors of at most 24 operands, and their addresses
+
+
+def _describe(what: str, device: int, operands, special=(), table: int = 0):
+    """Checks (name, tensor or None, rank) operands, f32 on CUDA device
+    `device`, and `special` ones, (name, tensor or None, rank, dtype).  Returns
+    the buffer that holds their descriptors, to be kept until the call
+    returns, and the address of each (None for None), the special ones last.
+    With `table` also the address of a table of the first `table` addresses
+    (an argument struct of the C ABI), put first."""
+    f32 = _torch().float32
+    buf = _CALL_BUFFER()
+    start = ctypes.addressof(buf)
+    here = start + 8 * table
+    values, at = [0] * table, []
+    for name, t, rank, *want in (*operands, *special) if special else operands:
         if t is None:
-            descs[name] = None
+            at.append(None)
             continue
-        if not t.is_cuda:
-            raise RemoraB200Error("remora_b200 ops take CUDA tensors (there is no CPU path)")
-        want = torch.int32 if name in ("lengths", "slots") else torch.float8_e4m3fn if name == "q" else torch.float32
-        if t.dtype != want:
-            raise RemoraUnsupportedError(f"{what}: {name} is {t.dtype}, not {want}")
-        if device is None:
-            device = t.device
-        elif t.device != device:
-            raise RemoraB200Error(f"{what}: {name} is on {t.device}, the others on {device}")
-        descs[name] = tensor_descriptor(t)
-    return descs
+        if t.dtype is not (want[0] if want else f32):
+            raise RemoraUnsupportedError(f"{what}: {name} is {t.dtype}, not {want[0] if want else f32}")
+        if t.get_device() != device:
+            if not t.is_cuda:
+                raise RemoraB200Error("remora_b200 ops take CUDA tensors (there is no CPU path)")
+            raise RemoraB200Error(f"{what}: {name} is on {t.device}, the first operand on cuda:{device}")
+        shape = t.shape
+        if len(shape) != rank:
+            raise RemoraShapeError(f"{what}: {name} has rank {len(shape)}, not {rank}")
+        base, off = t.data_ptr(), t.storage_offset()
+        if base:
+            base -= off * t.element_size()
+        at.append(here)
+        here += 24 + 16 * rank
+        values += (base, base, off, *shape, *t.stride())
+    for k in range(table):
+        values[k] = at[k] or 0
+    struct.pack_into(f"{len(values)}q", buf, 0, *values)
+    return (buf, start, *at[table:]) if table else (buf, *at)
 
 
-def _rank(what: str, t, *ranks: int) -> None:
-    if t is not None and t.dim() not in ranks:
-        raise RemoraShapeError(f"{what} has rank {t.dim()}, not {' or '.join(f'{r}' for r in ranks)}")
+def _cuda_index(t) -> int:
+    index = t.get_device()
+    if index < 0:
+        raise RemoraB200Error("remora_b200 ops take CUDA tensors (there is no CPU path)")
+    return index
 
 
-def _at(d):
-    return ctypes.addressof(d) if d is not None else None
+def _raw_stream(device: int) -> int:
+    """The current stream's handle, without a Stream object where torch can."""
+    torch = _torch()
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
 
 
-def _scratch(fn, what: str, device, *sizes):
-    """A byte tensor of the size that a _scratch entry point asks for."""
+def _scratch(fn, what: str, t, *sizes):
+    """(byte tensor, address, bytes) of the scratch that a _scratch entry point asks for."""
     n = ctypes.c_size_t()
     L.check(fn(*sizes, ctypes.byref(n)), what)
-    return _torch().empty((n.value,), dtype=_torch().uint8, device=device) if n.value else None
+    if not n.value:
+        return None, None, 0
+    buf = _torch().empty((n.value,), dtype=_torch().uint8, device=t.device)
+    return buf, buf.data_ptr(), n.value
 
 
-def _ptr(t):
-    return (t.data_ptr(), t.numel() * t.element_size()) if t is not None else (None, 0)
+def _rows_like(t, lengths):
+    """A contiguous result shaped as the f32 tensor t: zeros where some rows
+    will not be written (lengths or slots given), else memory as it comes."""
+    torch = _torch()
+    make = torch.empty_like if lengths is None else torch.zeros_like
+    return make(t, memory_format=torch.contiguous_format)
 
 
-def _fresh(lengths):
-    """torch.zeros where some rows will not be written, else torch.empty."""
-    return _torch().zeros if lengths is not None else _torch().empty
+_CONV_SPECS = tuple(L.RemoraCausalConvSpec(k, 0) for k in (0, 1))
+_SCAN_SPECS = tuple(L.RemoraSelectiveScanSpec(k, 0) for k in (0, 1))
+
+
+def _spec(specs, flag) -> int:
+    return ctypes.addressof(specs[1 if flag else 0])
 
 
 def rms_norm_fwd(x, w, *, residual=None, eps: float = 1e-6, out=None, sum_out=None):
     """s = x + residual; y = s / sqrt(mean(s^2) + eps) * w over the last axis
     (rank 1 to 4).  Returns y, and (y, s) with a residual.  `out` or `sum_out`
     may be x or the residual itself."""
-    torch = _torch()
-    _rank("rms_norm_fwd: x", x, 1, 2, 3, 4)
-    _rank("rms_norm_fwd: w", w, 1)
-    y = out if out is not None else torch.empty(x.shape, dtype=torch.float32, device=x.device)
-    s = sum_out
-    if s is None and residual is not None:
-        s = torch.empty(x.shape, dtype=torch.float32, device=x.device)
-    for name, t in (("residual", residual), ("out", y), ("sum_out", s)):
-        _rank(f"rms_norm_fwd: {name}", t, x.dim())
-    d = _operands("rms_norm_fwd", x=x, w=w, residual=residual, out=y, sum_out=s)
+    device, rank = _cuda_index(x), x.dim()
+    y = out if out is not None else _rows_like(x, None)
+    s = sum_out if sum_out is not None or residual is None else _rows_like(x, None)
+    keep, xd, rd, wd, yd, sd = _describe("rms_norm_fwd", device, (
+        ("x", x, rank), ("residual", residual, rank), ("w", w, 1), ("out", y, rank), ("sum_out", s, rank)))
     spec = L.RemoraNormSpec(eps, 0)
-    L.check(L.lib().remora_b200_rms_norm_fwd(_ctx(x).ptr, ctypes.addressof(spec), _at(d["x"]), _at(d["residual"]),
-                                             _at(d["w"]), _at(d["out"]), _at(d["sum_out"]), x.dim(), _stream(x)),
-            "rms_norm_fwd")
+    L.check(L.lib().remora_b200_rms_norm_fwd(context(device).ptr, ctypes.addressof(spec), xd, rd, wd, yd, sd, rank,
+                                             _raw_stream(device)), "rms_norm_fwd")
     return y if residual is None else (y, s)
 
 
@@ -460,22 +492,19 @@ def rms_norm_quant(x, w, *, residual=None, eps: float = 1e-6, group: int = 0, ou
     max(max|y| / 448, 2^-126).  Returns (q, scales), and (q, scales, s) with a
     residual."""
     torch = _torch()
-    _rank("rms_norm_quant: x", x, 1, 2, 3, 4)
-    _rank("rms_norm_quant: w", w, 1)
-    q = out if out is not None else torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    device, rank = _cuda_index(x), x.dim()
+    q = out
+    if q is None:
+        q = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
     if scales is None:
-        scales = torch.empty((*x.shape[:-1], x.shape[-1] // group if group > 0 else 1), dtype=torch.float32,
-                             device=x.device)
-    s = sum_out
-    if s is None and residual is not None:
-        s = torch.empty(x.shape, dtype=torch.float32, device=x.device)
-    for name, t in (("residual", residual), ("out", q), ("scales", scales), ("sum_out", s)):
-        _rank(f"rms_norm_quant: {name}", t, x.dim())
-    d = _operands("rms_norm_quant", x=x, w=w, residual=residual, q=q, scales=scales, sum_out=s)
+        scales = x.new_empty((*x.shape[:-1], x.shape[-1] // group if group > 0 and rank else 1))
+    s = sum_out if sum_out is not None or residual is None else _rows_like(x, None)
+    keep, xd, rd, wd, cd, sd, qd = _describe("rms_norm_quant", device, (
+        ("x", x, rank), ("residual", residual, rank), ("w", w, 1), ("scales", scales, rank), ("sum_out", s, rank)),
+        (("out", q, rank, torch.float8_e4m3fn),))
     spec = L.RemoraNormSpec(eps, group)
-    L.check(L.lib().remora_b200_rms_norm_quant(_ctx(x).ptr, ctypes.addressof(spec), _at(d["x"]), _at(d["residual"]),
-                                               _at(d["w"]), _at(d["q"]), _at(d["scales"]), _at(d["sum_out"]), x.dim(),
-                                               _stream(x)), "rms_norm_quant")
+    L.check(L.lib().remora_b200_rms_norm_quant(context(device).ptr, ctypes.addressof(spec), xd, rd, wd, qd, cd, sd,
+                                               rank, _raw_stream(device)), "rms_norm_quant")
     return (q, scales) if residual is None else (q, scales, s)
 
 
@@ -484,22 +513,18 @@ def rms_norm_bwd(s, w, dy, *, dsum=None, eps: float = 1e-6, out=None):
     (dx, dw), dx being the gradient of x and of the residual alike; dsum is
     the gradient that reaches s from its other readers.  `out` (dx) may be s,
     dy or dsum itself."""
-    torch = _torch()
-    _rank("rms_norm_bwd: s", s, 1, 2, 3, 4)
-    _rank("rms_norm_bwd: w", w, 1)
-    dx = out if out is not None else torch.empty(s.shape, dtype=torch.float32, device=s.device)
-    dw = torch.empty(w.shape, dtype=torch.float32, device=s.device)
-    for name, t in (("dy", dy), ("dsum", dsum), ("out", dx)):
-        _rank(f"rms_norm_bwd: {name}", t, s.dim())
-    d = _operands("rms_norm_bwd", s=s, w=w, dy=dy, dsum=dsum, out=dx, dw=dw)
-    lib, ctx = L.lib(), _ctx(s).ptr
-    dim = s.shape[-1]
-    scratch = _scratch(lib.remora_b200_rms_norm_bwd_scratch, "rms_norm_bwd", s.device, ctx,
-                       s.numel() // dim if dim else 0, dim)
+    device, rank = _cuda_index(s), s.dim()
+    dx = out if out is not None else _rows_like(s, None)
+    dw = _rows_like(w, None)
+    keep, sd, wd, gd, ed, xd, dwd = _describe("rms_norm_bwd", device, (
+        ("s", s, rank), ("w", w, 1), ("dy", dy, rank), ("dsum", dsum, rank), ("out", dx, rank), ("dw", dw, 1)))
+    lib, ctx = L.lib(), context(device).ptr
+    dim = s.shape[-1] if rank else 0
+    scratch, at, size = _scratch(lib.remora_b200_rms_norm_bwd_scratch, "rms_norm_bwd", s, ctx,
+                                 s.numel() // dim if dim else 0, dim)
     spec = L.RemoraNormSpec(eps, 0)
-    L.check(lib.remora_b200_rms_norm_bwd(ctx, ctypes.addressof(spec), _at(d["s"]), _at(d["w"]), _at(d["dy"]),
-                                         _at(d["dsum"]), _at(d["out"]), _at(d["dw"]), s.dim(), *_ptr(scratch),
-                                         _stream(s)), "rms_norm_bwd")
+    L.check(lib.remora_b200_rms_norm_bwd(ctx, ctypes.addressof(spec), sd, wd, gd, ed, xd, dwd, rank, at, size,
+                                         _raw_stream(device)), "rms_norm_bwd")
     return dx, dw
 
 
@@ -511,20 +536,16 @@ def causal_conv_fwd(x, w, bias=None, *, state=None, lengths=None, silu: bool = F
     return_state (or state_out, which may be `state` itself) returns
     (y, the state that continues the sequence), else y."""
     torch = _torch()
-    _rank("causal_conv_fwd: x", x, 3)
-    _rank("causal_conv_fwd: w", w, 2)
+    device = _cuda_index(x)
     if out is None:
-        out = _fresh(lengths)(x.shape, dtype=torch.float32, device=x.device)
-    if state_out is None and return_state:
-        state_out = torch.empty((x.shape[0], max(w.shape[1] - 1, 0), x.shape[2]), dtype=torch.float32, device=x.device)
-    for name, t, r in (("bias", bias, 1), ("state", state, 3), ("lengths", lengths, 1), ("out", out, 3),
-                       ("state_out", state_out, 3)):
-        _rank(f"causal_conv_fwd: {name}", t, r)
-    d = _operands("causal_conv_fwd", x=x, w=w, bias=bias, state=state, lengths=lengths, out=out, state_out=state_out)
-    spec = L.RemoraCausalConvSpec(int(bool(silu)), 0)
-    L.check(L.lib().remora_b200_causal_conv_fwd(_ctx(x).ptr, ctypes.addressof(spec), _at(d["x"]), _at(d["w"]),
-                                                _at(d["bias"]), _at(d["state"]), _at(d["lengths"]), _at(d["out"]),
-                                                _at(d["state_out"]), _stream(x)), "causal_conv_fwd")
+        out = _rows_like(x, lengths)
+    if state_out is None and return_state and x.dim() == 3 and w.dim() == 2:
+        state_out = x.new_empty((x.shape[0], max(w.shape[1] - 1, 0), x.shape[2]))
+    keep, xd, wd, bd, sd, yd, od, ld = _describe("causal_conv_fwd", device, (
+        ("x", x, 3), ("w", w, 2), ("bias", bias, 1), ("state", state, 3), ("out", out, 3),
+        ("state_out", state_out, 3)), (("lengths", lengths, 1, torch.int32),))
+    L.check(L.lib().remora_b200_causal_conv_fwd(context(device).ptr, _spec(_CONV_SPECS, silu), xd, wd, bd, sd, ld, yd,
+                                                od, _raw_stream(device)), "causal_conv_fwd")
     return out if state_out is None else (out, state_out)
 
 
@@ -532,26 +553,20 @@ def causal_conv_bwd(x, w, dy, bias=None, *, state=None, lengths=None, silu: bool
     """Gradients of causal_conv_fwd: (dx, dw, dbias, dstate), dbias and dstate
     None where bias or state is.  dstate_out is the gradient that reaches the
     returned state; `out` receives dx."""
-    torch = _torch()
-    _rank("causal_conv_bwd: x", x, 3)
-    _rank("causal_conv_bwd: w", w, 2)
-    B, T, D = x.shape
-    dx = out if out is not None else _fresh(lengths)(x.shape, dtype=torch.float32, device=x.device)
-    dw = torch.empty(w.shape, dtype=torch.float32, device=x.device)
-    dbias = torch.empty(bias.shape, dtype=torch.float32, device=x.device) if bias is not None else None
-    dstate = torch.empty(state.shape, dtype=torch.float32, device=x.device) if state is not None else None
-    for name, t, r in (("bias", bias, 1), ("state", state, 3), ("lengths", lengths, 1), ("dy", dy, 3), ("out", dx, 3),
-                       ("dstate_out", dstate_out, 3)):
-        _rank(f"causal_conv_bwd: {name}", t, r)
-    d = _operands("causal_conv_bwd", x=x, w=w, bias=bias, state=state, lengths=lengths, dy=dy, dstate_out=dstate_out,
-                  out=dx, dw=dw, dbias=dbias, dstate=dstate)
-    lib, ctx = L.lib(), _ctx(x).ptr
-    scratch = _scratch(lib.remora_b200_causal_conv_bwd_scratch, "causal_conv_bwd", x.device, ctx, B, T, D, w.shape[1])
-    spec = L.RemoraCausalConvSpec(int(bool(silu)), 0)
-    L.check(lib.remora_b200_causal_conv_bwd(ctx, ctypes.addressof(spec), _at(d["x"]), _at(d["w"]), _at(d["bias"]),
-                                            _at(d["state"]), _at(d["lengths"]), _at(d["dy"]), _at(d["dstate_out"]),
-                                            _at(d["out"]), _at(d["dw"]), _at(d["dbias"]), _at(d["dstate"]),
-                                            *_ptr(scratch), _stream(x)), "causal_conv_bwd")
+    device = _cuda_index(x)
+    dx = out if out is not None else _rows_like(x, lengths)
+    dw = _rows_like(w, None)
+    dbias = _rows_like(bias, None) if bias is not None else None
+    dstate = _rows_like(state, None) if state is not None else None
+    keep, xd, wd, bd, sd, gd, ed, dxd, dwd, dbd, dsd, ld = _describe("causal_conv_bwd", device, (
+        ("x", x, 3), ("w", w, 2), ("bias", bias, 1), ("state", state, 3), ("dy", dy, 3), ("dstate_out", dstate_out, 3),
+        ("out", dx, 3), ("dw", dw, 2), ("dbias", dbias, 1), ("dstate", dstate, 3)),
+        (("lengths", lengths, 1, _torch().int32),))
+    lib, ctx = L.lib(), context(device).ptr
+    scratch, at, size = _scratch(lib.remora_b200_causal_conv_bwd_scratch, "causal_conv_bwd", x, ctx, *x.shape,
+                                 w.shape[1])
+    L.check(lib.remora_b200_causal_conv_bwd(ctx, _spec(_CONV_SPECS, silu), xd, wd, bd, sd, ld, gd, ed, dxd, dwd, dbd, dsd,
+                                            at, size, _raw_stream(device)), "causal_conv_bwd")
     return dx, dw, dbias, dstate
 
 
@@ -560,30 +575,24 @@ def causal_conv_step(x, state, w, bias=None, *, silu: bool = False, slots=None, 
     moved on in place (or into state_out).  Row i uses state row slots[i], or
     row i without slots; a row whose slot is -1 or was named by an earlier row
     is left out (its y is zero, or as it was in a given `out`)."""
-    torch = _torch()
-    _rank("causal_conv_step: x", x, 2)
+    device = _cuda_index(x)
     if out is None:
-        out = _fresh(slots)(x.shape, dtype=torch.float32, device=x.device)
+        out = _rows_like(x, slots)
     if state_out is None:
         state_out = state
-    for name, t, r in (("state", state, 3), ("w", w, 2), ("bias", bias, 1), ("slots", slots, 1), ("out", out, 2),
-                       ("state_out", state_out, 3)):
-        _rank(f"causal_conv_step: {name}", t, r)
-    d = _operands("causal_conv_step", x=x, state=state, w=w, bias=bias, slots=slots, out=out, state_out=state_out)
-    spec = L.RemoraCausalConvSpec(int(bool(silu)), 0)
-    L.check(L.lib().remora_b200_causal_conv_step(_ctx(x).ptr, ctypes.addressof(spec), _at(d["x"]), _at(d["state"]),
-                                                 _at(d["w"]), _at(d["bias"]), _at(d["slots"]), _at(d["out"]),
-                                                 _at(d["state_out"]), _stream(x)), "causal_conv_step")
+    keep, xd, sd, wd, bd, yd, od, ld = _describe("causal_conv_step", device, (
+        ("x", x, 2), ("state", state, 3), ("w", w, 2), ("bias", bias, 1), ("out", out, 2), ("state_out", state_out, 3)),
+        (("slots", slots, 1, _torch().int32),))
+    L.check(L.lib().remora_b200_causal_conv_step(context(device).ptr, _spec(_CONV_SPECS, silu), xd, sd, wd, bd, ld, yd,
+                                                 od, _raw_stream(device)), "causal_conv_step")
     return out
 
 
-def _scan_inputs(what: str, u, delta, A, B, C, D, z, delta_bias, h0, lengths):
-    for name, t, *ranks in (("u", u, 3), ("delta", delta, 3), ("A", A, 2), ("B", B, 3, 4), ("C", C, 3, 4), ("D", D, 1),
-                            ("z", z, 3), ("delta_bias", delta_bias, 1), ("h0", h0, 3), ("lengths", lengths, 1)):
-        _rank(f"{what}: {name}", t, *ranks)
+def _groups(what: str, B, C, rank: int):
+    """B and C with their group axis: rank - 1 means one group."""
     if B.dim() != C.dim():
         raise RemoraShapeError(f"{what}: B has rank {B.dim()} and C rank {C.dim()}")
-    return (B, C) if B.dim() == 4 else (B.unsqueeze(2), C.unsqueeze(2))
+    return (B, C) if B.dim() == rank else (B.unsqueeze(-2), C.unsqueeze(-2))
 
 
 def selective_scan_fwd(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, softplus: bool = False, h0=None,
@@ -596,31 +605,28 @@ def selective_scan_fwd(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, so
     the state behind each sequence's end with return_state (or h_last, which
     may be h0 itself), then with save what selective_scan_bwd needs."""
     torch = _torch()
-    Bg, Cg = _scan_inputs("selective_scan_fwd", u, delta, A, B, C, D, z, delta_bias, h0, lengths)
+    device = _cuda_index(u)
+    Bg, Cg = _groups("selective_scan_fwd", B, C, 4)
     if out is None:
-        out = _fresh(lengths)(u.shape, dtype=torch.float32, device=u.device)
-    batch, length, dim = u.shape
-    states = A.shape[1]
-    if h_last is None and return_state:
-        h_last = torch.empty((batch, dim, states), dtype=torch.float32, device=u.device)
-    _rank("selective_scan_fwd: out", out, 3)
-    _rank("selective_scan_fwd: h_last", h_last, 3)
-    d = _operands("selective_scan_fwd", u=u, delta=delta, A=A, B=Bg, C=Cg, D=D, z=z, delta_bias=delta_bias, h0=h0,
-                  lengths=lengths, out=out, h_last=h_last)
-    args = L.RemoraSelectiveScanIn(*(_at(d[k]) for k in ("u", "delta", "A", "B", "C", "D", "z", "delta_bias", "h0",
-                                                          "lengths")))
-    lib, ctx = L.lib(), _ctx(u).ptr
-    scratch = _scratch(lib.remora_b200_selective_scan_fwd_scratch, "selective_scan_fwd", u.device, ctx, batch, length,
-                       dim, states, Bg.shape[2])
-    saved = None
+        out = _rows_like(u, lengths)
+    if h_last is None and return_state and u.dim() == 3 and A.dim() == 2:
+        h_last = u.new_empty((u.shape[0], u.shape[2], A.shape[1]))
+    keep, args, yd, hd = _describe("selective_scan_fwd", device, (
+        ("u", u, 3), ("delta", delta, 3), ("A", A, 2), ("B", Bg, 4), ("C", Cg, 4), ("D", D, 1), ("z", z, 3),
+        ("delta_bias", delta_bias, 1), ("h0", h0, 3), ("lengths", lengths, 1, torch.int32), ("out", out, 3),
+        ("h_last", h_last, 3)), table=10)
+    lib, ctx = L.lib(), context(device).ptr
+    sizes = (*u.shape, A.shape[1])
+    scratch, at, size = _scratch(lib.remora_b200_selective_scan_fwd_scratch, "selective_scan_fwd", u, ctx, *sizes,
+                                 Bg.shape[2])
+    saved, kept, kept_size = None, None, 0
     if save:
         n = ctypes.c_size_t()
-        L.check(lib.remora_b200_selective_scan_saved(batch, length, dim, states, ctypes.byref(n)), "selective_scan_fwd")
+        L.check(lib.remora_b200_selective_scan_saved(*sizes, ctypes.byref(n)), "selective_scan_fwd")
         saved = torch.empty((n.value // 4,), dtype=torch.float32, device=u.device)
-    spec = L.RemoraSelectiveScanSpec(int(bool(softplus)), 0)
-    L.check(lib.remora_b200_selective_scan_fwd(ctx, ctypes.addressof(spec), ctypes.addressof(args), _at(d["out"]),
-                                               _at(d["h_last"]), *_ptr(saved), *_ptr(scratch), _stream(u)),
-            "selective_scan_fwd")
+        kept, kept_size = (saved.data_ptr(), n.value) if n.value else (None, 0)
+    L.check(lib.remora_b200_selective_scan_fwd(ctx, _spec(_SCAN_SPECS, softplus), args, yd, hd, kept, kept_size, at,
+                                               size, _raw_stream(device)), "selective_scan_fwd")
     results = (out,) + ((h_last,) if h_last is not None else ()) + ((saved,) if save else ())
     return results if len(results) > 1 else out
 
@@ -631,37 +637,34 @@ def selective_scan_bwd(u, delta, A, B, C, dy, saved, D=None, *, z=None, delta_bi
     forward returned with save=True: (du, ddelta, dA, dB, dC, dD, dz,
     ddelta_bias, dh0), None where the input is None.  dh_last is the gradient
     that reaches the returned state."""
-    torch = _torch()
-    Bg, Cg = _scan_inputs("selective_scan_bwd", u, delta, A, B, C, D, z, delta_bias, h0, lengths)
-    _rank("selective_scan_bwd: dy", dy, 3)
-    _rank("selective_scan_bwd: dh_last", dh_last, 3)
-    _rank("selective_scan_bwd: saved", saved, 1)
+    device = _cuda_index(u)
+    Bg, Cg = _groups("selective_scan_bwd", B, C, 4)
 
-    def like(t, fresh):
-        return fresh(t.shape, dtype=torch.float32, device=u.device) if t is not None else None
+    def like(t):
+        return _rows_like(t, None) if t is not None else None
 
-    rows = _fresh(lengths)
-    grads = dict(du=like(u, rows), ddelta=like(delta, rows), dA=like(A, torch.empty), dB=like(Bg, rows),
-                 dC=like(Cg, rows), dD=like(D, torch.empty), dz=like(z, rows), ddelta_bias=like(delta_bias, torch.empty),
-                 dh0=like(h0, torch.empty))
-    d = _operands("selective_scan_bwd", u=u, delta=delta, A=A, B=Bg, C=Cg, D=D, z=z, delta_bias=delta_bias, h0=h0,
-                  lengths=lengths, dy=dy, dh_last=dh_last, saved=saved, **grads)
-    args = L.RemoraSelectiveScanIn(*(_at(d[k]) for k in ("u", "delta", "A", "B", "C", "D", "z", "delta_bias", "h0",
-                                                          "lengths")))
-    outs = L.RemoraSelectiveScanGrads(*(_at(d[k]) for k in grads))
-    if not saved.is_contiguous():
-        raise RemoraUnsupportedError("selective_scan_bwd: saved is not the forward's contiguous tensor")
-    lib, ctx = L.lib(), _ctx(u).ptr
-    batch, length, dim = u.shape
-    scratch = _scratch(lib.remora_b200_selective_scan_bwd_scratch, "selective_scan_bwd", u.device, ctx, batch, length,
-                       dim, A.shape[1], Bg.shape[2])
-    spec = L.RemoraSelectiveScanSpec(int(bool(softplus)), 0)
-    L.check(lib.remora_b200_selective_scan_bwd(ctx, ctypes.addressof(spec), ctypes.addressof(args), _at(d["dy"]),
-                                               _at(d["dh_last"]), *_ptr(saved), ctypes.addressof(outs), *_ptr(scratch),
-                                               _stream(u)), "selective_scan_bwd")
+    grads = (_rows_like(u, lengths), _rows_like(delta, lengths), like(A), _rows_like(Bg, lengths),
+             _rows_like(Cg, lengths), like(D), _rows_like(z, lengths) if z is not None else None, like(delta_bias),
+             like(h0))
+    keep, args, gd, hd, sd, *outs = _describe("selective_scan_bwd", device, (
+        ("u", u, 3), ("delta", delta, 3), ("A", A, 2), ("B", Bg, 4), ("C", Cg, 4), ("D", D, 1), ("z", z, 3),
+        ("delta_bias", delta_bias, 1), ("h0", h0, 3), ("lengths", lengths, 1, _torch().int32), ("dy", dy, 3),
+        ("dh_last", dh_last, 3),
+        ("saved", saved, 1), ("du", grads[0], 3), ("ddelta", grads[1], 3), ("dA", grads[2], 2), ("dB", grads[3], 4),
+        ("dC", grads[4], 4), ("dD", grads[5], 1), ("dz", grads[6], 3), ("ddelta_bias", grads[7], 1),
+        ("dh0", grads[8], 3)), table=10)
+    if saved is None or not saved.is_contiguous():
+        raise RemoraUnsupportedError("selective_scan_bwd: saved is not what selective_scan_fwd returned")
+    to = L.RemoraSelectiveScanGrads(*outs)
+    lib, ctx = L.lib(), context(device).ptr
+    scratch, at, size = _scratch(lib.remora_b200_selective_scan_bwd_scratch, "selective_scan_bwd", u, ctx, *u.shape,
+                                 A.shape[1], Bg.shape[2])
+    L.check(lib.remora_b200_selective_scan_bwd(ctx, _spec(_SCAN_SPECS, softplus), args, gd, hd, saved.data_ptr(),
+                                               4 * saved.numel(), ctypes.addressof(to), at, size, _raw_stream(device)),
+            "selective_scan_bwd")
     if B.dim() == 3:
-        grads["dB"], grads["dC"] = grads["dB"].squeeze(2), grads["dC"].squeeze(2)
-    return tuple(grads.values())
+        return (*grads[:3], grads[3].squeeze(2), grads[4].squeeze(2), *grads[5:])
+    return grads
 
 
 def selective_scan_step(state, u, delta, A, B, C, D=None, *, z=None, delta_bias=None, softplus: bool = False,
@@ -670,27 +673,16 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, *, z=None, delta_bias=
     the state [S, D, N] moved on in place (or into state_out).  Row i uses
     state row slots[i], or row i without slots; a row whose slot is -1 or was
     named by an earlier row is left out, as in causal_conv_step."""
-    torch = _torch()
-    for name, t, *ranks in (("state", state, 3), ("u", u, 2), ("delta", delta, 2), ("A", A, 2), ("B", B, 2, 3),
-                            ("C", C, 2, 3), ("D", D, 1), ("z", z, 2), ("delta_bias", delta_bias, 1),
-                            ("slots", slots, 1)):
-        _rank(f"selective_scan_step: {name}", t, *ranks)
-    if B.dim() != C.dim():
-        raise RemoraShapeError(f"selective_scan_step: B has rank {B.dim()} and C rank {C.dim()}")
-    if B.dim() == 2:
-        B, C = B.unsqueeze(1), C.unsqueeze(1)
+    device = _cuda_index(u)
+    Bg, Cg = _groups("selective_scan_step", B, C, 3)
     if out is None:
-        out = _fresh(slots)(u.shape, dtype=torch.float32, device=u.device)
+        out = _rows_like(u, slots)
     if state_out is None:
         state_out = state
-    _rank("selective_scan_step: out", out, 2)
-    _rank("selective_scan_step: state_out", state_out, 3)
-    d = _operands("selective_scan_step", state=state, u=u, delta=delta, A=A, B=B, C=C, D=D, z=z,
-                  delta_bias=delta_bias, slots=slots, out=out, state_out=state_out)
-    args = L.RemoraSelectiveStepIn(*(_at(d[k]) for k in ("state", "u", "delta", "A", "B", "C", "D", "z", "delta_bias",
-                                                          "slots")))
-    spec = L.RemoraSelectiveScanSpec(int(bool(softplus)), 0)
-    L.check(L.lib().remora_b200_selective_scan_step(_ctx(u).ptr, ctypes.addressof(spec), ctypes.addressof(args),
-                                                    _at(d["out"]), _at(d["state_out"]), _stream(u)),
-            "selective_scan_step")
+    keep, args, yd, od = _describe("selective_scan_step", device, (
+        ("state", state, 3), ("u", u, 2), ("delta", delta, 2), ("A", A, 2), ("B", Bg, 3), ("C", Cg, 3), ("D", D, 1),
+        ("z", z, 2), ("delta_bias", delta_bias, 1), ("slots", slots, 1, _torch().int32), ("out", out, 2),
+        ("state_out", state_out, 3)), table=10)
+    L.check(L.lib().remora_b200_selective_scan_step(context(device).ptr, _spec(_SCAN_SPECS, softplus), args, yd, od,
+                                                    _raw_stream(device)), "selective_scan_step")
     return out

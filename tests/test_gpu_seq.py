@@ -52,8 +52,8 @@ def norm_tol(D):
     return (D / 32 + 64) / 2 * E + 8 * E
 
 
-SHAPES = [(1, 1), (5, 3), (3, 31), (7, 128), (700, 33), (2, 1000), (600, 1000), (9, 2048), (1, 8192), (3, 8193), (2, 16384),
-          (2, 16388), (2, 20001), (1300, 64)]
+SHAPES = [(1, 1), (5, 3), (3, 31), (7, 128), (700, 33), (2, 1000), (600, 1000), (9, 2048), (1, 8192), (3, 8193),
+          (2, 16384), (2, 16388), (2, 20001), (1300, 64)]
 
 
 @pytest.mark.parametrize("rows,D", SHAPES)
@@ -116,8 +116,8 @@ def test_norm_in_place_and_strided(cuda, D):
     np.testing.assert_array_equal(to_host(flat), to_host(ops.rms_norm_fwd(r, w))[0, 0])
 
 
-@pytest.mark.parametrize("rows,D,group", [(3, 64, 0), (1, 2048, 0), (800, 128, 32), (5, 4096, 128), (4, 192, 64), (3, 77, 0),
-                                          (2, 20000, 0), (2, 20000, 32), (700, 1001, 0)])
+@pytest.mark.parametrize("rows,D,group", [(3, 64, 0), (1, 2048, 0), (800, 128, 32), (5, 4096, 128), (4, 192, 64),
+                                          (3, 77, 0), (2, 20000, 0), (2, 20000, 32), (700, 1001, 0)])
 @pytest.mark.parametrize("residual", [False, True])
 def test_norm_quant(cuda, rows, D, group, residual):
     rng = np.random.default_rng(rows + D + group)
@@ -224,7 +224,8 @@ def test_conv_forward_backward(cuda, B, T, D, W, silu, full):
     ry, rlast = ref.causal_conv(x0, w, b, state, lengths, silu)
     within(y, ry, conv_tol(x0, w, b, state, lengths, silu), "y")
     np.testing.assert_array_equal(to_host(last), rlast.astype(np.float32))
-    got = ops.causal_conv_bwd(d(x), d(w), d(dy), d(b), state=d(state), lengths=d(lengths), silu=silu, dstate_out=d(dlast))
+    got = ops.causal_conv_bwd(d(x), d(w), d(dy), d(b), state=d(state), lengths=d(lengths), silu=silu,
+                              dstate_out=d(dlast))
     want = ref.causal_conv_bwd(x0, w, b, state, lengths, silu, dy0, dlast)
     a = np.abs
     an = lambda v: None if v is None else a(v)  # noqa: E731
@@ -350,8 +351,8 @@ def scan_own(v, cuda):
 
 
 NAMES = ("du", "ddelta", "dA", "dB", "dC", "dD", "dz", "ddelta_bias", "dh0")
-SCANS = [(1, 1, 1, 1, 1), (2, 3, 5, 4, 1), (1, 17, 40, 16, 1), (2, 70, 34, 16, 2), (1, 200, 8, 16, 1), (2, 33, 12, 13, 3),
-         (1, 37, 6, 64, 1), (1, 50, 9, 33, 1), (2, 40, 64, 2, 1), (1, 45, 130, 8, 1), (1, 300, 3, 7, 1)]
+SCANS = [(1, 1, 1, 1, 1), (2, 3, 5, 4, 1), (1, 17, 40, 16, 1), (2, 70, 34, 16, 2), (1, 200, 8, 16, 1),
+         (2, 33, 12, 13, 3), (1, 37, 6, 64, 1), (1, 50, 9, 33, 1), (2, 40, 64, 2, 1), (1, 45, 130, 8, 1), (1, 300, 3, 7, 1)]
 
 
 @pytest.mark.parametrize("B,T,D,N,G", SCANS)
@@ -384,7 +385,8 @@ def test_scan_forward_backward(cuda, B, T, D, N, G, full):
     tol = (6 * T + 64) * E
     within(y, ry, my * tol, "y")
     within(last, rlast, mlast * tol, "h_last")
-    got = ops.selective_scan_bwd(*pos, dev(dy, cuda), saved, Dv, softplus=softplus, lengths=ln, dh_last=dev(dlast, cuda), **kw)
+    got = ops.selective_scan_bwd(*pos, dev(dy, cuda), saved, Dv, softplus=softplus, lengths=ln,
+                                 dh_last=dev(dlast, cuda), **kw)
     want = ref.selective_scan_bwd(*args, dyc, dlast)
     mag = ref.selective_scan_bwd(*args, dyc, dlast, absolute=True)
     for name, g in zip(NAMES, got):
@@ -702,6 +704,11 @@ def test_python_refusals(cuda):
     with pytest.raises(RemoraB200Error):
         ops.rms_norm_fwd(x, w, sum_out=x)
     y = torch.zeros((1, 3, 4), device=cuda)
+    with pytest.raises(RemoraShapeError):
+        ops.causal_conv_fwd(y[0], torch.zeros((4, 3), device=cuda))
+    with pytest.raises(RemoraShapeError):
+        ops.selective_scan_fwd(y, y, torch.zeros((4, 5), device=cuda), torch.zeros((1, 3, 5), device=cuda),
+                               torch.zeros((1, 3, 1, 5), device=cuda))
     with pytest.raises(RemoraB200Error):
         ops.causal_conv_fwd(y, torch.zeros((4, 3), device=cuda), out=y)
     with pytest.raises(RemoraUnsupportedError):

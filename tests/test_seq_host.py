@@ -179,17 +179,15 @@ def test_ops_take_cuda_tensors():
     import torch
 
     from remora_b200 import ops
-    from remora_b200.errors import RemoraB200Error, RemoraShapeError
+    from remora_b200.errors import RemoraB200Error
 
     t = torch.zeros
-    with pytest.raises(RemoraB200Error):
+    with pytest.raises(RemoraB200Error, match="CUDA"):
         ops.rms_norm_fwd(t(2, 4), t(4))
-    with pytest.raises(RemoraB200Error):
+    with pytest.raises(RemoraB200Error, match="CUDA"):
         ops.causal_conv_fwd(t(2, 3, 4), t(4, 3))
-    with pytest.raises(RemoraShapeError):
-        ops.causal_conv_fwd(t(3, 4), t(4, 3))
-    with pytest.raises(RemoraShapeError):
-        ops.selective_scan_fwd(t(2, 3, 4), t(2, 3, 4), t(4, 5), t(2, 3, 5), t(2, 3, 1, 5))
+    with pytest.raises(RemoraB200Error, match="CUDA"):
+        ops.selective_scan_fwd(t(2, 3, 4), t(2, 3, 4), t(4, 5), t(2, 3, 5), t(2, 3, 5))
 
 
 # ------------------------------------------------- the references' gradients
