@@ -174,19 +174,34 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// 1 / (1 + exp(-v)).  __expf is within 2 + 1.2 |v| units in the last place, so
-// the result is too; exp(-v) = inf gives 0.
-__device__ __forceinline__ float sigmoid(float v) { return __frcp_rn(1.0f + __expf(-v)); }
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// exp(v): v log2(e) in two parts, so that its rounding (|v| 2^-24) does not
+// show; within ex2.approx's 2^-22.
+__device__ __forceinline__ float exp_fast(float v) {
+  const float t = v * 1.4426950408889634f;
+  // log2(e) is the constant above plus 1.926e-8; inf - inf is kept out
+  const float r = fmaf(v, 1.4426950408889634f, -t) + v * 1.925963033500e-08f;
+  const float e = ex2(t);
+  return fabsf(v) < 3.0e38f ? fmaf(e, r * 0.6931471805599453f, e) : e;
+}
+
+// 1 / (1 + exp(-v)): within (6 + |v|) 2^-24; exp(-v) = inf gives 0.
+__device__ __forceinline__ float sigmoid(float v) { return rcp(1.0f + ex2(v * -1.4426950408889634f)); }
 
 // log(1 + exp(v)) = max(v, 0) + log1p(e), e = exp(-|v|) in (0, 1].  With
 // s = e / (2 + e) <= 1/3, log1p(e) = 2 atanh(s) = 2 s (1 + s^2/3 + s^4/5 + ..):
 // seven terms leave a relative remainder below 9^-7 / 15 = 1.4e-8.  *sig gets
 // the derivative 1 / (1 + exp(-v)).
 __device__ __forceinline__ float softplus(float v, float *sig) {
-  const float e = expf(-fabsf(v));
-  const float r = __frcp_rn(1.0f + e);
+  const float e = exp_fast(-fabsf(v));
+  const float r = rcp(1.0f + e);
   *sig = v >= 0.0f ? r : e * r;
-  const float s = __fdividef(e, 2.0f + e);
+  const float s = e * rcp(2.0f + e);
   const float q = s * s;
   float p = fmaf(q, 1.0f / 13, 1.0f / 11);
   p = fmaf(q, p, 1.0f / 9);

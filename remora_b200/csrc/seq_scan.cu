@@ -13,6 +13,7 @@
 // kernel joins them, and the main pass starts each piece from its own state.
 // That doubles the exponentials, so pieces are as few as fill the device.
 #include <algorithm>
+#include <type_traits>
 
 #include "seq_scan.cuh"
 
@@ -20,49 +21,83 @@ namespace remora {
 namespace seq {
 namespace {
 
-constexpr int kTile = 32;  // steps of b and c staged at a time
+constexpr int kTile = 32;   // steps of b and c staged at a time
+constexpr int64_t kBlocks = 148 * 8;  // blocks of a cut time axis: two rounds of 4 per SM
+constexpr int64_t kCutBelow = 148 * 3;
 
 // MAIN: writes y (and h_last, saved).  Otherwise the first pass of a cut time
 // axis: sum_h and sum_dt.  PADDED: N is not 4 NL; the states past N must stay
 // zero even where s u is not finite.
 template <int NL, bool PADDED, bool MAIN>
-__global__ void __launch_bounds__(kScanThreads) scan_fwd_kernel(const ScanArgs a) {
+__global__ void __launch_bounds__(kScanThreads, NL > 1 ? 4 : 2) scan_fwd_kernel(const ScanArgs a) {
   constexpr int NP = 4 * NL;
-  constexpr int GROUP = NL > 8 ? NL : 8;  // steps whose inputs are loaded together
+  constexpr int GROUP = save_every(NL);  // steps whose inputs are loaded together
   constexpr int PF = GROUP / NL;          // of them, per lane
   __shared__ __align__(16) float bs[2][kTile * NP];
   __shared__ __align__(16) float cs[2][MAIN ? kTile * NP : 4];
-  const Place<NL> at(a);
+  const Place<NL, kChan> at(a);
   const int64_t len = scan_length(a, at.b);
   const int64_t t0 = at.chunk * a.chunk, t_end = min(t0 + a.chunk, len);
   if (t0 >= len && t0 > 0) return;  // the first piece of an empty sequence hands h0 on
+  if (!MAIN && t_end == len) return;  // nothing follows
+  const int steps = (int)(t_end - t0);
   const int nv = a.states - 4 * at.q;  // of the four states, those below N
-  float A[4], h[4];
+  f2 A[kChan][2], h[kChan][2];
+  float bias[kChan], skip[kChan], total[kChan];
+  const float *up[kChan], *dp[kChan], *zp[kChan];
+  float *yp[kChan];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const bool on = at.live && k < nv;
-    A[k] = on ? a.a[at.d * a.a_d + (4 * at.q + k) * a.a_n] * kLog2e : 0.0f;
-    h[k] = 0.0f;
-    if (MAIN && on && a.chunks == 1 && a.h0.p)
-      h[k] = a.h0.p[at.b * a.h0.s0 + at.d * a.h0.s1 + (4 * at.q + k) * a.h0.s2];
+  for (int c = 0; c < kChan; ++c) {
+    float av[4], hv[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool on = k < nv;
+      av[k] = on ? a.a[at.d[c] * a.a_d + (4 * at.q + k) * a.a_n] * kLog2e : 0.0f;
+      hv[k] = 0.0f;
+      if (MAIN && on && a.chunks == 1 && a.h0.p)
+        hv[k] = a.h0.p[at.b * a.h0.s0 + at.d[c] * a.h0.s1 + (4 * at.q + k) * a.h0.s2];
+    }
+    if (MAIN && a.chunks > 1)
+      unpack(reinterpret_cast<const float4 *>(a.sum_h)[((at.b * a.chunks + at.chunk) * a.dim + at.d[c]) * NL + at.q], hv);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) A[c][k] = pair(av[2 * k], av[2 * k + 1]), h[c][k] = pair(hv[2 * k], hv[2 * k + 1]);
+    bias[c] = a.bias ? a.bias[at.d[c] * a.bias_s] : 0.0f;
+    skip[c] = MAIN && a.d ? a.d[at.d[c] * a.d_s] : 0.0f;
+    total[c] = 0.0f;
+    // a lane's own first step
+    up[c] = a.u.p + at.b * a.u.s0 + (t0 + at.q) * a.u.s1 + at.d[c] * a.u.s2;
+    dp[c] = a.delta.p + at.b * a.delta.s0 + (t0 + at.q) * a.delta.s1 + at.d[c] * a.delta.s2;
+    zp[c] = a.z.p + at.b * a.z.s0 + (t0 + at.q) * a.z.s1 + at.d[c] * a.z.s2;
+    yp[c] = a.y.p + at.b * a.y.s0 + (t0 + at.q) * a.y.s1 + at.d[c] * a.y.s2;
   }
-  if (MAIN && a.chunks > 1)
-    unpack(reinterpret_cast<const float4 *>(a.sum_h)[((at.b * a.chunks + at.chunk) * a.dim + at.d) * NL + at.q], h);
-  const float bias = a.bias ? a.bias[at.d * a.bias_s] : 0.0f;
-  const float skip = MAIN && a.d ? a.d[at.d * a.d_s] : 0.0f;
-  const float *up = a.u.p + at.b * a.u.s0 + at.d * a.u.s2;
-  const float *dp = a.delta.p + at.b * a.delta.s0 + at.d * a.delta.s2;
-  const float *zp = a.z.p + at.b * a.z.s0 + at.d * a.z.s2;
-  float *yp = a.y.p + at.b * a.y.s0 + at.d * a.y.s2;
-  float ru[PF], rd[PF], rz[PF], total = 0.0f;
-  auto fetch = [&](int64_t base) {
+  const bool gated = MAIN && a.z.p != nullptr;
+  float ru[kChan][PF], rd[kChan][PF], rz[kChan][PF];
+  auto fetch = [&](int base) {  // the inputs of steps base .. base + GROUP - 1 (zeros past the end), and on
+    if (base + GROUP <= steps) {
 #pragma unroll
-    for (int i = 0; i < PF; ++i) {
-      const int64_t t = base + i * NL + at.q;
-      const bool on = at.live && t < t_end;
-      ru[i] = on ? up[t * a.u.s1] : 0.0f;
-      rd[i] = on ? dp[t * a.delta.s1] : 0.0f;
-      if (MAIN && a.z.p) rz[i] = on ? zp[t * a.z.s1] : 0.0f;
+      for (int c = 0; c < kChan; ++c)
+#pragma unroll
+        for (int i = 0; i < PF; ++i) {
+          ru[c][i] = up[c][i * NL * a.u.s1];
+          rd[c][i] = dp[c][i * NL * a.delta.s1];
+          if (gated) rz[c][i] = zp[c][i * NL * a.z.s1];
+        }
+    } else {
+#pragma unroll
+      for (int c = 0; c < kChan; ++c)
+#pragma unroll
+        for (int i = 0; i < PF; ++i) {
+          const bool on = base + i * NL + at.q < steps;
+          ru[c][i] = on ? up[c][i * NL * a.u.s1] : 0.0f;
+          rd[c][i] = on ? dp[c][i * NL * a.delta.s1] : 0.0f;
+          if (gated) rz[c][i] = on ? zp[c][i * NL * a.z.s1] : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < kChan; ++c) {
+      up[c] += GROUP * a.u.s1;
+      dp[c] += GROUP * a.delta.s1;
+      if (gated) zp[c] += GROUP * a.z.s1;
     }
   };
   auto stage = [&](int buf, int64_t t) {
@@ -70,83 +105,134 @@ __global__ void __launch_bounds__(kScanThreads) scan_fwd_kernel(const ScanArgs a
     if (MAIN) stage_rows<NL, kTile>(cs[buf], a.c, a.vec_c, at.b, at.g, t, t_end, a.states);
     copy_commit();
   };
-  if (t0 < t_end) {
+  // what the steps of the next group need, from the inputs that have arrived
+  float s1[kChan][PF], su1[kChan][PF], y1[kChan][PF], w1[kChan][PF];
+  auto prepare = [&]() {
+#pragma unroll
+    for (int c = 0; c < kChan; ++c)
+#pragma unroll
+      for (int i = 0; i < PF; ++i) {
+        const float raw = rd[c][i] + bias[c];
+        float sig;
+        s1[c][i] = a.softplus ? softplus(raw, &sig) : raw;
+        su1[c][i] = s1[c][i] * ru[c][i];
+        if (MAIN) y1[c][i] = skip[c] * ru[c][i], w1[c][i] = gated ? rz[c][i] * sigmoid(rz[c][i]) : 1.0f;
+      }
+  };
+  // GROUP steps from `base` on, whose b and c rows start at bt and ct.  The
+  // inputs of the next group are prepared meanwhile, those of the one after
+  // it are on their way.
+  auto group = [&](auto whole, int base, const float *bt, const float *ct) {
+    constexpr bool FULL = decltype(whole)::value;
+    float s[kChan][PF], su[kChan][PF], y0[kChan][PF], w[kChan][PF];
+#pragma unroll
+    for (int c = 0; c < kChan; ++c)
+#pragma unroll
+      for (int i = 0; i < PF; ++i) {
+        s[c][i] = s1[c][i], su[c][i] = su1[c][i];
+        if (MAIN) y0[c][i] = y1[c][i], w[c][i] = w1[c][i];
+        if (!MAIN && (FULL || base + i * NL + at.q < steps)) total[c] += s[c][i];
+      }
+    prepare();
+    if (base + 2 * GROUP < steps) fetch(base + 2 * GROUP);
+#pragma unroll
+    for (int i = 0; i < PF; ++i) {
+      float part[kChan][NL];
+#pragma unroll
+      for (int j = 0; j < NL; ++j) {
+        const int t = i * NL + j;
+        float sj[kChan], suj[kChan];
+#pragma unroll
+        for (int c = 0; c < kChan; ++c) {
+          sj[c] = __shfl_sync(0xffffffffu, s[c][i], j, NL);
+          suj[c] = __shfl_sync(0xffffffffu, su[c][i], j, NL);
+          part[c][j] = 0.0f;
+        }
+        if (FULL || base + t < steps) {
+          const ulonglong2 b = *reinterpret_cast<const ulonglong2 *>(bt + t * NP + 4 * at.q);
+          const ulonglong2 cc = MAIN ? *reinterpret_cast<const ulonglong2 *>(ct + t * NP + 4 * at.q) : b;
+#pragma unroll
+          for (int c = 0; c < kChan; ++c) {
+            const f2 sp = both(sj[c]), sup = both(suj[c]);
+            f2 in0 = mul2(sup, b.x), in1 = mul2(sup, b.y);
+            if (PADDED) {
+              in0 = pair(nv > 0 ? lo(in0) : 0.0f, nv > 1 ? hi(in0) : 0.0f);
+              in1 = pair(nv > 2 ? lo(in1) : 0.0f, nv > 3 ? hi(in1) : 0.0f);
+            }
+            h[c][0] = fma2(ex2_2(mul2(sp, A[c][0])), h[c][0], in0);
+            h[c][1] = fma2(ex2_2(mul2(sp, A[c][1])), h[c][1], in1);
+            if (MAIN) {
+              const f2 y = fma2(h[c][1], cc.y, mul2(h[c][0], cc.x));
+              part[c][j] = lo(y) + hi(y);
+            }
+          }
+        }
+      }
+      if (MAIN) {
+#pragma unroll
+        for (int c = 0; c < kChan; ++c) {
+          transpose_sum<NL>(part[c], at.q);
+          if (at.live[c] && (FULL || base + i * NL + at.q < steps)) {
+            yp[c][i * NL * a.y.s1] = (part[c][0] + y0[c][i]) * w[c][i];
+          }
+        }
+      }
+    }
+    if (MAIN) {
+#pragma unroll
+      for (int c = 0; c < kChan; ++c) yp[c] += GROUP * a.y.s1;
+    }
+  };
+  if (steps > 0) {
     stage(0, t0);
-    fetch(t0);
+    fetch(0);
+    prepare();
+    fetch(GROUP);
   }
+  const int64_t kept = (a.length + GROUP - 1) / GROUP;
   int buf = 0;
-  for (int64_t tile = t0; tile < t_end; tile += kTile, buf ^= 1) {
-    if (tile + kTile < t_end)
-      stage(buf ^ 1, tile + kTile);
+  for (int tile = 0; tile < steps; tile += kTile, buf ^= 1) {
+    if (tile + kTile < steps)
+      stage(buf ^ 1, t0 + tile + kTile);
     else
       copy_commit();  // an empty group, so that the wait below counts alike
     copy_wait<1>();
     __syncthreads();
 #pragma unroll 1
-    for (int off = 0; off < kTile && tile + off < t_end; off += GROUP) {
-      const int64_t base = tile + off;
-      float s[PF], su[PF], u[PF], z[PF];
+    for (int base = tile; base < min(tile + kTile, steps); base += GROUP) {
+      if (MAIN && a.saved) {
 #pragma unroll
-      for (int i = 0; i < PF; ++i) {
-        const float raw = rd[i] + bias;
-        float sig;
-        s[i] = a.softplus ? softplus(raw, &sig) : raw;
-        u[i] = ru[i], z[i] = rz[i];
-        su[i] = s[i] * u[i];
-        if (!MAIN && base + i * NL + at.q < t_end) total += s[i];
+        for (int c = 0; c < kChan; ++c)
+          if (at.live[c])
+            reinterpret_cast<ulonglong2 *>(
+                a.saved)[((at.b * kept + (t0 + base) / GROUP) * a.dim + at.d[c]) * NL + at.q] =
+                make_ulonglong2(h[c][0], h[c][1]);
       }
-      if (base + GROUP < t_end) fetch(base + GROUP);
-      if (MAIN && a.saved && at.live && base % kSaveEvery == 0)
-        reinterpret_cast<float4 *>(
-            a.saved)[((at.b * ((a.length + kSaveEvery - 1) / kSaveEvery) + base / kSaveEvery) * a.dim + at.d) * NL +
-                     at.q] = make_float4(h[0], h[1], h[2], h[3]);
-      const bool full = base + GROUP <= t_end;
-#pragma unroll
-      for (int i = 0; i < PF; ++i) {
-        float part[NL];
-#pragma unroll
-        for (int j = 0; j < NL; ++j) {
-          part[j] = 0.0f;
-          const float sj = __shfl_sync(0xffffffffu, s[i], j, NL);
-          const float suj = __shfl_sync(0xffffffffu, su[i], j, NL);
-          if (full || base + i * NL + j < t_end) {
-            float b[4], c[4];
-            unpack(*reinterpret_cast<const float4 *>(&bs[buf][(off + i * NL + j) * NP + 4 * at.q]), b);
-            if (MAIN) unpack(*reinterpret_cast<const float4 *>(&cs[buf][(off + i * NL + j) * NP + 4 * at.q]), c);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float in = PADDED && k >= nv ? 0.0f : suj * b[k];
-              h[k] = fmaf(ex2(sj * A[k]), h[k], in);
-              if (MAIN) part[j] = fmaf(h[k], c[k], part[j]);
-            }
-          }
-        }
-        if (MAIN) {
-          transpose_sum<NL>(part, at.q);
-          const int64_t t = base + i * NL + at.q;
-          if (at.live && t < t_end) {
-            float y = fmaf(skip, u[i], part[0]);
-            if (a.z.p) y *= z[i] * sigmoid(z[i]);
-            yp[t * a.y.s1] = y;
-          }
-        }
-      }
+      const float *bt = &bs[buf][(base - tile) * NP], *ct = &cs[buf][MAIN ? (base - tile) * NP : 0];
+      if (base + GROUP <= steps)
+        group(std::true_type{}, base, bt, ct);
+      else
+        group(std::false_type{}, base, bt, ct);
     }
     __syncthreads();  // this buffer is filled again in the next turn
   }
-  if (MAIN) {
-    if (a.h_last.p && at.live && t_end == len) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (k < nv) a.h_last.p[at.b * a.h_last.s0 + at.d * a.h_last.s1 + (4 * at.q + k) * a.h_last.s2] = h[k];
-    }
-  } else {
+  for (int c = 0; c < kChan; ++c) {
+    const float hv[4] = {lo(h[c][0]), hi(h[c][0]), lo(h[c][1]), hi(h[c][1])};
+    if (MAIN) {
+      if (a.h_last.p && at.live[c] && t_end == len) {
 #pragma unroll
-    for (int o = 1; o < NL; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    if (at.live) {
-      const int64_t i = (at.b * a.chunks + at.chunk) * a.dim + at.d;
-      reinterpret_cast<float4 *>(a.sum_h)[i * NL + at.q] = make_float4(h[0], h[1], h[2], h[3]);
-      if (at.q == 0) a.sum_dt[i] = total;
+        for (int k = 0; k < 4; ++k)
+          if (k < nv) a.h_last.p[at.b * a.h_last.s0 + at.d[c] * a.h_last.s1 + (4 * at.q + k) * a.h_last.s2] = hv[k];
+      }
+    } else {
+#pragma unroll
+      for (int o = 1; o < NL; o <<= 1) total[c] += __shfl_xor_sync(0xffffffffu, total[c], o);
+      if (at.live[c]) {
+        const int64_t i = (at.b * a.chunks + at.chunk) * a.dim + at.d[c];
+        reinterpret_cast<float4 *>(a.sum_h)[i * NL + at.q] = make_float4(hv[0], hv[1], hv[2], hv[3]);
+        if (at.q == 0) a.sum_dt[i] = total[c];
+      }
     }
   }
 }
@@ -164,11 +250,22 @@ __global__ void __launch_bounds__(256) scan_combine_kernel(const ScanArgs a, int
   const bool on = n < a.states;
   const float A = on ? a.a[d * a.a_d + n * a.a_n] * kLog2e : 0.0f;
   float h = on && first.p ? first.p[b * first.s0 + d * first.s1 + n * first.s2] : 0.0f;
-  for (int64_t k = 0; k < used; ++k) {
-    const int64_t j = (b * a.chunks + (reverse ? used - 1 - k : k)) * a.dim + d;
-    const float own = a.sum_h[j * np + n], dt = a.sum_dt[j];
-    a.sum_h[j * np + n] = h;
-    h = fmaf(ex2(dt * A), h, own);
+  constexpr int U = 8;  // pieces whose sums are on their way together
+  for (int64_t k0 = 0; k0 < used; k0 += U) {
+    float own[U], dt[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int64_t j = (b * a.chunks + (reverse ? used - 1 - k0 - k : k0 + k)) * a.dim + d;
+      const bool summed = k0 + k + 1 < used;  // nothing follows the last
+      own[k] = summed ? a.sum_h[j * np + n] : 0.0f;
+      dt[k] = summed ? a.sum_dt[j] : 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      if (k0 + k >= used) break;
+      a.sum_h[((b * a.chunks + (reverse ? used - 1 - k0 - k : k0 + k)) * a.dim + d) * np + n] = h;
+      h = fmaf(ex2(dt[k] * A), h, own[k]);
+    }
   }
 }
 
@@ -273,10 +370,10 @@ bool vec_states(const DescView &v) {
 // warps, else as many as do, of at least 64 steps each.
 void cut_time(int64_t batch, int64_t length, int64_t dim, int states, int groups, int64_t *chunks, int64_t *chunk) {
   const int nl = lanes_for(states);
-  const int64_t per_block = kScanThreads / nl, per = dim / std::max(groups, 1);
+  const int64_t per_block = block_channels(nl, kChan), per = dim / std::max(groups, 1);
   const int64_t blocks = std::max<int64_t>(1, batch * groups * ((per + per_block - 1) / per_block));
   int64_t n = 1;
-  if (blocks < 148 * 3) n = std::max<int64_t>(1, std::min<int64_t>(148 * 5 / blocks, length / 64));
+  if (blocks < kCutBelow) n = std::max<int64_t>(1, std::min<int64_t>(kBlocks / blocks, length / 64));
   *chunk = std::max<int64_t>(kTile, ((length + n - 1) / n + kTile - 1) / kTile * kTile);
   *chunks = std::max<int64_t>(1, (length + *chunk - 1) / *chunk);
 }
@@ -288,6 +385,7 @@ size_t scratch_for(int64_t batch, int64_t dim, int states, int64_t chunks) {
 
 int check_sizes(int64_t batch, int64_t length, int64_t dim, int64_t states, int64_t groups, const char *what) {
   if (batch < 0 || length < 0 || dim < 0) return fail(REMORA_ERR_ARG, "%s: negative size", what);
+  if (length > kMaxLength) return fail(REMORA_ERR_LIMIT, "%s: more than 2^30 positions", what);
   if (states < 1 || states > kMaxStates)
     return fail(REMORA_ERR_UNSUPPORTED, "%s: %lld states (1..%d)", what, (long long)states, kMaxStates);
   if (groups < 1 || dim % groups)
@@ -360,8 +458,6 @@ int read_scan_in(const RemoraSelectiveScanSpec *spec, const RemoraSelectiveScanI
   if (have[9]) a->lengths = reinterpret_cast<const int *>(views[9].data(4)), a->lengths_s = views[9].strides[0];
   a->batch = B, a->length = L, a->dim = D, a->states = (int)N, a->groups = (int)G, a->softplus = spec->softplus != 0;
   a->per = D / G;
-  const int64_t per_block = kScanThreads / lanes_for((int)N);
-  a->blocks_d = (a->per + per_block - 1) / per_block;
   return REMORA_OK;
 }
 
@@ -384,7 +480,8 @@ extern "C" {
 int remora_b200_selective_scan_saved(int64_t batch, int64_t length, int64_t dim, int64_t states, size_t *bytes) {
   if (bytes == nullptr) return fail(REMORA_ERR_ARG, "selective_scan_saved: null pointer");
   REMORA_TRY(check_sizes(batch, length, dim, states, 1, "selective_scan_saved"));
-  *bytes = (size_t)(batch * ((length + kSaveEvery - 1) / kSaveEvery) * dim) * (size_t)(4 * lanes_for((int)states)) * 4;
+  const int nl = lanes_for((int)states), every = save_every(nl);
+  *bytes = (size_t)(batch * ((length + every - 1) / every) * dim) * (size_t)(4 * nl) * 4;
   return REMORA_OK;
 }
 
@@ -411,6 +508,8 @@ int remora_b200_selective_scan_fwd(RemoraB200Ctx *ctx, const RemoraSelectiveScan
   REMORA_TRY(read_f32(y, 3, &yv, "selective_scan y"));
   REMORA_TRY(read_optional(h_last, 3, &hv, &has_h, "selective_scan h_last"));
   REMORA_TRY(want_shape(yv, {a.batch, a.length, a.dim}, "selective_scan y"));
+  const int nl = lanes_for(a.states);
+  a.blocks_d = (a.per + block_channels(nl, kChan) - 1) / block_channels(nl, kChan);
   if (has_h) REMORA_TRY(want_shape(hv, {a.batch, a.dim, a.states}, "selective_scan h_last"));
   auto given = [&](int k) { return v[k].aligned != nullptr ? &v[k] : nullptr; };
   REMORA_TRY(want_apart({{&yv, "y", 4}, {has_h ? &hv : nullptr, "h_last", 4}},
@@ -420,7 +519,6 @@ int remora_b200_selective_scan_fwd(RemoraB200Ctx *ctx, const RemoraSelectiveScan
   a.y = op3(yv);
   if (has_h) a.h_last = op3(hv);
   cut_time(a.batch, a.length, a.dim, a.states, a.groups, &a.chunks, &a.chunk);
-  const int nl = lanes_for(a.states);
   if (saved != nullptr) {
     size_t need = 0;
     REMORA_TRY(remora_b200_selective_scan_saved(a.batch, a.length, a.dim, a.states, &need));

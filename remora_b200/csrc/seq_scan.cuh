@@ -4,12 +4,16 @@
 // and c in shared memory.
 //
 // Mapping.  A channel's N states are spread over NL neighbouring lanes of a
-// warp, four states each (NP = 4 NL >= N, the states past N are zero), so a
-// warp works on 32 / NL channels.  Time runs serially in a thread.  The
-// per-channel inputs are loaded by the lane that a step falls to (lane q of a
-// channel takes steps q, q + NL, ...) and broadcast by shuffle; sums over the
-// states go back to that lane by a transposed (reduce-scatter) shuffle, so
-// every per-channel value is loaded, transformed and stored once.
+// warp, four states each (NP = 4 NL >= N, the states past N are zero).  A
+// thread holds kChan channels, 32 / NL apart, so a warp works on 32 kChan / NL:
+// b and c of a step, which all channels read from shared memory, cost one
+// clock of the SM's shared-memory pipe per register that they fill, and are
+// used kChan times.  Time runs serially in a thread.  The per-channel inputs
+// are loaded by the lane that a step falls to (lane q of a channel takes steps
+// q, q + NL, ...) and broadcast by shuffle; sums over the states go back to
+// that lane by a transposed (reduce-scatter) shuffle, so every per-channel
+// value is loaded, transformed and stored once.  State arithmetic is done on
+// pairs of states (f32x2 instructions, each half rounded as the scalar form).
 #pragma once
 
 #include "seq.cuh"
@@ -18,8 +22,12 @@ namespace remora {
 namespace seq {
 
 constexpr int kScanThreads = 128;
-constexpr int kSaveEvery = 16;  // steps between the states that the forward keeps
+// Steps between the states that the forward keeps for the backward pass: what
+// fits a thread's registers there.
+constexpr int save_every(int nl) { return nl > 8 ? 16 : 8; }
 constexpr int kMaxStates = 64;
+constexpr int64_t kMaxLength = 1 << 30;
+constexpr int kChan = 2;  // channels per thread
 
 struct Op3 {  // [B, time, D], or [B, D, N]
   float *p;
@@ -45,16 +53,19 @@ struct ScanArgs {
   int64_t chunks;    // pieces of the time axis, each by blocks of its own
   int64_t chunk;     // their length, a multiple of 32
   int vec_b, vec_c;  // b, c rows can be copied 16 bytes at a time
-  float *saved;      // [B, ceil(L / kSaveEvery), D, NP]
+  float *saved;      // [B, ceil(L / save_every), D, NP]
   float *sum_h;      // [B, chunks, D, NP]: a piece's own end state, then its start state
   float *sum_dt;     // [B, chunks, D]: a piece's sum of steps
   // backward
   Op3 dy, dh_last, du, ddelta, dz, dh0;
   Op4 db, dc;
-  float *part_bc;  // [blocks_d, 2, B, L, G, N]
+  float *part_bc;  // [blocks_d, B, L, G, 2, N]
   float *part_a;   // [B * chunks, D, N]
   float *part_d;   // [B * chunks, 2, D]
 };
+
+// Channels of a block whose threads hold `chan` channels each.
+inline int64_t block_channels(int nl, int chan) { return (int64_t)kScanThreads / nl * chan; }
 
 // Lanes per channel for N states.
 inline int lanes_for(int states) {
@@ -75,20 +86,25 @@ __device__ __forceinline__ int64_t scan_length(const ScanArgs &a, int64_t b) {
 }
 
 // The place of a thread: block = ((b * chunks + chunk) * groups + g) * blocks_d + bd.
-template <int NL>
+// Channels past the group's last stand on its first one, with live false.
+template <int NL, int CHAN>
 struct Place {
-  int64_t bd, g, chunk, b, d;
+  int64_t bd, g, chunk, b, d[CHAN];
   int q;
-  bool live;
+  bool live[CHAN];
   __device__ __forceinline__ explicit Place(const ScanArgs &a) {
     int64_t i = blockIdx.x;
     bd = i % a.blocks_d, i /= a.blocks_d;
     g = i % a.groups, i /= a.groups;
     chunk = i % a.chunks, b = i / a.chunks;
     q = threadIdx.x % NL;
-    const int64_t in_group = bd * (kScanThreads / NL) + threadIdx.x / NL;
-    live = in_group < a.per;
-    d = g * a.per + (live ? in_group : 0);
+#pragma unroll
+    for (int c = 0; c < CHAN; ++c) {
+      const int64_t in_group = (bd * (kScanThreads / 32) + threadIdx.x / 32) * (32 / NL * CHAN) + c * (32 / NL) +
+                               threadIdx.x % 32 / NL;
+      live[c] = in_group < a.per;
+      d[c] = g * a.per + (live[c] ? in_group : 0);
+    }
   }
 };
 
@@ -145,7 +161,36 @@ __device__ __forceinline__ void transpose_sum(float (&v)[NL], int q) {
   }
 }
 
-__device__ __forceinline__ void unpack(const float4 &v, float (&o)[4]) { o[0] = v.x, o[1] = v.y, o[2] = v.z, o[3] = v.w; }
+__device__ __forceinline__ void unpack(const float4 &v, float (&o)[4]) {
+  o[0] = v.x, o[1] = v.y, o[2] = v.z, o[3] = v.w;
+}
+
+// Two f32 in a register pair, and the instructions on both at once.
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pair(float lo, float hi) {
+  f2 o;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(o) : "f"(lo), "f"(hi));
+  return o;
+}
+__device__ __forceinline__ f2 both(float v) { return pair(v, v); }
+__device__ __forceinline__ float lo(f2 v) { return __uint_as_float((unsigned)v); }
+__device__ __forceinline__ float hi(f2 v) { return __uint_as_float((unsigned)(v >> 32)); }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 o;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(o) : "l"(a), "l"(b));
+  return o;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 o;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(o) : "l"(a), "l"(b));
+  return o;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 o;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(o) : "l"(a), "l"(b), "l"(c));
+  return o;
+}
+__device__ __forceinline__ f2 ex2_2(f2 v) { return pair(ex2(lo(v)), ex2(hi(v))); }
 #endif
 
 }  // namespace seq

@@ -5,14 +5,16 @@
 //   dc_t[n] = sum_d dp h_t[n];  db_t[n] = sum_d G s u;  da[n] = sum_t G s (exp(s a) h_{t-1})[n]
 //   du = s sum_n G b + d dp;  ds = sum_n G a (exp(s a) h_{t-1}) + u sum_n G b;  ddelta = ds f'(delta + bias)
 //
-// A thread walks time from the end in pieces of kSaveEvery steps.  For each
-// it takes the state that the forward kept at the piece's start, runs the
-// recurrence forward once, keeping exp(s a) and exp(s a) h of every step in
-// registers, then the adjoint backward: one exponential per position, channel
-// and state in all.  db and dc sum over the channels of a group: over a warp
-// by shuffle, over a block through shared memory, over blocks by partial rows
-// in scratch that a second kernel adds in block order.
+// A thread walks time from the end in pieces of save_every steps.  For each it
+// takes the state that the forward kept at the piece's start, runs the
+// recurrence forward once, keeping exp(s a) h_{t-1} of every step in registers,
+// then the adjoint backward (the decay's second exponential costs less there
+// than the registers to keep it).  db and dc sum over the channels of a group:
+// over a thread's channels, over a warp by a transposed shuffle, over a block
+// through shared memory, over blocks by partial rows in scratch that a second
+// kernel adds in block order.
 #include <algorithm>
+#include <type_traits>
 
 #include "seq_scan.cuh"
 
@@ -20,8 +22,22 @@ namespace remora {
 namespace seq {
 namespace {
 
-constexpr int kSteps = kSaveEvery;
 constexpr int kWarps = kScanThreads / 32;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// Channels of a thread, steps of a piece, steps whose b, c, db and dc are in
+// shared memory together.
+template <int NL>
+struct Bwd {
+  static constexpr int kChan = NL > 8 ? 1 : 2;
+  static constexpr int kPiece = save_every(NL);
+  static constexpr int kTile = NL > 4 ? 16 : 32;
+};
+
+constexpr int64_t kBlocks = 148 * 8;  // blocks of a cut time axis
+constexpr int64_t kCutBelow = 148 * 2;
+
+int64_t bwd_channels(int nl) { return kScanThreads / nl * (nl > 8 ? 1 : 2); }  // of a block
 
 // Sums v over the 32 / NL channel lanes of a warp; CNT of the sums end in
 // v[0 .. CNT-1] of each lane, the sums FIRST .. FIRST + CNT - 1.
@@ -53,303 +69,376 @@ struct ChannelSum {
   __device__ static __forceinline__ bool stores(int lane) { return NL >= 4 || (lane & 3) < NL; }
 };
 
-template <int NL, bool PADDED>
-__global__ void __launch_bounds__(kScanThreads) scan_bwd_kernel(const ScanArgs a) {
-  constexpr int NP = 4 * NL;
-  constexpr int PF = kSteps / NL;
+template <int NL>
+__global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const ScanArgs a) {
+  constexpr int NP = 4 * NL, C = Bwd<NL>::kChan, T = Bwd<NL>::kPiece, TILE = Bwd<NL>::kTile;
+  constexpr int PF = T / NL;
   using Sum = ChannelSum<NL>;
-  __shared__ __align__(16) float bs[2][kSteps * NP], cs[2][kSteps * NP];
-  __shared__ __align__(16) float red[kWarps][kSteps][2 * NP];  // per step: db[NP], dc[NP]
-  const Place<NL> at(a);
+  __shared__ __align__(16) float bs[2][TILE * NP], cs[2][TILE * NP];
+  extern __shared__ __align__(16) float red[];  // [kWarps][TILE][2 NP]: per step db, dc
+  const Place<NL, C> at(a);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t len = scan_length(a, at.b);
   const int64_t t0 = at.chunk * a.chunk, t_end = min(t0 + a.chunk, len);
+  const int steps = t_end > t0 ? (int)(t_end - t0) : 0;
   const int64_t prow = at.b * a.chunks + at.chunk;
+  const int64_t kept = (a.length + T - 1) / T;
   const int nv = a.states - 4 * at.q;
-  float A[4], A2[4], G[4], dA[4];
+  f2 A[C][2], G[C][2], dA[C][2];
+  float bias[C], skip[C], sum_d[C], sum_bias[C];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const bool on = at.live && k < nv;
-    A[k] = on ? a.a[at.d * a.a_d + (4 * at.q + k) * a.a_n] : 0.0f;
-    A2[k] = A[k] * kLog2e;
-    G[k] = dA[k] = 0.0f;
-    if (on && a.chunks == 1 && a.dh_last.p)
-      G[k] = a.dh_last.p[at.b * a.dh_last.s0 + at.d * a.dh_last.s1 + (4 * at.q + k) * a.dh_last.s2];
-  }
-  if (a.chunks > 1 && (t0 < len || t0 == 0))
-    unpack(reinterpret_cast<const float4 *>(a.sum_h)[(prow * a.dim + at.d) * NL + at.q], G);
-  const float bias = a.bias ? a.bias[at.d * a.bias_s] : 0.0f;
-  const float skip = a.d ? a.d[at.d * a.d_s] : 0.0f;
-  const float *up = a.u.p + at.b * a.u.s0 + at.d * a.u.s2;
-  const float *dp = a.delta.p + at.b * a.delta.s0 + at.d * a.delta.s2;
-  const float *zp = a.z.p + at.b * a.z.s0 + at.d * a.z.s2;
-  const float *yp = a.dy.p + at.b * a.dy.s0 + at.d * a.dy.s2;
-  float ru[PF], rd[PF], rz[PF], ry[PF];
-  float4 rh = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  const int64_t kept = (a.length + kSaveEvery - 1) / kSaveEvery;
-  auto fetch = [&](int64_t base) {
+  for (int c = 0; c < C; ++c) {
+    float av[4], gv[4];
 #pragma unroll
-    for (int i = 0; i < PF; ++i) {
-      const int64_t t = base + i * NL + at.q;
-      const bool on = at.live && t < t_end;
-      ru[i] = on ? up[t * a.u.s1] : 0.0f;
-      rd[i] = on ? dp[t * a.delta.s1] : 0.0f;
-      ry[i] = on ? yp[t * a.dy.s1] : 0.0f;
-      if (a.z.p) rz[i] = on ? zp[t * a.z.s1] : 0.0f;
+    for (int k = 0; k < 4; ++k) {
+      const bool on = at.live[c] && k < nv;
+      av[k] = on ? a.a[at.d[c] * a.a_d + (4 * at.q + k) * a.a_n] * kLog2e : 0.0f;
+      gv[k] = 0.0f;
+      if (on && a.chunks == 1 && a.dh_last.p)
+        gv[k] = a.dh_last.p[at.b * a.dh_last.s0 + at.d[c] * a.dh_last.s1 + (4 * at.q + k) * a.dh_last.s2];
     }
-    if (at.live)
-      rh = reinterpret_cast<const float4 *>(a.saved)[((at.b * kept + base / kSaveEvery) * a.dim + at.d) * NL + at.q];
-  };
-  auto stage = [&](int buf, int64_t t) {
-    stage_rows<NL, kSteps>(bs[buf], a.b, a.vec_b, at.b, at.g, t, t_end, a.states);
-    stage_rows<NL, kSteps>(cs[buf], a.c, a.vec_c, at.b, at.g, t, t_end, a.states);
-    copy_commit();
-  };
-  float sum_d = 0.0f, sum_bias = 0.0f;
-  int buf = 0;
-  const int64_t last = t_end > t0 ? t0 + (t_end - 1 - t0) / kSteps * kSteps : t0 - kSteps;
-  if (last >= t0) {
-    stage(0, last);
-    fetch(last);
-  }
-  for (int64_t base = last; base >= t0; base -= kSteps, buf ^= 1) {
-    if (base - kSteps >= t0)
-      stage(buf ^ 1, base - kSteps);
-    else
-      copy_commit();
-    copy_wait<1>();
-    __syncthreads();  // b and c are there; red of the turn before is read
-    float s[PF], sig[PF], su[PF], u[PF], dyp[PF], dzf[PF], h[4];
-    unpack(rh, h);
+    if (a.chunks > 1 && at.live[c] && (t0 < len || t0 == 0))
+      unpack(reinterpret_cast<const float4 *>(a.sum_h)[(prow * a.dim + at.d[c]) * NL + at.q], gv);
 #pragma unroll
-    for (int i = 0; i < PF; ++i) {
-      const float raw = rd[i] + bias;
-      sig[i] = 1.0f;
-      s[i] = a.softplus ? softplus(raw, &sig[i]) : raw;
-      u[i] = ru[i];
-      su[i] = s[i] * u[i];
-      dyp[i] = ry[i];
-      dzf[i] = 0.0f;
-      if (a.z.p) {
-        const float sz = sigmoid(rz[i]);
-        dyp[i] = ry[i] * (rz[i] * sz);
-        dzf[i] = ry[i] * (sz * fmaf(rz[i], 1.0f - sz, 1.0f));
-      }
+    for (int k = 0; k < 2; ++k) {
+      A[c][k] = pair(av[2 * k], av[2 * k + 1]);
+      G[c][k] = pair(gv[2 * k], gv[2 * k + 1]);
+      dA[c][k] = 0;
     }
-    if (base - kSteps >= t0) fetch(base - kSteps);
-    float e[kSteps][4], eh[kSteps][4];
-    auto piece = [&](auto whole) {
-      constexpr bool FULL = decltype(whole)::value;
+    bias[c] = a.bias ? a.bias[at.d[c] * a.bias_s] : 0.0f;
+    skip[c] = a.d ? a.d[at.d[c] * a.d_s] : 0.0f;
+    sum_d[c] = sum_bias[c] = 0.0f;
+  }
+  const bool gated = a.z.p != nullptr;
+  float ru[C][PF], rd[C][PF], rz[C][PF], ry[C][PF];
+  ulonglong2 rh[C];
+  auto fetch = [&](int base) {  // the inputs of the piece from `base` on: zeros past the end and for no channel
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
 #pragma unroll
       for (int i = 0; i < PF; ++i) {
-        float part[NL];
+        const bool on = at.live[c] && base + i * NL + at.q < steps;
+        const int64_t t = t0 + base + i * NL + at.q;
+        ru[c][i] = on ? a.u.p[at.b * a.u.s0 + t * a.u.s1 + at.d[c] * a.u.s2] : 0.0f;
+        rd[c][i] = on ? a.delta.p[at.b * a.delta.s0 + t * a.delta.s1 + at.d[c] * a.delta.s2] : 0.0f;
+        ry[c][i] = on ? a.dy.p[at.b * a.dy.s0 + t * a.dy.s1 + at.d[c] * a.dy.s2] : 0.0f;
+        rz[c][i] = gated && on ? a.z.p[at.b * a.z.s0 + t * a.z.s1 + at.d[c] * a.z.s2] : 0.0f;
+      }
+      rh[c] = at.live[c] ? reinterpret_cast<const ulonglong2 *>(
+                               a.saved)[((at.b * kept + (t0 + base) / T) * a.dim + at.d[c]) * NL + at.q]
+                         : make_ulonglong2(0, 0);
+    }
+  };
+  auto stage = [&](int buf, int tile) {
+    stage_rows<NL, TILE>(bs[buf], a.b, a.vec_b, at.b, at.g, t0 + tile, t_end, a.states);
+    stage_rows<NL, TILE>(cs[buf], a.c, a.vec_c, at.b, at.g, t0 + tile, t_end, a.states);
+    copy_commit();
+  };
+  // the piece from `base` on; its rows of b, c and red start at bt, ct, rt
+  auto piece = [&](auto whole, int base, const float *bt, const float *ct, float *rt) {
+    constexpr bool FULL = decltype(whole)::value;
+    float s[C][PF], sig[C][PF], su[C][PF], u[C][PF], dyp[C][PF], dzf[C][PF];
+    f2 h[C][2], eh[T][C][2];
 #pragma unroll
-        for (int j = 0; j < NL; ++j) {
-          const int t = i * NL + j;
-          part[j] = 0.0f;
-          const float sj = __shfl_sync(0xffffffffu, s[i], j, NL);
-          const float suj = __shfl_sync(0xffffffffu, su[i], j, NL);
-          if (FULL || base + t < t_end) {
-            float b[4], c[4];
-            unpack(*reinterpret_cast<const float4 *>(&bs[buf][t * NP + 4 * at.q]), b);
-            unpack(*reinterpret_cast<const float4 *>(&cs[buf][t * NP + 4 * at.q]), c);
+    for (int c = 0; c < C; ++c) {
+      h[c][0] = rh[c].x, h[c][1] = rh[c].y;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              e[t][k] = ex2(sj * A2[k]);
-              eh[t][k] = e[t][k] * h[k];
-              h[k] = eh[t][k] + (PADDED && k >= nv ? 0.0f : suj * b[k]);
-              part[j] = fmaf(h[k], c[k], part[j]);
+      for (int i = 0; i < PF; ++i) {
+        const float raw = rd[c][i] + bias[c];
+        sig[c][i] = 1.0f;
+        s[c][i] = a.softplus ? softplus(raw, &sig[c][i]) : raw;
+        u[c][i] = ru[c][i];
+        su[c][i] = s[c][i] * u[c][i];
+        dyp[c][i] = ry[c][i];
+        dzf[c][i] = 0.0f;
+        if (gated) {
+          const float sz = sigmoid(rz[c][i]);
+          dyp[c][i] = ry[c][i] * (rz[c][i] * sz);
+          dzf[c][i] = ry[c][i] * (sz * fmaf(rz[c][i], 1.0f - sz, 1.0f));
+        }
+      }
+    }
+    if (base >= T) fetch(base - T);
+#pragma unroll
+    for (int i = 0; i < PF; ++i) {
+      float part[C][NL];
+#pragma unroll
+      for (int j = 0; j < NL; ++j) {
+        const int t = i * NL + j;
+        float sj[C], suj[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          sj[c] = __shfl_sync(0xffffffffu, s[c][i], j, NL);
+          suj[c] = __shfl_sync(0xffffffffu, su[c][i], j, NL);
+          part[c][j] = 0.0f;
+        }
+        if (FULL || base + t < steps) {
+          const ulonglong2 b = *reinterpret_cast<const ulonglong2 *>(bt + t * NP + 4 * at.q);
+          const ulonglong2 cc = *reinterpret_cast<const ulonglong2 *>(ct + t * NP + 4 * at.q);
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            const f2 sp = both(sj[c]), sup = both(suj[c]);
+            eh[t][c][0] = mul2(ex2_2(mul2(sp, A[c][0])), h[c][0]);
+            eh[t][c][1] = mul2(ex2_2(mul2(sp, A[c][1])), h[c][1]);
+            h[c][0] = fma2(sup, b.x, eh[t][c][0]);
+            h[c][1] = fma2(sup, b.y, eh[t][c][1]);
+            const f2 y = fma2(h[c][1], cc.y, mul2(h[c][0], cc.x));
+            part[c][j] = lo(y) + hi(y);
+          }
+        }
+      }
+      if (a.dz.p) {
+        const int64_t t = t0 + base + i * NL + at.q;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          transpose_sum<NL>(part[c], at.q);
+          if (at.live[c] && (FULL || base + i * NL + at.q < steps))
+            a.dz.p[at.b * a.dz.s0 + t * a.dz.s1 + at.d[c] * a.dz.s2] = dzf[c][i] * fmaf(skip[c], u[c][i], part[c][0]);
+        }
+      }
+    }
+    // a piece's share of da on its own: long sums in parts
+    f2 da[C][2];
+#pragma unroll
+    for (int c = 0; c < C; ++c) da[c][0] = da[c][1] = 0;
+#pragma unroll
+    for (int i = PF - 1; i >= 0; --i) {
+      float gb[C][NL], ga[C][NL];
+#pragma unroll
+      for (int j = NL - 1; j >= 0; --j) {
+        const int t = i * NL + j;
+        float sj[C], suj[C], dj[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          sj[c] = __shfl_sync(0xffffffffu, s[c][i], j, NL);
+          suj[c] = __shfl_sync(0xffffffffu, su[c][i], j, NL);
+          dj[c] = __shfl_sync(0xffffffffu, dyp[c][i], j, NL);
+          gb[c][j] = ga[c][j] = 0.0f;
+        }
+        if (FULL || base + t < steps) {
+          const ulonglong2 b = *reinterpret_cast<const ulonglong2 *>(bt + t * NP + 4 * at.q);
+          const ulonglong2 cc = *reinterpret_cast<const ulonglong2 *>(ct + t * NP + 4 * at.q);
+          f2 db[2], dc[2];
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            const f2 sp = both(sj[c]), sup = both(suj[c]), djp = both(dj[c]);
+            f2 g2, a2;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const f2 bk = k ? b.y : b.x, ck = k ? cc.y : cc.x, x = eh[t][c][k];
+              const f2 hk = fma2(sup, bk, x);
+              G[c][k] = fma2(ck, djp, G[c][k]);
+              db[k] = c ? fma2(G[c][k], sup, db[k]) : mul2(G[c][k], sup);
+              dc[k] = c ? fma2(hk, djp, dc[k]) : mul2(hk, djp);
+              const f2 gx = mul2(G[c][k], x);
+              g2 = k ? fma2(G[c][k], bk, g2) : mul2(G[c][k], bk);
+              a2 = k ? fma2(gx, A[c][k], a2) : mul2(gx, A[c][k]);
+              da[c][k] = fma2(gx, sp, da[c][k]);
+              G[c][k] = mul2(G[c][k], ex2_2(mul2(sp, A[c][k])));
+            }
+            gb[c][j] = lo(g2) + hi(g2);
+            ga[c][j] = lo(a2) + hi(a2);
+          }
+          float v[8] = {lo(db[0]), hi(db[0]), lo(db[1]), hi(db[1]), lo(dc[0]), hi(dc[0]), lo(dc[1]), hi(dc[1])};
+          Sum::run(v, lane);
+          if (Sum::stores(lane)) {
+            const int first = Sum::first(lane);
+#pragma unroll
+            for (int k = 0; k < Sum::kCount; ++k) {
+              const int f = first + k;
+              rt[t * 2 * NP + (f >> 2) * NP + 4 * at.q + (f & 3)] = v[k];
             }
           }
         }
-        transpose_sum<NL>(part, at.q);
-        const int64_t t = base + i * NL + at.q;
-        if (a.dz.p && at.live && t < t_end)
-          a.dz.p[at.b * a.dz.s0 + t * a.dz.s1 + at.d * a.dz.s2] = dzf[i] * fmaf(skip, u[i], part[0]);
       }
+      const int64_t t = t0 + base + i * NL + at.q;
 #pragma unroll
-      for (int i = PF - 1; i >= 0; --i) {
-        float gb[NL], ga[NL];
-#pragma unroll
-        for (int j = NL - 1; j >= 0; --j) {
-          const int t = i * NL + j;
-          gb[j] = ga[j] = 0.0f;
-          const float sj = __shfl_sync(0xffffffffu, s[i], j, NL);
-          const float suj = __shfl_sync(0xffffffffu, su[i], j, NL);
-          const float dj = __shfl_sync(0xffffffffu, dyp[i], j, NL);
-          if (FULL || base + t < t_end) {
-            float b[4], c[4], v[8];
-            unpack(*reinterpret_cast<const float4 *>(&bs[buf][t * NP + 4 * at.q]), b);
-            unpack(*reinterpret_cast<const float4 *>(&cs[buf][t * NP + 4 * at.q]), c);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const bool pad = PADDED && k >= nv;
-              const float hk = eh[t][k] + (pad ? 0.0f : suj * b[k]);
-              G[k] += pad ? 0.0f : c[k] * dj;
-              v[k] = G[k] * suj;
-              v[4 + k] = dj * hk;
-              gb[j] = fmaf(G[k], b[k], gb[j]);
-              const float geh = G[k] * eh[t][k];
-              dA[k] = fmaf(geh, sj, dA[k]);
-              ga[j] = fmaf(geh, A[k], ga[j]);
-              G[k] *= e[t][k];
-            }
-            if (PADDED || !at.live) {
-              // lanes without a channel hold zeros already but for b and c
-              // that are not finite; states past N are never stored
-#pragma unroll
-              for (int k = 0; k < 8; ++k)
-                if (!at.live) v[k] = 0.0f;
-            }
-            Sum::run(v, lane);
-            if (Sum::stores(lane)) {
-              const int first = Sum::first(lane);
-#pragma unroll
-              for (int k = 0; k < Sum::kCount; ++k) {
-                const int f = first + k;
-                red[warp][t][(f >> 2) * NP + 4 * at.q + (f & 3)] = v[k];
-              }
-            }
-          }
-        }
-        transpose_sum<NL>(gb, at.q);
-        transpose_sum<NL>(ga, at.q);
-        const int64_t t = base + i * NL + at.q;
-        if (at.live && t < t_end) {
-          const float ds = fmaf(u[i], gb[0], ga[0]) * sig[i];
-          a.du.p[at.b * a.du.s0 + t * a.du.s1 + at.d * a.du.s2] = fmaf(s[i], gb[0], skip * dyp[i]);
-          a.ddelta.p[at.b * a.ddelta.s0 + t * a.ddelta.s1 + at.d * a.ddelta.s2] = ds;
-          sum_d = fmaf(dyp[i], u[i], sum_d);
-          sum_bias += ds;
+      for (int c = 0; c < C; ++c) {
+        transpose_sum<NL>(gb[c], at.q);
+        transpose_sum<NL>(ga[c], at.q);
+        if (at.live[c] && (FULL || base + i * NL + at.q < steps)) {
+          // A is a log2(e): its log2(e) comes off the sum here
+          const float ds = fmaf(u[c][i], gb[c][0], ga[c][0] * kLn2) * sig[c][i];
+          a.du.p[at.b * a.du.s0 + t * a.du.s1 + at.d[c] * a.du.s2] = fmaf(s[c][i], gb[c][0], skip[c] * dyp[c][i]);
+          a.ddelta.p[at.b * a.ddelta.s0 + t * a.ddelta.s1 + at.d[c] * a.ddelta.s2] = ds;
+          sum_d[c] = fmaf(dyp[c][i], u[c][i], sum_d[c]);
+          sum_bias[c] += ds;
         }
       }
-    };
-    if (base + kSteps <= t_end)
-      piece(std::true_type{});
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) dA[c][k] = add2(dA[c][k], da[c][k]);
+  };
+  const int last = steps > 0 ? (steps - 1) / TILE * TILE : -TILE;
+  if (steps > 0) {
+    stage(0, last);
+    fetch((steps - 1) / T * T);
+  }
+  int buf = 0;
+  for (int tile = last; tile >= 0; tile -= TILE, buf ^= 1) {
+    if (tile > 0)
+      stage(buf ^ 1, tile - TILE);
     else
-      piece(std::false_type{});
+      copy_commit();  // an empty group, so that the wait below counts alike
+    copy_wait<1>();
+    __syncthreads();  // b and c are there; red of the turn before is read
+    float *rows = red + warp * TILE * 2 * NP;
+#pragma unroll 1
+    for (int base = (min(tile + TILE, steps) - 1) / T * T; base >= tile; base -= T) {
+      const int off = (base - tile) * NP;
+      if (base + T <= steps)
+        piece(std::true_type{}, base, bs[buf] + off, cs[buf] + off, rows + 2 * off);
+      else
+        piece(std::false_type{}, base, bs[buf] + off, cs[buf] + off, rows + 2 * off);
+    }
     __syncthreads();
     // join the warps; a row of part_bc is one channel block's share
-    const int64_t plane = a.batch * a.length * a.groups * a.states;
-    for (int i = threadIdx.x; i < kSteps * 2 * NP; i += kScanThreads) {
+    for (int i = threadIdx.x; i < TILE * 2 * NP; i += kScanThreads) {
       const int t = i / (2 * NP), f = i % (2 * NP), n = f % NP;
-      if (base + t >= t_end || n >= a.states) continue;
+      if (tile + t >= steps || n >= a.states) continue;
       float v = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) v += red[w][t][f];
+      for (int w = 0; w < kWarps; ++w) v += red[w * TILE * 2 * NP + i];
       const bool is_c = f >= NP;
+      const int64_t tt = t0 + tile + t;
       if (a.blocks_d == 1) {
         const Op4 &o = is_c ? a.dc : a.db;
-        o.p[at.b * o.s0 + (base + t) * o.s1 + at.g * o.s2 + n * o.s3] = v;
+        o.p[at.b * o.s0 + tt * o.s1 + at.g * o.s2 + n * o.s3] = v;
       } else {
-        a.part_bc[(at.bd * 2 + is_c) * plane + ((at.b * a.length + base + t) * a.groups + at.g) * a.states + n] = v;
+        const int64_t row = ((at.bd * a.batch + at.b) * a.length + tt) * a.groups + at.g;
+        a.part_bc[(row * 2 + is_c) * a.states + n] = v;
       }
     }
   }
-  if (a.dh0.p && at.live && t0 == 0) {
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+#pragma unroll
+    for (int o = 1; o < NL; o <<= 1) {
+      sum_d[c] += __shfl_xor_sync(0xffffffffu, sum_d[c], o);
+      sum_bias[c] += __shfl_xor_sync(0xffffffffu, sum_bias[c], o);
+    }
+    if (!at.live[c]) continue;
+    const float gv[4] = {lo(G[c][0]), hi(G[c][0]), lo(G[c][1]), hi(G[c][1])};
+    const float dv[4] = {lo(dA[c][0]), hi(dA[c][0]), lo(dA[c][1]), hi(dA[c][1])};
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (k < nv) a.dh0.p[at.b * a.dh0.s0 + at.d * a.dh0.s1 + (4 * at.q + k) * a.dh0.s2] = G[k];
-  }
-#pragma unroll
-  for (int o = 1; o < NL; o <<= 1) {
-    sum_d += __shfl_xor_sync(0xffffffffu, sum_d, o);
-    sum_bias += __shfl_xor_sync(0xffffffffu, sum_bias, o);
-  }
-  if (at.live) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (k < nv) a.part_a[(prow * a.dim + at.d) * a.states + 4 * at.q + k] = dA[k];
+      if (k < nv) {
+        if (a.dh0.p && t0 == 0) a.dh0.p[at.b * a.dh0.s0 + at.d[c] * a.dh0.s1 + (4 * at.q + k) * a.dh0.s2] = gv[k];
+        a.part_a[(prow * a.dim + at.d[c]) * a.states + 4 * at.q + k] = dv[k];
+      }
     if (at.q == 0) {
-      a.part_d[prow * 2 * a.dim + at.d] = sum_d;
-      a.part_d[(prow * 2 + 1) * a.dim + at.d] = sum_bias;
+      a.part_d[prow * 2 * a.dim + at.d[c]] = sum_d[c];
+      a.part_d[(prow * 2 + 1) * a.dim + at.d[c]] = sum_bias[c];
     }
   }
 }
 
-// First pass of a cut time axis: the adjoint that leaves a piece at its start
-// when none enters at its end, and the piece's sum of steps.
-template <int NL, bool PADDED>
-__global__ void __launch_bounds__(kScanThreads) scan_adjoint_kernel(const ScanArgs a) {
-  constexpr int NP = 4 * NL;
-  constexpr int PF = kSteps / NL;
-  __shared__ __align__(16) float cs[2][kSteps * NP];
-  const Place<NL> at(a);
+// First pass of a cut time axis: the adjoint that leaves a piece of it at its
+// start when none enters at its end, and the piece's sum of steps.
+template <int NL>
+__global__ void __launch_bounds__(kScanThreads, NL > 1 ? 4 : 2) scan_adjoint_kernel(const ScanArgs a) {
+  constexpr int NP = 4 * NL, C = Bwd<NL>::kChan, T = Bwd<NL>::kPiece, TILE = Bwd<NL>::kTile;
+  constexpr int PF = T / NL;
+  __shared__ __align__(16) float cs[2][TILE * NP];
+  const Place<NL, C> at(a);
   const int64_t len = scan_length(a, at.b);
   const int64_t t0 = at.chunk * a.chunk, t_end = min(t0 + a.chunk, len);
-  if (t0 >= len && t0 > 0) return;
+  if (t0 == 0 || t0 >= len) return;  // nothing lies ahead of the first
+  const int steps = (int)(t_end - t0);
   const int nv = a.states - 4 * at.q;
-  float A2[4], G[4] = {0.0f, 0.0f, 0.0f, 0.0f}, total = 0.0f;
+  f2 A[C][2], G[C][2];
+  float bias[C], total[C];
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    A2[k] = at.live && k < nv ? a.a[at.d * a.a_d + (4 * at.q + k) * a.a_n] * kLog2e : 0.0f;
-  const float bias = a.bias ? a.bias[at.d * a.bias_s] : 0.0f;
-  const float *dp = a.delta.p + at.b * a.delta.s0 + at.d * a.delta.s2;
-  const float *zp = a.z.p + at.b * a.z.s0 + at.d * a.z.s2;
-  const float *yp = a.dy.p + at.b * a.dy.s0 + at.d * a.dy.s2;
-  float rd[PF], rz[PF], ry[PF];
-  auto fetch = [&](int64_t base) {
+  for (int c = 0; c < C; ++c) {
+    float av[4];
 #pragma unroll
-    for (int i = 0; i < PF; ++i) {
-      const int64_t t = base + i * NL + at.q;
-      const bool on = at.live && t < t_end;
-      rd[i] = on ? dp[t * a.delta.s1] : 0.0f;
-      ry[i] = on ? yp[t * a.dy.s1] : 0.0f;
-      if (a.z.p) rz[i] = on ? zp[t * a.z.s1] : 0.0f;
-    }
+    for (int k = 0; k < 4; ++k) av[k] = k < nv ? a.a[at.d[c] * a.a_d + (4 * at.q + k) * a.a_n] * kLog2e : 0.0f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) A[c][k] = pair(av[2 * k], av[2 * k + 1]), G[c][k] = 0;
+    bias[c] = a.bias ? a.bias[at.d[c] * a.bias_s] : 0.0f;
+    total[c] = 0.0f;
+  }
+  const bool gated = a.z.p != nullptr;
+  float rd[C][PF], rz[C][PF], ry[C][PF];
+  auto fetch = [&](int base) {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < PF; ++i) {
+        const bool on = base + i * NL + at.q < steps;
+        const int64_t t = t0 + base + i * NL + at.q;
+        rd[c][i] = on ? a.delta.p[at.b * a.delta.s0 + t * a.delta.s1 + at.d[c] * a.delta.s2] : 0.0f;
+        ry[c][i] = on ? a.dy.p[at.b * a.dy.s0 + t * a.dy.s1 + at.d[c] * a.dy.s2] : 0.0f;
+        rz[c][i] = gated && on ? a.z.p[at.b * a.z.s0 + t * a.z.s1 + at.d[c] * a.z.s2] : 0.0f;
+      }
   };
-  auto stage = [&](int buf, int64_t t) {
-    stage_rows<NL, kSteps>(cs[buf], a.c, a.vec_c, at.b, at.g, t, t_end, a.states);
+  auto stage = [&](int buf, int tile) {
+    stage_rows<NL, TILE>(cs[buf], a.c, a.vec_c, at.b, at.g, t0 + tile, t_end, a.states);
     copy_commit();
   };
+  auto piece = [&](auto whole, int base, const float *ct) {
+    constexpr bool FULL = decltype(whole)::value;
+    float s[C][PF], dyp[C][PF];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < PF; ++i) {
+        const float raw = rd[c][i] + bias[c];
+        float sig;
+        s[c][i] = a.softplus ? softplus(raw, &sig) : raw;
+        dyp[c][i] = gated ? ry[c][i] * (rz[c][i] * sigmoid(rz[c][i])) : ry[c][i];
+        if (FULL || base + i * NL + at.q < steps) total[c] += s[c][i];
+      }
+    if (base >= T) fetch(base - T);
+#pragma unroll
+    for (int t = T - 1; t >= 0; --t) {
+      float sj[C], dj[C];
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        sj[c] = __shfl_sync(0xffffffffu, s[c][t / NL], t % NL, NL);
+        dj[c] = __shfl_sync(0xffffffffu, dyp[c][t / NL], t % NL, NL);
+      }
+      if (FULL || base + t < steps) {
+        const ulonglong2 cc = *reinterpret_cast<const ulonglong2 *>(ct + t * NP + 4 * at.q);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const f2 sp = both(sj[c]), djp = both(dj[c]);
+          G[c][0] = mul2(fma2(cc.x, djp, G[c][0]), ex2_2(mul2(sp, A[c][0])));
+          G[c][1] = mul2(fma2(cc.y, djp, G[c][1]), ex2_2(mul2(sp, A[c][1])));
+        }
+      }
+    }
+  };
+  const int last = (steps - 1) / TILE * TILE;
+  stage(0, last);
+  fetch((steps - 1) / T * T);
   int buf = 0;
-  const int64_t last = t_end > t0 ? t0 + (t_end - 1 - t0) / kSteps * kSteps : t0 - kSteps;
-  if (last >= t0) {
-    stage(0, last);
-    fetch(last);
-  }
-  for (int64_t base = last; base >= t0; base -= kSteps, buf ^= 1) {
-    if (base - kSteps >= t0)
-      stage(buf ^ 1, base - kSteps);
+  for (int tile = last; tile >= 0; tile -= TILE, buf ^= 1) {
+    if (tile > 0)
+      stage(buf ^ 1, tile - TILE);
     else
       copy_commit();
     copy_wait<1>();
     __syncthreads();
-    float s[PF], dyp[PF];
-#pragma unroll
-    for (int i = 0; i < PF; ++i) {
-      const float raw = rd[i] + bias;
-      float sig;
-      s[i] = a.softplus ? softplus(raw, &sig) : raw;
-      dyp[i] = a.z.p ? ry[i] * (rz[i] * sigmoid(rz[i])) : ry[i];
-      if (base + i * NL + at.q < t_end) total += s[i];
+#pragma unroll 1
+    for (int base = (min(tile + TILE, steps) - 1) / T * T; base >= tile; base -= T) {
+      if (base + T <= steps)
+        piece(std::true_type{}, base, cs[buf] + (base - tile) * NP);
+      else
+        piece(std::false_type{}, base, cs[buf] + (base - tile) * NP);
     }
-    if (base - kSteps >= t0) fetch(base - kSteps);
-#pragma unroll
-    for (int i = PF - 1; i >= 0; --i)
-#pragma unroll
-      for (int j = NL - 1; j >= 0; --j) {
-        const int t = i * NL + j;
-        const float sj = __shfl_sync(0xffffffffu, s[i], j, NL);
-        const float dj = __shfl_sync(0xffffffffu, dyp[i], j, NL);
-        if (base + t < t_end) {
-          float c[4];
-          unpack(*reinterpret_cast<const float4 *>(&cs[buf][t * NP + 4 * at.q]), c);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            G[k] += PADDED && k >= nv ? 0.0f : c[k] * dj;
-            G[k] *= ex2(sj * A2[k]);
-          }
-        }
-      }
     __syncthreads();
   }
 #pragma unroll
-  for (int o = 1; o < NL; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  if (at.live) {
-    const int64_t i = (at.b * a.chunks + at.chunk) * a.dim + at.d;
-    reinterpret_cast<float4 *>(a.sum_h)[i * NL + at.q] = make_float4(G[0], G[1], G[2], G[3]);
-    if (at.q == 0) a.sum_dt[i] = total;
+  for (int c = 0; c < C; ++c) {
+#pragma unroll
+    for (int o = 1; o < NL; o <<= 1) total[c] += __shfl_xor_sync(0xffffffffu, total[c], o);
+    if (!at.live[c]) continue;
+    const int64_t i = (at.b * a.chunks + at.chunk) * a.dim + at.d[c];
+    reinterpret_cast<ulonglong2 *>(a.sum_h)[i * NL + at.q] = make_ulonglong2(G[c][0], G[c][1]);
+    if (at.q == 0) a.sum_dt[i] = total[c];
   }
 }
 
@@ -361,10 +450,12 @@ __global__ void __launch_bounds__(256) join_bc_kernel(const ScanArgs a) {
   const int64_t n = i % a.states, g = i / a.states % a.groups, bt = i / a.states / a.groups;
   const int64_t t = bt % a.length, b = bt / a.length;
   if (t >= scan_length(a, b)) return;
+  const float *p = a.part_bc + (bt * a.groups + g) * 2 * a.states + n;
   float vb = 0.0f, vc = 0.0f;
-  for (int64_t k = 0; k < a.blocks_d; ++k) {
-    vb += a.part_bc[2 * k * plane + i];
-    vc += a.part_bc[(2 * k + 1) * plane + i];
+#pragma unroll 8
+  for (int64_t k = 0; k < a.blocks_d; ++k, p += 2 * plane) {
+    vb += p[0];
+    vc += p[a.states];
   }
   a.db.p[b * a.db.s0 + t * a.db.s1 + g * a.db.s2 + n * a.db.s3] = vb;
   a.dc.p[b * a.dc.s0 + t * a.dc.s1 + g * a.dc.s2 + n * a.dc.s3] = vc;
@@ -377,10 +468,10 @@ Op3 op3(const DescView &v) {
 
 // As the forward's: pieces only where the channels give too few warps.
 void cut_time(int64_t batch, int64_t length, int64_t dim, int nl, int64_t groups, int64_t *chunks, int64_t *chunk) {
-  const int64_t per_block = kScanThreads / nl, per = dim / std::max<int64_t>(groups, 1);
+  const int64_t per_block = bwd_channels(nl), per = dim / std::max<int64_t>(groups, 1);
   const int64_t blocks = std::max<int64_t>(1, batch * groups * ((per + per_block - 1) / per_block));
   int64_t n = 1;
-  if (blocks < 148) n = std::max<int64_t>(1, std::min<int64_t>(148 * 2 / blocks, length / 64));
+  if (blocks < kCutBelow) n = std::max<int64_t>(1, std::min<int64_t>(kBlocks / blocks, length / 64));
   *chunk = std::max<int64_t>(32, ((length + n - 1) / n + 31) / 32 * 32);
   *chunks = std::max<int64_t>(1, (length + *chunk - 1) / *chunk);
 }
@@ -394,7 +485,7 @@ Layout layout_for(int64_t batch, int64_t length, int64_t dim, int states, int64_
   Layout l = {};
   const int nl = lanes_for(states);
   cut_time(batch, length, dim, nl, groups, &l.chunks, &l.chunk);
-  const int64_t per_block = kScanThreads / nl, per = dim / std::max<int64_t>(groups, 1);
+  const int64_t per_block = bwd_channels(nl), per = dim / std::max<int64_t>(groups, 1);
   const int64_t blocks_d = (per + per_block - 1) / per_block;
   size_t at = 0;
   auto take = [&](int64_t n) {
@@ -411,31 +502,30 @@ Layout layout_for(int64_t batch, int64_t length, int64_t dim, int states, int64_
   return l;
 }
 
-int launch_bwd(const ScanArgs &a, int nl, bool adjoint, cudaStream_t stream) {
+template <int NL>
+int launch_one(const ScanArgs &a, bool adjoint, cudaStream_t stream) {
   const unsigned grid = (unsigned)(a.batch * a.chunks * a.groups * a.blocks_d);
-  const bool padded = a.states != 4 * nl;
   note_launch();
-#define REMORA_SCAN_CASE(NL)                                                        \
-  case NL:                                                                          \
-    if (adjoint && padded)                                                          \
-      scan_adjoint_kernel<NL, true><<<grid, kScanThreads, 0, stream>>>(a);          \
-    else if (adjoint)                                                               \
-      scan_adjoint_kernel<NL, false><<<grid, kScanThreads, 0, stream>>>(a);         \
-    else if (padded)                                                                \
-      scan_bwd_kernel<NL, true><<<grid, kScanThreads, 0, stream>>>(a);              \
-    else                                                                            \
-      scan_bwd_kernel<NL, false><<<grid, kScanThreads, 0, stream>>>(a);             \
-    break;
-  switch (nl) {
-    REMORA_SCAN_CASE(1)
-    REMORA_SCAN_CASE(2)
-    REMORA_SCAN_CASE(4)
-    REMORA_SCAN_CASE(8)
-    REMORA_SCAN_CASE(16)
+  if (adjoint) {
+    scan_adjoint_kernel<NL><<<grid, kScanThreads, 0, stream>>>(a);
+  } else {
+    constexpr int kRed = kWarps * Bwd<NL>::kTile * 8 * NL * 4, kStatic = 4 * Bwd<NL>::kTile * 4 * NL * 4;
+    if (kRed + kStatic > 48 * 1024)
+      REMORA_CUDA_TRY(cudaFuncSetAttribute(scan_bwd_kernel<NL>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRed));
+    scan_bwd_kernel<NL><<<grid, kScanThreads, kRed, stream>>>(a);
   }
-#undef REMORA_SCAN_CASE
   REMORA_CUDA_TRY(cudaGetLastError());
   return REMORA_OK;
+}
+
+int launch_bwd(const ScanArgs &a, int nl, bool adjoint, cudaStream_t stream) {
+  switch (nl) {
+  case 1: return launch_one<1>(a, adjoint, stream);
+  case 2: return launch_one<2>(a, adjoint, stream);
+  case 4: return launch_one<4>(a, adjoint, stream);
+  case 8: return launch_one<8>(a, adjoint, stream);
+  default: return launch_one<16>(a, adjoint, stream);
+  }
 }
 
 }  // namespace
@@ -466,6 +556,8 @@ int remora_b200_selective_scan_bwd(RemoraB200Ctx *ctx, const RemoraSelectiveScan
   DescView v[10], gy, gh, o[9];
   bool has_gh, have[9];
   REMORA_TRY(read_scan_in(spec, in, &a, v, "selective_scan_bwd"));
+  const int nl = lanes_for(a.states);
+  a.blocks_d = (a.per + bwd_channels(nl) - 1) / bwd_channels(nl);
   if (grads == nullptr) return fail(REMORA_ERR_ARG, "selective_scan_bwd: null gradients");
   REMORA_TRY(read_f32(dy, 3, &gy, "selective_scan dy"));
   REMORA_TRY(read_optional(dh_last, 3, &gh, &has_gh, "selective_scan dh_last"));
@@ -500,7 +592,6 @@ int remora_b200_selective_scan_bwd(RemoraB200Ctx *ctx, const RemoraSelectiveScan
                          {given(4), "c", 4}, {given(5), "d", 4}, {given(6), "z", 4}, {given(7), "delta_bias", 4},
                          {given(8), "h0", 4}, {given(9), "lengths", 4}, {&gy, "dy", 4},
                          {has_gh ? &gh : nullptr, "dh_last", 4}}));
-  const int nl = lanes_for(a.states);
   const Layout l = layout_for(B, L, D, a.states, G);
   size_t need = 0;
   REMORA_TRY(remora_b200_selective_scan_saved(B, L, D, N, &need));
