@@ -44,8 +44,7 @@ __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 4 : 2) scan_fwd_kernel(
   const int nv = a.states - 4 * at.q;  // of the four states, those below N
   f2 A[kChan][2], h[kChan][2];
   float bias[kChan], skip[kChan], total[kChan];
-  const float *up[kChan], *dp[kChan], *zp[kChan];
-  float *yp[kChan];
+  const Lane<NL, kChan> lu(a.u, at, t0), ld(a.delta, at, t0), lz(a.z, at, t0), ly(a.y, at, t0);
 #pragma unroll
   for (int c = 0; c < kChan; ++c) {
     float av[4], hv[4];
@@ -64,23 +63,18 @@ __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 4 : 2) scan_fwd_kernel(
     bias[c] = a.bias ? a.bias[at.d[c] * a.bias_s] : 0.0f;
     skip[c] = MAIN && a.d ? a.d[at.d[c] * a.d_s] : 0.0f;
     total[c] = 0.0f;
-    // a lane's own first step
-    up[c] = a.u.p + at.b * a.u.s0 + (t0 + at.q) * a.u.s1 + at.d[c] * a.u.s2;
-    dp[c] = a.delta.p + at.b * a.delta.s0 + (t0 + at.q) * a.delta.s1 + at.d[c] * a.delta.s2;
-    zp[c] = a.z.p + at.b * a.z.s0 + (t0 + at.q) * a.z.s1 + at.d[c] * a.z.s2;
-    yp[c] = a.y.p + at.b * a.y.s0 + (t0 + at.q) * a.y.s1 + at.d[c] * a.y.s2;
   }
   const bool gated = MAIN && a.z.p != nullptr;
   float ru[kChan][PF], rd[kChan][PF], rz[kChan][PF];
-  auto fetch = [&](int base) {  // the inputs of steps base .. base + GROUP - 1 (zeros past the end), and on
+  auto fetch = [&](int base) {  // the inputs of steps base .. base + GROUP - 1, zeros past the end
     if (base + GROUP <= steps) {
 #pragma unroll
       for (int c = 0; c < kChan; ++c)
 #pragma unroll
         for (int i = 0; i < PF; ++i) {
-          ru[c][i] = up[c][i * NL * a.u.s1];
-          rd[c][i] = dp[c][i * NL * a.delta.s1];
-          if (gated) rz[c][i] = zp[c][i * NL * a.z.s1];
+          ru[c][i] = lu(c, base + i * NL);
+          rd[c][i] = ld(c, base + i * NL);
+          if (gated) rz[c][i] = lz(c, base + i * NL);
         }
     } else {
 #pragma unroll
@@ -88,16 +82,10 @@ __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 4 : 2) scan_fwd_kernel(
 #pragma unroll
         for (int i = 0; i < PF; ++i) {
           const bool on = base + i * NL + at.q < steps;
-          ru[c][i] = on ? up[c][i * NL * a.u.s1] : 0.0f;
-          rd[c][i] = on ? dp[c][i * NL * a.delta.s1] : 0.0f;
-          if (gated) rz[c][i] = on ? zp[c][i * NL * a.z.s1] : 0.0f;
+          ru[c][i] = on ? lu(c, base + i * NL) : 0.0f;
+          rd[c][i] = on ? ld(c, base + i * NL) : 0.0f;
+          if (gated) rz[c][i] = on ? lz(c, base + i * NL) : 0.0f;
         }
-    }
-#pragma unroll
-    for (int c = 0; c < kChan; ++c) {
-      up[c] += GROUP * a.u.s1;
-      dp[c] += GROUP * a.delta.s1;
-      if (gated) zp[c] += GROUP * a.z.s1;
     }
   };
   auto stage = [&](int buf, int64_t t) {
@@ -173,14 +161,10 @@ __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 4 : 2) scan_fwd_kernel(
         for (int c = 0; c < kChan; ++c) {
           transpose_sum<NL>(part[c], at.q);
           if (at.live[c] && (FULL || base + i * NL + at.q < steps)) {
-            yp[c][i * NL * a.y.s1] = (part[c][0] + y0[c][i]) * w[c][i];
+            ly(c, base + i * NL) = (part[c][0] + y0[c][i]) * w[c][i];
           }
         }
       }
-    }
-    if (MAIN) {
-#pragma unroll
-      for (int c = 0; c < kChan; ++c) yp[c] += GROUP * a.y.s1;
     }
   };
   if (steps > 0) {
@@ -516,6 +500,9 @@ int remora_b200_selective_scan_fwd(RemoraB200Ctx *ctx, const RemoraSelectiveScan
                         {{given(0), "u", 4}, {given(1), "delta", 4}, {given(2), "a", 4}, {given(3), "b", 4},
                          {given(4), "c", 4}, {given(5), "d", 4}, {given(6), "z", 4}, {given(7), "delta_bias", 4},
                          {given(8), "h0", 4}, {given(9), "lengths", 4}}, {&v[8]}));
+  for (int k : {0, 1, 6})
+    if (v[k].aligned) REMORA_TRY(check_reach(v[k], nl, kChan, "selective_scan_fwd"));
+  REMORA_TRY(check_reach(yv, nl, kChan, "selective_scan_fwd"));
   a.y = op3(yv);
   if (has_h) a.h_last = op3(hv);
   cut_time(a.batch, a.length, a.dim, a.states, a.groups, &a.chunks, &a.chunk);

@@ -67,6 +67,17 @@ struct ScanArgs {
 // Channels of a block whose threads hold `chan` channels each.
 inline int64_t block_channels(int nl, int chan) { return (int64_t)kScanThreads / nl * chan; }
 
+// Lane's 32-bit offsets reach the block's channels and a lane group's steps.
+inline int check_reach(const DescView &v, int nl, int chan, const char *what) {
+  auto size = [](int64_t x) { return x < 0 ? -x : x; };
+  const int64_t most = (int64_t)1 << 30;
+  if (size(v.strides[1]) > most || size(v.strides[2]) > most ||
+      size(v.strides[2]) * (block_channels(nl, chan) - 1) + size(v.strides[1]) * (nl - 1) >= most)
+    return fail(REMORA_ERR_LIMIT, "%s: strides of %lld and %lld elements spread a block's channels over 2^30", what,
+                (long long)v.strides[1], (long long)v.strides[2]);
+  return REMORA_OK;
+}
+
 // Lanes per channel for N states.
 inline int lanes_for(int states) {
   int nl = 1;
@@ -86,25 +97,54 @@ __device__ __forceinline__ int64_t scan_length(const ScanArgs &a, int64_t b) {
 }
 
 // The place of a thread: block = ((b * chunks + chunk) * groups + g) * blocks_d + bd.
-// Channels past the group's last stand on its first one, with live false.
+// Channels past the group's last stand on the block's first, with live false.
 template <int NL, int CHAN>
 struct Place {
+  static constexpr int kChannels = kScanThreads / NL * CHAN;  // of a block
   int64_t bd, g, chunk, b, d[CHAN];
+  int64_t first;    // the block's first channel
+  int local[CHAN];  // a channel's place in the block
   int q;
-  bool live[CHAN];
+  bool live[CHAN], whole;  // whole: the block has no dead channel
   __device__ __forceinline__ explicit Place(const ScanArgs &a) {
-    int64_t i = blockIdx.x;
-    bd = i % a.blocks_d, i /= a.blocks_d;
-    g = i % a.groups, i /= a.groups;
-    chunk = i % a.chunks, b = i / a.chunks;
+    unsigned i = blockIdx.x;
+    const unsigned groups = a.groups, blocks_d = (unsigned)a.blocks_d, chunks = (unsigned)a.chunks;
+    bd = i % blocks_d, i /= blocks_d;
+    g = i % groups, i /= groups;
+    chunk = i % chunks, b = i / chunks;
     q = threadIdx.x % NL;
+    first = g * a.per + bd * kChannels;
+    const int64_t left = a.per - bd * kChannels;
+    whole = left >= kChannels;
 #pragma unroll
     for (int c = 0; c < CHAN; ++c) {
-      const int64_t in_group = (bd * (kScanThreads / 32) + threadIdx.x / 32) * (32 / NL * CHAN) + c * (32 / NL) +
-                               threadIdx.x % 32 / NL;
-      live[c] = in_group < a.per;
-      d[c] = g * a.per + (live[c] ? in_group : 0);
+      local[c] = (threadIdx.x / 32 * CHAN + c) * (32 / NL) + threadIdx.x % 32 / NL;
+      live[c] = local[c] < left;
+      if (!live[c]) local[c] = 0;
+      d[c] = first + local[c];
     }
+  }
+};
+
+// A lane's elements of a [B, time, D] operand: a base address that the whole
+// block shares, moved along time, and a 32-bit offset per channel.  The offset
+// counts from the lowest of the block's addresses, so it is never negative.
+template <int NL, int CHAN>
+struct Lane {
+  char *base;
+  int64_t step;  // bytes per time step
+  unsigned off[CHAN];
+  __device__ __forceinline__ Lane(const Op3 &o, const Place<NL, CHAN> &at, int64_t t0) {
+    const int64_t low = (o.s2 < 0 ? o.s2 * (at.kChannels - 1) : 0) + (o.s1 < 0 ? o.s1 * (NL - 1) : 0);
+    base = reinterpret_cast<char *>(o.p + (at.b * o.s0 + t0 * o.s1 + at.first * o.s2 + low));
+    step = o.s1 * 4;
+#pragma unroll
+    for (int c = 0; c < CHAN; ++c)
+      off[c] = (unsigned)((at.local[c] * o.s2 + at.q * o.s1 - low) * 4);
+  }
+  // step t + q of channel c
+  __device__ __forceinline__ float &operator()(int c, int t) const {
+    return *reinterpret_cast<float *>(base + t * step + off[c]);
   }
 };
 

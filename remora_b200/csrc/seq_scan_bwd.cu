@@ -112,21 +112,25 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const ScanArg
   const bool gated = a.z.p != nullptr;
   float ru[C][PF], rd[C][PF], rz[C][PF], ry[C][PF];
   ulonglong2 rh[C];
-  auto fetch = [&](int base) {  // the inputs of the piece from `base` on: zeros past the end and for no channel
+  const Lane<NL, C> lu(a.u, at, t0), ld(a.delta, at, t0), lz(a.z, at, t0), ly(a.dy, at, t0);
+  const Lane<NL, C> ldu(a.du, at, t0), ldd(a.ddelta, at, t0), ldz(a.dz, at, t0);
+  // the states kept at the pieces' starts: [piece, local channel, q]
+  const ulonglong2 *hp = reinterpret_cast<const ulonglong2 *>(a.saved) +
+                         ((at.b * kept + t0 / T) * a.dim + at.first) * NL;
+  const int64_t hstep = a.dim * NL;
+  auto fetch = [&](int base) {  // the inputs of the piece from `base` on, zeros past the end
+    const bool full = base + T <= steps;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
 #pragma unroll
       for (int i = 0; i < PF; ++i) {
-        const bool on = at.live[c] && base + i * NL + at.q < steps;
-        const int64_t t = t0 + base + i * NL + at.q;
-        ru[c][i] = on ? a.u.p[at.b * a.u.s0 + t * a.u.s1 + at.d[c] * a.u.s2] : 0.0f;
-        rd[c][i] = on ? a.delta.p[at.b * a.delta.s0 + t * a.delta.s1 + at.d[c] * a.delta.s2] : 0.0f;
-        ry[c][i] = on ? a.dy.p[at.b * a.dy.s0 + t * a.dy.s1 + at.d[c] * a.dy.s2] : 0.0f;
-        rz[c][i] = gated && on ? a.z.p[at.b * a.z.s0 + t * a.z.s1 + at.d[c] * a.z.s2] : 0.0f;
+        const bool on = full || base + i * NL + at.q < steps;
+        ru[c][i] = on ? lu(c, base + i * NL) : 0.0f;
+        rd[c][i] = on ? ld(c, base + i * NL) : 0.0f;
+        ry[c][i] = on ? ly(c, base + i * NL) : 0.0f;
+        rz[c][i] = gated && on ? lz(c, base + i * NL) : 0.0f;
       }
-      rh[c] = at.live[c] ? reinterpret_cast<const ulonglong2 *>(
-                               a.saved)[((at.b * kept + (t0 + base) / T) * a.dim + at.d[c]) * NL + at.q]
-                         : make_ulonglong2(0, 0);
+      rh[c] = (hp + base / T * hstep)[(unsigned)(at.local[c] * NL + at.q)];
     }
   };
   auto stage = [&](int buf, int tile) {
@@ -156,6 +160,15 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const ScanArg
           dyp[c][i] = ry[c][i] * (rz[c][i] * sz);
           dzf[c][i] = ry[c][i] * (sz * fmaf(rz[c][i], 1.0f - sz, 1.0f));
         }
+      }
+    }
+    if (!at.whole) {  // dead channels must add nothing to the sums over channels
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        if (at.live[c]) continue;
+        h[c][0] = h[c][1] = 0;
+#pragma unroll
+        for (int i = 0; i < PF; ++i) s[c][i] = su[c][i] = dyp[c][i] = 0.0f;
       }
     }
     if (base >= T) fetch(base - T);
@@ -188,12 +201,11 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const ScanArg
         }
       }
       if (a.dz.p) {
-        const int64_t t = t0 + base + i * NL + at.q;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
           transpose_sum<NL>(part[c], at.q);
           if (at.live[c] && (FULL || base + i * NL + at.q < steps))
-            a.dz.p[at.b * a.dz.s0 + t * a.dz.s1 + at.d[c] * a.dz.s2] = dzf[c][i] * fmaf(skip[c], u[c][i], part[c][0]);
+            ldz(c, base + i * NL) = dzf[c][i] * fmaf(skip[c], u[c][i], part[c][0]);
         }
       }
     }
@@ -251,7 +263,6 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const ScanArg
           }
         }
       }
-      const int64_t t = t0 + base + i * NL + at.q;
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         transpose_sum<NL>(gb[c], at.q);
@@ -259,8 +270,8 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const ScanArg
         if (at.live[c] && (FULL || base + i * NL + at.q < steps)) {
           // A is a log2(e): its log2(e) comes off the sum here
           const float ds = fmaf(u[c][i], gb[c][0], ga[c][0] * kLn2) * sig[c][i];
-          a.du.p[at.b * a.du.s0 + t * a.du.s1 + at.d[c] * a.du.s2] = fmaf(s[c][i], gb[c][0], skip[c] * dyp[c][i]);
-          a.ddelta.p[at.b * a.ddelta.s0 + t * a.ddelta.s1 + at.d[c] * a.ddelta.s2] = ds;
+          ldu(c, base + i * NL) = fmaf(s[c][i], gb[c][0], skip[c] * dyp[c][i]);
+          ldd(c, base + i * NL) = ds;
           sum_d[c] = fmaf(dyp[c][i], u[c][i], sum_d[c]);
           sum_bias[c] += ds;
         }
@@ -362,16 +373,17 @@ __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 4 : 2) scan_adjoint_ker
   }
   const bool gated = a.z.p != nullptr;
   float rd[C][PF], rz[C][PF], ry[C][PF];
+  const Lane<NL, C> ld(a.delta, at, t0), lz(a.z, at, t0), ly(a.dy, at, t0);
   auto fetch = [&](int base) {
+    const bool full = base + T <= steps;
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int i = 0; i < PF; ++i) {
-        const bool on = base + i * NL + at.q < steps;
-        const int64_t t = t0 + base + i * NL + at.q;
-        rd[c][i] = on ? a.delta.p[at.b * a.delta.s0 + t * a.delta.s1 + at.d[c] * a.delta.s2] : 0.0f;
-        ry[c][i] = on ? a.dy.p[at.b * a.dy.s0 + t * a.dy.s1 + at.d[c] * a.dy.s2] : 0.0f;
-        rz[c][i] = gated && on ? a.z.p[at.b * a.z.s0 + t * a.z.s1 + at.d[c] * a.z.s2] : 0.0f;
+        const bool on = full || base + i * NL + at.q < steps;
+        rd[c][i] = on ? ld(c, base + i * NL) : 0.0f;
+        ry[c][i] = on ? ly(c, base + i * NL) : 0.0f;
+        rz[c][i] = gated && on ? lz(c, base + i * NL) : 0.0f;
       }
   };
   auto stage = [&](int buf, int tile) {
@@ -598,6 +610,11 @@ int remora_b200_selective_scan_bwd(RemoraB200Ctx *ctx, const RemoraSelectiveScan
   REMORA_TRY(want_scratch(saved, saved_bytes, need, "selective_scan_bwd (saved)"));
   REMORA_TRY(want_scratch(scratch, scratch_bytes, l.total * 4, "selective_scan_bwd"));
   if (D == 0) return REMORA_OK;
+  const int chan = nl > 8 ? 1 : 2;
+  for (int k : {0, 1, 6})
+    if (v[k].aligned) REMORA_TRY(check_reach(v[k], nl, chan, "selective_scan_bwd"));
+  for (const DescView *x : {&gy, &o[0], &o[1], have[6] ? &o[6] : &o[0]})
+    REMORA_TRY(check_reach(*x, nl, chan, "selective_scan_bwd"));
   a.dy = op3(gy);
   if (has_gh) a.dh_last = op3(gh);
   a.du = op3(o[0]), a.ddelta = op3(o[1]);
