@@ -129,6 +129,7 @@ __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 4 : 2) scan_fwd_kernel(
 #pragma unroll
       for (int j = 0; j < NL; ++j) {
         const int t = i * NL + j;
+        keep_order();
         float sj[kChan], suj[kChan];
 #pragma unroll
         for (int c = 0; c < kChan; ++c) {

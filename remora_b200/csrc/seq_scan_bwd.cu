@@ -178,6 +178,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const ScanArg
 #pragma unroll
       for (int j = 0; j < NL; ++j) {
         const int t = i * NL + j;
+        keep_order();
         float sj[C], suj[C];
 #pragma unroll
         for (int c = 0; c < C; ++c) {
@@ -219,6 +220,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const ScanArg
 #pragma unroll
       for (int j = NL - 1; j >= 0; --j) {
         const int t = i * NL + j;
+        keep_order();
         float sj[C], suj[C], dj[C];
 #pragma unroll
         for (int c = 0; c < C; ++c) {
@@ -406,6 +408,7 @@ __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 4 : 2) scan_adjoint_ker
     if (base >= T) fetch(base - T);
 #pragma unroll
     for (int t = T - 1; t >= 0; --t) {
+      keep_order();
       float sj[C], dj[C];
 #pragma unroll
       for (int c = 0; c < C; ++c) {
