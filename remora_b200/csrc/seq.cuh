@@ -211,6 +211,33 @@ __device__ __forceinline__ float softplus(float v, float *sig) {
   p = fmaf(q, p, 1.0f);
   return fmaxf(v, 0.0f) + 2.0f * s * p;
 }
+
+// Two f32 in a register pair, and the instructions on both at once.
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pair(float lo, float hi) {
+  f2 o;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(o) : "f"(lo), "f"(hi));
+  return o;
+}
+__device__ __forceinline__ f2 both(float v) { return pair(v, v); }
+__device__ __forceinline__ float lo(f2 v) { return __uint_as_float((unsigned)v); }
+__device__ __forceinline__ float hi(f2 v) { return __uint_as_float((unsigned)(v >> 32)); }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 o;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(o) : "l"(a), "l"(b));
+  return o;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 o;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(o) : "l"(a), "l"(b));
+  return o;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 o;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(o) : "l"(a), "l"(b), "l"(c));
+  return o;
+}
+__device__ __forceinline__ f2 ex2_2(f2 v) { return pair(ex2(lo(v)), ex2(hi(v))); }
 #endif
 
 constexpr float kLog2e = 1.4426950408889634f;

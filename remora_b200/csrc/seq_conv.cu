@@ -5,11 +5,12 @@
 //   g = dy * dy/dp;  dx[s] = sum_k w[k] g[s + W-1 - k];  dw[k] = sum_t g[t] x[t - (W-1) + k]
 //
 // Two products per tap and element against 8 bytes of HBM: bound by HBM.  A
-// thread walks a run of time steps of VEC channels (16-byte accesses where
-// every address and stride allows it) with the last W rows in registers, so
-// each row is read once but for the W-1 rows ahead of a run, which its
-// neighbour in the block has just brought into L1.
+// thread walks a run of time steps of VEC channels (8-byte accesses where
+// every address and stride allows it, 256 bytes per warp and row) with the last
+// W rows in registers, so each row is read once but for the W-1 rows ahead of
+// a run, which its neighbour in the block has just brought into L1.
 #include <algorithm>
+#include <type_traits>
 
 #include "seq.cuh"
 
@@ -19,7 +20,14 @@ namespace {
 
 constexpr int kMinWidth = 2, kMaxWidth = 8;
 constexpr int kLanes = 32;  // threads along the channels
-constexpr int kRuns = 8;    // runs of time steps per block
+constexpr int kRuns = 4;    // runs of time steps per block
+// Rows that a thread loads together while it works on as many, and channels of
+// a thread where rows are aligned for it.  Forward of 1 x 8192 x 4096: 47 us
+// with 8 rows of 2 channels, 55 with 4 of 4, 54 with 4 of 2.  Backward of 8 x
+// 2048 x 4096: 165 us with 4 of 2 at 6 blocks per SM, 180 with 2 of 4, 191 with
+// 4 of 1.
+constexpr int kFwdRows = 8, kBwdRows = 4;
+constexpr int kVec = 2;
 
 struct Op3 {  // [B, time, D]
   float *p;
@@ -56,6 +64,9 @@ __device__ __forceinline__ Vec<VEC> load(const float *p) {
   if constexpr (VEC == 4) {
     const float4 q = *reinterpret_cast<const float4 *>(p);
     o.v[0] = q.x, o.v[1] = q.y, o.v[2] = q.z, o.v[3] = q.w;
+  } else if constexpr (VEC == 2) {
+    const float2 q = *reinterpret_cast<const float2 *>(p);
+    o.v[0] = q.x, o.v[1] = q.y;
   } else {
     o.v[0] = *p;
   }
@@ -66,8 +77,18 @@ template <int VEC>
 __device__ __forceinline__ void store(float *p, const Vec<VEC> &o) {
   if constexpr (VEC == 4)
     *reinterpret_cast<float4 *>(p) = make_float4(o.v[0], o.v[1], o.v[2], o.v[3]);
+  else if constexpr (VEC == 2)
+    *reinterpret_cast<float2 *>(p) = make_float2(o.v[0], o.v[1]);
   else
     *p = o.v[0];
+}
+
+template <int VEC>
+__device__ __forceinline__ Vec<VEC> fma(const Vec<VEC> &a, const Vec<VEC> &b, const Vec<VEC> &c) {
+  Vec<VEC> o;
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) o.v[j] = fmaf(a.v[j], b.v[j], c.v[j]);
+  return o;
 }
 
 template <int VEC>
@@ -116,11 +137,11 @@ __global__ void __launch_bounds__(kLanes *kRuns) conv_fwd_kernel(const ConvArgs 
   auto step = [&](const Vec<VEC> &now) {
     Vec<VEC> o = bias;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
+    for (int k = 0; k < W - 1; ++k) o = fma(w[k], win[k], o);
+    o = fma(w[W - 1], now, o);
+    if (a.silu) {
 #pragma unroll
-      for (int k = 0; k < W - 1; ++k) o.v[j] = fmaf(w[k].v[j], win[k].v[j], o.v[j]);
-      o.v[j] = fmaf(w[W - 1].v[j], now.v[j], o.v[j]);
-      if (a.silu) o.v[j] *= sigmoid(o.v[j]);
+      for (int j = 0; j < VEC; ++j) o.v[j] *= sigmoid(o.v[j]);
     }
     store<VEC>(y, o);
     y += a.y.t;
@@ -128,13 +149,22 @@ __global__ void __launch_bounds__(kLanes *kRuns) conv_fwd_kernel(const ConvArgs 
     for (int k = 0; k + 1 < W - 1; ++k) win[k] = win[k + 1];
     win[W - 2] = now;
   };
+  // the next U rows are on their way while the last U are worked on
+  constexpr int U = kFwdRows;
+  Vec<VEC> r[U], n[U];
   int64_t t = t0;
-  constexpr int U = 8;  // rows in flight per thread
-  for (; t + U <= t1; t += U) {
-    Vec<VEC> r[U];
+  if (t + U <= t1) {
 #pragma unroll
-    for (int k = 0; k < U; ++k) r[k] = load<VEC>(x + k * a.x.t);
+    for (int k = 0; k < U; ++k) n[k] = load<VEC>(x + k * a.x.t);
+  }
+  for (; t + U <= t1; t += U) {
     x += U * a.x.t;
+#pragma unroll
+    for (int k = 0; k < U; ++k) r[k] = n[k];
+    if (t + 2 * U <= t1) {
+#pragma unroll
+      for (int k = 0; k < U; ++k) n[k] = load<VEC>(x + k * a.x.t);
+    }
 #pragma unroll
     for (int k = 0; k < U; ++k) step(r[k]);
   }
@@ -152,7 +182,7 @@ __global__ void __launch_bounds__(kLanes *kRuns) conv_fwd_kernel(const ConvArgs 
 // A run of rows s in [t0, t0 + run) of dx needs g[s .. s + W-1]: the walk goes
 // W-1 steps past the run, and dw takes the steps inside it only.
 template <int W, int VEC>
-__global__ void __launch_bounds__(kLanes *kRuns) conv_bwd_kernel(const ConvArgs a) {
+__global__ void __launch_bounds__(kLanes *kRuns, W <= 4 ? 6 : W <= 6 ? 4 : 3) conv_bwd_kernel(const ConvArgs a) {
   __shared__ float sum[kRuns][kLanes * VEC];
   const int64_t bd = blockIdx.x % a.blocks_d, rest = blockIdx.x / a.blocks_d;
   const int64_t bt = rest % a.blocks_t, b = rest / a.blocks_t;
@@ -177,59 +207,73 @@ __global__ void __launch_bounds__(kLanes *kRuns) conv_bwd_kernel(const ConvArgs 
     for (int k = 0; k < W - 1; ++k) win[k + 1] = row_at<W, VEC>(a, b, t0 - (W - 1) + k, d);
     const float *x = a.x.p + b * a.x.b + d * a.x.d;
     const float *dy = a.dy.p + b * a.dy.b + d * a.dy.d;
-    auto step = [&](int64_t t, const Vec<VEC> &xr, const Vec<VEC> &gr) {
+    float *dxp = a.dx.p + b * a.dx.b + d * a.dx.d + (t0 - (W - 1)) * a.dx.t;  // row t - (W-1)
+    // One step.  INNER: t lies in the run, W-1 steps or more behind its start;
+    // otherwise the step may lie past the run's or the sequence's end, and its
+    // row of dx ahead of the run, in the state or in state_out.
+    auto step = [&](auto inner, int64_t t, const Vec<VEC> &xr, const Vec<VEC> &gr) {
+      constexpr bool INNER = decltype(inner)::value;
 #pragma unroll
       for (int k = 0; k + 1 < W; ++k) win[k] = win[k + 1], g[k] = g[k + 1];
       win[W - 1] = xr;
       Vec<VEC> now = gr, o = zero<VEC>();
+      if (a.silu) {
+        Vec<VEC> p = bias;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        if (a.silu) {
-          float p = bias.v[j];
+        for (int k = 0; k < W; ++k) p = fma(w[k], win[k], p);
 #pragma unroll
-          for (int k = 0; k < W; ++k) p = fmaf(w[k].v[j], win[k].v[j], p);
-          const float s = sigmoid(p);
-          now.v[j] *= s * fmaf(p, 1.0f - s, 1.0f);
+        for (int j = 0; j < VEC; ++j) {
+          const float s = sigmoid(p.v[j]);
+          now.v[j] *= s * fmaf(p.v[j], 1.0f - s, 1.0f);
         }
-        if (t >= len) now.v[j] = 0.0f;  // whatever a NaN in the window made of it
-        if (t < t1) {
+      }
+      if (!INNER && t >= len) now = zero<VEC>();  // whatever a NaN in the window made of it
+      if (INNER || t < t1) {
 #pragma unroll
-          for (int k = 0; k < W; ++k) dw[k].v[j] = fmaf(now.v[j], win[k].v[j], dw[k].v[j]);
-          db.v[j] += now.v[j];
-        }
+        for (int k = 0; k < W; ++k) dw[k] = fma(now, win[k], dw[k]);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) db.v[j] += now.v[j];
       }
       g[W - 1] = now;
       const int64_t s = t - (W - 1);
       // rows ahead of the run belong to the run before, or to the state
-      if (s >= t0 || (t0 == 0 && a.dstate.p != nullptr)) {
+      if (INNER || s >= t0 || (t0 == 0 && a.dstate.p != nullptr)) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j)
-#pragma unroll
-          for (int k = 0; k < W; ++k) o.v[j] = fmaf(w[k].v[j], g[W - 1 - k].v[j], o.v[j]);
-        const int64_t i = s - len + (W - 1);  // the row of state_out that is this row
-        if (a.dstate_out.p != nullptr && i >= 0) {
-          const Vec<VEC> e = load<VEC>(a.dstate_out.p + b * a.dstate_out.b + i * a.dstate_out.t + d * a.dstate_out.d);
+        for (int k = 0; k < W; ++k) o = fma(w[k], g[W - 1 - k], o);
+        if (!INNER && a.dstate_out.p != nullptr && t >= len) {  // this row is row t - len of state_out
+          const Vec<VEC> e =
+              load<VEC>(a.dstate_out.p + b * a.dstate_out.b + (t - len) * a.dstate_out.t + d * a.dstate_out.d);
 #pragma unroll
           for (int j = 0; j < VEC; ++j) o.v[j] += e.v[j];
         }
-        if (s >= 0)
-          store<VEC>(a.dx.p + b * a.dx.b + s * a.dx.t + d * a.dx.d, o);
+        if (INNER || s >= 0)
+          store<VEC>(dxp, o);
         else
           store<VEC>(a.dstate.p + b * a.dstate.b + (s + W - 1) * a.dstate.t + d * a.dstate.d, o);
       }
+      dxp += a.dx.t;
     };
-    int64_t t = t0;
-    constexpr int U = 4;  // rows of x and of dy in flight per thread
+    using Inner = std::true_type;
+    using Edge = std::false_type;
     const int64_t end = t1 + W - 1, full = min(end, len);
-    for (; t + U <= full; t += U) {
-      Vec<VEC> xr[U], gr[U];
+    int64_t t = t0;
+    for (; t < min(t0 + W - 1, full); ++t) step(Edge{}, t, load<VEC>(x + t * a.x.t), load<VEC>(dy + t * a.dy.t));
+    constexpr int U = kBwdRows;
+    Vec<VEC> xr[U], gr[U], xn[U], gn[U];
+    auto fetch = [&](int64_t at) {
 #pragma unroll
-      for (int k = 0; k < U; ++k) xr[k] = load<VEC>(x + (t + k) * a.x.t), gr[k] = load<VEC>(dy + (t + k) * a.dy.t);
+      for (int k = 0; k < U; ++k) xn[k] = load<VEC>(x + (at + k) * a.x.t), gn[k] = load<VEC>(dy + (at + k) * a.dy.t);
+    };
+    if (t + U <= t1) fetch(t);
+    for (; t + U <= t1; t += U) {
 #pragma unroll
-      for (int k = 0; k < U; ++k) step(t + k, xr[k], gr[k]);
+      for (int k = 0; k < U; ++k) xr[k] = xn[k], gr[k] = gn[k];
+      if (t + 2 * U <= t1) fetch(t + U);
+#pragma unroll
+      for (int k = 0; k < U; ++k) step(Inner{}, t + k, xr[k], gr[k]);
     }
-    for (; t < full; ++t) step(t, load<VEC>(x + t * a.x.t), load<VEC>(dy + t * a.dy.t));
-    for (; t < end; ++t) step(t, zero<VEC>(), zero<VEC>());
+    for (; t < full; ++t) step(Edge{}, t, load<VEC>(x + t * a.x.t), load<VEC>(dy + t * a.dy.t));
+    for (; t < end; ++t) step(Edge{}, t, zero<VEC>(), zero<VEC>());
   }
   // the block's runs, joined in their order
 #pragma unroll
@@ -294,30 +338,35 @@ __global__ void __launch_bounds__(128) conv_step_kernel(const StepArgs a) {
 }
 
 // ------------------------------------------------------------------ host --
-// Time steps per thread: longer runs read fewer rows twice ((W-1) / run),
-// shorter ones keep the device full when there are few rows.
-int run_for(int64_t batch, int64_t length, int64_t dim, int vec) {
-  int run = 32;
+// Time steps per thread, `most` at most: longer runs read fewer rows twice
+// ((W-1) / run), shorter ones keep the device full when there are few rows.
+// On 8 x 2048 x 4096: forward 83 us with 32 steps and 84 with 64, backward
+// 165 with 32 and 152 with 64 or 128.
+constexpr int kFwdRun = 32, kBwdRun = 64;
+
+int run_for(int most, int64_t batch, int64_t length, int64_t dim, int vec) {
+  int run = most;
   while (run > 8 && batch * ((length + run - 1) / run) * ((dim + vec - 1) / vec) < 148 * 1024) run /= 2;
   return run;
 }
 
-bool vec_rows(const DescView &v) {
+// Whether every row can be read `vec` channels at a time.
+bool vec_rows(const DescView &v, int vec) {
   if (v.sizes[v.rank - 1] > 1 && v.strides[v.rank - 1] != 1) return false;
-  if (reinterpret_cast<uintptr_t>(v.data(4)) & 15) return false;
+  if (reinterpret_cast<uintptr_t>(v.data(4)) % (4 * vec)) return false;
   for (int d = 0; d < v.rank - 1; ++d)
-    if (v.sizes[d] > 1 && (v.strides[d] & 3)) return false;
+    if (v.sizes[d] > 1 && v.strides[d] % vec) return false;
   return true;
 }
 
-template <int VEC>
-int launch_conv(int width, bool bwd, const ConvArgs &a, cudaStream_t stream) {
+template <int VEC, bool BWD>
+int launch_conv(int width, const ConvArgs &a, cudaStream_t stream) {
   const unsigned grid = (unsigned)(a.batch * a.blocks_t * a.blocks_d);
   const dim3 block(kLanes, kRuns);
   note_launch();
 #define REMORA_CONV_CASE(W)                                    \
   case W:                                                      \
-    if (bwd)                                                   \
+    if constexpr (BWD)                                         \
       conv_bwd_kernel<W, VEC><<<grid, block, 0, stream>>>(a);  \
     else                                                       \
       conv_fwd_kernel<W, VEC><<<grid, block, 0, stream>>>(a);  \
@@ -365,12 +414,12 @@ int check_width(int64_t width, const char *what) {
 // The grid is sized for the shorter runs, so the size does not depend on the
 // alignment of the operands.
 int64_t bwd_parts(int64_t batch, int64_t length, int64_t dim) {
-  const int run = std::min(run_for(batch, length, dim, 1), run_for(batch, length, dim, 4));
+  const int run = std::min(run_for(kBwdRun, batch, length, dim, 1), run_for(kBwdRun, batch, length, dim, kVec));
   return batch * std::max<int64_t>(1, (length + (int64_t)run * kRuns - 1) / ((int64_t)run * kRuns));
 }
 
-int set_grid(ConvArgs &a, int vec, const char *what) {
-  a.run = run_for(a.batch, a.length, a.dim, vec);
+int set_grid(ConvArgs &a, int most, int vec, const char *what) {
+  a.run = run_for(most, a.batch, a.length, a.dim, vec);
   a.blocks_d = (a.dim + kLanes * vec - 1) / (kLanes * vec);
   a.blocks_t = std::max<int64_t>(1, (a.length + (int64_t)a.run * kRuns - 1) / ((int64_t)a.run * kRuns));
   if (a.batch * a.blocks_t * a.blocks_d > 0x7fffffff) return fail(REMORA_ERR_LIMIT, "%s: too many blocks", what);
@@ -424,12 +473,14 @@ int remora_b200_causal_conv_fwd(RemoraB200Ctx *ctx, const RemoraCausalConvSpec *
   if (has_b) a.bias = reinterpret_cast<const float *>(bv.data(4)), a.bias_d = bv.strides[0];
   if (has_l) a.lengths = reinterpret_cast<const int *>(lv.data(4)), a.lengths_b = lv.strides[0];
   a.batch = B, a.length = L, a.dim = D, a.silu = spec->silu != 0;
-  const bool vec = D % 4 == 0 && vec_rows(xv) && vec_rows(yv) && (!has_s || vec_rows(sv)) && (!has_o || vec_rows(ov));
-  REMORA_TRY(set_grid(a, vec ? 4 : 1, "causal_conv_fwd"));
+  constexpr int V = kVec;
+  const bool vec = D % V == 0 && vec_rows(xv, V) && vec_rows(yv, V) && (!has_s || vec_rows(sv, V)) &&
+                   (!has_o || vec_rows(ov, V));
+  REMORA_TRY(set_grid(a, kFwdRun, vec ? V : 1, "causal_conv_fwd"));
   DeviceGuard guard;
   REMORA_TRY(guard.enter(ctx));
-  return vec ? launch_conv<4>((int)W, false, a, (cudaStream_t)stream)
-             : launch_conv<1>((int)W, false, a, (cudaStream_t)stream);
+  return vec ? launch_conv<V, false>((int)W, a, (cudaStream_t)stream)
+             : launch_conv<1, false>((int)W, a, (cudaStream_t)stream);
 }
 
 int remora_b200_causal_conv_bwd_scratch(RemoraB200Ctx *ctx, int64_t batch, int64_t length, int64_t dim, int64_t width,
@@ -492,13 +543,14 @@ int remora_b200_causal_conv_bwd(RemoraB200Ctx *ctx, const RemoraCausalConvSpec *
   if (has_l) a.lengths = reinterpret_cast<const int *>(lv.data(4)), a.lengths_b = lv.strides[0];
   a.batch = B, a.length = L, a.dim = D, a.silu = spec->silu != 0;
   a.part = static_cast<float *>(scratch);
-  const bool vec = D % 4 == 0 && vec_rows(xv) && vec_rows(gv) && vec_rows(dxv) && (!has_s || vec_rows(sv)) &&
-                   (!has_e || vec_rows(ev)) && (!has_ds || vec_rows(dsv));
-  REMORA_TRY(set_grid(a, vec ? 4 : 1, "causal_conv_bwd"));
+  constexpr int V = kVec;
+  const bool vec = D % V == 0 && vec_rows(xv, V) && vec_rows(gv, V) && vec_rows(dxv, V) &&
+                   (!has_s || vec_rows(sv, V)) && (!has_e || vec_rows(ev, V)) && (!has_ds || vec_rows(dsv, V));
+  REMORA_TRY(set_grid(a, kBwdRun, vec ? V : 1, "causal_conv_bwd"));
   DeviceGuard guard;
   REMORA_TRY(guard.enter(ctx));
   if (B > 0)
-    REMORA_TRY(vec ? launch_conv<4>((int)W, true, a, stream) : launch_conv<1>((int)W, true, a, stream));
+    REMORA_TRY((vec ? launch_conv<V, true>((int)W, a, stream) : launch_conv<1, true>((int)W, a, stream)));
   // a row of part: W rows of dw and one of dbias, each over the channels
   const Columns to = {reinterpret_cast<float *>(dwv.data(4)), D, dwv.strides[1], dwv.strides[0], W * D,
                       has_db ? reinterpret_cast<float *>(dbv.data(4)) : nullptr, has_db ? dbv.strides[0] : 0};
@@ -543,7 +595,7 @@ int remora_b200_causal_conv_step(RemoraB200Ctx *ctx, const RemoraCausalConvSpec 
   if (has_b) a.bias = reinterpret_cast<const float *>(bv.data(4)), a.bias_d = bv.strides[0];
   if (has_l) a.slots = reinterpret_cast<const int *>(lv.data(4)), a.slots_b = lv.strides[0];
   a.rows = S, a.dim = D, a.silu = spec->silu != 0;
-  const bool vec = D % 4 == 0 && vec_rows(xv) && vec_rows(yv) && vec_rows(sv) && vec_rows(ov);
+  const bool vec = D % 4 == 0 && vec_rows(xv, 4) && vec_rows(yv, 4) && vec_rows(sv, 4) && vec_rows(ov, 4);
   DeviceGuard guard;
   REMORA_TRY(guard.enter(ctx));
   return vec ? launch_step<4>((int)W, B, a, (cudaStream_t)stream) : launch_step<1>((int)W, B, a, (cudaStream_t)stream);

@@ -254,6 +254,8 @@ __global__ void __launch_bounds__(256) scan_combine_kernel(const ScanArgs a, int
   }
 }
 
+constexpr int64_t kManyBlocks = 148 * 4;
+
 struct TokenArgs {
   Op3 state, state_out, b, c;  // b, c: [B, G, N]
   const float *u, *delta, *z, *a, *d, *bias;
@@ -262,72 +264,99 @@ struct TokenArgs {
   const int *slots;
   int64_t slots_s;
   int64_t batch, rows, dim, per;
-  int states, softplus, vec;
+  int states, groups, softplus, vec;
 };
 
-// Four states of one channel and row per thread; bound by the states' bytes.
-template <int NL>
+// Four states of one channel per thread, of R batch rows, R either 1 or NL.
+// Bound by the states' bytes: with R = NL the decay rates are read once for R
+// rows, R states are on their way at once, and what belongs to a row and
+// channel alone (the step, the gate, y) is worked out by one of the NL lanes.
+template <int NL, int R>
 __global__ void __launch_bounds__(kScanThreads) scan_step_kernel(const TokenArgs a) {
-  const int64_t i = blockIdx.y;
-  int64_t slot = i;
-  bool live = true;
-  if (a.slots != nullptr) {
-    slot = a.slots[i * a.slots_s];
-    bool again = false;
-    for (int64_t k = threadIdx.x; k < i; k += kScanThreads) again |= a.slots[k * a.slots_s] == slot;
-    live = !__syncthreads_or(again) && slot >= 0 && slot < a.rows;
-  }
+  const int64_t i0 = (int64_t)blockIdx.y * R;
   const int q = threadIdx.x % NL;
   const int64_t d = (int64_t)blockIdx.x * (kScanThreads / NL) + threadIdx.x / NL;
-  live = live && d < a.dim;
-  const int nv = live ? a.states - 4 * q : 0;
-  float sum = 0.0f, u = 0.0f;
-  if (live) {
-    const int64_t g = d / a.per;
-    const float *hp = a.state.p + slot * a.state.s0 + d * a.state.s1 + 4 * q * a.state.s2;
-    const float *ap = a.a + d * a.a_d + 4 * q * a.a_n;
-    const float *bp = a.b.p + i * a.b.s0 + g * a.b.s1 + 4 * q * a.b.s2;
-    const float *cp = a.c.p + i * a.c.s0 + g * a.c.s1 + 4 * q * a.c.s2;
-    float h[4], A[4], b[4], c[4];
-    if (a.vec) {
-      if (nv > 0) {
-        unpack(*reinterpret_cast<const float4 *>(hp), h);
-        unpack(*reinterpret_cast<const float4 *>(ap), A);
-        unpack(*reinterpret_cast<const float4 *>(bp), b);
-        unpack(*reinterpret_cast<const float4 *>(cp), c);
-      }
-    } else {
+  int64_t slot[R];
+  bool on[R];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (k < nv) h[k] = hp[k * a.state.s2], A[k] = ap[k * a.a_n], b[k] = bp[k * a.b.s2], c[k] = cp[k * a.c.s2];
+  for (int r = 0; r < R; ++r) {
+    const int64_t i = i0 + r;
+    slot[r] = i;
+    on[r] = i < a.batch;
+    if (a.slots != nullptr) {
+      slot[r] = on[r] ? a.slots[i * a.slots_s] : -1;
+      bool again = false;
+      for (int64_t k = threadIdx.x; k < i && on[r]; k += kScanThreads) again |= a.slots[k * a.slots_s] == slot[r];
+      on[r] = !__syncthreads_or(again) && slot[r] >= 0 && slot[r] < a.rows;
     }
-    u = a.u[i * a.u_b + d * a.u_d];
-    float s = a.delta[i * a.delta_b + d * a.delta_d] + (a.bias ? a.bias[d * a.bias_s] : 0.0f), sig;
-    if (a.softplus) s = softplus(s, &sig);
-    const float su = s * u;
+    on[r] = on[r] && d < a.dim;
+  }
+  const int own = R > 1 ? q : 0;  // the row whose per-channel values this lane has
+  const int64_t i = i0 + own;
+  bool mine = false;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (k < nv) {
-        h[k] = fmaf(ex2(s * (A[k] * kLog2e)), h[k], su * b[k]);
-        sum = fmaf(h[k], c[k], sum);
-      }
-    float *ho = a.state_out.p + slot * a.state_out.s0 + d * a.state_out.s1 + 4 * q * a.state_out.s2;
+  for (int r = 0; r < R; ++r) mine = r == own ? on[r] : mine;
+  const int nv = d < a.dim ? a.states - 4 * q : 0;
+  const int64_t g = a.groups == 1 ? 0 : (unsigned)d / (unsigned)a.per;
+  float h[R][4], b[R][4], c[R][4], A[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  auto get = [&](const float *p, int64_t stride, float (&v)[4]) {
     if (a.vec) {
-      if (nv > 0) *reinterpret_cast<float4 *>(ho) = make_float4(h[0], h[1], h[2], h[3]);
+      unpack(*reinterpret_cast<const float4 *>(p), v);
     } else {
 #pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = k < nv ? p[k * stride] : 0.0f;
+    }
+  };
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (on[r] && nv > 0) get(a.state.p + slot[r] * a.state.s0 + d * a.state.s1 + 4 * q * a.state.s2, a.state.s2, h[r]);
+  float u = 0.0f, s = 0.0f, z = 0.0f, sig;
+  if (mine) {
+    u = a.u[i * a.u_b + d * a.u_d];
+    s = a.delta[i * a.delta_b + d * a.delta_d] + (a.bias ? a.bias[d * a.bias_s] : 0.0f);
+    if (a.z) z = a.z[i * a.z_b + d * a.z_d];
+  }
+  if (nv > 0) get(a.a + d * a.a_d + 4 * q * a.a_n, a.a_n, A);
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (on[r] && nv > 0) {
+      get(a.b.p + (i0 + r) * a.b.s0 + g * a.b.s1 + 4 * q * a.b.s2, a.b.s2, b[r]);
+      get(a.c.p + (i0 + r) * a.c.s0 + g * a.c.s1 + 4 * q * a.c.s2, a.c.s2, c[r]);
+    }
+  if (a.softplus) s = softplus(s, &sig);
+  const float su = s * u;
+  float part[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float sr = R > 1 ? __shfl_sync(0xffffffffu, s, r, NL) : s;
+    const float sur = R > 1 ? __shfl_sync(0xffffffffu, su, r, NL) : su;
+    part[r] = 0.0f;
+    if (on[r] && nv > 0) {
+#pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (k < nv) ho[k * a.state_out.s2] = h[k];
+        if (k < nv) {
+          h[r][k] = fmaf(ex2(sr * (A[k] * kLog2e)), h[r][k], sur * b[r][k]);
+          part[r] = fmaf(h[r][k], c[r][k], part[r]);
+        }
+      float *o = a.state_out.p + slot[r] * a.state_out.s0 + d * a.state_out.s1 + 4 * q * a.state_out.s2;
+      if (a.vec) {
+        *reinterpret_cast<float4 *>(o) = make_float4(h[r][0], h[r][1], h[r][2], h[r][3]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k < nv) o[k * a.state_out.s2] = h[r][k];
+      }
     }
   }
+  if constexpr (R > 1) {
+    transpose_sum<NL>(part, q);
+  } else {
 #pragma unroll
-  for (int o = 1; o < NL; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (live && q == 0) {
-    float y = fmaf(a.d ? a.d[d * a.d_s] : 0.0f, u, sum);
-    if (a.z) {
-      const float z = a.z[i * a.z_b + d * a.z_d];
-      y *= z * sigmoid(z);
-    }
+    for (int o = 1; o < NL; o <<= 1) part[0] += __shfl_xor_sync(0xffffffffu, part[0], o);
+  }
+  if (mine && (R > 1 || q == 0)) {
+    float y = fmaf(a.d ? a.d[d * a.d_s] : 0.0f, u, part[0]);
+    if (a.z) y *= z * sigmoid(z);
     a.y[i * a.y_b + d * a.y_d] = y;
   }
 }
@@ -579,21 +608,34 @@ int remora_b200_selective_scan_step(RemoraB200Ctx *ctx, const RemoraSelectiveSca
   if (has_i) a.bias = reinterpret_cast<const float *>(iv.data(4)), a.bias_s = iv.strides[0];
   if (has_l) a.slots = reinterpret_cast<const int *>(lv.data(4)), a.slots_s = lv.strides[0];
   a.y = reinterpret_cast<float *>(yv.data(4)), a.y_b = yv.strides[0], a.y_d = yv.strides[1];
-  a.batch = B, a.rows = S, a.dim = D, a.per = D / G, a.states = (int)N, a.softplus = spec->softplus != 0;
+  a.batch = B, a.rows = S, a.dim = D, a.per = D / G, a.states = (int)N, a.groups = (int)G;
+  a.softplus = spec->softplus != 0;
   a.vec = vec_states(sv) && vec_states(ov) && vec_states(av) && vec_states(bv) && vec_states(cv);
   const int nl = lanes_for(a.states);
-  const dim3 grid((unsigned)((D + kScanThreads / nl - 1) / (kScanThreads / nl)), (unsigned)B);
+  if (D > 0x7fffffff) return fail(REMORA_ERR_LIMIT, "selective_scan_step: more than 2^31 - 1 channels");
+  // R = NL rows per thread once that leaves every SM some blocks
+  const int64_t blocks = (D + kScanThreads / nl - 1) / (kScanThreads / nl);
+  const bool many = nl > 1 && blocks * (B / nl) >= kManyBlocks;
+  const dim3 grid((unsigned)blocks, (unsigned)(many ? (B + nl - 1) / nl : B));
   DeviceGuard guard;
   REMORA_TRY(guard.enter(ctx));
   cudaStream_t s = (cudaStream_t)stream;
   note_launch();
+#define REMORA_STEP_CASE(NL)                                        \
+  case NL:                                                          \
+    if (many)                                                       \
+      scan_step_kernel<NL, NL><<<grid, kScanThreads, 0, s>>>(a);    \
+    else                                                            \
+      scan_step_kernel<NL, 1><<<grid, kScanThreads, 0, s>>>(a);     \
+    break;
   switch (nl) {
-  case 1: scan_step_kernel<1><<<grid, kScanThreads, 0, s>>>(a); break;
-  case 2: scan_step_kernel<2><<<grid, kScanThreads, 0, s>>>(a); break;
-  case 4: scan_step_kernel<4><<<grid, kScanThreads, 0, s>>>(a); break;
-  case 8: scan_step_kernel<8><<<grid, kScanThreads, 0, s>>>(a); break;
-  default: scan_step_kernel<16><<<grid, kScanThreads, 0, s>>>(a); break;
+  case 1: scan_step_kernel<1, 1><<<grid, kScanThreads, 0, s>>>(a); break;
+    REMORA_STEP_CASE(2)
+    REMORA_STEP_CASE(4)
+    REMORA_STEP_CASE(8)
+    REMORA_STEP_CASE(16)
   }
+#undef REMORA_STEP_CASE
   REMORA_CUDA_TRY(cudaGetLastError());
   return REMORA_OK;
 }
