@@ -13,6 +13,7 @@
 // kernel joins them, and the main pass starts each piece from its own state.
 // That doubles the exponentials, so pieces are as few as fill the device.
 #include <algorithm>
+#include <cstdlib>
 #include <type_traits>
 
 #include "seq_scan.cuh"
@@ -256,14 +257,22 @@ __global__ void __launch_bounds__(256) scan_combine_kernel(const ScanArgs a, int
 
 constexpr int64_t kManyBlocks = 148 * 4;
 
+// An operand of one token per row and its strides along up to three axes.
+// They are 32-bit, so that an index times a stride, a 64-bit sum, is one
+// instruction; the host refuses larger ones.
+struct Token {
+  float *p;
+  int s0, s1, s2;
+  __device__ __forceinline__ float *operator()(int i, int j, int k) const {
+    return p + ((int64_t)i * s0 + (int64_t)j * s1 + (int64_t)k * s2);
+  }
+};
+
 struct TokenArgs {
-  Op3 state, state_out, b, c;  // b, c: [B, G, N]
-  const float *u, *delta, *z, *a, *d, *bias;
-  float *y;
-  int64_t u_b, u_d, delta_b, delta_d, z_b, z_d, y_b, y_d, a_d, a_n, d_s, bias_s;
+  Token state, state_out, b, c, a, u, delta, z, y, d, bias;
   const int *slots;
-  int64_t slots_s;
-  int64_t batch, rows, dim, per;
+  int slots_s;
+  int batch, rows, dim, per;
   int states, groups, softplus, vec;
 };
 
@@ -272,60 +281,61 @@ struct TokenArgs {
 // rows, R states are on their way at once, and what belongs to a row and
 // channel alone (the step, the gate, y) is worked out by one of the NL lanes.
 template <int NL, int R>
-__global__ void __launch_bounds__(kScanThreads) scan_step_kernel(const TokenArgs a) {
-  const int64_t i0 = (int64_t)blockIdx.y * R;
-  const int q = threadIdx.x % NL;
-  const int64_t d = (int64_t)blockIdx.x * (kScanThreads / NL) + threadIdx.x / NL;
-  int64_t slot[R];
+__global__ void __launch_bounds__(kScanThreads, NL > 4 ? 2 : 7) scan_step_kernel(const TokenArgs a) {
+  const int i0 = (int)blockIdx.y * R;
+  const int q = threadIdx.x % NL, d = (int)blockIdx.x * (kScanThreads / NL) + threadIdx.x / NL;
+  int slot[R];
   bool on[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int64_t i = i0 + r;
+    const int i = i0 + r;
     slot[r] = i;
     on[r] = i < a.batch;
     if (a.slots != nullptr) {
-      slot[r] = on[r] ? a.slots[i * a.slots_s] : -1;
+      slot[r] = on[r] ? a.slots[(int64_t)i * a.slots_s] : -1;
       bool again = false;
-      for (int64_t k = threadIdx.x; k < i && on[r]; k += kScanThreads) again |= a.slots[k * a.slots_s] == slot[r];
+      for (int k = threadIdx.x; k < i && on[r]; k += kScanThreads)
+        again |= a.slots[(int64_t)k * a.slots_s] == slot[r];
       on[r] = !__syncthreads_or(again) && slot[r] >= 0 && slot[r] < a.rows;
     }
-    on[r] = on[r] && d < a.dim;
   }
+  const int nv = d < a.dim ? a.states - 4 * q : 0;
   const int own = R > 1 ? q : 0;  // the row whose per-channel values this lane has
-  const int64_t i = i0 + own;
   bool mine = false;
 #pragma unroll
-  for (int r = 0; r < R; ++r) mine = r == own ? on[r] : mine;
-  const int nv = d < a.dim ? a.states - 4 * q : 0;
-  const int64_t g = a.groups == 1 ? 0 : (unsigned)d / (unsigned)a.per;
+  for (int r = 0; r < R; ++r) mine = r == own ? on[r] && d < a.dim : mine;
   float h[R][4], b[R][4], c[R][4], A[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  auto get = [&](const float *p, int64_t stride, float (&v)[4]) {
+  auto get = [&](const float *p, int stride, float (&v)[4]) {
     if (a.vec) {
       unpack(*reinterpret_cast<const float4 *>(p), v);
     } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = k < nv ? p[k * stride] : 0.0f;
+      for (int k = 0; k < 4; ++k) v[k] = k < nv ? p[(int64_t)k * stride] : 0.0f;
     }
   };
 #pragma unroll
   for (int r = 0; r < R; ++r)
-    if (on[r] && nv > 0) get(a.state.p + slot[r] * a.state.s0 + d * a.state.s1 + 4 * q * a.state.s2, a.state.s2, h[r]);
+    if (on[r] && nv > 0) get(a.state(slot[r], d, 4 * q), a.state.s2, h[r]);
   float u = 0.0f, s = 0.0f, z = 0.0f, sig;
   if (mine) {
-    u = a.u[i * a.u_b + d * a.u_d];
-    s = a.delta[i * a.delta_b + d * a.delta_d] + (a.bias ? a.bias[d * a.bias_s] : 0.0f);
-    if (a.z) z = a.z[i * a.z_b + d * a.z_d];
+    u = *a.u(i0 + own, d, 0);
+    s = *a.delta(i0 + own, d, 0);
+    if (a.bias.p) s += *a.bias(0, d, 0);
+    if (a.z.p) z = *a.z(i0 + own, d, 0);
   }
-  if (nv > 0) get(a.a + d * a.a_d + 4 * q * a.a_n, a.a_n, A);
+  if (nv > 0) get(a.a(0, d, 4 * q), a.a.s2, A);
+  const int g = a.groups > 1 ? (int)((unsigned)d / (unsigned)a.per) : 0;
 #pragma unroll
   for (int r = 0; r < R; ++r)
     if (on[r] && nv > 0) {
-      get(a.b.p + (i0 + r) * a.b.s0 + g * a.b.s1 + 4 * q * a.b.s2, a.b.s2, b[r]);
-      get(a.c.p + (i0 + r) * a.c.s0 + g * a.c.s1 + 4 * q * a.c.s2, a.c.s2, c[r]);
+      get(a.b(i0 + r, g, 4 * q), a.b.s2, b[r]);
+      get(a.c(i0 + r, g, 4 * q), a.c.s2, c[r]);
     }
   if (a.softplus) s = softplus(s, &sig);
   const float su = s * u;
   float part[R];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) A[k] *= kLog2e;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const float sr = R > 1 ? __shfl_sync(0xffffffffu, s, r, NL) : s;
@@ -334,17 +344,17 @@ __global__ void __launch_bounds__(kScanThreads) scan_step_kernel(const TokenArgs
     if (on[r] && nv > 0) {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (k < nv) {
-          h[r][k] = fmaf(ex2(sr * (A[k] * kLog2e)), h[r][k], sur * b[r][k]);
+        if (a.vec || k < nv) {
+          h[r][k] = fmaf(ex2(sr * A[k]), h[r][k], sur * b[r][k]);
           part[r] = fmaf(h[r][k], c[r][k], part[r]);
         }
-      float *o = a.state_out.p + slot[r] * a.state_out.s0 + d * a.state_out.s1 + 4 * q * a.state_out.s2;
+      float *o = a.state_out(slot[r], d, 4 * q);
       if (a.vec) {
         *reinterpret_cast<float4 *>(o) = make_float4(h[r][0], h[r][1], h[r][2], h[r][3]);
       } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (k < nv) o[k * a.state_out.s2] = h[r][k];
+          if (k < nv) o[(int64_t)k * a.state_out.s2] = h[r][k];
       }
     }
   }
@@ -355,9 +365,10 @@ __global__ void __launch_bounds__(kScanThreads) scan_step_kernel(const TokenArgs
     for (int o = 1; o < NL; o <<= 1) part[0] += __shfl_xor_sync(0xffffffffu, part[0], o);
   }
   if (mine && (R > 1 || q == 0)) {
-    float y = fmaf(a.d ? a.d[d * a.d_s] : 0.0f, u, part[0]);
-    if (a.z) y *= z * sigmoid(z);
-    a.y[i * a.y_b + d * a.y_d] = y;
+    float y = part[0];
+    if (a.d.p) y = fmaf(*a.d(0, d, 0), u, y);
+    if (a.z.p) y *= z * sigmoid(z);
+    *a.y(i0 + own, d, 0) = y;
   }
 }
 
@@ -598,21 +609,32 @@ int remora_b200_selective_scan_step(RemoraB200Ctx *ctx, const RemoraSelectiveSca
                          {&cv, "c", 4}, {has_d ? &dv : nullptr, "d", 4}, {has_z ? &zv : nullptr, "z", 4},
                          {has_i ? &iv : nullptr, "delta_bias", 4}, {has_l ? &lv : nullptr, "slots", 4}}, {&sv}));
   if (B == 0 || D == 0) return REMORA_OK;
+  if (std::max(std::max(D, S), N) > 0x3fffffff) return fail(REMORA_ERR_LIMIT, "selective_scan_step: more than 2^30 rows");
   TokenArgs a = {};
-  a.state = op3(sv), a.state_out = op3(ov), a.b = op3(bv), a.c = op3(cv);
-  a.u = reinterpret_cast<const float *>(uv.data(4)), a.u_b = uv.strides[0], a.u_d = uv.strides[1];
-  a.delta = reinterpret_cast<const float *>(ev.data(4)), a.delta_b = ev.strides[0], a.delta_d = ev.strides[1];
-  a.a = reinterpret_cast<const float *>(av.data(4)), a.a_d = av.strides[0], a.a_n = av.strides[1];
-  if (has_d) a.d = reinterpret_cast<const float *>(dv.data(4)), a.d_s = dv.strides[0];
-  if (has_z) a.z = reinterpret_cast<const float *>(zv.data(4)), a.z_b = zv.strides[0], a.z_d = zv.strides[1];
-  if (has_i) a.bias = reinterpret_cast<const float *>(iv.data(4)), a.bias_s = iv.strides[0];
-  if (has_l) a.slots = reinterpret_cast<const int *>(lv.data(4)), a.slots_s = lv.strides[0];
-  a.y = reinterpret_cast<float *>(yv.data(4)), a.y_b = yv.strides[0], a.y_d = yv.strides[1];
-  a.batch = B, a.rows = S, a.dim = D, a.per = D / G, a.states = (int)N, a.groups = (int)G;
+  // each operand's place in Token: row, channel (or group), state
+  struct {
+    const DescView *v;
+    int row, channel, state;
+    Token *to;
+  } const places[] = {{&sv, 0, 1, 2, &a.state}, {&ov, 0, 1, 2, &a.state_out}, {&bv, 0, 1, 2, &a.b}, {&cv, 0, 1, 2, &a.c},
+                      {&av, -1, 0, 1, &a.a},    {&uv, 0, 1, -1, &a.u},        {&ev, 0, 1, -1, &a.delta},
+                      {&yv, 0, 1, -1, &a.y},    {has_z ? &zv : nullptr, 0, 1, -1, &a.z},
+                      {has_d ? &dv : nullptr, -1, 0, -1, &a.d}, {has_i ? &iv : nullptr, -1, 0, -1, &a.bias},
+                      {has_l ? &lv : nullptr, 0, -1, -1, nullptr}};
+  for (const auto &x : places) {
+    if (x.v == nullptr) continue;
+    for (int k = 0; k < x.v->rank; ++k)
+      if (std::abs(x.v->strides[k]) > 0x7fffffff)
+        return fail(REMORA_ERR_LIMIT, "selective_scan_step: a stride of %lld elements (at most 2^31 - 1)",
+                    (long long)x.v->strides[k]);
+    auto stride = [&](int k) { return k < 0 ? 0 : (int)x.v->strides[k]; };
+    if (x.to) *x.to = {reinterpret_cast<float *>(x.v->data(4)), stride(x.row), stride(x.channel), stride(x.state)};
+  }
+  if (has_l) a.slots = reinterpret_cast<const int *>(lv.data(4)), a.slots_s = (int)lv.strides[0];
+  a.batch = (int)B, a.rows = (int)S, a.dim = (int)D, a.per = (int)(D / G), a.states = (int)N, a.groups = (int)G;
   a.softplus = spec->softplus != 0;
   a.vec = vec_states(sv) && vec_states(ov) && vec_states(av) && vec_states(bv) && vec_states(cv);
   const int nl = lanes_for(a.states);
-  if (D > 0x7fffffff) return fail(REMORA_ERR_LIMIT, "selective_scan_step: more than 2^31 - 1 channels");
   // R = NL rows per thread once that leaves every SM some blocks
   const int64_t blocks = (D + kScanThreads / nl - 1) / (kScanThreads / nl);
   const bool many = nl > 1 && blocks * (B / nl) >= kManyBlocks;
