@@ -1,4 +1,5 @@
-"""Build libremora_b200.so in-tree with nvcc for sm_100a.
+"""Build libremora_b200.so in-tree with nvcc for sm_100a, and the Python
+binding's host code (_binding.so) with the host compiler.
 
 Usage: python -m remora_b200.csrc.build  (or build() from Python).  Object
 files go to remora_b200/csrc/_build/; the shared library lands next to the
@@ -7,10 +8,12 @@ package so a plain snapshot of the repository carries it.
 
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -18,6 +21,7 @@ HERE = Path(__file__).resolve().parent
 PKG = HERE.parent
 ROOT = PKG.parent
 OUT = PKG / "libremora_b200.so"
+BINDING = PKG / "_binding.so"
 BUILD = HERE / "_build"
 
 SOURCES = sorted(HERE.glob("*.cu"))
@@ -62,10 +66,45 @@ def _compile(src: Path, verbose: bool) -> Path:
     return obj
 
 
+def _build_binding(verbose: bool) -> None:
+    """_binding.so: binding.cpp against the headers of the installed torch."""
+    src = HERE / "binding.cpp"
+    if BINDING.exists() and BINDING.stat().st_mtime >= src.stat().st_mtime:
+        return
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not spec.submodule_search_locations:
+        raise RuntimeError("building remora_b200._binding needs the torch headers")
+    torch_dir = Path(next(iter(spec.submodule_search_locations)))
+    cxx = _host_compiler()[1:] or ["g++"]
+    cmd = [
+        *cxx,
+        "-O2",
+        "-std=c++17",
+        "-fPIC",
+        "-shared",
+        f"-I{torch_dir / 'include'}",
+        f"-I{torch_dir / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
+        f"-I{sysconfig.get_paths()['include']}",
+        str(src),
+        "-o",
+        str(BINDING),
+        f"-L{torch_dir / 'lib'}",
+        "-ltorch_python",
+        "-ltorch_cpu",
+        "-lc10",
+        f"-Wl,-rpath,{torch_dir / 'lib'}",
+    ]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+
+
 def build(verbose: bool = False, jobs: int | None = None) -> Path:
     BUILD.mkdir(exist_ok=True)
     with ThreadPoolExecutor(max_workers=jobs or min(8, os.cpu_count() or 1)) as ex:
+        binding = ex.submit(_build_binding, verbose)
         objs = list(ex.map(lambda s: _compile(s, verbose), SOURCES))
+        binding.result()
     if not OUT.exists() or any(o.stat().st_mtime > OUT.stat().st_mtime for o in objs):
         cmd = [
             NVCC,

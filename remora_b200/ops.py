@@ -10,7 +10,6 @@ computes on the host.
 from __future__ import annotations
 
 import ctypes
-import struct
 from typing import Any, Sequence
 
 from remora_b200 import _lib as L
@@ -389,46 +388,53 @@ def append(a, b, out=None):
 # rows of a given `out` stay as they were.
 #
 # A single-token call costs what the host does, so the operands of a call are
-# checked and laid out in one loop, as one buffer of descriptors, and results
-# are made by the cheapest torch call for each.
-_CALL_BUFFER = ctypes.c_char * 3072  # descriptors of at most 24 operands, and their addresses
+# checked and laid out natively (csrc/binding.cpp), and results are made by the
+# cheapest torch call for each.
+def _describe(what: str, device: int, operands, table: int = 0):
+    """Checks (name, tensor or None, rank[, dtype]) operands, f32 unless a
+    dtype is given, on CUDA device `device`.  Returns the buffer that holds
+    their descriptors, to be kept until the call returns, and the address of
+    each (None for None).  With `table`, one address stands for the first
+    `table`: that of a struct of their addresses."""
+    described = _binding().describe(device, operands, table)
+    if described is None:
+        _refuse(what, device, operands)
+    return described
 
 
-def _describe(what: str, device: int, operands, special=(), table: int = 0):
-    """Checks (name, tensor or None, rank) operands, f32 on CUDA device
-    `device`, and `special` ones, (name, tensor or None, rank, dtype).  Returns
-    the buffer that holds their descriptors, to be kept until the call
-    returns, and the address of each (None for None), the special ones last.
-    With `table` also the address of a table of the first `table` addresses
-    (an argument struct of the C ABI), put first."""
-    f32 = _torch().float32
-    buf = _CALL_BUFFER()
-    start = ctypes.addressof(buf)
-    here = start + 8 * table
-    values, at = [0] * table, []
-    for name, t, rank, *want in (*operands, *special) if special else operands:
+def _binding():
+    global _binding_module
+    if _binding_module is None:
+        _torch()  # its libraries are the binding's
+        try:
+            from remora_b200 import _binding as module
+        except ImportError as e:
+            raise RemoraB200Error(f"remora_b200._binding is not built; run `python -m remora_b200.csrc.build` ({e})")
+        _binding_module = module
+    return _binding_module
+
+
+_binding_module = None
+
+
+def _refuse(what: str, device: int, operands) -> None:
+    """Raises for the first operand that describe() does not take."""
+    torch = _torch()
+    for name, t, rank, *dtype in operands:
+        want = dtype[0] if dtype else torch.float32
         if t is None:
-            at.append(None)
             continue
-        if t.dtype is not (want[0] if want else f32):
-            raise RemoraUnsupportedError(f"{what}: {name} is {t.dtype}, not {want[0] if want else f32}")
+        if not isinstance(t, torch.Tensor):
+            raise RemoraB200Error(f"{what}: {name} is a {type(t).__name__}, not a tensor")
+        if not t.is_cuda:
+            raise RemoraB200Error("remora_b200 ops take CUDA tensors (there is no CPU path)")
+        if t.dtype != want:
+            raise RemoraUnsupportedError(f"{what}: {name} is {t.dtype}, not {want}")
         if t.get_device() != device:
-            if not t.is_cuda:
-                raise RemoraB200Error("remora_b200 ops take CUDA tensors (there is no CPU path)")
             raise RemoraB200Error(f"{what}: {name} is on {t.device}, the first operand on cuda:{device}")
-        shape = t.shape
-        if len(shape) != rank:
-            raise RemoraShapeError(f"{what}: {name} has rank {len(shape)}, not {rank}")
-        base, off = t.data_ptr(), t.storage_offset()
-        if base:
-            base -= off * t.element_size()
-        at.append(here)
-        here += 24 + 16 * rank
-        values += (base, base, off, *shape, *t.stride())
-    for k in range(table):
-        values[k] = at[k] or 0
-    struct.pack_into(f"{len(values)}q", buf, 0, *values)
-    return (buf, start, *at[table:]) if table else (buf, *at)
+        if t.dim() != rank:
+            raise RemoraShapeError(f"{what}: {name} has rank {t.dim()}, not {rank}")
+    raise RemoraUnsupportedError(f"{what}: an operand has no dense storage, or a rank over {L.MAX_RANK}")
 
 
 def _cuda_index(t) -> int:
@@ -500,8 +506,8 @@ def rms_norm_quant(x, w, *, residual=None, eps: float = 1e-6, group: int = 0, ou
         scales = x.new_empty((*x.shape[:-1], x.shape[-1] // group if group > 0 and rank else 1))
     s = sum_out if sum_out is not None or residual is None else _rows_like(x, None)
     keep, xd, rd, wd, cd, sd, qd = _describe("rms_norm_quant", device, (
-        ("x", x, rank), ("residual", residual, rank), ("w", w, 1), ("scales", scales, rank), ("sum_out", s, rank)),
-        (("out", q, rank, torch.float8_e4m3fn),))
+        ("x", x, rank), ("residual", residual, rank), ("w", w, 1), ("scales", scales, rank), ("sum_out", s, rank),
+        ("out", q, rank, torch.float8_e4m3fn)))
     spec = L.RemoraNormSpec(eps, group)
     L.check(L.lib().remora_b200_rms_norm_quant(context(device).ptr, ctypes.addressof(spec), xd, rd, wd, qd, cd, sd,
                                                rank, _raw_stream(device)), "rms_norm_quant")
@@ -543,7 +549,7 @@ def causal_conv_fwd(x, w, bias=None, *, state=None, lengths=None, silu: bool = F
         state_out = x.new_empty((x.shape[0], max(w.shape[1] - 1, 0), x.shape[2]))
     keep, xd, wd, bd, sd, yd, od, ld = _describe("causal_conv_fwd", device, (
         ("x", x, 3), ("w", w, 2), ("bias", bias, 1), ("state", state, 3), ("out", out, 3),
-        ("state_out", state_out, 3)), (("lengths", lengths, 1, torch.int32),))
+        ("state_out", state_out, 3), ("lengths", lengths, 1, torch.int32)))
     L.check(L.lib().remora_b200_causal_conv_fwd(context(device).ptr, _spec(_CONV_SPECS, silu), xd, wd, bd, sd, ld, yd,
                                                 od, _raw_stream(device)), "causal_conv_fwd")
     return out if state_out is None else (out, state_out)
@@ -560,8 +566,8 @@ def causal_conv_bwd(x, w, dy, bias=None, *, state=None, lengths=None, silu: bool
     dstate = _rows_like(state, None) if state is not None else None
     keep, xd, wd, bd, sd, gd, ed, dxd, dwd, dbd, dsd, ld = _describe("causal_conv_bwd", device, (
         ("x", x, 3), ("w", w, 2), ("bias", bias, 1), ("state", state, 3), ("dy", dy, 3), ("dstate_out", dstate_out, 3),
-        ("out", dx, 3), ("dw", dw, 2), ("dbias", dbias, 1), ("dstate", dstate, 3)),
-        (("lengths", lengths, 1, _torch().int32),))
+        ("out", dx, 3), ("dw", dw, 2), ("dbias", dbias, 1), ("dstate", dstate, 3),
+        ("lengths", lengths, 1, _torch().int32)))
     lib, ctx = L.lib(), context(device).ptr
     scratch, at, size = _scratch(lib.remora_b200_causal_conv_bwd_scratch, "causal_conv_bwd", x, ctx, *x.shape,
                                  w.shape[1])
@@ -581,8 +587,8 @@ def causal_conv_step(x, state, w, bias=None, *, silu: bool = False, slots=None, 
     if state_out is None:
         state_out = state
     keep, xd, sd, wd, bd, yd, od, ld = _describe("causal_conv_step", device, (
-        ("x", x, 2), ("state", state, 3), ("w", w, 2), ("bias", bias, 1), ("out", out, 2), ("state_out", state_out, 3)),
-        (("slots", slots, 1, _torch().int32),))
+        ("x", x, 2), ("state", state, 3), ("w", w, 2), ("bias", bias, 1), ("out", out, 2), ("state_out", state_out, 3),
+        ("slots", slots, 1, _torch().int32)))
     L.check(L.lib().remora_b200_causal_conv_step(context(device).ptr, _spec(_CONV_SPECS, silu), xd, sd, wd, bd, ld, yd,
                                                  od, _raw_stream(device)), "causal_conv_step")
     return out

@@ -190,6 +190,40 @@ def test_ops_take_cuda_tensors():
         ops.selective_scan_fwd(t(2, 3, 4), t(2, 3, 4), t(4, 5), t(2, 3, 5), t(2, 3, 5))
 
 
+def test_binding_lays_out_descriptors():
+    """The binding's buffer holds the descriptors that tensor_descriptor makes
+    (the view's start in `offset`), and refuses what does not fit."""
+    import torch
+
+    from remora_b200 import _binding
+    from remora_b200.abi import tensor_descriptor
+
+    base = torch.arange(120.0).reshape(4, 5, 6)
+    views = [base, base[1:, ::2, 3:].permute(2, 0, 1), base[0, 0, 0], torch.zeros(0, 3), base[:, :1].expand(4, 5, 6)]
+    operands = tuple((f"t{k}", t, t.dim()) for k, t in enumerate(views)) + (
+        ("none", None, 2), ("ints", torch.arange(3, dtype=torch.int32), 1, torch.int32))
+    for table in (0, 2, len(operands)):
+        buf, *at = _binding.describe(-1, operands, table)
+        if table:
+            first = ctypes.cast(at[0], ctypes.POINTER(ctypes.c_uint64))
+            at = [first[k] or None for k in range(table)] + at[1:]
+        assert len(at) == len(operands) and at[5] is None
+        for (_, t, *_rest), address in zip(operands, at):
+            if t is None:
+                continue
+            want = tensor_descriptor(t)
+            if not t.numel():
+                want.allocated = want.aligned = 0
+            assert ctypes.string_at(address, ctypes.sizeof(want)) == bytes(want)
+    one = torch.zeros(2, 3)
+    for bad in (("x", one, 3), ("x", one.double(), 2), ("x", one, 2, torch.int32), ("x", 3.0, 0), ("x", one.to_sparse(), 2)):
+        assert _binding.describe(-1, (bad,), 0) is None
+    assert _binding.describe(0, (("x", one, 2),), 0) is None  # another device
+    for wrong in ((-1, [("x", one, 2)], 0), (-1, (("x", one),), 0), (-1, (("x", one, 2, "f32"),), 0), (-1, (("x", one, 2),), 2)):
+        with pytest.raises((TypeError, ValueError)):
+            _binding.describe(*wrong)
+
+
 # ------------------------------------------------- the references' gradients
 def central(f, x, eps=1e-5):
     g = np.zeros_like(x)
