@@ -18,8 +18,8 @@
  *    that the caller did not share.
  *  - `lengths` (int32, one per sequence, may be NULL): sequence b is
  *    lengths[b] positions long, taken as 0 below 0 and as L above L.  Rows
- *    behind a sequence's end are neither read nor written, in inputs, outputs
- *    and gradients.
+ *    behind a sequence's end are never read; in outputs and gradients they
+ *    stay as they were, or become zero where the spec's zero_rest is set.
  *  - Outputs must not overlap inputs or each other, except where an entry
  *    point says so; views that interleave (columns of one wider array) do not
  *    count as overlapping.  Input gradients of one array passed twice are two
@@ -80,8 +80,9 @@ int remora_b200_rms_norm_bwd(RemoraB200Ctx *ctx, const RemoraNormSpec *spec,
 /* Depthwise causal convolution along time                                  */
 /* ------------------------------------------------------------------------ */
 typedef struct {
-  int32_t silu; /* 1: y = p / (1 + exp(-p)) of the convolution's p          */
-  int32_t reserved_;
+  int32_t silu;      /* 1: y = p / (1 + exp(-p)) of the convolution's p     */
+  int32_t zero_rest; /* 1: rows of y and dx that belong to no sequence
+                        (behind an end; of a token left out) are set to zero */
 } RemoraCausalConvSpec;
 
 /* p[b,t,d] = bias[d] + sum_k w[d,k] x[b, t - (W-1) + k, d], W taps (2..8), x
@@ -116,8 +117,8 @@ int remora_b200_causal_conv_bwd(
    [S,W-1,D] (slots int32 [B]; NULL: row i, B <= S); state_out [S,W-1,D]
    (exactly state for an update in place) gets the moved window in the same
    row, its other rows stay as they were.  A row whose slot is outside 0..S-1
-   (-1 for padding) or was named by an earlier row is left out: its y and all
-   states stay as they were. */
+   (-1 for padding) or was named by an earlier row is left out: all states and,
+   without zero_rest, its y stay as they were. */
 int remora_b200_causal_conv_step(RemoraB200Ctx *ctx,
                                  const RemoraCausalConvSpec *spec,
                                  const RemoraMemRef2 *x,
@@ -132,8 +133,9 @@ int remora_b200_causal_conv_step(RemoraB200Ctx *ctx,
 /* Selective state space scan                                               */
 /* ------------------------------------------------------------------------ */
 typedef struct {
-  int32_t softplus; /* 1: the step is softplus(delta + delta_bias)           */
-  int32_t reserved_;
+  int32_t softplus;  /* 1: the step is softplus(delta + delta_bias)          */
+  int32_t zero_rest; /* 1: rows of y, du, ddelta, dz, db and dc that belong to
+                        no sequence are set to zero                          */
 } RemoraSelectiveScanSpec;
 
 /* Inputs of the scan over [B,L,D] with N states (1..64) per channel:

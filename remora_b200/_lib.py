@@ -134,11 +134,11 @@ class RemoraNormSpec(ctypes.Structure):
 
 
 class RemoraCausalConvSpec(ctypes.Structure):
-    _fields_ = [("silu", ctypes.c_int32), ("reserved_", ctypes.c_int32)]
+    _fields_ = [("silu", ctypes.c_int32), ("zero_rest", ctypes.c_int32)]
 
 
 class RemoraSelectiveScanSpec(ctypes.Structure):
-    _fields_ = [("softplus", ctypes.c_int32), ("reserved_", ctypes.c_int32)]
+    _fields_ = [("softplus", ctypes.c_int32), ("zero_rest", ctypes.c_int32)]
 
 
 class RemoraSelectiveScanIn(ctypes.Structure):

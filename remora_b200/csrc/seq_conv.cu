@@ -47,7 +47,7 @@ struct ConvArgs {
   int64_t batch, length, dim;
   int64_t blocks_d, blocks_t;  // grid: batch x blocks_t x blocks_d, flattened
   int run;                     // time steps per thread
-  int silu;
+  int silu, zero_rest;
   // backward
   Op3 dy, dx, dstate, dstate_out;
   float *part;  // [batch * blocks_t, (W + 1), dim]
@@ -105,6 +105,11 @@ __device__ __forceinline__ int64_t length_of(const int *lengths, int64_t stride,
   return n < 0 ? 0 : n > length ? length : n;
 }
 
+template <int VEC>
+__device__ __forceinline__ void zero_rows(const Op3 &o, int64_t b, int64_t from, int64_t to, int64_t d) {
+  for (int64_t t = from; t < to; ++t) store<VEC>(o.p + b * o.b + t * o.t + d * o.d, zero<VEC>());
+}
+
 // Row e of the state followed by the sequence: e < 0 is state row e + W-1.
 template <int W, int VEC>
 __device__ __forceinline__ Vec<VEC> row_at(const ConvArgs &a, int64_t b, int64_t e, int64_t d) {
@@ -121,6 +126,7 @@ __global__ void __launch_bounds__(kLanes *kRuns) conv_fwd_kernel(const ConvArgs 
   if (d >= a.dim) return;
   const int64_t len = length_of(a.lengths, a.lengths_b, b, a.length);
   const int64_t t0 = (bt * kRuns + threadIdx.y) * a.run;
+  if (a.zero_rest) zero_rows<VEC>(a.y, b, max(t0, len), min(t0 + a.run, a.length), d);
   if (t0 >= len && t0 > 0) return;
   const int64_t t1 = min(t0 + a.run, len);
   Vec<VEC> w[W], win[W - 1], bias = zero<VEC>();
@@ -192,6 +198,7 @@ __global__ void __launch_bounds__(kLanes *kRuns, W <= 4 ? 6 : W <= 6 ? 4 : 3) co
   Vec<VEC> dw[W], db = zero<VEC>();
 #pragma unroll
   for (int k = 0; k < W; ++k) dw[k] = zero<VEC>();
+  if (a.zero_rest && d < a.dim) zero_rows<VEC>(a.dx, b, max(t0, len), min(t0 + a.run, a.length), d);
   if (d < a.dim && (t0 < len || t0 == 0)) {
     const int64_t t1 = min(t0 + a.run, len);  // rows [t0, t1) of dx and of the sums
     Vec<VEC> w[W], win[W], g[W], bias = zero<VEC>();  // win: x rows t-(W-1) .. t; g: g[t-(W-1)] .. g[t]
@@ -303,7 +310,7 @@ struct StepArgs {
   const int *slots;
   int64_t slots_b;
   int64_t rows, dim;
-  int silu;
+  int silu, zero_rest;
 };
 
 template <int W, int VEC>
@@ -318,7 +325,11 @@ __global__ void __launch_bounds__(128) conv_step_kernel(const StepArgs a) {
     live = !__syncthreads_or(again) && slot >= 0 && slot < a.rows;
   }
   const int64_t d = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * VEC;
-  if (!live || d >= a.dim) return;
+  if (d >= a.dim) return;
+  if (!live) {
+    if (a.zero_rest) store<VEC>(a.y + i * a.y_b + d * a.y_d, zero<VEC>());
+    return;
+  }
   const float *s = a.state.p + slot * a.state.b + d * a.state.d;
   float *so = a.state_out.p + slot * a.state_out.b + d * a.state_out.d;
   Vec<VEC> win[W], o = zero<VEC>();
@@ -472,7 +483,7 @@ int remora_b200_causal_conv_fwd(RemoraB200Ctx *ctx, const RemoraCausalConvSpec *
   a.w = reinterpret_cast<const float *>(wv.data(4)), a.w_d = wv.strides[0], a.w_k = wv.strides[1];
   if (has_b) a.bias = reinterpret_cast<const float *>(bv.data(4)), a.bias_d = bv.strides[0];
   if (has_l) a.lengths = reinterpret_cast<const int *>(lv.data(4)), a.lengths_b = lv.strides[0];
-  a.batch = B, a.length = L, a.dim = D, a.silu = spec->silu != 0;
+  a.batch = B, a.length = L, a.dim = D, a.silu = spec->silu != 0, a.zero_rest = spec->zero_rest != 0;
   constexpr int V = kVec;
   const bool vec = D % V == 0 && vec_rows(xv, V) && vec_rows(yv, V) && (!has_s || vec_rows(sv, V)) &&
                    (!has_o || vec_rows(ov, V));
@@ -541,7 +552,7 @@ int remora_b200_causal_conv_bwd(RemoraB200Ctx *ctx, const RemoraCausalConvSpec *
   a.w = reinterpret_cast<const float *>(wv.data(4)), a.w_d = wv.strides[0], a.w_k = wv.strides[1];
   if (has_b) a.bias = reinterpret_cast<const float *>(bv.data(4)), a.bias_d = bv.strides[0];
   if (has_l) a.lengths = reinterpret_cast<const int *>(lv.data(4)), a.lengths_b = lv.strides[0];
-  a.batch = B, a.length = L, a.dim = D, a.silu = spec->silu != 0;
+  a.batch = B, a.length = L, a.dim = D, a.silu = spec->silu != 0, a.zero_rest = spec->zero_rest != 0;
   a.part = static_cast<float *>(scratch);
   constexpr int V = kVec;
   const bool vec = D % V == 0 && vec_rows(xv, V) && vec_rows(gv, V) && vec_rows(dxv, V) &&
@@ -594,7 +605,7 @@ int remora_b200_causal_conv_step(RemoraB200Ctx *ctx, const RemoraCausalConvSpec 
   a.w = reinterpret_cast<const float *>(wv.data(4)), a.w_d = wv.strides[0], a.w_k = wv.strides[1];
   if (has_b) a.bias = reinterpret_cast<const float *>(bv.data(4)), a.bias_d = bv.strides[0];
   if (has_l) a.slots = reinterpret_cast<const int *>(lv.data(4)), a.slots_b = lv.strides[0];
-  a.rows = S, a.dim = D, a.silu = spec->silu != 0;
+  a.rows = S, a.dim = D, a.silu = spec->silu != 0, a.zero_rest = spec->zero_rest != 0;
   const bool vec = D % 4 == 0 && vec_rows(xv, 4) && vec_rows(yv, 4) && vec_rows(sv, 4) && vec_rows(ov, 4);
   DeviceGuard guard;
   REMORA_TRY(guard.enter(ctx));

@@ -39,13 +39,15 @@ __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 4 : 2) scan_fwd_kernel(
   const Place<NL, kChan> at(a);
   const int64_t len = scan_length(a, at.b);
   const int64_t t0 = at.chunk * a.chunk, t_end = min(t0 + a.chunk, len);
+  const Lane<NL, kChan> ly(a.y, at, t0);
+  if (MAIN && a.zero_rest) zero_rows(ly, at, a, t0, len);
   if (t0 >= len && t0 > 0) return;  // the first piece of an empty sequence hands h0 on
   if (!MAIN && t_end == len) return;  // nothing follows
   const int steps = (int)(t_end - t0);
   const int nv = a.states - 4 * at.q;  // of the four states, those below N
   f2 A[kChan][2], h[kChan][2];
   float bias[kChan], skip[kChan], total[kChan];
-  const Lane<NL, kChan> lu(a.u, at, t0), ld(a.delta, at, t0), lz(a.z, at, t0), ly(a.y, at, t0);
+  const Lane<NL, kChan> lu(a.u, at, t0), ld(a.delta, at, t0), lz(a.z, at, t0);
 #pragma unroll
   for (int c = 0; c < kChan; ++c) {
     float av[4], hv[4];
@@ -273,7 +275,7 @@ struct TokenArgs {
   const int *slots;
   int slots_s;
   int batch, rows, dim, per;
-  int states, groups, softplus, vec;
+  int states, groups, softplus, zero_rest, vec;
 };
 
 // Four states of one channel per thread, of R batch rows, R either 1 or NL.
@@ -369,6 +371,8 @@ __global__ void __launch_bounds__(kScanThreads, NL > 4 ? 2 : 7) scan_step_kernel
     if (a.d.p) y = fmaf(*a.d(0, d, 0), u, y);
     if (a.z.p) y *= z * sigmoid(z);
     *a.y(i0 + own, d, 0) = y;
+  } else if (a.zero_rest && !mine && d < a.dim && i0 + own < a.batch && (R > 1 || q == 0)) {
+    *a.y(i0 + own, d, 0) = 0.0f;
   }
 }
 
@@ -482,6 +486,7 @@ int read_scan_in(const RemoraSelectiveScanSpec *spec, const RemoraSelectiveScanI
   if (have[8]) a->h0 = op3(views[8]);
   if (have[9]) a->lengths = reinterpret_cast<const int *>(views[9].data(4)), a->lengths_s = views[9].strides[0];
   a->batch = B, a->length = L, a->dim = D, a->states = (int)N, a->groups = (int)G, a->softplus = spec->softplus != 0;
+  a->zero_rest = spec->zero_rest != 0;
   a->per = D / G;
   return REMORA_OK;
 }
@@ -632,7 +637,7 @@ int remora_b200_selective_scan_step(RemoraB200Ctx *ctx, const RemoraSelectiveSca
   }
   if (has_l) a.slots = reinterpret_cast<const int *>(lv.data(4)), a.slots_s = (int)lv.strides[0];
   a.batch = (int)B, a.rows = (int)S, a.dim = (int)D, a.per = (int)(D / G), a.states = (int)N, a.groups = (int)G;
-  a.softplus = spec->softplus != 0;
+  a.softplus = spec->softplus != 0, a.zero_rest = spec->zero_rest != 0;
   a.vec = vec_states(sv) && vec_states(ov) && vec_states(av) && vec_states(bv) && vec_states(cv);
   const int nl = lanes_for(a.states);
   // R = NL rows per thread once that leaves every SM some blocks

@@ -47,7 +47,7 @@ struct ScanArgs {
   const int *lengths;
   int64_t lengths_s;
   int64_t batch, length, dim;
-  int states, groups, softplus;
+  int states, groups, softplus, zero_rest;
   int64_t per;       // channels per group
   int64_t blocks_d;  // channel blocks per group
   int64_t chunks;    // pieces of the time axis, each by blocks of its own
@@ -147,6 +147,17 @@ struct Lane {
     return *reinterpret_cast<float *>(base + t * step + off[c]);
   }
 };
+
+// Sets the rows of a chunk that lie behind the sequence's end to zero.
+template <int NL, int CHAN>
+__device__ __forceinline__ void zero_rows(const Lane<NL, CHAN> &o, const Place<NL, CHAN> &at, const ScanArgs &a,
+                                          int64_t t0, int64_t len) {
+  const int upto = (int)(min(t0 + a.chunk, a.length) - t0);
+  for (int t = (int)(max(t0, len) - t0); t < upto; t += NL)
+#pragma unroll
+    for (int c = 0; c < CHAN; ++c)
+      if (at.live[c] && t + at.q < upto) o(c, t) = 0.0f;
+}
 
 __device__ __forceinline__ void copy_async4(float *dst, const float *src, bool on) {
   const uint32_t s = static_cast<uint32_t>(__cvta_generic_to_shared(dst));

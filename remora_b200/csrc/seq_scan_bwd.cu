@@ -114,6 +114,19 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const ScanArg
   ulonglong2 rh[C];
   const Lane<NL, C> lu(a.u, at, t0), ld(a.delta, at, t0), lz(a.z, at, t0), ly(a.dy, at, t0);
   const Lane<NL, C> ldu(a.du, at, t0), ldd(a.ddelta, at, t0), ldz(a.dz, at, t0);
+  if (a.zero_rest) {
+    zero_rows(ldu, at, a, t0, len);
+    zero_rows(ldd, at, a, t0, len);
+    if (a.dz.p) zero_rows(ldz, at, a, t0, len);
+    if (a.blocks_d == 1) {  // else by join_bc_kernel
+      const int64_t from = max(t0, len), rows = min(t0 + a.chunk, a.length) - from;
+      for (int64_t i = threadIdx.x; i < rows * a.states; i += kScanThreads) {
+        const int64_t t = from + i / a.states, n = i % a.states;
+        a.db.p[at.b * a.db.s0 + t * a.db.s1 + at.g * a.db.s2 + n * a.db.s3] = 0.0f;
+        a.dc.p[at.b * a.dc.s0 + t * a.dc.s1 + at.g * a.dc.s2 + n * a.dc.s3] = 0.0f;
+      }
+    }
+  }
   // the states kept at the pieces' starts: [piece, local channel, q]
   const ulonglong2 *hp = reinterpret_cast<const ulonglong2 *>(a.saved) +
                          ((at.b * kept + t0 / T) * a.dim + at.first) * NL;
@@ -464,11 +477,12 @@ __global__ void __launch_bounds__(256) join_bc_kernel(const ScanArgs a) {
   if (i >= plane) return;
   const int64_t n = i % a.states, g = i / a.states % a.groups, bt = i / a.states / a.groups;
   const int64_t t = bt % a.length, b = bt / a.length;
-  if (t >= scan_length(a, b)) return;
+  const bool rest = t >= scan_length(a, b);
+  if (rest && !a.zero_rest) return;
   const float *p = a.part_bc + (bt * a.groups + g) * 2 * a.states + n;
   float vb = 0.0f, vc = 0.0f;
 #pragma unroll 8
-  for (int64_t k = 0; k < a.blocks_d; ++k, p += 2 * plane) {
+  for (int64_t k = 0; k < (rest ? 0 : a.blocks_d); ++k, p += 2 * plane) {
     vb += p[0];
     vc += p[a.states];
   }

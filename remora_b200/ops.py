@@ -461,20 +461,20 @@ def _scratch(fn, what: str, t, *sizes):
     return buf, buf.data_ptr(), n.value
 
 
-def _rows_like(t, lengths):
-    """A contiguous result shaped as the f32 tensor t: zeros where some rows
-    will not be written (lengths or slots given), else memory as it comes."""
+def _like(t):
+    """An unset contiguous result shaped as the f32 tensor t (None for None)."""
     torch = _torch()
-    make = torch.empty_like if lengths is None else torch.zeros_like
-    return make(t, memory_format=torch.contiguous_format)
+    return torch.empty_like(t, memory_format=torch.contiguous_format) if t is not None else None
 
 
-_CONV_SPECS = tuple(L.RemoraCausalConvSpec(k, 0) for k in (0, 1))
-_SCAN_SPECS = tuple(L.RemoraSelectiveScanSpec(k, 0) for k in (0, 1))
+# indexed by the flag and by zero_rest: set for results made here, whose rows
+# outside every sequence shall be zero, not for a caller's
+_CONV_SPECS = tuple(tuple(L.RemoraCausalConvSpec(k, zero) for zero in (0, 1)) for k in (0, 1))
+_SCAN_SPECS = tuple(tuple(L.RemoraSelectiveScanSpec(k, zero) for zero in (0, 1)) for k in (0, 1))
 
 
-def _spec(specs, flag) -> int:
-    return ctypes.addressof(specs[1 if flag else 0])
+def _spec(specs, flag, made_here: bool) -> int:
+    return ctypes.addressof(specs[1 if flag else 0][1 if made_here else 0])
 
 
 def rms_norm_fwd(x, w, *, residual=None, eps: float = 1e-6, out=None, sum_out=None):
@@ -482,8 +482,8 @@ def rms_norm_fwd(x, w, *, residual=None, eps: float = 1e-6, out=None, sum_out=No
     (rank 1 to 4).  Returns y, and (y, s) with a residual.  `out` or `sum_out`
     may be x or the residual itself."""
     device, rank = _cuda_index(x), x.dim()
-    y = out if out is not None else _rows_like(x, None)
-    s = sum_out if sum_out is not None or residual is None else _rows_like(x, None)
+    y = out if out is not None else _like(x)
+    s = sum_out if sum_out is not None or residual is None else _like(x)
     keep, xd, rd, wd, yd, sd = _describe("rms_norm_fwd", device, (
         ("x", x, rank), ("residual", residual, rank), ("w", w, 1), ("out", y, rank), ("sum_out", s, rank)))
     spec = L.RemoraNormSpec(eps, 0)
@@ -504,7 +504,7 @@ def rms_norm_quant(x, w, *, residual=None, eps: float = 1e-6, group: int = 0, ou
         q = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
     if scales is None:
         scales = x.new_empty((*x.shape[:-1], x.shape[-1] // group if group > 0 and rank else 1))
-    s = sum_out if sum_out is not None or residual is None else _rows_like(x, None)
+    s = sum_out if sum_out is not None or residual is None else _like(x)
     keep, xd, rd, wd, cd, sd, qd = _describe("rms_norm_quant", device, (
         ("x", x, rank), ("residual", residual, rank), ("w", w, 1), ("scales", scales, rank), ("sum_out", s, rank),
         ("out", q, rank, torch.float8_e4m3fn)))
@@ -520,8 +520,8 @@ def rms_norm_bwd(s, w, dy, *, dsum=None, eps: float = 1e-6, out=None):
     the gradient that reaches s from its other readers.  `out` (dx) may be s,
     dy or dsum itself."""
     device, rank = _cuda_index(s), s.dim()
-    dx = out if out is not None else _rows_like(s, None)
-    dw = _rows_like(w, None)
+    dx = out if out is not None else _like(s)
+    dw = _like(w)
     keep, sd, wd, gd, ed, xd, dwd = _describe("rms_norm_bwd", device, (
         ("s", s, rank), ("w", w, 1), ("dy", dy, rank), ("dsum", dsum, rank), ("out", dx, rank), ("dw", dw, 1)))
     lib, ctx = L.lib(), context(device).ptr
@@ -543,16 +543,15 @@ def causal_conv_fwd(x, w, bias=None, *, state=None, lengths=None, silu: bool = F
     (y, the state that continues the sequence), else y."""
     torch = _torch()
     device = _cuda_index(x)
-    if out is None:
-        out = _rows_like(x, lengths)
+    y = out if out is not None else _like(x)
     if state_out is None and return_state and x.dim() == 3 and w.dim() == 2:
         state_out = x.new_empty((x.shape[0], max(w.shape[1] - 1, 0), x.shape[2]))
     keep, xd, wd, bd, sd, yd, od, ld = _describe("causal_conv_fwd", device, (
-        ("x", x, 3), ("w", w, 2), ("bias", bias, 1), ("state", state, 3), ("out", out, 3),
+        ("x", x, 3), ("w", w, 2), ("bias", bias, 1), ("state", state, 3), ("out", y, 3),
         ("state_out", state_out, 3), ("lengths", lengths, 1, torch.int32)))
-    L.check(L.lib().remora_b200_causal_conv_fwd(context(device).ptr, _spec(_CONV_SPECS, silu), xd, wd, bd, sd, ld, yd,
-                                                od, _raw_stream(device)), "causal_conv_fwd")
-    return out if state_out is None else (out, state_out)
+    L.check(L.lib().remora_b200_causal_conv_fwd(context(device).ptr, _spec(_CONV_SPECS, silu, out is None), xd, wd, bd,
+                                                sd, ld, yd, od, _raw_stream(device)), "causal_conv_fwd")
+    return y if state_out is None else (y, state_out)
 
 
 def causal_conv_bwd(x, w, dy, bias=None, *, state=None, lengths=None, silu: bool = False, dstate_out=None, out=None):
@@ -560,10 +559,10 @@ def causal_conv_bwd(x, w, dy, bias=None, *, state=None, lengths=None, silu: bool
     None where bias or state is.  dstate_out is the gradient that reaches the
     returned state; `out` receives dx."""
     device = _cuda_index(x)
-    dx = out if out is not None else _rows_like(x, lengths)
-    dw = _rows_like(w, None)
-    dbias = _rows_like(bias, None) if bias is not None else None
-    dstate = _rows_like(state, None) if state is not None else None
+    dx = out if out is not None else _like(x)
+    dw = _like(w)
+    dbias = _like(bias)
+    dstate = _like(state)
     keep, xd, wd, bd, sd, gd, ed, dxd, dwd, dbd, dsd, ld = _describe("causal_conv_bwd", device, (
         ("x", x, 3), ("w", w, 2), ("bias", bias, 1), ("state", state, 3), ("dy", dy, 3), ("dstate_out", dstate_out, 3),
         ("out", dx, 3), ("dw", dw, 2), ("dbias", dbias, 1), ("dstate", dstate, 3),
@@ -571,8 +570,8 @@ def causal_conv_bwd(x, w, dy, bias=None, *, state=None, lengths=None, silu: bool
     lib, ctx = L.lib(), context(device).ptr
     scratch, at, size = _scratch(lib.remora_b200_causal_conv_bwd_scratch, "causal_conv_bwd", x, ctx, *x.shape,
                                  w.shape[1])
-    L.check(lib.remora_b200_causal_conv_bwd(ctx, _spec(_CONV_SPECS, silu), xd, wd, bd, sd, ld, gd, ed, dxd, dwd, dbd, dsd,
-                                            at, size, _raw_stream(device)), "causal_conv_bwd")
+    L.check(lib.remora_b200_causal_conv_bwd(ctx, _spec(_CONV_SPECS, silu, out is None), xd, wd, bd, sd, ld, gd, ed, dxd,
+                                            dwd, dbd, dsd, at, size, _raw_stream(device)), "causal_conv_bwd")
     return dx, dw, dbias, dstate
 
 
@@ -582,16 +581,15 @@ def causal_conv_step(x, state, w, bias=None, *, silu: bool = False, slots=None, 
     row i without slots; a row whose slot is -1 or was named by an earlier row
     is left out (its y is zero, or as it was in a given `out`)."""
     device = _cuda_index(x)
-    if out is None:
-        out = _rows_like(x, slots)
+    y = out if out is not None else _like(x)
     if state_out is None:
         state_out = state
     keep, xd, sd, wd, bd, yd, od, ld = _describe("causal_conv_step", device, (
-        ("x", x, 2), ("state", state, 3), ("w", w, 2), ("bias", bias, 1), ("out", out, 2), ("state_out", state_out, 3),
+        ("x", x, 2), ("state", state, 3), ("w", w, 2), ("bias", bias, 1), ("out", y, 2), ("state_out", state_out, 3),
         ("slots", slots, 1, _torch().int32)))
-    L.check(L.lib().remora_b200_causal_conv_step(context(device).ptr, _spec(_CONV_SPECS, silu), xd, sd, wd, bd, ld, yd,
-                                                 od, _raw_stream(device)), "causal_conv_step")
-    return out
+    L.check(L.lib().remora_b200_causal_conv_step(context(device).ptr, _spec(_CONV_SPECS, silu, out is None), xd, sd, wd,
+                                                 bd, ld, yd, od, _raw_stream(device)), "causal_conv_step")
+    return y
 
 
 def _groups(what: str, B, C, rank: int):
@@ -613,13 +611,12 @@ def selective_scan_fwd(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, so
     torch = _torch()
     device = _cuda_index(u)
     Bg, Cg = _groups("selective_scan_fwd", B, C, 4)
-    if out is None:
-        out = _rows_like(u, lengths)
+    y = out if out is not None else _like(u)
     if h_last is None and return_state and u.dim() == 3 and A.dim() == 2:
         h_last = u.new_empty((u.shape[0], u.shape[2], A.shape[1]))
     keep, args, yd, hd = _describe("selective_scan_fwd", device, (
         ("u", u, 3), ("delta", delta, 3), ("A", A, 2), ("B", Bg, 4), ("C", Cg, 4), ("D", D, 1), ("z", z, 3),
-        ("delta_bias", delta_bias, 1), ("h0", h0, 3), ("lengths", lengths, 1, torch.int32), ("out", out, 3),
+        ("delta_bias", delta_bias, 1), ("h0", h0, 3), ("lengths", lengths, 1, torch.int32), ("out", y, 3),
         ("h_last", h_last, 3)), table=10)
     lib, ctx = L.lib(), context(device).ptr
     sizes = (*u.shape, A.shape[1])
@@ -631,10 +628,10 @@ def selective_scan_fwd(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, so
         L.check(lib.remora_b200_selective_scan_saved(*sizes, ctypes.byref(n)), "selective_scan_fwd")
         saved = torch.empty((n.value // 4,), dtype=torch.float32, device=u.device)
         kept, kept_size = (saved.data_ptr(), n.value) if n.value else (None, 0)
-    L.check(lib.remora_b200_selective_scan_fwd(ctx, _spec(_SCAN_SPECS, softplus), args, yd, hd, kept, kept_size, at,
-                                               size, _raw_stream(device)), "selective_scan_fwd")
-    results = (out,) + ((h_last,) if h_last is not None else ()) + ((saved,) if save else ())
-    return results if len(results) > 1 else out
+    L.check(lib.remora_b200_selective_scan_fwd(ctx, _spec(_SCAN_SPECS, softplus, out is None), args, yd, hd, kept,
+                                               kept_size, at, size, _raw_stream(device)), "selective_scan_fwd")
+    results = (y,) + ((h_last,) if h_last is not None else ()) + ((saved,) if save else ())
+    return results if len(results) > 1 else y
 
 
 def selective_scan_bwd(u, delta, A, B, C, dy, saved, D=None, *, z=None, delta_bias=None, softplus: bool = False,
@@ -646,12 +643,7 @@ def selective_scan_bwd(u, delta, A, B, C, dy, saved, D=None, *, z=None, delta_bi
     device = _cuda_index(u)
     Bg, Cg = _groups("selective_scan_bwd", B, C, 4)
 
-    def like(t):
-        return _rows_like(t, None) if t is not None else None
-
-    grads = (_rows_like(u, lengths), _rows_like(delta, lengths), like(A), _rows_like(Bg, lengths),
-             _rows_like(Cg, lengths), like(D), _rows_like(z, lengths) if z is not None else None, like(delta_bias),
-             like(h0))
+    grads = tuple(_like(t) for t in (u, delta, A, Bg, Cg, D, z, delta_bias, h0))
     keep, args, gd, hd, sd, *outs = _describe("selective_scan_bwd", device, (
         ("u", u, 3), ("delta", delta, 3), ("A", A, 2), ("B", Bg, 4), ("C", Cg, 4), ("D", D, 1), ("z", z, 3),
         ("delta_bias", delta_bias, 1), ("h0", h0, 3), ("lengths", lengths, 1, _torch().int32), ("dy", dy, 3),
@@ -665,7 +657,7 @@ def selective_scan_bwd(u, delta, A, B, C, dy, saved, D=None, *, z=None, delta_bi
     lib, ctx = L.lib(), context(device).ptr
     scratch, at, size = _scratch(lib.remora_b200_selective_scan_bwd_scratch, "selective_scan_bwd", u, ctx, *u.shape,
                                  A.shape[1], Bg.shape[2])
-    L.check(lib.remora_b200_selective_scan_bwd(ctx, _spec(_SCAN_SPECS, softplus), args, gd, hd, saved.data_ptr(),
+    L.check(lib.remora_b200_selective_scan_bwd(ctx, _spec(_SCAN_SPECS, softplus, True), args, gd, hd, saved.data_ptr(),
                                                4 * saved.numel(), ctypes.addressof(to), at, size, _raw_stream(device)),
             "selective_scan_bwd")
     if B.dim() == 3:
@@ -681,14 +673,13 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, *, z=None, delta_bias=
     named by an earlier row is left out, as in causal_conv_step."""
     device = _cuda_index(u)
     Bg, Cg = _groups("selective_scan_step", B, C, 3)
-    if out is None:
-        out = _rows_like(u, slots)
+    y = out if out is not None else _like(u)
     if state_out is None:
         state_out = state
     keep, args, yd, od = _describe("selective_scan_step", device, (
         ("state", state, 3), ("u", u, 2), ("delta", delta, 2), ("A", A, 2), ("B", Bg, 3), ("C", Cg, 3), ("D", D, 1),
-        ("z", z, 2), ("delta_bias", delta_bias, 1), ("slots", slots, 1, _torch().int32), ("out", out, 2),
+        ("z", z, 2), ("delta_bias", delta_bias, 1), ("slots", slots, 1, _torch().int32), ("out", y, 2),
         ("state_out", state_out, 3)), table=10)
-    L.check(L.lib().remora_b200_selective_scan_step(context(device).ptr, _spec(_SCAN_SPECS, softplus), args, yd, od,
-                                                    _raw_stream(device)), "selective_scan_step")
-    return out
+    L.check(L.lib().remora_b200_selective_scan_step(context(device).ptr, _spec(_SCAN_SPECS, softplus, out is None), args,
+                                                    yd, od, _raw_stream(device)), "selective_scan_step")
+    return y
