@@ -151,8 +151,8 @@ __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 4 : 2) scan_fwd_kernel(
               in0 = pair(nv > 0 ? lo(in0) : 0.0f, nv > 1 ? hi(in0) : 0.0f);
               in1 = pair(nv > 2 ? lo(in1) : 0.0f, nv > 3 ? hi(in1) : 0.0f);
             }
-            h[c][0] = fma2(ex2_2(mul2(sp, A[c][0])), h[c][0], in0);
-            h[c][1] = fma2(ex2_2(mul2(sp, A[c][1])), h[c][1], in1);
+            h[c][0] = fma2(decay2(sp, A[c][0]), h[c][0], in0);
+            h[c][1] = fma2(decay2(sp, A[c][1]), h[c][1], in1);
             if (MAIN) {
               const f2 y = fma2(h[c][1], cc.y, mul2(h[c][0], cc.x));
               part[c][j] = lo(y) + hi(y);
@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(kScanThreads, NL > 4 ? 2 : 7) scan_step_kernel
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         if (a.vec || k < nv) {
-          h[r][k] = fmaf(ex2(sr * A[k]), h[r][k], sur * b[r][k]);
+          h[r][k] = fmaf(decay(sr, A[k]), h[r][k], sur * b[r][k]);
           part[r] = fmaf(h[r][k], c[r][k], part[r]);
         }
       float *o = a.state_out(slot[r], d, 4 * q);
@@ -402,7 +402,7 @@ void cut_time(int64_t batch, int64_t length, int64_t dim, int states, int groups
   const int64_t per_block = block_channels(nl, kChan), per = dim / std::max(groups, 1);
   const int64_t blocks = std::max<int64_t>(1, batch * groups * ((per + per_block - 1) / per_block));
   int64_t n = 1;
-  if (blocks < kCutBelow) n = std::max<int64_t>(1, std::min<int64_t>(kBlocks / blocks, length / 64));
+  if (blocks < kCutBelow) n = std::max<int64_t>(1, std::min<int64_t>(kBlocks / blocks, length / 16));
   *chunk = std::max<int64_t>(kTile, ((length + n - 1) / n + kTile - 1) / kTile * kTile);
   *chunks = std::max<int64_t>(1, (length + *chunk - 1) / *chunk);
 }

@@ -34,7 +34,7 @@ struct Bwd {
   static constexpr int kTile = NL > 4 ? 16 : 32;
 };
 
-constexpr int64_t kBlocks = 148 * 8;  // blocks of a cut time axis
+constexpr int64_t kBlocks = 148 * 16;  // blocks of a cut time axis
 constexpr int64_t kCutBelow = 148 * 2;
 
 int64_t bwd_channels(int nl) { return kScanThreads / nl * (nl > 8 ? 1 : 2); }  // of a block
@@ -205,8 +205,8 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const ScanArg
 #pragma unroll
           for (int c = 0; c < C; ++c) {
             const f2 sp = both(sj[c]), sup = both(suj[c]);
-            eh[t][c][0] = mul2(ex2_2(mul2(sp, A[c][0])), h[c][0]);
-            eh[t][c][1] = mul2(ex2_2(mul2(sp, A[c][1])), h[c][1]);
+            eh[t][c][0] = mul2(decay2(sp, A[c][0]), h[c][0]);
+            eh[t][c][1] = mul2(decay2(sp, A[c][1]), h[c][1]);
             h[c][0] = fma2(sup, b.x, eh[t][c][0]);
             h[c][1] = fma2(sup, b.y, eh[t][c][1]);
             const f2 y = fma2(h[c][1], cc.y, mul2(h[c][0], cc.x));
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const ScanArg
               g2 = k ? fma2(G[c][k], bk, g2) : mul2(G[c][k], bk);
               a2 = k ? fma2(gx, A[c][k], a2) : mul2(gx, A[c][k]);
               da[c][k] = fma2(gx, sp, da[c][k]);
-              G[c][k] = mul2(G[c][k], ex2_2(mul2(sp, A[c][k])));
+              G[c][k] = mul2(G[c][k], decay2(sp, A[c][k]));
             }
             gb[c][j] = lo(g2) + hi(g2);
             ga[c][j] = lo(a2) + hi(a2);
@@ -433,8 +433,8 @@ __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 4 : 2) scan_adjoint_ker
 #pragma unroll
         for (int c = 0; c < C; ++c) {
           const f2 sp = both(sj[c]), djp = both(dj[c]);
-          G[c][0] = mul2(fma2(cc.x, djp, G[c][0]), ex2_2(mul2(sp, A[c][0])));
-          G[c][1] = mul2(fma2(cc.y, djp, G[c][1]), ex2_2(mul2(sp, A[c][1])));
+          G[c][0] = mul2(fma2(cc.x, djp, G[c][0]), decay2(sp, A[c][0]));
+          G[c][1] = mul2(fma2(cc.y, djp, G[c][1]), decay2(sp, A[c][1]));
         }
       }
     }
@@ -482,10 +482,11 @@ __global__ void __launch_bounds__(256) join_bc_kernel(const ScanArgs a) {
   const float *p = a.part_bc + (bt * a.groups + g) * 2 * a.states + n;
   float vb = 0.0f, vc = 0.0f;
 #pragma unroll 8
-  for (int64_t k = 0; k < (rest ? 0 : a.blocks_d); ++k, p += 2 * plane) {
+  for (int64_t k = 0; k < a.blocks_d; ++k, p += 2 * plane) {
     vb += p[0];
     vc += p[a.states];
   }
+  if (rest) vb = vc = 0.0f;  // their shares were never written
   a.db.p[b * a.db.s0 + t * a.db.s1 + g * a.db.s2 + n * a.db.s3] = vb;
   a.dc.p[b * a.dc.s0 + t * a.dc.s1 + g * a.dc.s2 + n * a.dc.s3] = vc;
 }
@@ -500,7 +501,7 @@ void cut_time(int64_t batch, int64_t length, int64_t dim, int nl, int64_t groups
   const int64_t per_block = bwd_channels(nl), per = dim / std::max<int64_t>(groups, 1);
   const int64_t blocks = std::max<int64_t>(1, batch * groups * ((per + per_block - 1) / per_block));
   int64_t n = 1;
-  if (blocks < kCutBelow) n = std::max<int64_t>(1, std::min<int64_t>(kBlocks / blocks, length / 64));
+  if (blocks < kCutBelow) n = std::max<int64_t>(1, std::min<int64_t>(kBlocks / blocks, length / 16));
   *chunk = std::max<int64_t>(32, ((length + n - 1) / n + 31) / 32 * 32);
   *chunks = std::max<int64_t>(1, (length + *chunk - 1) / *chunk);
 }
