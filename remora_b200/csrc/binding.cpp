@@ -1,16 +1,20 @@
-// binding.cpp — the host side of a call from Python: lays out the descriptors
-// of a call's tensors in one buffer.  In Python this costs a microsecond per
-// tensor, more than the rest of a single-token call.
+// binding.cpp — the host side of a call from Python: makes the results that
+// the caller did not give and lays out the descriptors of a call's tensors in
+// one buffer.  In Python this costs a microsecond and more per tensor, more than
+// the rest of a single-token call.
 //
-//   describe(device, operands, table) -> (buffer, address, ...) or None
+//   describe(device, operands, table) -> (buffer, results, address, ...) or None
 //
-// operands: a tuple of (name, tensor or None, rank) or, for other types than
-// f32, (name, tensor or None, rank, dtype).  The buffer (bytes, to be kept until
-// the call returns) holds a RemoraMemRefN for each tensor; its address follows
-// in the tuple, None for None.  With table = k > 0 the first k addresses form an
-// argument struct at the buffer's start, whose address stands for them.  None is
-// returned when an operand is not a tensor of its type, rank and device: the
-// caller says which.
+// operands: a tuple of (name, tensor or None, rank), with a dtype as fourth
+// field for other types than f32, and for a result, as fifth field, what it is
+// made like where it was not given: a tensor whose shape it gets or a tuple of
+// sizes (None: left out).  `results` holds the operands with five fields, given
+// or made (contiguous and unset).  The buffer (bytes, to be kept until the call returns) holds a RemoraMemRefN for
+// each tensor; its address follows in the tuple, None for None.  With table = k
+// > 0 the first k addresses form an argument struct at the buffer's start, whose
+// address stands for them.  None is returned when an operand is not a tensor of
+// its type, rank and device: the caller says which.
+#include <ATen/ops/empty.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -37,25 +41,27 @@ PyObject *layout(PyObject *const *args, Py_ssize_t nargs) {
     PyErr_SetString(PyExc_ValueError, "describe: too many operands, or a table longer than they are");
     return nullptr;
   }
+  at::Tensor results[kMaxOperands];
   const at::Tensor *tensors[kMaxOperands];
   int64_t starts[kMaxOperands];  // all that may throw is done before memory is taken
   int64_t words = table;
   for (Py_ssize_t k = 0; k < n; ++k) {
     PyObject *item = PyTuple_GET_ITEM(operands, k);
     const Py_ssize_t fields = PyTuple_Check(item) ? PyTuple_GET_SIZE(item) : 0;
-    if (fields != 3 && fields != 4) {
-      PyErr_SetString(PyExc_TypeError, "describe: an operand is (name, tensor, rank) or (name, tensor, rank, dtype)");
+    if (fields < 3 || fields > 5) {
+      PyErr_SetString(PyExc_TypeError, "describe: an operand is (name, tensor, rank[, dtype[, shape]])");
       return nullptr;
     }
     PyObject *value = PyTuple_GET_ITEM(item, 1);
     tensors[k] = nullptr;
-    if (value == Py_None) continue;
-    if (!THPVariable_Check(value)) Py_RETURN_NONE;
-    const at::Tensor &t = THPVariable_Unpack(value);
+    PyObject *shape = fields == 5 ? PyTuple_GET_ITEM(item, 4) : Py_None;
+    const bool make = value == Py_None && shape != Py_None;
+    if (value == Py_None && !make) continue;
+    if (!make && !THPVariable_Check(value)) Py_RETURN_NONE;
     const long rank = PyLong_AsLong(PyTuple_GET_ITEM(item, 2));
     if (PyErr_Occurred()) return nullptr;
     at::ScalarType type = at::kFloat;
-    if (fields == 4) {
+    if (fields >= 4) {
       PyObject *d = PyTuple_GET_ITEM(item, 3);
       if (!THPDtype_Check(d)) {
         PyErr_SetString(PyExc_TypeError, "describe: the fourth field is a torch dtype");
@@ -63,6 +69,23 @@ PyObject *layout(PyObject *const *args, Py_ssize_t nargs) {
       }
       type = reinterpret_cast<THPDtype *>(d)->scalar_type;
     }
+    if (make) {
+      int64_t sizes[kMaxRank] = {0};
+      at::IntArrayRef of;
+      if (THPVariable_Check(shape)) {
+        of = THPVariable_Unpack(shape).sizes();
+      } else if (PyTuple_Check(shape) && PyTuple_GET_SIZE(shape) <= kMaxRank) {
+        for (Py_ssize_t d = 0; d < PyTuple_GET_SIZE(shape); ++d) sizes[d] = PyLong_AsLongLong(PyTuple_GET_ITEM(shape, d));
+        if (PyErr_Occurred()) return nullptr;
+        of = at::IntArrayRef(sizes, PyTuple_GET_SIZE(shape));
+      } else {
+        PyErr_SetString(PyExc_TypeError, "describe: the fifth field is a tensor or a tuple of at most 10 sizes");
+        return nullptr;
+      }
+      const at::Device place = device < 0 ? at::Device(at::kCPU) : at::Device(at::kCUDA, (at::DeviceIndex)device);
+      results[k] = at::empty(of, at::TensorOptions().dtype(type).device(place));
+    }
+    const at::Tensor &t = make ? results[k] : THPVariable_Unpack(value);
     if (t.scalar_type() != type || t.dim() != rank || rank > kMaxRank || t.get_device() != device ||
         !t.has_storage())
       Py_RETURN_NONE;
@@ -75,13 +98,29 @@ PyObject *layout(PyObject *const *args, Py_ssize_t nargs) {
   if (buffer == nullptr) return nullptr;
   char *base = PyBytes_AS_STRING(buffer);
   int64_t *out = reinterpret_cast<int64_t *>(base), *to = out + table;
-  PyObject *result = PyTuple_New(1 + (table ? 1 : 0) + n - table);
+  Py_ssize_t count = 0;
+  for (Py_ssize_t k = 0; k < n; ++k) count += PyTuple_GET_SIZE(PyTuple_GET_ITEM(operands, k)) == 5;
+  PyObject *made = PyTuple_New(count);
+  PyObject *result = made ? PyTuple_New(2 + (table ? 1 : 0) + n - table) : nullptr;
   if (result == nullptr) {
+    Py_XDECREF(made);
     Py_DECREF(buffer);
     return nullptr;
   }
+  count = 0;
+  for (Py_ssize_t k = 0; k < n; ++k) {
+    PyObject *item = PyTuple_GET_ITEM(operands, k);
+    if (PyTuple_GET_SIZE(item) != 5) continue;
+    PyObject *out = PyTuple_GET_ITEM(item, 1);
+    if (results[k].defined())
+      out = THPVariable_Wrap(results[k]);
+    else
+      Py_INCREF(out);
+    PyTuple_SET_ITEM(made, count++, out);
+  }
   PyTuple_SET_ITEM(result, 0, buffer);
-  Py_ssize_t at = 1;
+  PyTuple_SET_ITEM(result, 1, made);
+  Py_ssize_t at = 2;
   if (table) PyTuple_SET_ITEM(result, at++, PyLong_FromVoidPtr(base));
   for (Py_ssize_t k = 0; k < n; ++k) {
     const int64_t here = tensors[k] ? (int64_t)reinterpret_cast<uintptr_t>(to) : 0;
@@ -124,7 +163,7 @@ PyObject *describe(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
 
 PyMethodDef methods[] = {
     {"describe", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(describe)), METH_FASTCALL,
-     "describe(device, operands, table) -> (buffer, address, ...) or None"},
+     "describe(device, operands, table) -> (buffer, results, address, ...) or None"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_binding", "Descriptors of a call's tensors.", -1, methods,

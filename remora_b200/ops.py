@@ -388,14 +388,15 @@ def append(a, b, out=None):
 # rows of a given `out` stay as they were.
 #
 # A single-token call costs what the host does, so the operands of a call are
-# checked and laid out natively (csrc/binding.cpp), and results are made by the
-# cheapest torch call for each.
+# checked and laid out, and its results made, natively (csrc/binding.cpp).
 def _describe(what: str, device: int, operands, table: int = 0):
-    """Checks (name, tensor or None, rank[, dtype]) operands, f32 unless a
-    dtype is given, on CUDA device `device`.  Returns the buffer that holds
-    their descriptors, to be kept until the call returns, and the address of
-    each (None for None).  With `table`, one address stands for the first
-    `table`: that of a struct of their addresses."""
+    """Checks (name, tensor or None, rank[, dtype[, shape]]) operands, f32
+    unless a dtype is given, on CUDA device `device`; one with a shape (a
+    tensor's, or a tuple) is a result, made where it is None.  Returns the
+    buffer that holds their descriptors, to be kept until the call returns,
+    the tuple of results, and the address of each operand (None for None).
+    With `table`, one address stands for the first `table`: that of a struct
+    of their addresses."""
     described = _binding().describe(device, operands, table)
     if described is None:
         _refuse(what, device, operands)
@@ -420,8 +421,8 @@ _binding_module = None
 def _refuse(what: str, device: int, operands) -> None:
     """Raises for the first operand that describe() does not take."""
     torch = _torch()
-    for name, t, rank, *dtype in operands:
-        want = dtype[0] if dtype else torch.float32
+    for name, t, rank, *more in operands:
+        want = more[0] if more else torch.float32
         if t is None:
             continue
         if not isinstance(t, torch.Tensor):
@@ -461,12 +462,6 @@ def _scratch(fn, what: str, t, *sizes):
     return buf, buf.data_ptr(), n.value
 
 
-def _like(t):
-    """An unset contiguous result shaped as the f32 tensor t (None for None)."""
-    torch = _torch()
-    return torch.empty_like(t, memory_format=torch.contiguous_format) if t is not None else None
-
-
 # indexed by the flag and by zero_rest: set for results made here, whose rows
 # outside every sequence shall be zero, not for a caller's
 _CONV_SPECS = tuple(tuple(L.RemoraCausalConvSpec(k, zero) for zero in (0, 1)) for k in (0, 1))
@@ -481,11 +476,10 @@ def rms_norm_fwd(x, w, *, residual=None, eps: float = 1e-6, out=None, sum_out=No
     """s = x + residual; y = s / sqrt(mean(s^2) + eps) * w over the last axis
     (rank 1 to 4).  Returns y, and (y, s) with a residual.  `out` or `sum_out`
     may be x or the residual itself."""
-    device, rank = _cuda_index(x), x.dim()
-    y = out if out is not None else _like(x)
-    s = sum_out if sum_out is not None or residual is None else _like(x)
-    keep, xd, rd, wd, yd, sd = _describe("rms_norm_fwd", device, (
-        ("x", x, rank), ("residual", residual, rank), ("w", w, 1), ("out", y, rank), ("sum_out", s, rank)))
+    device, rank, f32 = _cuda_index(x), x.dim(), _torch().float32
+    keep, (y, s), xd, rd, wd, yd, sd = _describe("rms_norm_fwd", device, (
+        ("x", x, rank), ("residual", residual, rank), ("w", w, 1), ("out", out, rank, f32, x),
+        ("sum_out", sum_out, rank, f32, residual)))
     spec = L.RemoraNormSpec(eps, 0)
     L.check(L.lib().remora_b200_rms_norm_fwd(context(device).ptr, ctypes.addressof(spec), xd, rd, wd, yd, sd, rank,
                                              _raw_stream(device)), "rms_norm_fwd")
@@ -498,16 +492,11 @@ def rms_norm_quant(x, w, *, residual=None, eps: float = 1e-6, group: int = 0, ou
     max(max|y| / 448, 2^-126).  Returns (q, scales), and (q, scales, s) with a
     residual."""
     torch = _torch()
-    device, rank = _cuda_index(x), x.dim()
-    q = out
-    if q is None:
-        q = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
-    if scales is None:
-        scales = x.new_empty((*x.shape[:-1], x.shape[-1] // group if group > 0 and rank else 1))
-    s = sum_out if sum_out is not None or residual is None else _like(x)
-    keep, xd, rd, wd, cd, sd, qd = _describe("rms_norm_quant", device, (
-        ("x", x, rank), ("residual", residual, rank), ("w", w, 1), ("scales", scales, rank), ("sum_out", s, rank),
-        ("out", q, rank, torch.float8_e4m3fn)))
+    device, rank, f32 = _cuda_index(x), x.dim(), torch.float32
+    columns = x.shape[-1] // group if group > 0 and rank else 1
+    keep, (scales, s, q), xd, rd, wd, cd, sd, qd = _describe("rms_norm_quant", device, (
+        ("x", x, rank), ("residual", residual, rank), ("w", w, 1), ("scales", scales, rank, f32, (*x.shape[:-1], columns)),
+        ("sum_out", sum_out, rank, f32, residual), ("out", out, rank, torch.float8_e4m3fn, x)))
     spec = L.RemoraNormSpec(eps, group)
     L.check(L.lib().remora_b200_rms_norm_quant(context(device).ptr, ctypes.addressof(spec), xd, rd, wd, qd, cd, sd,
                                                rank, _raw_stream(device)), "rms_norm_quant")
@@ -519,11 +508,10 @@ def rms_norm_bwd(s, w, dy, *, dsum=None, eps: float = 1e-6, out=None):
     (dx, dw), dx being the gradient of x and of the residual alike; dsum is
     the gradient that reaches s from its other readers.  `out` (dx) may be s,
     dy or dsum itself."""
-    device, rank = _cuda_index(s), s.dim()
-    dx = out if out is not None else _like(s)
-    dw = _like(w)
-    keep, sd, wd, gd, ed, xd, dwd = _describe("rms_norm_bwd", device, (
-        ("s", s, rank), ("w", w, 1), ("dy", dy, rank), ("dsum", dsum, rank), ("out", dx, rank), ("dw", dw, 1)))
+    device, rank, f32 = _cuda_index(s), s.dim(), _torch().float32
+    keep, (dx, dw), sd, wd, gd, ed, xd, dwd = _describe("rms_norm_bwd", device, (
+        ("s", s, rank), ("w", w, 1), ("dy", dy, rank), ("dsum", dsum, rank), ("out", out, rank, f32, s),
+        ("dw", None, 1, f32, w)))
     lib, ctx = L.lib(), context(device).ptr
     dim = s.shape[-1] if rank else 0
     scratch, at, size = _scratch(lib.remora_b200_rms_norm_bwd_scratch, "rms_norm_bwd", s, ctx,
@@ -542,13 +530,11 @@ def causal_conv_fwd(x, w, bias=None, *, state=None, lengths=None, silu: bool = F
     return_state (or state_out, which may be `state` itself) returns
     (y, the state that continues the sequence), else y."""
     torch = _torch()
-    device = _cuda_index(x)
-    y = out if out is not None else _like(x)
-    if state_out is None and return_state and x.dim() == 3 and w.dim() == 2:
-        state_out = x.new_empty((x.shape[0], max(w.shape[1] - 1, 0), x.shape[2]))
-    keep, xd, wd, bd, sd, yd, od, ld = _describe("causal_conv_fwd", device, (
-        ("x", x, 3), ("w", w, 2), ("bias", bias, 1), ("state", state, 3), ("out", y, 3),
-        ("state_out", state_out, 3), ("lengths", lengths, 1, torch.int32)))
+    device, f32 = _cuda_index(x), torch.float32
+    wanted = (x.shape[0], w.shape[1] - 1, x.shape[2]) if return_state and x.dim() == 3 and w.dim() == 2 else None
+    keep, (y, state_out), xd, wd, bd, sd, yd, od, ld = _describe("causal_conv_fwd", device, (
+        ("x", x, 3), ("w", w, 2), ("bias", bias, 1), ("state", state, 3), ("out", out, 3, f32, x),
+        ("state_out", state_out, 3, f32, wanted), ("lengths", lengths, 1, torch.int32)))
     L.check(L.lib().remora_b200_causal_conv_fwd(context(device).ptr, _spec(_CONV_SPECS, silu, out is None), xd, wd, bd,
                                                 sd, ld, yd, od, _raw_stream(device)), "causal_conv_fwd")
     return y if state_out is None else (y, state_out)
@@ -558,15 +544,12 @@ def causal_conv_bwd(x, w, dy, bias=None, *, state=None, lengths=None, silu: bool
     """Gradients of causal_conv_fwd: (dx, dw, dbias, dstate), dbias and dstate
     None where bias or state is.  dstate_out is the gradient that reaches the
     returned state; `out` receives dx."""
-    device = _cuda_index(x)
-    dx = out if out is not None else _like(x)
-    dw = _like(w)
-    dbias = _like(bias)
-    dstate = _like(state)
-    keep, xd, wd, bd, sd, gd, ed, dxd, dwd, dbd, dsd, ld = _describe("causal_conv_bwd", device, (
+    torch = _torch()
+    device, f32 = _cuda_index(x), torch.float32
+    keep, (dx, dw, dbias, dstate), xd, wd, bd, sd, gd, ed, dxd, dwd, dbd, dsd, ld = _describe("causal_conv_bwd", device, (
         ("x", x, 3), ("w", w, 2), ("bias", bias, 1), ("state", state, 3), ("dy", dy, 3), ("dstate_out", dstate_out, 3),
-        ("out", dx, 3), ("dw", dw, 2), ("dbias", dbias, 1), ("dstate", dstate, 3),
-        ("lengths", lengths, 1, _torch().int32)))
+        ("out", out, 3, f32, x), ("dw", None, 2, f32, w), ("dbias", None, 1, f32, bias),
+        ("dstate", None, 3, f32, state), ("lengths", lengths, 1, torch.int32)))
     lib, ctx = L.lib(), context(device).ptr
     scratch, at, size = _scratch(lib.remora_b200_causal_conv_bwd_scratch, "causal_conv_bwd", x, ctx, *x.shape,
                                  w.shape[1])
@@ -580,13 +563,13 @@ def causal_conv_step(x, state, w, bias=None, *, silu: bool = False, slots=None, 
     moved on in place (or into state_out).  Row i uses state row slots[i], or
     row i without slots; a row whose slot is -1 or was named by an earlier row
     is left out (its y is zero, or as it was in a given `out`)."""
+    torch = _torch()
     device = _cuda_index(x)
-    y = out if out is not None else _like(x)
     if state_out is None:
         state_out = state
-    keep, xd, sd, wd, bd, yd, od, ld = _describe("causal_conv_step", device, (
-        ("x", x, 2), ("state", state, 3), ("w", w, 2), ("bias", bias, 1), ("out", y, 2), ("state_out", state_out, 3),
-        ("slots", slots, 1, _torch().int32)))
+    keep, (y,), xd, sd, wd, bd, yd, od, ld = _describe("causal_conv_step", device, (
+        ("x", x, 2), ("state", state, 3), ("w", w, 2), ("bias", bias, 1), ("out", out, 2, torch.float32, x),
+        ("state_out", state_out, 3), ("slots", slots, 1, torch.int32)))
     L.check(L.lib().remora_b200_causal_conv_step(context(device).ptr, _spec(_CONV_SPECS, silu, out is None), xd, sd, wd,
                                                  bd, ld, yd, od, _raw_stream(device)), "causal_conv_step")
     return y
@@ -611,13 +594,12 @@ def selective_scan_fwd(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, so
     torch = _torch()
     device = _cuda_index(u)
     Bg, Cg = _groups("selective_scan_fwd", B, C, 4)
-    y = out if out is not None else _like(u)
-    if h_last is None and return_state and u.dim() == 3 and A.dim() == 2:
-        h_last = u.new_empty((u.shape[0], u.shape[2], A.shape[1]))
-    keep, args, yd, hd = _describe("selective_scan_fwd", device, (
+    f32 = torch.float32
+    wanted = (u.shape[0], u.shape[2], A.shape[1]) if return_state and u.dim() == 3 and A.dim() == 2 else None
+    keep, (y, h_last), args, yd, hd = _describe("selective_scan_fwd", device, (
         ("u", u, 3), ("delta", delta, 3), ("A", A, 2), ("B", Bg, 4), ("C", Cg, 4), ("D", D, 1), ("z", z, 3),
-        ("delta_bias", delta_bias, 1), ("h0", h0, 3), ("lengths", lengths, 1, torch.int32), ("out", y, 3),
-        ("h_last", h_last, 3)), table=10)
+        ("delta_bias", delta_bias, 1), ("h0", h0, 3), ("lengths", lengths, 1, torch.int32), ("out", out, 3, f32, u),
+        ("h_last", h_last, 3, f32, wanted)), table=10)
     lib, ctx = L.lib(), context(device).ptr
     sizes = (*u.shape, A.shape[1])
     scratch, at, size = _scratch(lib.remora_b200_selective_scan_fwd_scratch, "selective_scan_fwd", u, ctx, *sizes,
@@ -643,14 +625,13 @@ def selective_scan_bwd(u, delta, A, B, C, dy, saved, D=None, *, z=None, delta_bi
     device = _cuda_index(u)
     Bg, Cg = _groups("selective_scan_bwd", B, C, 4)
 
-    grads = tuple(_like(t) for t in (u, delta, A, Bg, Cg, D, z, delta_bias, h0))
-    keep, args, gd, hd, sd, *outs = _describe("selective_scan_bwd", device, (
+    f32 = _torch().float32
+    keep, grads, args, gd, hd, sd, *outs = _describe("selective_scan_bwd", device, (
         ("u", u, 3), ("delta", delta, 3), ("A", A, 2), ("B", Bg, 4), ("C", Cg, 4), ("D", D, 1), ("z", z, 3),
         ("delta_bias", delta_bias, 1), ("h0", h0, 3), ("lengths", lengths, 1, _torch().int32), ("dy", dy, 3),
-        ("dh_last", dh_last, 3),
-        ("saved", saved, 1), ("du", grads[0], 3), ("ddelta", grads[1], 3), ("dA", grads[2], 2), ("dB", grads[3], 4),
-        ("dC", grads[4], 4), ("dD", grads[5], 1), ("dz", grads[6], 3), ("ddelta_bias", grads[7], 1),
-        ("dh0", grads[8], 3)), table=10)
+        ("dh_last", dh_last, 3), ("saved", saved, 1), ("du", None, 3, f32, u), ("ddelta", None, 3, f32, delta),
+        ("dA", None, 2, f32, A), ("dB", None, 4, f32, Bg), ("dC", None, 4, f32, Cg), ("dD", None, 1, f32, D),
+        ("dz", None, 3, f32, z), ("ddelta_bias", None, 1, f32, delta_bias), ("dh0", None, 3, f32, h0)), table=10)
     if saved is None or not saved.is_contiguous():
         raise RemoraUnsupportedError("selective_scan_bwd: saved is not what selective_scan_fwd returned")
     to = L.RemoraSelectiveScanGrads(*outs)
@@ -673,12 +654,12 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, *, z=None, delta_bias=
     named by an earlier row is left out, as in causal_conv_step."""
     device = _cuda_index(u)
     Bg, Cg = _groups("selective_scan_step", B, C, 3)
-    y = out if out is not None else _like(u)
+    torch = _torch()
     if state_out is None:
         state_out = state
-    keep, args, yd, od = _describe("selective_scan_step", device, (
+    keep, (y,), args, yd, od = _describe("selective_scan_step", device, (
         ("state", state, 3), ("u", u, 2), ("delta", delta, 2), ("A", A, 2), ("B", Bg, 3), ("C", Cg, 3), ("D", D, 1),
-        ("z", z, 2), ("delta_bias", delta_bias, 1), ("slots", slots, 1, _torch().int32), ("out", y, 2),
+        ("z", z, 2), ("delta_bias", delta_bias, 1), ("slots", slots, 1, torch.int32), ("out", out, 2, torch.float32, u),
         ("state_out", state_out, 3)), table=10)
     L.check(L.lib().remora_b200_selective_scan_step(context(device).ptr, _spec(_SCAN_SPECS, softplus, out is None), args,
                                                     yd, od, _raw_stream(device)), "selective_scan_step")

@@ -203,7 +203,8 @@ def test_binding_lays_out_descriptors():
     operands = tuple((f"t{k}", t, t.dim()) for k, t in enumerate(views)) + (
         ("none", None, 2), ("ints", torch.arange(3, dtype=torch.int32), 1, torch.int32))
     for table in (0, 2, len(operands)):
-        buf, *at = _binding.describe(-1, operands, table)
+        buf, results, *at = _binding.describe(-1, operands, table)
+        assert results == ()
         if table:
             first = ctypes.cast(at[0], ctypes.POINTER(ctypes.c_uint64))
             at = [first[k] or None for k in range(table)] + at[1:]
@@ -216,6 +217,15 @@ def test_binding_lays_out_descriptors():
                 want.allocated = want.aligned = 0
             assert ctypes.string_at(address, ctypes.sizeof(want)) == bytes(want)
     one = torch.zeros(2, 3)
+    got = _binding.describe(-1, (("a", None, 2, torch.float32, one.t()), ("b", one, 2, torch.float32, one),
+                                 ("c", None, 2, torch.float32, None), ("d", None, 1, torch.int32, (7,))), 0)
+    made, given, absent, ints = got[1]
+    assert made.shape == (3, 2) and made.is_contiguous() and made.dtype == torch.float32
+    assert given is one and absent is None and ints.shape == (7,) and ints.dtype == torch.int32
+    assert got[4] is None
+    for address, t in zip((got[2], got[3], got[5]), (made, one, ints)):
+        want = tensor_descriptor(t)
+        assert ctypes.string_at(address, ctypes.sizeof(want)) == bytes(want)
     for bad in (("x", one, 3), ("x", one.double(), 2), ("x", one, 2, torch.int32), ("x", 3.0, 0), ("x", one.to_sparse(), 2)):
         assert _binding.describe(-1, (bad,), 0) is None
     assert _binding.describe(0, (("x", one, 2),), 0) is None  # another device
