@@ -36,6 +36,10 @@ inline int read_f32(const void *desc, int rank, DescView *out, const char *what)
   return REMORA_OK;
 }
 
+// An axis of one element has no stride to speak of: 0, whatever it says, so
+// that no check of strides trips over it.
+inline int64_t stride_of(const DescView &v, int d) { return v.sizes[d] > 1 ? v.strides[d] : 0; }
+
 // As read_f32, and leaves *have false for a null descriptor.
 inline int read_optional(const void *desc, int rank, DescView *out, bool *have, const char *what) {
   *have = desc != nullptr;
@@ -60,53 +64,76 @@ inline bool same_view(const DescView &a, const DescView &b) {
   return true;
 }
 
-// Byte range of a view's elements.
-inline void byte_range(const DescView &v, int esize, uintptr_t *lo, uintptr_t *hi) {
-  int64_t mn = 0, mx = 0;
-  for (int d = 0; d < v.rank; ++d) {
-    const int64_t span = (v.sizes[d] - 1) * v.strides[d];
-    (span < 0 ? mn : mx) += span;
+// Whether two views share a byte: whether the difference of their addresses is
+// a sum of index times stride over the axes of both.  The axes, all made to
+// count upwards, are tried from the largest stride down; what those below can
+// still add up to leaves one or two indices to try on each of an ordinary
+// view's axes.  Views so irregular that this takes long count as overlapping.
+struct Overlap {
+  struct Axis {
+    int64_t stride, size;
+  } axes[2 * (REMORA_MAX_RANK + 1)];
+  int count = 0;
+  int64_t rest[2 * (REMORA_MAX_RANK + 1) + 1];  // the most that axes from here on add up to
+  int64_t target;
+  int budget = 1 << 14;
+
+  void add(int64_t stride, int64_t size) {
+    if (size <= 1 || stride == 0) return;
+    if (stride < 0) {  // from the other end
+      target -= stride * (size - 1);
+      stride = -stride;
+    }
+    for (int k = 0; k < count; ++k)
+      if (axes[k].stride == stride) {
+        axes[k].size += size - 1;
+        return;
+      }
+    axes[count++] = {stride, size};
   }
-  const uintptr_t base = reinterpret_cast<uintptr_t>(v.aligned) + (uintptr_t)(v.offset * esize);
-  *lo = base + (uintptr_t)(mn * esize);
-  *hi = base + (uintptr_t)(mx * esize) + (uintptr_t)esize;
+
+  bool hits(int i, int64_t left) {
+    if (left < 0 || left > rest[i]) return false;
+    if (i == count || left == 0) return true;
+    if (--budget < 0) return true;
+    int64_t k = left / axes[i].stride;
+    if (k > axes[i].size - 1) k = axes[i].size - 1;
+    for (; k >= 0 && left - k * axes[i].stride <= rest[i + 1]; --k)
+      if (hits(i + 1, left - k * axes[i].stride)) return true;
+    return false;
+  }
+};
+
+// Byte range of a view's elements.
+inline void byte_range(const DescView &v, int esize, char **lo, char **hi) {
+  *lo = *hi = v.aligned + v.offset * esize;
+  for (int d = 0; d < v.rank; ++d) {
+    const int64_t span = (v.sizes[d] - 1) * v.strides[d] * esize;
+    (span < 0 ? *lo : *hi) += span;
+  }
+  *hi += esize;
 }
 
-// Whether two views may share a byte.  Ranges that meet are still apart when
-// both views are columns of rows with one pitch (strides that are multiples
-// of it, but for a unit stride along the row) and their columns are apart.
 inline bool may_overlap(const DescView &a, int ea, const DescView &b, int eb) {
   if (a.numel() == 0 || b.numel() == 0) return false;
-  uintptr_t alo, ahi, blo, bhi;
+  char *alo, *ahi, *blo, *bhi;
   byte_range(a, ea, &alo, &ahi);
   byte_range(b, eb, &blo, &bhi);
   if (ahi <= blo || bhi <= alo) return false;
-  int64_t pitch = 0;  // bytes: the largest common row pitch of the two
-  const DescView *vs[2] = {&a, &b};
-  const int es[2] = {ea, eb};
-  int64_t extent[2] = {ea, eb};
-  for (int k = 0; k < 2; ++k)
-    for (int d = 0; d < vs[k]->rank; ++d) {
-      if (vs[k]->sizes[d] <= 1) continue;
-      const int64_t st = vs[k]->strides[d] * es[k];
-      if (st == es[k]) {
-        extent[k] = vs[k]->sizes[d] * (int64_t)es[k];
-        continue;
-      }
-      if (st <= 0) return true;
-      int64_t x = pitch, y = st;  // gcd
-      while (y) {
-        const int64_t t = x % y;
-        x = y;
-        y = t;
-      }
-      pitch = x;
+  Overlap o;
+  o.target = (b.aligned + b.offset * eb) - (a.aligned + a.offset * ea);
+  for (int d = 0; d < a.rank; ++d) o.add(a.strides[d] * ea, a.sizes[d]);
+  for (int d = 0; d < b.rank; ++d) o.add(-b.strides[d] * eb, b.sizes[d]);
+  o.add(1, ea);
+  o.add(-1, eb);
+  for (int i = 1; i < o.count; ++i)  // the largest stride first
+    for (int k = i; k > 0 && o.axes[k - 1].stride < o.axes[k].stride; --k) {
+      const Overlap::Axis t = o.axes[k];
+      o.axes[k] = o.axes[k - 1], o.axes[k - 1] = t;
     }
-  if (pitch == 0) return true;
-  // b's columns start `gap` bytes behind a's, in a's row or the next
-  int64_t gap = ((b.aligned + b.offset * eb) - (a.aligned + a.offset * ea)) % pitch;
-  if (gap < 0) gap += pitch;
-  return gap < extent[0] || gap + extent[1] > pitch;
+  o.rest[o.count] = 0;
+  for (int i = o.count - 1; i >= 0; --i) o.rest[i] = o.rest[i + 1] + o.axes[i].stride * (o.axes[i].size - 1);
+  return o.hits(0, o.target);
 }
 
 // An output whose own elements share addresses (a stride of 0 over more than

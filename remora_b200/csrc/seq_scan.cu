@@ -377,14 +377,6 @@ __global__ void __launch_bounds__(kScanThreads, NL > 4 ? 2 : 7) scan_step_kernel
 }
 
 // ------------------------------------------------------------------ host --
-Op3 op3(const DescView &v) {
-  return {reinterpret_cast<float *>(v.data(4)), v.strides[0], v.strides[1], v.strides[2]};
-}
-
-Op4 op4(const DescView &v) {
-  return {reinterpret_cast<float *>(v.data(4)), v.strides[0], v.strides[1], v.strides[2], v.strides[3]};
-}
-
 // Rows that 16-byte copies can take: unit stride, a multiple of four states,
 // every row 16-byte aligned.
 bool vec_states(const DescView &v) {
@@ -614,7 +606,7 @@ int remora_b200_selective_scan_step(RemoraB200Ctx *ctx, const RemoraSelectiveSca
                          {&cv, "c", 4}, {has_d ? &dv : nullptr, "d", 4}, {has_z ? &zv : nullptr, "z", 4},
                          {has_i ? &iv : nullptr, "delta_bias", 4}, {has_l ? &lv : nullptr, "slots", 4}}, {&sv}));
   if (B == 0 || D == 0) return REMORA_OK;
-  if (std::max(std::max(D, S), N) > 0x3fffffff) return fail(REMORA_ERR_LIMIT, "selective_scan_step: more than 2^30 rows");
+  if (std::max(D, S) > 0x3fffffff) return fail(REMORA_ERR_LIMIT, "selective_scan_step: more than 2^30 rows");
   TokenArgs a = {};
   // each operand's place in Token: row, channel (or group), state
   struct {
@@ -629,13 +621,13 @@ int remora_b200_selective_scan_step(RemoraB200Ctx *ctx, const RemoraSelectiveSca
   for (const auto &x : places) {
     if (x.v == nullptr) continue;
     for (int k = 0; k < x.v->rank; ++k)
-      if (std::abs(x.v->strides[k]) > 0x7fffffff)
+      if (std::abs(stride_of(*x.v, k)) > 0x7fffffff)
         return fail(REMORA_ERR_LIMIT, "selective_scan_step: a stride of %lld elements (at most 2^31 - 1)",
                     (long long)x.v->strides[k]);
-    auto stride = [&](int k) { return k < 0 ? 0 : (int)x.v->strides[k]; };
+    auto stride = [&](int k) { return k < 0 ? 0 : (int)stride_of(*x.v, k); };
     if (x.to) *x.to = {reinterpret_cast<float *>(x.v->data(4)), stride(x.row), stride(x.channel), stride(x.state)};
   }
-  if (has_l) a.slots = reinterpret_cast<const int *>(lv.data(4)), a.slots_s = (int)lv.strides[0];
+  if (has_l) a.slots = reinterpret_cast<const int *>(lv.data(4)), a.slots_s = (int)stride_of(lv, 0);
   a.batch = (int)B, a.rows = (int)S, a.dim = (int)D, a.per = (int)(D / G), a.states = (int)N, a.groups = (int)G;
   a.softplus = spec->softplus != 0, a.zero_rest = spec->zero_rest != 0;
   a.vec = vec_states(sv) && vec_states(ov) && vec_states(av) && vec_states(bv) && vec_states(cv);

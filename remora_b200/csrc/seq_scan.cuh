@@ -69,12 +69,12 @@ inline int64_t block_channels(int nl, int chan) { return (int64_t)kScanThreads /
 
 // Lane's 32-bit offsets reach the block's channels and a lane group's steps.
 inline int check_reach(const DescView &v, int nl, int chan, const char *what) {
-  auto size = [](int64_t x) { return x < 0 ? -x : x; };
   const int64_t most = (int64_t)1 << 30;
-  if (size(v.strides[1]) > most || size(v.strides[2]) > most ||
-      size(v.strides[2]) * (block_channels(nl, chan) - 1) + size(v.strides[1]) * (nl - 1) >= most)
-    return fail(REMORA_ERR_LIMIT, "%s: strides of %lld and %lld elements spread a block's channels over 2^30", what,
-                (long long)v.strides[1], (long long)v.strides[2]);
+  const int64_t s1 = stride_of(v, 1) < 0 ? -stride_of(v, 1) : stride_of(v, 1);
+  const int64_t s2 = stride_of(v, 2) < 0 ? -stride_of(v, 2) : stride_of(v, 2);
+  if (s1 > most || s2 > most || s2 * (block_channels(nl, chan) - 1) + s1 * (nl - 1) >= most)
+    return fail(REMORA_ERR_LIMIT, "%s: time and channel strides of %lld and %lld elements spread a block over 2^30", what,
+                (long long)s1, (long long)s2);
   return REMORA_OK;
 }
 
@@ -83,6 +83,14 @@ inline int lanes_for(int states) {
   int nl = 1;
   while (nl * 4 < states) nl *= 2;
   return nl;
+}
+
+inline Op3 op3(const DescView &v) {
+  return {reinterpret_cast<float *>(v.data(4)), stride_of(v, 0), stride_of(v, 1), stride_of(v, 2)};
+}
+
+inline Op4 op4(const DescView &v) {
+  return {reinterpret_cast<float *>(v.data(4)), stride_of(v, 0), stride_of(v, 1), stride_of(v, 2), stride_of(v, 3)};
 }
 
 int read_scan_in(const RemoraSelectiveScanSpec *spec, const RemoraSelectiveScanIn *in, ScanArgs *a, DescView views[10],

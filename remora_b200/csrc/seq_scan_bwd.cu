@@ -492,10 +492,6 @@ __global__ void __launch_bounds__(256) join_bc_kernel(const ScanArgs a) {
 }
 
 // ------------------------------------------------------------------ host --
-Op3 op3(const DescView &v) {
-  return {reinterpret_cast<float *>(v.data(4)), v.strides[0], v.strides[1], v.strides[2]};
-}
-
 // As the forward's: pieces only where the channels give too few warps.
 void cut_time(int64_t batch, int64_t length, int64_t dim, int nl, int64_t groups, int64_t *chunks, int64_t *chunk) {
   const int64_t per_block = bwd_channels(nl), per = dim / std::max<int64_t>(groups, 1);
@@ -636,8 +632,7 @@ int remora_b200_selective_scan_bwd(RemoraB200Ctx *ctx, const RemoraSelectiveScan
   a.dy = op3(gy);
   if (has_gh) a.dh_last = op3(gh);
   a.du = op3(o[0]), a.ddelta = op3(o[1]);
-  a.db = {reinterpret_cast<float *>(o[3].data(4)), o[3].strides[0], o[3].strides[1], o[3].strides[2], o[3].strides[3]};
-  a.dc = {reinterpret_cast<float *>(o[4].data(4)), o[4].strides[0], o[4].strides[1], o[4].strides[2], o[4].strides[3]};
+  a.db = op4(o[3]), a.dc = op4(o[4]);
   if (have[6]) a.dz = op3(o[6]);
   if (have[8]) a.dh0 = op3(o[8]);
   a.chunks = l.chunks, a.chunk = l.chunk;

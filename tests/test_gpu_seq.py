@@ -509,6 +509,120 @@ def test_scan_bad_values_stay_in_their_channel(cuda, N):
     np.testing.assert_allclose(y, want, rtol=1e-4, atol=1e-5)
 
 
+def test_offsets_past_32_bits(cuda):
+    """Rows whose addresses lie more than 2^32 bytes apart, and axes of one
+    element with strides that mean nothing."""
+    import torch
+
+    rng = np.random.default_rng(13)
+    far = 1 << 30  # elements: 4 GiB
+    buf = torch.empty(2 * far + (1 << 20), dtype=torch.float32, device=cuda)
+    D, N, T = 20, 16, 9
+    wide = buf.as_strided((3, T, D), (far, 4 * D, 1))
+    x = dev(rnd(rng, 3, T, D), cuda)
+    wide.copy_(x)
+    w = dev(rnd(rng, D), cuda)
+    np.testing.assert_array_equal(to_host(ops.rms_norm_fwd(wide, w)), to_host(ops.rms_norm_fwd(x, w)))
+    cw, cb = dev(rnd(rng, D, 4), cuda), dev(rnd(rng, D), cuda)
+    np.testing.assert_array_equal(to_host(ops.causal_conv_fwd(wide, cw, cb)), to_host(ops.causal_conv_fwd(x, cw, cb)))
+    A, b, c = dev(-np.abs(rnd(rng, D, N)), cuda), dev(rnd(rng, 3, T, N), cuda), dev(rnd(rng, 3, T, N), cuda)
+    want = ops.selective_scan_fwd(x, x, A, b, c, softplus=True, z=x, save=True, return_state=True)
+    out = buf.as_strided((3, T, D), (far, 4 * D, 1), D)  # beside the input
+    got = ops.selective_scan_fwd(wide, wide, A, b, c, softplus=True, z=wide, save=True, return_state=True, out=out)
+    for g, r in zip(got, want):
+        np.testing.assert_array_equal(to_host(g), to_host(r))
+    for g, r in zip(ops.selective_scan_bwd(wide, wide, A, b, c, wide, got[2], z=wide, softplus=True),
+                    ops.selective_scan_bwd(x, x, A, b, c, x, want[2], z=x, softplus=True)):
+        if g is not None:
+            np.testing.assert_array_equal(to_host(g), to_host(r))
+    state = buf.as_strided((3, D, N), (far, N, 1), 1 << 12)
+    state.copy_(want[1])
+    y = ops.selective_scan_step(state, x[:, 0], x[:, 1], A, b[:, 0], c[:, 0], softplus=True)
+    plain = want[1].clone()
+    np.testing.assert_array_equal(to_host(y), to_host(ops.selective_scan_step(plain, x[:, 0], x[:, 1], A, b[:, 0],
+                                                                             c[:, 0], softplus=True)))
+    np.testing.assert_array_equal(to_host(state), to_host(plain))
+    one = x[:1, :1].as_strided((1, 1, D), (1 << 40, 1 << 40, 1))
+    y = ops.selective_scan_fwd(one, one, A, b[:1, :1], c[:1, :1], softplus=True)
+    np.testing.assert_array_equal(to_host(y)[0, 0], to_host(ops.selective_scan_fwd(x, x, A, b, c, softplus=True))[0, 0])
+    del buf
+
+
+def test_negative_strides_through_the_c_abi(cuda):
+    """Descriptors may run backwards (torch views cannot): time and channels
+    reversed give the reversed arrays' results."""
+    import ctypes
+
+    import torch
+
+    from remora_b200 import _lib as L
+    from remora_b200.abi import make_memref_descriptor, tensor_descriptor
+    from remora_b200.runtime import context
+
+    rng = np.random.default_rng(14)
+    B, T, D, N = 2, 21, 70, 16
+    u, delta = dev(rnd(rng, B, T, D), cuda), dev(rnd(rng, B, T, D), cuda)
+    A, b, c = dev(-np.abs(rnd(rng, D, N)), cuda), dev(rnd(rng, B, T, 1, N), cuda), dev(rnd(rng, B, T, 1, N), cuda)
+    back = make_memref_descriptor(u.data_ptr(), (B, T, D), (T * D, -D, -1), offset=(T - 1) * D + D - 1)
+    y, out = torch.zeros_like(u), torch.zeros_like(u)
+    rev = make_memref_descriptor(out.data_ptr(), (B, T, D), (T * D, -D, -1), offset=(T - 1) * D + D - 1)
+    want = ops.selective_scan_fwd(u.flip(1, 2).contiguous(), delta, A, b, c, softplus=True)
+    descs = [tensor_descriptor(t) for t in (delta, A, b, c)]
+    spec = L.RemoraSelectiveScanSpec(1, 0)
+    stream = ctypes.c_void_p(torch.cuda.current_stream(cuda).cuda_stream)
+    for to, result in ((tensor_descriptor(y), lambda: y), (rev, lambda: out.flip(1, 2))):
+        args = L.RemoraSelectiveScanIn(ctypes.addressof(back), *(ctypes.addressof(x) for x in descs))
+        n = ctypes.c_size_t()
+        lib, ctx = L.lib(), context(0).ptr
+        L.check(lib.remora_b200_selective_scan_fwd_scratch(ctx, B, T, D, N, 1, ctypes.byref(n)))
+        scratch = torch.empty(n.value + 16, dtype=torch.uint8, device=cuda)
+        L.check(lib.remora_b200_selective_scan_fwd(ctx, ctypes.addressof(spec), ctypes.addressof(args),
+                                                   ctypes.addressof(to), None, None, 0, scratch.data_ptr(), n.value,
+                                                   stream))
+        np.testing.assert_array_equal(to_host(result()), to_host(want))
+    cw = dev(rnd(rng, D, 3), cuda)
+    conv = L.RemoraCausalConvSpec(0, 0)
+    wd, to = tensor_descriptor(cw), tensor_descriptor(y)
+    L.check(lib.remora_b200_causal_conv_fwd(ctx, ctypes.addressof(conv), ctypes.addressof(back), ctypes.addressof(wd),
+                                            None, None, None, ctypes.addressof(to), None, stream))
+    np.testing.assert_array_equal(to_host(y), to_host(ops.causal_conv_fwd(u.flip(1, 2).contiguous(), cw)))
+
+
+def test_rows_of_no_sequence(cuda):
+    """Zero in results made by the call, as they were in a caller's."""
+    import torch
+
+    rng = np.random.default_rng(15)
+    B, T = 3, 90
+    lengths = torch.tensor([90, 0, 41], dtype=torch.int32, device=cuda)
+    for D, N, G in ((10, 16, 1), (200, 5, 2)):
+        v = scan_inputs(rng, B, T, D, N, G, True)
+        pos, Dv, kw = scan_own(v, cuda)
+        y, saved = ops.selective_scan_fwd(*pos, Dv, softplus=True, lengths=lengths, save=True, **kw)
+        grads = ops.selective_scan_bwd(*pos, pos[0], saved, Dv, softplus=True, lengths=lengths, **kw)
+        for t in (y, grads[0], grads[1], grads[3], grads[4], grads[6]):
+            t = to_host(t)
+            assert (t[1] == 0).all() and (t[2, 41:] == 0).all() and (t[2, :41] != 0).any()
+        kept = torch.full((B, T, D), 7.0, device=cuda)
+        ops.selective_scan_fwd(*pos, Dv, softplus=True, lengths=lengths, out=kept, **kw)
+        kept = to_host(kept)
+        assert (kept[1] == 7).all() and (kept[2, 41:] == 7).all()
+        np.testing.assert_array_equal(kept[2, :41], to_host(y)[2, :41])
+
+
+def test_norm_of_four_axes(cuda):
+    rng = np.random.default_rng(16)
+    x = dev(rnd(rng, 3, 2, 5, 4, 12), cuda)[:, 1].permute(1, 0, 2, 3)  # axes that do not collapse
+    w = dev(rnd(rng, 12), cuda)
+    y = ops.rms_norm_fwd(x, w)
+    np.testing.assert_array_equal(to_host(y), to_host(ops.rms_norm_fwd(x.contiguous(), w)))
+    q, sc = ops.rms_norm_quant(x, w)
+    q2, sc2 = ops.rms_norm_quant(x.contiguous(), w)
+    np.testing.assert_array_equal(to_host(q.float()), to_host(q2.float()))
+    np.testing.assert_array_equal(to_host(sc), to_host(sc2))
+    assert sc.shape == (5, 3, 4, 1)
+
+
 # ------------------------------------------- together, streams and graphs
 def block(ops_in, p, state=None):
     """One residual block: norm, in-projection, conv, scan, out-projection."""
@@ -602,9 +716,6 @@ def test_block_gradient_against_differences(cuda):
     dyv = ops.gemm(dxz.reshape(B * T, -1), p["win"].t()).view(B, T, M)
     dx, dw = ops.rms_norm_bwd(s, p["w"], dyv)
     host = {k: to_host(a).astype(np.float64) for k, a in p.items()}
-
-    class Host(dict):
-        pass
 
     def loss(xx, pp):
         yv, _ = ref.rms_norm(xx, pp["w"], res.astype(np.float64), 1e-6)

@@ -175,6 +175,33 @@ def test_scan_refusals():
     assert bwd([outs[0], outs[0], *outs[2:]]) == L.ERR_ARG  # one array for two gradients
 
 
+def test_overlap_is_decided_by_the_elements():
+    """Against enumeration: random small views of one buffer as s and dx of a
+    norm's backward, refused as overlapping exactly where they share an element
+    and are not the same view; the others are refused for want of scratch."""
+    rng = np.random.default_rng(0)
+    spec = L.RemoraNormSpec(1e-6, 0)
+    seen = set()
+    for _ in range(400):
+        n, d = int(rng.integers(1, 5)), int(rng.integers(1, 6))
+        views, cells = [], []
+        for _ in range(2):
+            strides = [int(rng.integers(-14, 15)), int(rng.choice([-2, -1, 1, 2, 3]))]
+            strides = [x if x or k else 9 for k, x in enumerate(strides)]
+            off = int(rng.integers(60, 90))
+            views.append(desc(n, d, at=BASE, strides=strides, offset=off))
+            cells.append({off + i * strides[0] + j * strides[1] for i in range(n) for j in range(d)})
+        r, w = desc(n, d, at=BASE + (1 << 17)), desc(d, at=BASE + (1 << 18), strides=[1])
+        st = L.lib().remora_b200_rms_norm_bwd(FAKE, ctypes.addressof(spec), ad(views[1]), ad(w), ad(r), None,
+                                              ad(views[0]), ad(desc(d, at=BASE + (1 << 19))), 2, None, 0, None)
+        in_place = (views[0].offset == views[1].offset and (n == 1 or views[0].stride0 == views[1].stride0)
+                    and (d == 1 or views[0].stride1 == views[1].stride1))
+        shared = bool(cells[0] & cells[1]) and not in_place
+        assert st == (L.ERR_ARG if shared else L.ERR_LIMIT), L.last_error()
+        seen.add((shared, in_place))
+    assert {(True, False), (False, False)} <= seen
+
+
 def test_ops_take_cuda_tensors():
     import torch
 
