@@ -9,7 +9,8 @@
 // where it stays between the row's sum and the outputs that need it.  A row is
 // held by blockDim.x threads, V groups of VEC consecutive elements each: 16-byte
 // accesses (VEC 4) where the row length, every row stride and every address
-// allow it, else 4-byte ones.  Rows too long for that are read again from L2.
+// allow it, else 4-byte ones.  Rows that are too long for that, or whose elements
+// are not consecutive, are read again from L2.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -61,37 +62,95 @@ struct Pack {
 };
 
 template <int VEC>
-__device__ __forceinline__ Pack<VEC> load(const float *p, int64_t inner, int64_t c) {
+__device__ __forceinline__ Pack<VEC> load(const float *p) {
   Pack<VEC> o;
-  if (VEC == 4) {
-    const float4 q = *reinterpret_cast<const float4 *>(p + c);
-    o.v[0] = q.x, o.v[VEC > 1 ? 1 : 0] = q.y, o.v[VEC > 2 ? 2 : 0] = q.z, o.v[VEC > 3 ? 3 : 0] = q.w;
+  if constexpr (VEC == 4) {
+    const float4 q = *reinterpret_cast<const float4 *>(p);
+    o.v[0] = q.x, o.v[1] = q.y, o.v[2] = q.z, o.v[3] = q.w;
   } else {
-    o.v[0] = p[c * inner];
+    o.v[0] = *p;
   }
   return o;
 }
 
 template <int VEC>
-__device__ __forceinline__ void store(float *p, int64_t inner, int64_t c, const Pack<VEC> &o) {
-  if (VEC == 4)
-    *reinterpret_cast<float4 *>(p + c) =
-        make_float4(o.v[0], o.v[VEC > 1 ? 1 : 0], o.v[VEC > 2 ? 2 : 0], o.v[VEC > 3 ? 3 : 0]);
+__device__ __forceinline__ void store(float *p, const Pack<VEC> &o) {
+  if constexpr (VEC == 4)
+    *reinterpret_cast<float4 *>(p) = make_float4(o.v[0], o.v[1], o.v[2], o.v[3]);
   else
-    p[c * inner] = o.v[0];
+    *p = o.v[0];
 }
 
 template <int VEC>
-__device__ __forceinline__ void store_e4m3(uint8_t *p, int64_t inner, int64_t c, const Pack<VEC> &o, float inv) {
-  if (VEC == 4) {
-    const float2 lo = make_float2(o.v[0] * inv, o.v[VEC > 1 ? 1 : 0] * inv);
-    const float2 hi = make_float2(o.v[VEC > 2 ? 2 : 0] * inv, o.v[VEC > 3 ? 3 : 0] * inv);
-    const uint32_t b = (uint32_t)__nv_cvt_float2_to_fp8x2(lo, __NV_SATFINITE, __NV_E4M3) |
-                       (uint32_t)__nv_cvt_float2_to_fp8x2(hi, __NV_SATFINITE, __NV_E4M3) << 16;
-    *reinterpret_cast<uint32_t *>(p + c) = b;
+__device__ __forceinline__ void store_e4m3(uint8_t *p, const Pack<VEC> &o, float inv) {
+  if constexpr (VEC == 4) {
+    const float2 lo = make_float2(o.v[0] * inv, o.v[1] * inv), hi = make_float2(o.v[2] * inv, o.v[3] * inv);
+    *reinterpret_cast<uint32_t *>(p) = (uint32_t)__nv_cvt_float2_to_fp8x2(lo, __NV_SATFINITE, __NV_E4M3) |
+                                       (uint32_t)__nv_cvt_float2_to_fp8x2(hi, __NV_SATFINITE, __NV_E4M3) << 16;
   } else {
-    p[c * inner] = __nv_cvt_float_to_fp8(o.v[0] * inv, __NV_SATFINITE, __NV_E4M3);
+    *p = __nv_cvt_float_to_fp8(o.v[0] * inv, __NV_SATFINITE, __NV_E4M3);
   }
+}
+
+// The elements c .. c + VEC-1 of a row of `dim`.  SHIFT: the row does not start at
+// a 16-byte boundary, its groups of four do: the first and the last may lie
+// partly outside the row, are read element by element there, and give zeros for
+// what is not in it.
+template <int VEC, bool SHIFT>
+__device__ __forceinline__ Pack<VEC> load_in(const float *p, int c, int dim) {
+  if constexpr (SHIFT) {
+    if (c < 0 || c + VEC > dim) {
+      Pack<VEC> o;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) o.v[k] = c + k >= 0 && c + k < dim ? p[c + k] : 0.0f;
+      return o;
+    }
+  }
+  return load<VEC>(p + c);
+}
+
+// As load_in, for an operand whose row starts at a boundary of its own.
+template <int VEC, bool SHIFT>
+__device__ __forceinline__ Pack<VEC> load_w(const float *p, int c, int dim) {
+  if constexpr (SHIFT) {
+    Pack<VEC> o;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) o.v[k] = c + k >= 0 && c + k < dim ? p[c + k] : 0.0f;
+    return o;
+  }
+  return load<VEC>(p + c);
+}
+
+template <int VEC, bool SHIFT>
+__device__ __forceinline__ void store_in(float *p, int c, int dim, const Pack<VEC> &o) {
+  if constexpr (SHIFT) {
+    if (c < 0 || c + VEC > dim) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k)
+        if (c + k >= 0 && c + k < dim) p[c + k] = o.v[k];
+      return;
+    }
+  }
+  store<VEC>(p + c, o);
+}
+
+template <int VEC, bool SHIFT>
+__device__ __forceinline__ void store_e4m3_in(uint8_t *p, int c, int dim, const Pack<VEC> &o, float inv) {
+  if constexpr (SHIFT) {
+    if (c < 0 || c + VEC > dim) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k)
+        if (c + k >= 0 && c + k < dim) p[c + k] = __nv_cvt_float_to_fp8(o.v[k] * inv, __NV_SATFINITE, __NV_E4M3);
+      return;
+    }
+  }
+  store_e4m3<VEC>(p + c, o, inv);
+}
+
+// Elements of a row ahead of its first 16-byte boundary's group.
+template <bool SHIFT>
+__device__ __forceinline__ int shift_of(const float *row) {
+  return SHIFT ? (int)(reinterpret_cast<uintptr_t>(row) >> 2) & 3 : 0;
 }
 
 // max that keeps a NaN of either side
@@ -127,20 +186,22 @@ __device__ __forceinline__ float row_reduce(float v, float *part) {
 }
 
 // One row per blockDim.x threads, held in registers.
-template <int VEC, int V, int MODE>
+template <int VEC, bool SHIFT, int V, int MODE>
 __global__ void __launch_bounds__(1024) norm_kernel(const NormArgs a) {
   __shared__ float part[32 * 32];
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   const bool live = row < a.rows;
+  const int dim = (int)a.dim;
   const float *x = reinterpret_cast<const float *>(a.x.base) + (live ? row_offset(a.x, a.lead, row) : 0);
   const float *r = reinterpret_cast<const float *>(a.r.base) + (live && a.has_r ? row_offset(a.r, a.lead, row) : 0);
+  const int shift = shift_of<SHIFT>(x);
   Pack<VEC> s[V];
   float ss = 0.0f;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const int64_t c = (int64_t)(j * blockDim.x + threadIdx.x) * VEC;
-    if (live && c < a.dim) {
-      s[j] = load<VEC>(x, a.x.inner, c);
+    const int c = (j * blockDim.x + threadIdx.x) * VEC - shift;
+    if (live && c < dim) {
+      s[j] = load_in<VEC, SHIFT>(x, c, dim);
     } else {
 #pragma unroll
       for (int k = 0; k < VEC; ++k) s[j].v[k] = 0.0f;
@@ -149,9 +210,9 @@ __global__ void __launch_bounds__(1024) norm_kernel(const NormArgs a) {
   if (a.has_r) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int64_t c = (int64_t)(j * blockDim.x + threadIdx.x) * VEC;
-      if (live && c < a.dim) {
-        const Pack<VEC> q = load<VEC>(r, a.r.inner, c);
+      const int c = (j * blockDim.x + threadIdx.x) * VEC - shift;
+      if (live && c < dim) {
+        const Pack<VEC> q = load_in<VEC, SHIFT>(r, c, dim);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) s[j].v[k] += q.v[k];
       }
@@ -161,22 +222,23 @@ __global__ void __launch_bounds__(1024) norm_kernel(const NormArgs a) {
   for (int j = 0; j < V; ++j)
 #pragma unroll
     for (int k = 0; k < VEC; ++k) ss = fmaf(s[j].v[k], s[j].v[k], ss);
+  ss = row_reduce<false>(ss, part);
+  // written behind the sum: 82 us ahead of it, 75 behind (8192 x 4096 to e4m3)
   if (a.has_s && live) {
     float *so = reinterpret_cast<float *>(a.s.base) + row_offset(a.s, a.lead, row);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int64_t c = (int64_t)(j * blockDim.x + threadIdx.x) * VEC;
-      if (c < a.dim) store<VEC>(so, a.s.inner, c, s[j]);
+      const int c = (j * blockDim.x + threadIdx.x) * VEC - shift;
+      if (c < dim) store_in<VEC, SHIFT>(so, c, dim, s[j]);
     }
   }
-  ss = row_reduce<false>(ss, part);
   const float rstd = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
   float amax = 0.0f;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const int64_t c = (int64_t)(j * blockDim.x + threadIdx.x) * VEC;
-    if (c < a.dim) {
-      const Pack<VEC> w = load<VEC>(a.w, a.w_stride, c);
+    const int c = (j * blockDim.x + threadIdx.x) * VEC - shift;
+    if (c < dim) {
+      const Pack<VEC> w = load_w<VEC, SHIFT>(a.w, c, dim);
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
         s[j].v[k] = s[j].v[k] * rstd * w.v[k];
@@ -189,8 +251,8 @@ __global__ void __launch_bounds__(1024) norm_kernel(const NormArgs a) {
     float *y = reinterpret_cast<float *>(a.y.base) + row_offset(a.y, a.lead, row);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int64_t c = (int64_t)(j * blockDim.x + threadIdx.x) * VEC;
-      if (c < a.dim) store<VEC>(y, a.y.inner, c, s[j]);
+      const int c = (j * blockDim.x + threadIdx.x) * VEC - shift;
+      if (c < dim) store_in<VEC, SHIFT>(y, c, dim, s[j]);
     }
     return;
   }
@@ -204,23 +266,23 @@ __global__ void __launch_bounds__(1024) norm_kernel(const NormArgs a) {
     const float inv = 1.0f / scale;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int64_t c = (int64_t)(j * blockDim.x + threadIdx.x) * VEC;
-      if (c < a.dim) store_e4m3<VEC>(q, a.y.inner, c, s[j], inv);
+      const int c = (j * blockDim.x + threadIdx.x) * VEC - shift;
+      if (c < dim) store_e4m3_in<VEC, SHIFT>(q, c, dim, s[j], inv);
     }
   } else {
     // a group is group / 4 neighbouring threads of one j: 8, 16 or 32 lanes
     const int lanes = a.group / VEC;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int64_t c = (int64_t)(j * blockDim.x + threadIdx.x) * VEC;
+      const int c = (j * blockDim.x + threadIdx.x) * VEC - shift;
       float m = 0.0f;
 #pragma unroll
       for (int k = 0; k < VEC; ++k) m = max_nan(m, fabsf(s[j].v[k]));
       for (int o = lanes >> 1; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
       const float scale = max_nan(m / kE4M3Max, kMinScale);
-      if (live && c < a.dim) {
+      if (live && c < dim) {
         if ((threadIdx.x & (lanes - 1)) == 0) sc[(c / a.group) * a.scales.inner] = scale;
-        store_e4m3<VEC>(q, a.y.inner, c, s[j], 1.0f / scale);
+        store_e4m3_in<VEC, SHIFT>(q, c, dim, s[j], 1.0f / scale);
       }
     }
   }
@@ -267,7 +329,7 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const NormArgs a) {
     for (int64_t c = threadIdx.x; c < a.dim; c += blockDim.x) {
       Pack<1> o;
       o.v[0] = value(c);
-      store_e4m3<1>(q, a.y.inner, c, o, inv);
+      store_e4m3<1>(q + c * a.y.inner, o, inv);
     }
   } else {
     // a warp per group; its lanes' elements were written by other threads
@@ -283,7 +345,7 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const NormArgs a) {
       for (int k = threadIdx.x & 31; k < a.group; k += 32) {
         Pack<1> o;
         o.v[0] = value(g * a.group + k);
-        store_e4m3<1>(q, a.y.inner, g * a.group + k, o, inv);
+        store_e4m3<1>(q + (g * a.group + k) * a.y.inner, o, inv);
       }
     }
   }
@@ -303,19 +365,23 @@ struct NormBwdArgs {
 
 // As norm_kernel, over several rows per thread group: each thread keeps its
 // columns' part of dw in registers and writes it once.
-template <int VEC, int V>
+template <int VEC, bool SHIFT, int V>
 __global__ void __launch_bounds__(512) norm_bwd_kernel(const NormBwdArgs a) {
   __shared__ float part[2 * 32 * 32];
+  const int dim = (int)a.dim;
+  const int64_t slot = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  const int64_t slots = (int64_t)gridDim.x * blockDim.y;
+  // the rows of a slot are a multiple of four apart: one shift for all of them
+  const int shift =
+      shift_of<SHIFT>(reinterpret_cast<const float *>(a.s.base) + (slot < a.rows ? row_offset(a.s, a.lead, slot) : 0));
   Pack<VEC> w[V], dw[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const int64_t c = (int64_t)(j * blockDim.x + threadIdx.x) * VEC;
+    const int c = (j * blockDim.x + threadIdx.x) * VEC - shift;
 #pragma unroll
     for (int k = 0; k < VEC; ++k) w[j].v[k] = dw[j].v[k] = 0.0f;
-    if (c < a.dim) w[j] = load<VEC>(a.w, a.w_stride, c);
+    if (c < dim) w[j] = load_w<VEC, SHIFT>(a.w, c, dim);
   }
-  const int64_t slot = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  const int64_t slots = (int64_t)gridDim.x * blockDim.y;
   // every thread of the block takes the same number of turns
   for (int64_t base = (int64_t)blockIdx.x * blockDim.y; base < a.rows; base += slots) {
     const int64_t row = base + threadIdx.y;
@@ -328,13 +394,13 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const NormBwdArgs a) {
     float ss = 0.0f, sg = 0.0f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int64_t c = (int64_t)(j * blockDim.x + threadIdx.x) * VEC;
+      const int c = (j * blockDim.x + threadIdx.x) * VEC - shift;
 #pragma unroll
       for (int k = 0; k < VEC; ++k) sv[j].v[k] = gv[j].v[k] = dv[j].v[k] = 0.0f;
-      if (live && c < a.dim) {
-        sv[j] = load<VEC>(s, a.s.inner, c);
-        gv[j] = load<VEC>(dy, a.dy.inner, c);
-        if (a.has_ds) dv[j] = load<VEC>(ds, a.ds.inner, c);
+      if (live && c < dim) {
+        sv[j] = load_in<VEC, SHIFT>(s, c, dim);
+        gv[j] = load_in<VEC, SHIFT>(dy, c, dim);
+        if (a.has_ds) dv[j] = load_in<VEC, SHIFT>(ds, c, dim);
       }
     }
 #pragma unroll
@@ -365,7 +431,7 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const NormBwdArgs a) {
     float *dx = reinterpret_cast<float *>(a.dx.base) + (live ? row_offset(a.dx, a.lead, row) : 0);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int64_t c = (int64_t)(j * blockDim.x + threadIdx.x) * VEC;
+      const int c = (j * blockDim.x + threadIdx.x) * VEC - shift;
       Pack<VEC> o;
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
@@ -373,16 +439,15 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const NormBwdArgs a) {
         o.v[k] = fmaf(rstd, fmaf(-xh, coef, gv[j].v[k] * w[j].v[k]), dv[j].v[k]);
         dw[j].v[k] = fmaf(gv[j].v[k], xh, dw[j].v[k]);
       }
-      if (live && c < a.dim) store<VEC>(dx, a.dx.inner, c, o);
+      if (live && c < dim) store_in<VEC, SHIFT>(dx, c, dim, o);
     }
   }
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const int64_t c = (int64_t)(j * blockDim.x + threadIdx.x) * VEC;
-    if (c < a.dim) {
+    const int c = (j * blockDim.x + threadIdx.x) * VEC - shift;
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) a.part[slot * a.dim + c + k] = dw[j].v[k];
-    }
+    for (int k = 0; k < VEC; ++k)
+      if (c + k >= 0 && c + k < dim) a.part[slot * a.dim + c + k] = dw[j].v[k];
   }
 }
 
@@ -505,12 +570,45 @@ bool one_stride(const DescView &v, Rows *r) {
   return true;
 }
 
+// Whether a row's elements are consecutive.
+bool unit_rows(const DescView &v) { return v.strides[v.rank - 1] == 1 || v.sizes[v.rank - 1] == 1; }
+
 bool aligned_rows(const DescView &v, int esize, int vec_bytes) {
-  if (v.strides[v.rank - 1] != 1 && v.sizes[v.rank - 1] != 1) return false;
   if (reinterpret_cast<uintptr_t>(v.data(esize)) % vec_bytes) return false;
   for (int d = 0; d < v.rank - 1; ++d)
     if (v.sizes[d] > 1 && (v.strides[d] * esize) % vec_bytes) return false;
   return true;
+}
+
+// How the register kernels read rows: 16 bytes at a time where every row of
+// every operand starts at such a boundary; also where the rows do not, but all
+// operands' rows start equally far from one (arrays of an odd row length);
+// element by element where they differ; not at all where a row's elements are
+// not consecutive.  12000 x 2731 with a residual: SHIFTED us shifted, 121 single.
+enum class Access { kVector, kShifted, kSingle, kNone };
+
+struct Operand {
+  const DescView *v;  // may be null
+  int esize;
+};
+
+Access access_for(int64_t dim, const DescView &w, std::initializer_list<Operand> operands) {
+  bool aligned = dim % 4 == 0, alike = true;
+  const DescView *first = nullptr;
+  if (!unit_rows(w)) return Access::kNone;
+  for (const Operand &o : operands) {
+    if (o.v == nullptr) continue;
+    if (!unit_rows(*o.v)) return Access::kNone;
+    aligned = aligned && aligned_rows(*o.v, o.esize, 4 * o.esize);
+    // in elements from a boundary, modulo four
+    if (first == nullptr) first = o.v;
+    alike = alike && (reinterpret_cast<uintptr_t>(o.v->data(o.esize)) / o.esize) % 4 ==
+                         (reinterpret_cast<uintptr_t>(first->data(4)) / 4) % 4;
+    for (int d = 0; d < o.v->rank - 1; ++d)
+      alike = alike && (o.v->sizes[d] <= 1 || (o.v->strides[d] - first->strides[d]) % 4 == 0);
+  }
+  if (aligned && reinterpret_cast<uintptr_t>(w.data(4)) % 16 == 0) return Access::kVector;
+  return alike ? Access::kShifted : Access::kSingle;
 }
 
 int check_rank(int rank) {
@@ -543,15 +641,21 @@ struct Tiling {
   bool fits;
 };
 
-// Four vectors per thread (64 bytes of each operand in flight) when the rows
-// fill the device; one, over more threads, when there are few rows and the
-// call waits for the latency of a single row.
-Tiling tile_for(int64_t rows, int64_t dim, int vec, int max_threads) {
-  const int64_t vecs = (dim + vec - 1) / vec;
-  const int max_v = vec == 4 ? 4 : 8;
+// Four vectors (or eight single elements) per thread, 64 (32) bytes of each
+// operand in flight, when the rows fill the device; one, over more threads, when
+// there are few rows and the call waits for the latency of a single row.  No
+// more than a warp's threads leave each something to do.  Rows that are a little
+// too long for shifted vectors are read by single elements.
+Tiling tile_for(int64_t rows, int64_t dim, Access *access, int max_threads, int max_single) {
   Tiling t = {32, 1, 1, false};
-  const int64_t want_v = rows >= 592 ? (vec == 4 ? 4 : 8) : 1;
-  for (int v = (int)std::min<int64_t>(want_v, max_v); v <= max_v; v *= 2) {
+  if (*access == Access::kNone) return t;
+  if (*access == Access::kShifted && (dim + 3 + 3) / 4 > (int64_t)max_threads * 4) *access = Access::kSingle;
+  const int vec = *access == Access::kSingle ? 1 : 4, max_v = vec == 4 ? 4 : max_single;
+  const int64_t vecs = (dim + (*access == Access::kShifted ? 3 : 0) + vec - 1) / vec;
+  int v = 1;
+  if (rows >= 592)
+    while (v < (vec == 4 ? 4 : 8) && vecs > 32 * v) v *= 2;
+  for (; v <= max_v; v *= 2) {
     const int64_t threads = ((vecs + v - 1) / v + 31) / 32 * 32;
     if (threads > max_threads) continue;
     t.threads = (int)threads;
@@ -564,21 +668,31 @@ Tiling tile_for(int64_t rows, int64_t dim, int vec, int max_threads) {
   return t;
 }
 
-template <int VEC, int MODE>
+template <int VEC, bool SHIFT, int MODE>
 int launch_norm(const NormArgs &a, const Tiling &t, cudaStream_t stream) {
   const dim3 block(t.threads, t.per_block);
   const unsigned grid = (unsigned)((a.rows + t.per_block - 1) / t.per_block);
   note_launch();
   switch (t.v) {
-  case 1: norm_kernel<VEC, 1, MODE><<<grid, block, 0, stream>>>(a); break;
-  case 2: norm_kernel<VEC, 2, MODE><<<grid, block, 0, stream>>>(a); break;
-  case 4: norm_kernel<VEC, 4, MODE><<<grid, block, 0, stream>>>(a); break;
+  case 1: norm_kernel<VEC, SHIFT, 1, MODE><<<grid, block, 0, stream>>>(a); break;
+  case 2: norm_kernel<VEC, SHIFT, 2, MODE><<<grid, block, 0, stream>>>(a); break;
+  case 4: norm_kernel<VEC, SHIFT, 4, MODE><<<grid, block, 0, stream>>>(a); break;
   default:
-    if constexpr (VEC == 1) norm_kernel<VEC, 8, MODE><<<grid, block, 0, stream>>>(a);
+    if constexpr (VEC == 1) norm_kernel<VEC, SHIFT, 8, MODE><<<grid, block, 0, stream>>>(a);
     break;
   }
   REMORA_CUDA_TRY(cudaGetLastError());
   return REMORA_OK;
+}
+
+template <int MODE>
+int launch_norm(Access access, const NormArgs &a, const Tiling &t, cudaStream_t stream) {
+  if (access == Access::kVector) return launch_norm<4, false, MODE>(a, t, stream);
+  if constexpr (MODE != kQuantGroup) {
+    if (access == Access::kShifted) return launch_norm<4, true, MODE>(a, t, stream);
+    return launch_norm<1, false, MODE>(a, t, stream);
+  }
+  return REMORA_OK;  // not reached: groups are vectors or go to norm_long_kernel
 }
 
 int norm_forward(RemoraB200Ctx *ctx, const RemoraNormSpec *spec, const void *x, const void *residual,
@@ -628,10 +742,9 @@ int norm_forward(RemoraB200Ctx *ctx, const RemoraNormSpec *spec, const void *x, 
   a.y = rows_of(yv, quant ? 1 : 4);
   a.lead = sh.lead;
   bool one = one_stride(xv, &a.x) & one_stride(yv, &a.y);
-  bool vec = sh.dim % 4 == 0 && aligned_rows(xv, 4, 16) && aligned_rows(yv, quant ? 1 : 4, quant ? 4 : 16) &&
-             (wv.strides[0] == 1) && reinterpret_cast<uintptr_t>(wv.data(4)) % 16 == 0;
-  if (has_r) a.r = rows_of(rv, 4), one = one_stride(rv, &a.r) && one, vec = vec && aligned_rows(rv, 4, 16);
-  if (has_s) a.s = rows_of(sv, 4), one = one_stride(sv, &a.s) && one, vec = vec && aligned_rows(sv, 4, 16);
+  Access access = access_for(sh.dim, wv, {{&xv, 4}, {&yv, quant ? 1 : 4}, {rp, 4}, {sp, 4}});
+  if (has_r) a.r = rows_of(rv, 4), one = one_stride(rv, &a.r) && one;
+  if (has_s) a.s = rows_of(sv, 4), one = one_stride(sv, &a.s) && one;
   if (quant) a.scales = rows_of(cv, 4), one = one_stride(cv, &a.scales) && one;
   if (!one) {  // back to the strides of three axes
     a.x = rows_of(xv, 4), a.y = rows_of(yv, quant ? 1 : 4);
@@ -645,10 +758,10 @@ int norm_forward(RemoraB200Ctx *ctx, const RemoraNormSpec *spec, const void *x, 
   a.rows = sh.rows, a.dim = sh.dim, a.eps = spec->eps, a.group = (int)std::min<int64_t>(group, 1 << 30);
   a.has_r = has_r, a.has_s = has_s;
   const int mode = !quant ? kPlain : group == sh.dim && spec->group == 0 ? kQuantRow : kQuantGroup;
-  const Tiling t = tile_for(sh.rows, sh.dim, vec ? 4 : 1, 1024);
+  const Tiling t = tile_for(sh.rows, sh.dim, &access, 1024, 8);
   DeviceGuard guard;
   REMORA_TRY(guard.enter(ctx));
-  if (!t.fits || (mode == kQuantGroup && !vec)) {
+  if (!t.fits || (mode == kQuantGroup && access != Access::kVector)) {
     const unsigned threads = (unsigned)std::min<int64_t>(1024, (sh.dim + 31) / 32 * 32);
     note_launch();
     if (mode == kPlain)
@@ -660,10 +773,9 @@ int norm_forward(RemoraB200Ctx *ctx, const RemoraNormSpec *spec, const void *x, 
     REMORA_CUDA_TRY(cudaGetLastError());
     return REMORA_OK;
   }
-  if (mode == kPlain) return vec ? launch_norm<4, kPlain>(a, t, stream) : launch_norm<1, kPlain>(a, t, stream);
-  if (mode == kQuantRow)
-    return vec ? launch_norm<4, kQuantRow>(a, t, stream) : launch_norm<1, kQuantRow>(a, t, stream);
-  return launch_norm<4, kQuantGroup>(a, t, stream);
+  if (mode == kPlain) return launch_norm<kPlain>(access, a, t, stream);
+  if (mode == kQuantRow) return launch_norm<kQuantRow>(access, a, t, stream);
+  return launch_norm<kQuantGroup>(access, a, t, stream);
 }
 
 // The last block's thread groups past the rows write a (zero) part too.
@@ -676,16 +788,21 @@ size_t bwd_scratch(int64_t rows, int64_t dim) {
   return ((size_t)bwd_slots(rows) * dim + (size_t)rows) * 4;
 }
 
-template <int VEC>
+template <int VEC, bool SHIFT>
 int launch_bwd(const NormBwdArgs &a, const Tiling &t, unsigned grid, cudaStream_t stream) {
   const dim3 block(t.threads, t.per_block);
   note_launch();
   switch (t.v) {
-  case 1: norm_bwd_kernel<VEC, 1><<<grid, block, 0, stream>>>(a); break;
-  case 2: norm_bwd_kernel<VEC, 2><<<grid, block, 0, stream>>>(a); break;
-  case 4: norm_bwd_kernel<VEC, 4><<<grid, block, 0, stream>>>(a); break;
+  case 1: norm_bwd_kernel<VEC, SHIFT, 1><<<grid, block, 0, stream>>>(a); break;
+  case 2: norm_bwd_kernel<VEC, SHIFT, 2><<<grid, block, 0, stream>>>(a); break;
+  case 4: norm_bwd_kernel<VEC, SHIFT, 4><<<grid, block, 0, stream>>>(a); break;
   default:
-    if constexpr (VEC == 1) norm_bwd_kernel<VEC, 8><<<grid, block, 0, stream>>>(a);
+    if constexpr (VEC == 1) {
+      if (t.v == 8)
+        norm_bwd_kernel<VEC, SHIFT, 8><<<grid, block, 0, stream>>>(a);
+      else
+        norm_bwd_kernel<VEC, SHIFT, 16><<<grid, block, 0, stream>>>(a);
+    }
     break;
   }
   REMORA_CUDA_TRY(cudaGetLastError());
@@ -769,9 +886,8 @@ int remora_b200_rms_norm_bwd(RemoraB200Ctx *ctx, const RemoraNormSpec *spec, con
   a.lead.one = one_stride(sv, &b.s) & one_stride(gv, &b.dy) & one_stride(xv, &b.dx);
   if (has_ds) a.lead.one = one_stride(dv, &b.ds) && a.lead.one;
   if (a.lead.one) a.s = b.s, a.dy = b.dy, a.dx = b.dx, a.ds = b.ds;
-  const bool vec = sh.dim % 4 == 0 && aligned_rows(sv, 4, 16) && aligned_rows(gv, 4, 16) && aligned_rows(xv, 4, 16) &&
-                   (!has_ds || aligned_rows(dv, 4, 16)) && wv.strides[0] == 1 &&
-                   reinterpret_cast<uintptr_t>(wv.data(4)) % 16 == 0;
+  Access access = access_for(sh.dim, wv, {{&sv, 4}, {&gv, 4}, {&xv, 4}, {dp, 4}});
+  if (access == Access::kShifted && !a.lead.one) access = Access::kSingle;  // a slot's rows share one shift
   a.w = reinterpret_cast<const float *>(wv.data(4)), a.w_stride = wv.strides[0];
   a.rows = sh.rows, a.dim = sh.dim, a.eps = spec->eps, a.has_ds = has_ds;
   a.part = static_cast<float *>(scratch);
@@ -779,13 +895,21 @@ int remora_b200_rms_norm_bwd(RemoraB200Ctx *ctx, const RemoraNormSpec *spec, con
   DeviceGuard guard;
   REMORA_TRY(guard.enter(ctx));
   if (sh.rows > 0) {
-    const Tiling t = tile_for(sh.rows, sh.dim, vec ? 4 : 1, 512);
+    const Tiling t = tile_for(sh.rows, sh.dim, &access, 512, 16);
     if (t.fits) {
       const int64_t per_sm = std::max(1, 512 / (t.threads * t.per_block));
-      const int64_t grid = std::min<int64_t>((sh.rows + t.per_block - 1) / t.per_block,
-                                             std::min<int64_t>(ctx->sm_count * per_sm, kBwdMaxSlots / t.per_block));
+      int64_t grid = std::min<int64_t>((sh.rows + t.per_block - 1) / t.per_block,
+                                       std::min<int64_t>(ctx->sm_count * per_sm, kBwdMaxSlots / t.per_block));
+      // where a slot has several rows (an SM's worth of blocks and more), they are
+      // a multiple of four apart
+      if (grid * t.per_block < sh.rows) grid -= grid % 4;
       parts = grid * t.per_block;
-      REMORA_TRY(vec ? launch_bwd<4>(a, t, (unsigned)grid, stream) : launch_bwd<1>(a, t, (unsigned)grid, stream));
+      if (access == Access::kVector)
+        REMORA_TRY((launch_bwd<4, false>(a, t, (unsigned)grid, stream)));
+      else if (access == Access::kShifted)
+        REMORA_TRY((launch_bwd<4, true>(a, t, (unsigned)grid, stream)));
+      else
+        REMORA_TRY((launch_bwd<1, false>(a, t, (unsigned)grid, stream)));
     } else {
       parts = std::min<int64_t>(sh.rows, kLongParts);
       a.rstd = a.part + bwd_slots(sh.rows) * sh.dim;

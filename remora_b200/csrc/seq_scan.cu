@@ -278,12 +278,13 @@ struct TokenArgs {
   int states, groups, softplus, zero_rest, vec;
 };
 
-// Four states of one channel per thread, of R batch rows, R either 1 or NL.
-// Bound by the states' bytes: with R = NL the decay rates are read once for R
-// rows, R states are on their way at once, and what belongs to a row and
-// channel alone (the step, the gate, y) is worked out by one of the NL lanes.
+// Four states of one channel per thread, of R batch rows, R either 1 or the
+// smaller of NL and 4.  Bound by the states' bytes: with R > 1 the decay rates
+// are read once for R rows, R states are on their way at once, and what belongs
+// to a row and channel alone (the step, the gate, y) is worked out by one of the
+// NL lanes.
 template <int NL, int R>
-__global__ void __launch_bounds__(kScanThreads, NL > 4 ? 2 : 7) scan_step_kernel(const TokenArgs a) {
+__global__ void __launch_bounds__(kScanThreads, 7) scan_step_kernel(const TokenArgs a) {
   const int i0 = (int)blockIdx.y * R;
   const int q = threadIdx.x % NL, d = (int)blockIdx.x * (kScanThreads / NL) + threadIdx.x / NL;
   int slot[R];
@@ -302,7 +303,7 @@ __global__ void __launch_bounds__(kScanThreads, NL > 4 ? 2 : 7) scan_step_kernel
     }
   }
   const int nv = d < a.dim ? a.states - 4 * q : 0;
-  const int own = R > 1 ? q : 0;  // the row whose per-channel values this lane has
+  const int own = q % R;  // the row whose per-channel values this lane has
   bool mine = false;
 #pragma unroll
   for (int r = 0; r < R; ++r) mine = r == own ? on[r] && d < a.dim : mine;
@@ -360,18 +361,17 @@ __global__ void __launch_bounds__(kScanThreads, NL > 4 ? 2 : 7) scan_step_kernel
       }
     }
   }
-  if constexpr (R > 1) {
-    transpose_sum<NL>(part, q);
-  } else {
 #pragma unroll
-    for (int o = 1; o < NL; o <<= 1) part[0] += __shfl_xor_sync(0xffffffffu, part[0], o);
-  }
-  if (mine && (R > 1 || q == 0)) {
+  for (int o = R; o < NL; o <<= 1)
+#pragma unroll
+    for (int r = 0; r < R; ++r) part[r] += __shfl_xor_sync(0xffffffffu, part[r], o);
+  transpose_sum<R>(part, own);
+  if (mine && q < R) {
     float y = part[0];
     if (a.d.p) y = fmaf(*a.d(0, d, 0), u, y);
     if (a.z.p) y *= z * sigmoid(z);
     *a.y(i0 + own, d, 0) = y;
-  } else if (a.zero_rest && !mine && d < a.dim && i0 + own < a.batch && (R > 1 || q == 0)) {
+  } else if (a.zero_rest && !mine && d < a.dim && i0 + own < a.batch && q < R) {
     *a.y(i0 + own, d, 0) = 0.0f;
   }
 }
@@ -632,10 +632,11 @@ int remora_b200_selective_scan_step(RemoraB200Ctx *ctx, const RemoraSelectiveSca
   a.softplus = spec->softplus != 0, a.zero_rest = spec->zero_rest != 0;
   a.vec = vec_states(sv) && vec_states(ov) && vec_states(av) && vec_states(bv) && vec_states(cv);
   const int nl = lanes_for(a.states);
-  // R = NL rows per thread once that leaves every SM some blocks
+  // several rows per thread once that leaves every SM some blocks
   const int64_t blocks = (D + kScanThreads / nl - 1) / (kScanThreads / nl);
-  const bool many = nl > 1 && blocks * (B / nl) >= kManyBlocks;
-  const dim3 grid((unsigned)blocks, (unsigned)(many ? (B + nl - 1) / nl : B));
+  const int rows = nl < 4 ? nl : 4;
+  const bool many = nl > 1 && blocks * (B / rows) >= kManyBlocks;
+  const dim3 grid((unsigned)blocks, (unsigned)(many ? (B + rows - 1) / rows : B));
   DeviceGuard guard;
   REMORA_TRY(guard.enter(ctx));
   cudaStream_t s = (cudaStream_t)stream;
@@ -643,7 +644,7 @@ int remora_b200_selective_scan_step(RemoraB200Ctx *ctx, const RemoraSelectiveSca
 #define REMORA_STEP_CASE(NL)                                        \
   case NL:                                                          \
     if (many)                                                       \
-      scan_step_kernel<NL, NL><<<grid, kScanThreads, 0, s>>>(a);    \
+      scan_step_kernel<NL, (NL < 4 ? NL : 4)><<<grid, kScanThreads, 0, s>>>(a); \
     else                                                            \
       scan_step_kernel<NL, 1><<<grid, kScanThreads, 0, s>>>(a);     \
     break;

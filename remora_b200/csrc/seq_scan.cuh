@@ -24,7 +24,7 @@ namespace seq {
 constexpr int kScanThreads = 128;
 // Steps between the states that the forward keeps for the backward pass: what
 // fits a thread's registers there.
-constexpr int save_every(int nl) { return nl > 8 ? 16 : 8; }
+constexpr int save_every(int nl) { return nl > 8 ? 16 : nl > 1 ? 8 : 4; }
 constexpr int kMaxStates = 64;
 constexpr int64_t kMaxLength = 1 << 30;
 constexpr int kChan = 2;  // channels per thread

@@ -25,11 +25,13 @@ namespace {
 constexpr int kWarps = kScanThreads / 32;
 constexpr float kLn2 = 0.6931471805599453f;
 
+constexpr int bwd_chan(int nl) { return nl > 8 || nl < 4 ? 1 : 2; }
+
 // Channels of a thread, steps of a piece, steps whose b, c, db and dc are in
 // shared memory together.
 template <int NL>
 struct Bwd {
-  static constexpr int kChan = NL > 8 ? 1 : 2;
+  static constexpr int kChan = bwd_chan(NL);
   static constexpr int kPiece = save_every(NL);
   static constexpr int kTile = NL > 4 ? 16 : 32;
 };
@@ -37,7 +39,7 @@ struct Bwd {
 constexpr int64_t kBlocks = 148 * 16;  // blocks of a cut time axis
 constexpr int64_t kCutBelow = 148 * 2;
 
-int64_t bwd_channels(int nl) { return kScanThreads / nl * (nl > 8 ? 1 : 2); }  // of a block
+int64_t bwd_channels(int nl) { return kScanThreads / nl * bwd_chan(nl); }  // of a block
 
 // Sums v over the 32 / NL channel lanes of a warp; CNT of the sums end in
 // v[0 .. CNT-1] of each lane, the sums FIRST .. FIRST + CNT - 1.
@@ -624,7 +626,7 @@ int remora_b200_selective_scan_bwd(RemoraB200Ctx *ctx, const RemoraSelectiveScan
   REMORA_TRY(want_scratch(saved, saved_bytes, need, "selective_scan_bwd (saved)"));
   REMORA_TRY(want_scratch(scratch, scratch_bytes, l.total * 4, "selective_scan_bwd"));
   if (D == 0) return REMORA_OK;
-  const int chan = nl > 8 ? 1 : 2;
+  const int chan = bwd_chan(nl);
   for (int k : {0, 1, 6})
     if (v[k].aligned) REMORA_TRY(check_reach(v[k], nl, chan, "selective_scan_bwd"));
   for (const DescView *x : {&gy, &o[0], &o[1], have[6] ? &o[6] : &o[0]})
