@@ -9,6 +9,11 @@
 // every address and stride allows it, 256 bytes per warp and row) with the last
 // W rows in registers, so each row is read once but for the W-1 rows ahead of
 // a run, which its neighbour in the block has just brought into L1.
+//
+// Measured on B200 (a copy runs at 6.46 TB/s): forward with SiLU of 8 x 2048 x 4096
+// 83 us, 6.5 TB/s, of 1 x 8192 x 4096 46 us, 5.9 TB/s; backward of 8 x 2048 x 4096
+// 152 us and 5 us for the join of dw and dbias, 5.3 TB/s, where the instructions
+// (recomputed pre-activations, 4 W products per element) begin to count.
 #include <algorithm>
 #include <type_traits>
 

@@ -13,6 +13,12 @@
 // over a thread's channels, over a warp by a transposed shuffle, over a block
 // through shared memory, over blocks by partial rows in scratch that a second
 // kernel adds in block order.
+//
+// Bound by issue: some 260 instructions per warp, step and pair of channels (8
+// states per thread), of which the sums over channels and states are a third; 255
+// registers leave 8 warps per SM, which issue every other clock.  Measured on B200
+// for 4 x 2048 x 2048 x 16: 467 us, first pass of the adjoint 95, joins 22; with
+// decays kept instead of recomputed, one channel per thread and spilling 1439.
 #include <algorithm>
 #include <type_traits>
 

@@ -53,7 +53,7 @@ def norm_tol(D):
 
 
 SHAPES = [(1, 1), (5, 3), (3, 31), (7, 128), (700, 33), (2, 1000), (600, 1000), (9, 2048), (1, 8192), (3, 8193),
-          (2, 16384), (2, 16388), (2, 20001), (1300, 64)]
+          (2, 16384), (2, 16388), (2, 20001), (1300, 64), (9000, 37), (4001, 1003)]
 
 
 @pytest.mark.parametrize("rows,D", SHAPES)
