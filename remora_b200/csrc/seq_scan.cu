@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 4 : 2) scan_fwd_kernel(
   const Place<NL, kChan> at(a);
   const int64_t len = scan_length(a, at.b);
   const int64_t t0 = at.chunk * a.chunk, t_end = min(t0 + a.chunk, len);
-  const Lane<NL, kChan> ly(a.y, at, t0);
+  Lane<NL, kChan> ly(a.y, at, t0);
   if (MAIN && a.zero_rest) zero_rows(ly, at, a, t0, len);
   if (t0 >= len && t0 > 0) return;  // the first piece of an empty sequence hands h0 on
   if (!MAIN && t_end == len) return;  // nothing follows
@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 4 : 2) scan_fwd_kernel(
   const int nv = a.states - 4 * at.q;  // of the four states, those below N
   f2 A[kChan][2], h[kChan][2];
   float bias[kChan], skip[kChan], total[kChan];
-  const Lane<NL, kChan> lu(a.u, at, t0), ld(a.delta, at, t0), lz(a.z, at, t0);
+  Lane<NL, kChan> lu(a.u, at, t0), ld(a.delta, at, t0), lz(a.z, at, t0);
 #pragma unroll
   for (int c = 0; c < kChan; ++c) {
     float av[4], hv[4];
@@ -76,15 +76,17 @@ __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 4 : 2) scan_fwd_kernel(
   }
   const bool gated = MAIN && a.z.p != nullptr;
   float ru[kChan][PF], rd[kChan][PF], rz[kChan][PF];
-  auto fetch = [&](int base) {  // the inputs of steps base .. base + GROUP - 1, zeros past the end
+  // the inputs of steps base .. base + GROUP - 1, zeros past the end, and on to
+  // the next
+  auto fetch = [&](int base) {
     if (base + GROUP <= steps) {
 #pragma unroll
       for (int c = 0; c < kChan; ++c)
 #pragma unroll
         for (int i = 0; i < PF; ++i) {
-          ru[c][i] = lu(c, base + i * NL);
-          rd[c][i] = ld(c, base + i * NL);
-          if (gated) rz[c][i] = lz(c, base + i * NL);
+          ru[c][i] = lu(c, i * NL);
+          rd[c][i] = ld(c, i * NL);
+          if (gated) rz[c][i] = lz(c, i * NL);
         }
     } else {
 #pragma unroll
@@ -92,11 +94,12 @@ __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 4 : 2) scan_fwd_kernel(
 #pragma unroll
         for (int i = 0; i < PF; ++i) {
           const bool on = base + i * NL + at.q < steps;
-          ru[c][i] = on ? lu(c, base + i * NL) : 0.0f;
-          rd[c][i] = on ? ld(c, base + i * NL) : 0.0f;
-          if (gated) rz[c][i] = on ? lz(c, base + i * NL) : 0.0f;
+          ru[c][i] = on ? lu(c, i * NL) : 0.0f;
+          rd[c][i] = on ? ld(c, i * NL) : 0.0f;
+          if (gated) rz[c][i] = on ? lz(c, i * NL) : 0.0f;
         }
     }
+    lu.go(GROUP), ld.go(GROUP), lz.go(GROUP);
   };
   auto stage = [&](int buf, int64_t t) {
     stage_rows<NL, kTile>(bs[buf], a.b, a.vec_b, at.b, at.g, t, t_end, a.states);
@@ -172,7 +175,7 @@ __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 4 : 2) scan_fwd_kernel(
         for (int c = 0; c < kChan; ++c) {
           transpose_sum<NL>(part[c], at.q);
           if (at.live[c] && (FULL || base + i * NL + at.q < steps)) {
-            ly(c, base + i * NL) = (part[c][0] + y0[c][i]) * w[c][i];
+            ly(c, i * NL) = (part[c][0] + y0[c][i]) * w[c][i];
           }
         }
       }
@@ -208,6 +211,7 @@ __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 4 : 2) scan_fwd_kernel(
         group(std::true_type{}, base, bt, ct);
       else
         group(std::false_type{}, base, bt, ct);
+      if (MAIN) ly.go(GROUP);
     }
     __syncthreads();  // this buffer is filled again in the next turn
   }

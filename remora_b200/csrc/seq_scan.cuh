@@ -150,7 +150,8 @@ struct Lane {
     for (int c = 0; c < CHAN; ++c)
       off[c] = (unsigned)((at.local[c] * o.s2 + at.q * o.s1 - low) * 4);
   }
-  // step t + q of channel c
+  __device__ __forceinline__ void go(int64_t steps) { base += steps * step; }
+  // step t + q of channel c, t counted from where the base has got to
   __device__ __forceinline__ float &operator()(int c, int t) const {
     return *reinterpret_cast<float *>(base + t * step + off[c]);
   }

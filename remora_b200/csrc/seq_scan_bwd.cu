@@ -120,8 +120,8 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const ScanArg
   const bool gated = a.z.p != nullptr;
   float ru[C][PF], rd[C][PF], rz[C][PF], ry[C][PF];
   ulonglong2 rh[C];
-  const Lane<NL, C> lu(a.u, at, t0), ld(a.delta, at, t0), lz(a.z, at, t0), ly(a.dy, at, t0);
-  const Lane<NL, C> ldu(a.du, at, t0), ldd(a.ddelta, at, t0), ldz(a.dz, at, t0);
+  Lane<NL, C> lu(a.u, at, t0), ld(a.delta, at, t0), lz(a.z, at, t0), ly(a.dy, at, t0);
+  Lane<NL, C> ldu(a.du, at, t0), ldd(a.ddelta, at, t0), ldz(a.dz, at, t0);
   if (a.zero_rest) {
     zero_rows(ldu, at, a, t0, len);
     zero_rows(ldd, at, a, t0, len);
@@ -139,20 +139,24 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const ScanArg
   const ulonglong2 *hp = reinterpret_cast<const ulonglong2 *>(a.saved) +
                          ((at.b * kept + t0 / T) * a.dim + at.first) * NL;
   const int64_t hstep = a.dim * NL;
-  auto fetch = [&](int base) {  // the inputs of the piece from `base` on, zeros past the end
+  // the inputs of the piece from `base` on, zeros past the end, and back to the
+  // piece before it
+  auto fetch = [&](int base) {
     const bool full = base + T <= steps;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
 #pragma unroll
       for (int i = 0; i < PF; ++i) {
         const bool on = full || base + i * NL + at.q < steps;
-        ru[c][i] = on ? lu(c, base + i * NL) : 0.0f;
-        rd[c][i] = on ? ld(c, base + i * NL) : 0.0f;
-        ry[c][i] = on ? ly(c, base + i * NL) : 0.0f;
-        rz[c][i] = gated && on ? lz(c, base + i * NL) : 0.0f;
+        ru[c][i] = on ? lu(c, i * NL) : 0.0f;
+        rd[c][i] = on ? ld(c, i * NL) : 0.0f;
+        ry[c][i] = on ? ly(c, i * NL) : 0.0f;
+        rz[c][i] = gated && on ? lz(c, i * NL) : 0.0f;
       }
-      rh[c] = (hp + base / T * hstep)[(unsigned)(at.local[c] * NL + at.q)];
+      rh[c] = hp[(unsigned)(at.local[c] * NL + at.q)];
     }
+    lu.go(-T), ld.go(-T), ly.go(-T), lz.go(-T);
+    hp -= hstep;
   };
   auto stage = [&](int buf, int tile) {
     stage_rows<NL, TILE>(bs[buf], a.b, a.vec_b, at.b, at.g, t0 + tile, t_end, a.states);
@@ -227,7 +231,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const ScanArg
         for (int c = 0; c < C; ++c) {
           transpose_sum<NL>(part[c], at.q);
           if (at.live[c] && (FULL || base + i * NL + at.q < steps))
-            ldz(c, base + i * NL) = dzf[c][i] * fmaf(skip[c], u[c][i], part[c][0]);
+            ldz(c, i * NL) = dzf[c][i] * fmaf(skip[c], u[c][i], part[c][0]);
         }
       }
     }
@@ -293,8 +297,8 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const ScanArg
         if (at.live[c] && (FULL || base + i * NL + at.q < steps)) {
           // A is a log2(e): its log2(e) comes off the sum here
           const float ds = fmaf(u[c][i], gb[c][0], ga[c][0] * kLn2) * sig[c][i];
-          ldu(c, base + i * NL) = fmaf(s[c][i], gb[c][0], skip[c] * dyp[c][i]);
-          ldd(c, base + i * NL) = ds;
+          ldu(c, i * NL) = fmaf(s[c][i], gb[c][0], skip[c] * dyp[c][i]);
+          ldd(c, i * NL) = ds;
           sum_d[c] = fmaf(dyp[c][i], u[c][i], sum_d[c]);
           sum_bias[c] += ds;
         }
@@ -304,11 +308,15 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const ScanArg
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int k = 0; k < 2; ++k) dA[c][k] = add2(dA[c][k], da[c][k]);
+    ldu.go(-T), ldd.go(-T), ldz.go(-T);
   };
   const int last = steps > 0 ? (steps - 1) / TILE * TILE : -TILE;
   if (steps > 0) {
+    const int end = (steps - 1) / T * T;
+    lu.go(end), ld.go(end), ly.go(end), lz.go(end), ldu.go(end), ldd.go(end), ldz.go(end);
+    hp += end / T * hstep;
     stage(0, last);
-    fetch((steps - 1) / T * T);
+    fetch(end);
   }
   int buf = 0;
   for (int tile = last; tile >= 0; tile -= TILE, buf ^= 1) {
@@ -396,7 +404,7 @@ __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 4 : 2) scan_adjoint_ker
   }
   const bool gated = a.z.p != nullptr;
   float rd[C][PF], rz[C][PF], ry[C][PF];
-  const Lane<NL, C> ld(a.delta, at, t0), lz(a.z, at, t0), ly(a.dy, at, t0);
+  Lane<NL, C> ld(a.delta, at, t0), lz(a.z, at, t0), ly(a.dy, at, t0);
   auto fetch = [&](int base) {
     const bool full = base + T <= steps;
 #pragma unroll
@@ -404,10 +412,11 @@ __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 4 : 2) scan_adjoint_ker
 #pragma unroll
       for (int i = 0; i < PF; ++i) {
         const bool on = full || base + i * NL + at.q < steps;
-        rd[c][i] = on ? ld(c, base + i * NL) : 0.0f;
-        ry[c][i] = on ? ly(c, base + i * NL) : 0.0f;
-        rz[c][i] = gated && on ? lz(c, base + i * NL) : 0.0f;
+        rd[c][i] = on ? ld(c, i * NL) : 0.0f;
+        ry[c][i] = on ? ly(c, i * NL) : 0.0f;
+        rz[c][i] = gated && on ? lz(c, i * NL) : 0.0f;
       }
+    ld.go(-T), ly.go(-T), lz.go(-T);
   };
   auto stage = [&](int buf, int tile) {
     stage_rows<NL, TILE>(cs[buf], a.c, a.vec_c, at.b, at.g, t0 + tile, t_end, a.states);
@@ -448,8 +457,10 @@ __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 4 : 2) scan_adjoint_ker
     }
   };
   const int last = (steps - 1) / TILE * TILE;
+  const int end = (steps - 1) / T * T;
+  ld.go(end), ly.go(end), lz.go(end);
   stage(0, last);
-  fetch((steps - 1) / T * T);
+  fetch(end);
   int buf = 0;
   for (int tile = last; tile >= 0; tile -= TILE, buf ^= 1) {
     if (tile > 0)
@@ -544,8 +555,7 @@ int launch_one(const ScanArgs &a, bool adjoint, cudaStream_t stream) {
     scan_adjoint_kernel<NL><<<grid, kScanThreads, 0, stream>>>(a);
   } else {
     constexpr int kRed = kWarps * Bwd<NL>::kTile * 8 * NL * 4, kStatic = 4 * Bwd<NL>::kTile * 4 * NL * 4;
-    if (kRed + kStatic > 48 * 1024)
-      REMORA_CUDA_TRY(cudaFuncSetAttribute(scan_bwd_kernel<NL>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRed));
+    static_assert(kRed + kStatic <= 48 * 1024, "shared memory that needs no attribute");
     scan_bwd_kernel<NL><<<grid, kScanThreads, kRed, stream>>>(a);
   }
   REMORA_CUDA_TRY(cudaGetLastError());
@@ -631,7 +641,6 @@ int remora_b200_selective_scan_bwd(RemoraB200Ctx *ctx, const RemoraSelectiveScan
   REMORA_TRY(remora_b200_selective_scan_saved(B, L, D, N, &need));
   REMORA_TRY(want_scratch(saved, saved_bytes, need, "selective_scan_bwd (saved)"));
   REMORA_TRY(want_scratch(scratch, scratch_bytes, l.total * 4, "selective_scan_bwd"));
-  if (D == 0) return REMORA_OK;
   const int chan = bwd_chan(nl);
   for (int k : {0, 1, 6})
     if (v[k].aligned) REMORA_TRY(check_reach(v[k], nl, chan, "selective_scan_bwd"));
@@ -652,17 +661,17 @@ int remora_b200_selective_scan_bwd(RemoraB200Ctx *ctx, const RemoraSelectiveScan
     return fail(REMORA_ERR_LIMIT, "selective_scan_bwd: too many blocks");
   DeviceGuard guard;
   REMORA_TRY(guard.enter(ctx));
-  if (B > 0) {
+  if (B > 0 && D > 0) {
     if (a.chunks > 1) {
       REMORA_TRY(launch_bwd(a, nl, true, stream));
       REMORA_TRY(combine_chunks(a, nl, true, stream));
     }
     REMORA_TRY(launch_bwd(a, nl, false, stream));
-    if (a.blocks_d > 1 && L > 0) {
-      note_launch();
-      join_bc_kernel<<<(unsigned)((B * L * G * N + 255) / 256), 256, 0, stream>>>(a);
-      REMORA_CUDA_TRY(cudaGetLastError());
-    }
+  }
+  if (B * L > 0 && a.blocks_d != 1) {  // no channels: zeros
+    note_launch();
+    join_bc_kernel<<<(unsigned)((B * L * G * N + 255) / 256), 256, 0, stream>>>(a);
+    REMORA_CUDA_TRY(cudaGetLastError());
   }
   const Columns da = {reinterpret_cast<float *>(o[2].data(4)), N, o[2].strides[0], o[2].strides[1], D * N, nullptr, 0};
   REMORA_TRY(reduce_rows(a.part_a, B * a.chunks, D * N, da, stream));

@@ -439,6 +439,8 @@ def _refuse(what: str, device: int, operands) -> None:
 
 
 def _cuda_index(t) -> int:
+    if not isinstance(t, _torch().Tensor):
+        raise RemoraB200Error(f"the first operand is a {type(t).__name__}, not a tensor")
     index = t.get_device()
     if index < 0:
         raise RemoraB200Error("remora_b200 ops take CUDA tensors (there is no CPU path)")
