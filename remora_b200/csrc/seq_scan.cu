@@ -188,6 +188,8 @@ __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 4 : 2) scan_fwd_kernel(
     fetch(GROUP);
   }
   const int64_t kept = (a.length + GROUP - 1) / GROUP;
+  // the states kept at the groups' starts: [group, local channel, q]
+  ulonglong2 *keep = reinterpret_cast<ulonglong2 *>(a.saved) + ((at.b * kept + t0 / GROUP) * a.dim + at.first) * NL;
   int buf = 0;
   for (int tile = 0; tile < steps; tile += kTile, buf ^= 1) {
     if (tile + kTile < steps)
@@ -201,10 +203,8 @@ __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 4 : 2) scan_fwd_kernel(
       if (MAIN && a.saved) {
 #pragma unroll
         for (int c = 0; c < kChan; ++c)
-          if (at.live[c])
-            reinterpret_cast<ulonglong2 *>(
-                a.saved)[((at.b * kept + (t0 + base) / GROUP) * a.dim + at.d[c]) * NL + at.q] =
-                make_ulonglong2(h[c][0], h[c][1]);
+          if (at.live[c]) keep[(unsigned)(at.local[c] * NL + at.q)] = make_ulonglong2(h[c][0], h[c][1]);
+        keep += a.dim * NL;
       }
       const float *bt = &bs[buf][(base - tile) * NP], *ct = &cs[buf][MAIN ? (base - tile) * NP : 0];
       if (base + GROUP <= steps)

@@ -310,6 +310,16 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const ScanArg
       for (int k = 0; k < 2; ++k) dA[c][k] = add2(dA[c][k], da[c][k]);
     ldu.go(-T), ldd.go(-T), ldz.go(-T);
   };
+  // In a tile's join a thread has one column, jf (state jn of db or dc), and every
+  // JROWS-th step.
+  constexpr int JROWS = kScanThreads / (2 * NP);
+  const int jf = threadIdx.x % (2 * NP), jt = threadIdx.x / (2 * NP), jn = jf % NP;
+  const bool jc = jf >= NP;
+  const Op4 &jo = jc ? a.dc : a.db;
+  const int64_t jstep = a.blocks_d == 1 ? jo.s1 : (int64_t)a.groups * 2 * a.states;
+  float *jp = a.blocks_d == 1
+                  ? jo.p + (at.b * jo.s0 + t0 * jo.s1 + at.g * jo.s2 + jn * jo.s3)
+                  : a.part_bc + ((((at.bd * a.batch + at.b) * a.length + t0) * a.groups + at.g) * 2 + jc) * a.states + jn;
   const int last = steps > 0 ? (steps - 1) / TILE * TILE : -TILE;
   if (steps > 0) {
     const int end = (steps - 1) / T * T;
@@ -337,20 +347,13 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const ScanArg
     }
     __syncthreads();
     // join the warps; a row of part_bc is one channel block's share
-    for (int i = threadIdx.x; i < TILE * 2 * NP; i += kScanThreads) {
-      const int t = i / (2 * NP), f = i % (2 * NP), n = f % NP;
-      if (tile + t >= steps || n >= a.states) continue;
-      float v = 0.0f;
+    if (jn < a.states) {
+#pragma unroll 4
+      for (int t = jt; t < TILE && tile + t < steps; t += JROWS) {
+        float v = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) v += red[w * TILE * 2 * NP + i];
-      const bool is_c = f >= NP;
-      const int64_t tt = t0 + tile + t;
-      if (a.blocks_d == 1) {
-        const Op4 &o = is_c ? a.dc : a.db;
-        o.p[at.b * o.s0 + tt * o.s1 + at.g * o.s2 + n * o.s3] = v;
-      } else {
-        const int64_t row = ((at.bd * a.batch + at.b) * a.length + tt) * a.groups + at.g;
-        a.part_bc[(row * 2 + is_c) * a.states + n] = v;
+        for (int w = 0; w < kWarps; ++w) v += red[w * TILE * 2 * NP + t * 2 * NP + jf];
+        jp[(tile + t) * jstep] = v;
       }
     }
   }
