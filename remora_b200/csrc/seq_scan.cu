@@ -272,14 +272,18 @@ __global__ void __launch_bounds__(256) scan_combine_kernel(const ScanArgs a, int
 constexpr int64_t kManyBlocks = 148 * 4;
 
 // An operand of one token per row and its strides along up to three axes.
-// They are 32-bit, so that an index times a stride, a 64-bit sum, is one
-// instruction; the host refuses larger ones.
+// They are 32-bit and in bytes, so that an index times a stride added to an
+// address is one instruction; the host refuses larger ones.  at() is what a
+// thread's rows share, row() adds the row's part.
 struct Token {
   float *p;
   int s0, s1, s2;
-  __device__ __forceinline__ float *operator()(int i, int j, int k) const {
-    return p + ((int64_t)i * s0 + (int64_t)j * s1 + (int64_t)k * s2);
+  __device__ __forceinline__ static float *add(float *o, int i, int bytes) {
+    return reinterpret_cast<float *>(reinterpret_cast<char *>(o) + (int64_t)i * bytes);
   }
+  __device__ __forceinline__ float *at(int j, int k) const { return add(add(p, j, s1), k, s2); }
+  __device__ __forceinline__ float *row(float *o, int i) const { return add(o, i, s0); }
+  __device__ __forceinline__ float *operator()(int i, int j) const { return row(add(p, j, s1), i); }
 };
 
 struct TokenArgs {
@@ -287,15 +291,15 @@ struct TokenArgs {
   const int *slots;
   int slots_s;
   int batch, rows, dim, per;
-  int states, groups, softplus, zero_rest, vec;
+  int states, groups, softplus, zero_rest;
 };
 
 // Four states of one channel per thread, of R batch rows, R either 1 or the
 // smaller of NL and 4.  Bound by the states' bytes: with R > 1 the decay rates
 // are read once for R rows, R states are on their way at once, and what belongs
 // to a row and channel alone (the step, the gate, y) is worked out by one of the
-// NL lanes.
-template <int NL, int R>
+// NL lanes.  VEC: four states are one aligned load, and none is past N.
+template <int NL, int R, bool VEC>
 __global__ void __launch_bounds__(kScanThreads, 7) scan_step_kernel(const TokenArgs a) {
   const int i0 = (int)blockIdx.y * R;
   const int q = threadIdx.x % NL, d = (int)blockIdx.x * (kScanThreads / NL) + threadIdx.x / NL;
@@ -319,57 +323,69 @@ __global__ void __launch_bounds__(kScanThreads, 7) scan_step_kernel(const TokenA
   bool mine = false;
 #pragma unroll
   for (int r = 0; r < R; ++r) mine = r == own ? on[r] && d < a.dim : mine;
-  float h[R][4], b[R][4], c[R][4], A[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  auto get = [&](const float *p, int stride, float (&v)[4]) {
-    if (a.vec) {
-      unpack(*reinterpret_cast<const float4 *>(p), v);
+  f2 h[R][2], b[R][2], c[R][2], A[2] = {0, 0};
+  auto get = [&](float *p, int stride, f2 (&v)[2]) {
+    if (VEC) {
+      const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(p);
+      v[0] = w.x, v[1] = w.y;
     } else {
+      float w[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = k < nv ? p[(int64_t)k * stride] : 0.0f;
+      for (int k = 0; k < 4; ++k) w[k] = k < nv ? *Token::add(p, k, stride) : 0.0f;
+      v[0] = pair(w[0], w[1]), v[1] = pair(w[2], w[3]);
     }
   };
+  {
+    float *p = a.state.at(d, 4 * q);
 #pragma unroll
-  for (int r = 0; r < R; ++r)
-    if (on[r] && nv > 0) get(a.state(slot[r], d, 4 * q), a.state.s2, h[r]);
+    for (int r = 0; r < R; ++r)
+      if (on[r] && nv > 0) get(a.state.row(p, slot[r]), a.state.s2, h[r]);
+  }
   float u = 0.0f, s = 0.0f, z = 0.0f, sig;
   if (mine) {
-    u = *a.u(i0 + own, d, 0);
-    s = *a.delta(i0 + own, d, 0);
-    if (a.bias.p) s += *a.bias(0, d, 0);
-    if (a.z.p) z = *a.z(i0 + own, d, 0);
+    u = *a.u(i0 + own, d);
+    s = *a.delta(i0 + own, d);
+    if (a.bias.p) s += *a.bias(0, d);
+    if (a.z.p) z = *a.z(i0 + own, d);
   }
-  if (nv > 0) get(a.a(0, d, 4 * q), a.a.s2, A);
-  const int g = a.groups > 1 ? (int)((unsigned)d / (unsigned)a.per) : 0;
+  if (nv > 0) get(a.a.at(d, 4 * q), a.a.s2, A);
+  {
+    const int g = a.groups > 1 ? (int)((unsigned)d / (unsigned)a.per) : 0;
+    float *pb = a.b.row(a.b.at(g, 4 * q), i0), *pc = a.c.row(a.c.at(g, 4 * q), i0);
 #pragma unroll
-  for (int r = 0; r < R; ++r)
-    if (on[r] && nv > 0) {
-      get(a.b(i0 + r, g, 4 * q), a.b.s2, b[r]);
-      get(a.c(i0 + r, g, 4 * q), a.c.s2, c[r]);
-    }
+    for (int r = 0; r < R; ++r)
+      if (on[r] && nv > 0) {
+        get(a.b.row(pb, r), a.b.s2, b[r]);
+        get(a.c.row(pc, r), a.c.s2, c[r]);
+      }
+  }
   if (a.softplus) s = softplus(s, &sig);
   const float su = s * u;
   float part[R];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) A[k] *= kLog2e;
+  A[0] = mul2(A[0], both(kLog2e)), A[1] = mul2(A[1], both(kLog2e));
+  float *po = a.state_out.at(d, 4 * q);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const float sr = R > 1 ? __shfl_sync(0xffffffffu, s, r, NL) : s;
-    const float sur = R > 1 ? __shfl_sync(0xffffffffu, su, r, NL) : su;
+    const f2 sr = both(R > 1 ? __shfl_sync(0xffffffffu, s, r, NL) : s);
+    const f2 sur = both(R > 1 ? __shfl_sync(0xffffffffu, su, r, NL) : su);
     part[r] = 0.0f;
     if (on[r] && nv > 0) {
+      f2 v[2];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (a.vec || k < nv) {
-          h[r][k] = fmaf(decay(sr, A[k]), h[r][k], sur * b[r][k]);
-          part[r] = fmaf(h[r][k], c[r][k], part[r]);
-        }
-      float *o = a.state_out(slot[r], d, 4 * q);
-      if (a.vec) {
-        *reinterpret_cast<float4 *>(o) = make_float4(h[r][0], h[r][1], h[r][2], h[r][3]);
+      for (int k = 0; k < 2; ++k) {
+        v[k] = fma2(decay2(sr, A[k]), h[r][k], mul2(sur, b[r][k]));
+        // past N: s u may not be finite
+        if (!VEC) v[k] = pair(2 * k < nv ? lo(v[k]) : 0.0f, 2 * k + 1 < nv ? hi(v[k]) : 0.0f);
+      }
+      const f2 sum = fma2(v[1], c[r][1], mul2(v[0], c[r][0]));
+      part[r] = lo(sum) + hi(sum);
+      float *o = a.state_out.row(po, slot[r]);
+      if (VEC) {
+        *reinterpret_cast<ulonglong2 *>(o) = make_ulonglong2(v[0], v[1]);
       } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (k < nv) o[(int64_t)k * a.state_out.s2] = h[r][k];
+          if (k < nv) *Token::add(o, k, a.state_out.s2) = k & 1 ? hi(v[k / 2]) : lo(v[k / 2]);
       }
     }
   }
@@ -380,11 +396,11 @@ __global__ void __launch_bounds__(kScanThreads, 7) scan_step_kernel(const TokenA
   transpose_sum<R>(part, own);
   if (mine && q < R) {
     float y = part[0];
-    if (a.d.p) y = fmaf(*a.d(0, d, 0), u, y);
+    if (a.d.p) y = fmaf(*a.d(0, d), u, y);
     if (a.z.p) y *= z * sigmoid(z);
-    *a.y(i0 + own, d, 0) = y;
+    *a.y(i0 + own, d) = y;
   } else if (a.zero_rest && !mine && d < a.dim && i0 + own < a.batch && q < R) {
-    *a.y(i0 + own, d, 0) = 0.0f;
+    *a.y(i0 + own, d) = 0.0f;
   }
 }
 
@@ -633,16 +649,16 @@ int remora_b200_selective_scan_step(RemoraB200Ctx *ctx, const RemoraSelectiveSca
   for (const auto &x : places) {
     if (x.v == nullptr) continue;
     for (int k = 0; k < x.v->rank; ++k)
-      if (std::abs(stride_of(*x.v, k)) > 0x7fffffff)
-        return fail(REMORA_ERR_LIMIT, "selective_scan_step: a stride of %lld elements (at most 2^31 - 1)",
+      if (std::abs(stride_of(*x.v, k)) > 0x1fffffff)
+        return fail(REMORA_ERR_LIMIT, "selective_scan_step: a stride of %lld elements (at most 2^29 - 1)",
                     (long long)x.v->strides[k]);
-    auto stride = [&](int k) { return k < 0 ? 0 : (int)stride_of(*x.v, k); };
+    auto stride = [&](int k) { return k < 0 ? 0 : (int)stride_of(*x.v, k) * 4; };
     if (x.to) *x.to = {reinterpret_cast<float *>(x.v->data(4)), stride(x.row), stride(x.channel), stride(x.state)};
   }
   if (has_l) a.slots = reinterpret_cast<const int *>(lv.data(4)), a.slots_s = (int)stride_of(lv, 0);
   a.batch = (int)B, a.rows = (int)S, a.dim = (int)D, a.per = (int)(D / G), a.states = (int)N, a.groups = (int)G;
   a.softplus = spec->softplus != 0, a.zero_rest = spec->zero_rest != 0;
-  a.vec = vec_states(sv) && vec_states(ov) && vec_states(av) && vec_states(bv) && vec_states(cv);
+  const bool vec = vec_states(sv) && vec_states(ov) && vec_states(av) && vec_states(bv) && vec_states(cv);
   const int nl = lanes_for(a.states);
   // several rows per thread once that leaves every SM some blocks
   const int64_t blocks = (D + kScanThreads / nl - 1) / (kScanThreads / nl);
@@ -653,20 +669,27 @@ int remora_b200_selective_scan_step(RemoraB200Ctx *ctx, const RemoraSelectiveSca
   REMORA_TRY(guard.enter(ctx));
   cudaStream_t s = (cudaStream_t)stream;
   note_launch();
-#define REMORA_STEP_CASE(NL)                                        \
-  case NL:                                                          \
-    if (many)                                                       \
-      scan_step_kernel<NL, (NL < 4 ? NL : 4)><<<grid, kScanThreads, 0, s>>>(a); \
-    else                                                            \
-      scan_step_kernel<NL, 1><<<grid, kScanThreads, 0, s>>>(a);     \
+#define REMORA_STEP_LAUNCH(NL, R)                                     \
+  if (vec)                                                            \
+    scan_step_kernel<NL, R, true><<<grid, kScanThreads, 0, s>>>(a);   \
+  else                                                                \
+    scan_step_kernel<NL, R, false><<<grid, kScanThreads, 0, s>>>(a);
+#define REMORA_STEP_CASE(NL)                        \
+  case NL:                                          \
+    if (many) {                                     \
+      REMORA_STEP_LAUNCH(NL, (NL < 4 ? NL : 4))     \
+    } else {                                        \
+      REMORA_STEP_LAUNCH(NL, 1)                     \
+    }                                               \
     break;
   switch (nl) {
-  case 1: scan_step_kernel<1, 1><<<grid, kScanThreads, 0, s>>>(a); break;
+  case 1: REMORA_STEP_LAUNCH(1, 1) break;
     REMORA_STEP_CASE(2)
     REMORA_STEP_CASE(4)
     REMORA_STEP_CASE(8)
     REMORA_STEP_CASE(16)
   }
+#undef REMORA_STEP_LAUNCH
 #undef REMORA_STEP_CASE
   REMORA_CUDA_TRY(cudaGetLastError());
   return REMORA_OK;
