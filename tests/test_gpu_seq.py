@@ -456,6 +456,52 @@ def test_scan_steps_continue_a_prompt(cuda, D, N, G):
     within(state, rlast, mlast * tol, "state")
 
 
+@pytest.mark.parametrize("N,G", [(16, 1), (16, 3), (13, 1), (12, 2), (8, 1), (7, 1), (24, 1), (64, 2), (33, 1), (4, 1)])
+@pytest.mark.parametrize("pool", [False, True])
+def test_scan_step_of_many_rows(cuda, N, G, pool):
+    """Several rows per thread, the last group of them not full; in a pool some
+    rows are left out: padding, out of range, named before in the same group of
+    rows and in an earlier one."""
+    rng = np.random.default_rng(N * 10 + G)
+    B, D = 251, 300
+    S = B + 30 if pool else B
+    v = {k: None if a is None else a[:, 0] if k in ("u", "delta", "B", "C", "z") else a
+         for k, a in scan_inputs(rng, B, 1, D, N, G, True).items()}
+    h = rnd(rng, S, D, N)
+    slots = np.arange(B, dtype=np.int32)
+    out = np.zeros(B, bool)
+    if pool:
+        slots = rng.permutation(S)[:B].astype(np.int32)
+        slots[[0, 101, 102]], slots[9], slots[10], slots[250] = -1, slots[8], S, slots[3]
+        out[[0, 9, 10, 101, 102, 250]] = True
+    args = (*(v[k][:, None] if k in ("u", "delta", "B", "C", "z") else v[k]
+              for k in ("u", "delta", "A", "B", "C", "D", "z", "bias")), True, h[np.where(out, 0, slots)], 1 - out)
+    ry, rlast = ref.selective_scan(*args)
+    my, mlast = ref.selective_scan(*args, absolute=True)
+    tol = (6 + 64) * E
+    d = {k: dev(a, cuda) for k, a in v.items()}
+    state = dev(h, cuda)
+    y = ops.selective_scan_step(state, d["u"], d["delta"], d["A"], d["B"], d["C"], d["D"], z=d["z"],
+                                delta_bias=d["bias"], softplus=True, slots=dev(slots, cuda) if pool else None)
+    within(y, ry[:, 0], my[:, 0] * tol, "y")
+    after = to_host(state)
+    within(after[slots[~out]], rlast[~out], mlast[~out] * tol, "state")
+    rest = np.setdiff1d(np.arange(S), slots[~out])
+    np.testing.assert_array_equal(after[rest], h[rest])
+
+
+def test_scan_without_channels(cuda):
+    """No channels: the gradients of b and c are sums of nothing."""
+    import torch
+
+    z = lambda *s: torch.zeros(s, device=cuda)
+    bc = torch.ones(2, 5, 3, device=cuda)
+    y, h, saved = ops.selective_scan_fwd(z(2, 5, 0), z(2, 5, 0), z(0, 3), bc, bc, return_state=True, save=True)
+    assert y.shape == (2, 5, 0) and h.shape == (2, 0, 3)
+    got = ops.selective_scan_bwd(z(2, 5, 0), z(2, 5, 0), z(0, 3), bc, bc, z(2, 5, 0), saved)
+    assert (got[3] == 0).all() and (got[4] == 0).all() and got[3].shape == bc.shape
+
+
 def test_scan_strided_views_equal_contiguous(cuda):
     import torch
 

@@ -175,6 +175,30 @@ def test_scan_refusals():
     assert bwd([outs[0], outs[0], *outs[2:]]) == L.ERR_ARG  # one array for two gradients
 
 
+def test_scan_step_refusals():
+    far = [BASE + (k << 40) for k in range(12)]
+    spec = L.RemoraSelectiveScanSpec(1, 0)
+    good = dict(state=desc(4, 6, 5, at=far[0]), u=desc(2, 6, at=far[1]), delta=desc(2, 6, at=far[2]),
+                a=desc(6, 5, at=far[3]), b=desc(2, 2, 5, at=far[4]), c=desc(2, 2, 5, at=far[5]), d=None, z=None,
+                delta_bias=None, slots=None)
+
+    def step(y=desc(2, 6, at=far[6]), out=None, **kw):
+        m = {**good, **kw}
+        args = L.RemoraSelectiveStepIn(*(ad(v) for v in m.values()))
+        return L.lib().remora_b200_selective_scan_step(FAKE, ctypes.addressof(spec), ctypes.addressof(args), ad(y),
+                                                       ad(out or m["state"]), None)
+
+    assert step(u=None) == L.ERR_ARG
+    assert step(state=desc(1, 6, 5, at=far[0])) == L.ERR_SHAPE  # two rows, one state
+    assert step(state=desc(4, 6, 4, at=far[0])) == L.ERR_SHAPE
+    assert step(b=desc(2, 4, 5, at=far[4])) == L.ERR_SHAPE  # six channels in four groups
+    assert step(slots=desc(3, at=far[7])) == L.ERR_SHAPE
+    assert step(y=desc(2, 6, at=far[1])) == L.ERR_ARG
+    assert step(out=desc(4, 6, 5, at=far[0] + 8)) == L.ERR_ARG  # neither the state nor apart from it
+    assert step(state=desc(4, 6, 5, at=far[0], strides=[1 << 29, 5, 1])) == L.ERR_LIMIT
+    assert step(u=desc(2, 6, at=far[1], strides=[-(1 << 29), 1], offset=1 << 29)) == L.ERR_LIMIT
+
+
 def test_overlap_is_decided_by_the_elements():
     """Against enumeration: random small views of one buffer as s and dx of a
     norm's backward, refused as overlapping exactly where they share an element
