@@ -272,14 +272,14 @@ __global__ void __launch_bounds__(256) scan_combine_kernel(const ScanArgs a, int
 constexpr int64_t kManyBlocks = 148 * 4;
 
 // An operand of one token per row and its strides along up to three axes.
-// They are 32-bit and in bytes, so that an index times a stride added to an
-// address is one instruction; the host refuses larger ones.  at() is what a
-// thread's rows share, row() adds the row's part.
+// They are 32-bit, and four times an index is, so that a stride times an index
+// added to an address is one instruction; the host refuses larger ones.  at() is
+// what a thread's rows share, row() adds the row's part.
 struct Token {
   float *p;
   int s0, s1, s2;
-  __device__ __forceinline__ static float *add(float *o, int i, int bytes) {
-    return reinterpret_cast<float *>(reinterpret_cast<char *>(o) + (int64_t)i * bytes);
+  __device__ __forceinline__ static float *add(float *o, int i, int stride) {
+    return reinterpret_cast<float *>(reinterpret_cast<char *>(o) + (int64_t)(4 * i) * stride);
   }
   __device__ __forceinline__ float *at(int j, int k) const { return add(add(p, j, s1), k, s2); }
   __device__ __forceinline__ float *row(float *o, int i) const { return add(o, i, s0); }
@@ -634,7 +634,8 @@ int remora_b200_selective_scan_step(RemoraB200Ctx *ctx, const RemoraSelectiveSca
                          {&cv, "c", 4}, {has_d ? &dv : nullptr, "d", 4}, {has_z ? &zv : nullptr, "z", 4},
                          {has_i ? &iv : nullptr, "delta_bias", 4}, {has_l ? &lv : nullptr, "slots", 4}}, {&sv}));
   if (B == 0 || D == 0) return REMORA_OK;
-  if (std::max(D, S) > 0x3fffffff) return fail(REMORA_ERR_LIMIT, "selective_scan_step: more than 2^30 rows");
+  if (std::max(D, S) > 0x1fffffff)
+    return fail(REMORA_ERR_LIMIT, "selective_scan_step: 2^29 channels or rows of state, or more");
   TokenArgs a = {};
   // each operand's place in Token: row, channel (or group), state
   struct {
@@ -649,10 +650,10 @@ int remora_b200_selective_scan_step(RemoraB200Ctx *ctx, const RemoraSelectiveSca
   for (const auto &x : places) {
     if (x.v == nullptr) continue;
     for (int k = 0; k < x.v->rank; ++k)
-      if (std::abs(stride_of(*x.v, k)) > 0x1fffffff)
-        return fail(REMORA_ERR_LIMIT, "selective_scan_step: a stride of %lld elements (at most 2^29 - 1)",
+      if (std::abs(stride_of(*x.v, k)) > 0x7fffffff)
+        return fail(REMORA_ERR_LIMIT, "selective_scan_step: a stride of %lld elements (at most 2^31 - 1)",
                     (long long)x.v->strides[k]);
-    auto stride = [&](int k) { return k < 0 ? 0 : (int)stride_of(*x.v, k) * 4; };
+    auto stride = [&](int k) { return k < 0 ? 0 : (int)stride_of(*x.v, k); };
     if (x.to) *x.to = {reinterpret_cast<float *>(x.v->data(4)), stride(x.row), stride(x.channel), stride(x.state)};
   }
   if (has_l) a.slots = reinterpret_cast<const int *>(lv.data(4)), a.slots_s = (int)stride_of(lv, 0);

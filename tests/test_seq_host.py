@@ -195,8 +195,9 @@ def test_scan_step_refusals():
     assert step(slots=desc(3, at=far[7])) == L.ERR_SHAPE
     assert step(y=desc(2, 6, at=far[1])) == L.ERR_ARG
     assert step(out=desc(4, 6, 5, at=far[0] + 8)) == L.ERR_ARG  # neither the state nor apart from it
-    assert step(state=desc(4, 6, 5, at=far[0], strides=[1 << 29, 5, 1])) == L.ERR_LIMIT
-    assert step(u=desc(2, 6, at=far[1], strides=[-(1 << 29), 1], offset=1 << 29)) == L.ERR_LIMIT
+    assert step(state=desc(4, 6, 5, at=far[0], strides=[1 << 31, 5, 1])) == L.ERR_LIMIT
+    assert step(state=desc(1 << 29, 6, 5, at=far[0])) == L.ERR_LIMIT
+    assert step(u=desc(2, 6, at=far[1], strides=[-(1 << 31), 1], offset=1 << 31)) == L.ERR_LIMIT
 
 
 def test_overlap_is_decided_by_the_elements():
