@@ -47,34 +47,50 @@ constexpr int64_t kCutBelow = 148 * 2;
 
 int64_t bwd_channels(int nl) { return kScanThreads / nl * bwd_chan(nl); }  // of a block
 
-// Sums v over the 32 / NL channel lanes of a warp; CNT of the sums end in
-// v[0 .. CNT-1] of each lane, the sums FIRST .. FIRST + CNT - 1.
+// The sums over a warp's channels: lanes of the same q.  Each lane leaves its four
+// states of db and of dc in shared memory, and after kSteps steps each lane adds
+// up four states of one step's db or dc over all channels (over a kParts-th of
+// them, and the parts by shuffles).  Rows are kRow floats apart, so that eight
+// lanes, which read 16 bytes each at once, meet 32 banks.
 template <int NL>
 struct ChannelSum {
-  static constexpr int kLanesD = 32 / NL;
-  static constexpr int kCount = kLanesD >= 8 ? 1 : 8 / kLanesD;
-  __device__ static __forceinline__ void run(float (&v)[8], int lane) {
-    int half = 4;
-#pragma unroll
-    for (int o = 16; o >= NL; o >>= 1) {
-      if (half >= 1) {
-        const bool up = lane & o;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (k < half) {
-            const float send = up ? v[k] : v[k + half];
-            const float keep = up ? v[k + half] : v[k];
-            v[k] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-          }
-        half >>= 1;
-      } else {
-        v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
-      }
-    }
+  static constexpr int kSteps = 16 / NL < save_every(NL) ? 16 / NL : save_every(NL);
+  static constexpr int kParts = 16 / (NL * kSteps);
+  static constexpr int kEach = 32 / NL / kParts;
+  static constexpr int kRow = 128 + 4 * NL % 32;
+  static constexpr int kFloats = kSteps * 2 * kRow;
+  float *to;          // where the lane leaves its states of step 0
+  const float *from;  // the first of the values that it adds up
+  int out;            // where their sum goes, from a step's row of db and dc
+  bool stores;
+  __device__ __forceinline__ ChannelSum(float *room, int lane) {
+    const int q = lane % NL, which = lane / NL % 2, step = lane / (2 * NL) % kSteps, part = lane / (2 * NL * kSteps);
+    to = room + 4 * lane;
+    from = room + (step * 2 + which) * kRow + part * kEach * 4 * NL + 4 * q;
+    out = (step * 2 + which) * 4 * NL + 4 * q;
+    stores = part == 0;
   }
-  __device__ static __forceinline__ int first(int lane) { return lane / (NL > 4 ? NL : 4) * kCount; }
-  // of the lanes that hold the same sum, one stores it
-  __device__ static __forceinline__ bool stores(int lane) { return NL >= 4 || (lane & 3) < NL; }
+  __device__ __forceinline__ void put(int step, const f2 (&db)[2], const f2 (&dc)[2]) const {
+    *reinterpret_cast<ulonglong2 *>(to + step * 2 * kRow) = make_ulonglong2(db[0], db[1]);
+    *reinterpret_cast<ulonglong2 *>(to + (step * 2 + 1) * kRow) = make_ulonglong2(dc[0], dc[1]);
+  }
+  // all lanes of the warp, after the last put of kSteps steps
+  __device__ __forceinline__ void add_up(float *row) const {
+    __syncwarp();
+    ulonglong2 sum = *reinterpret_cast<const ulonglong2 *>(from);
+#pragma unroll
+    for (int k = 1; k < kEach; ++k) {
+      const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(from + k * 4 * NL);
+      sum.x = add2(sum.x, v.x), sum.y = add2(sum.y, v.y);
+    }
+    __syncwarp();  // read, before the next step is put there
+#pragma unroll
+    for (int o = 16; o >= 2 * NL * kSteps; o >>= 1) {
+      sum.x = add2(sum.x, __shfl_xor_sync(0xffffffffu, sum.x, o));
+      sum.y = add2(sum.y, __shfl_xor_sync(0xffffffffu, sum.y, o));
+    }
+    if (stores) *reinterpret_cast<ulonglong2 *>(row + out) = sum;
+  }
 };
 
 // Two blocks per SM, and three for one lane per channel (4 x 2000 x 2000 x 4: 163
@@ -83,11 +99,11 @@ template <int NL>
 __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 2 : 3) scan_bwd_kernel(const ScanArgs a) {
   constexpr int NP = 4 * NL, C = Bwd<NL>::kChan, T = Bwd<NL>::kPiece, TILE = Bwd<NL>::kTile;
   constexpr int PF = T / NL;
-  using Sum = ChannelSum<NL>;
   __shared__ __align__(16) float bs[2][TILE * NP], cs[2][TILE * NP];
-  extern __shared__ __align__(16) float red[];  // [kWarps][TILE][2 NP]: per step db, dc
+  extern __shared__ __align__(16) float red[];  // [kWarps][TILE][2 NP]: per step db, dc; room for ChannelSum
   const Place<NL, C> at(a);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int warp = threadIdx.x >> 5;
+  const ChannelSum<NL> over(red + kWarps * TILE * 2 * NP + warp * ChannelSum<NL>::kFloats, threadIdx.x & 31);
   const int64_t len = scan_length(a, at.b);
   const int64_t t0 = at.chunk * a.chunk, t_end = min(t0 + a.chunk, len);
   const int steps = t_end > t0 ? (int)(t_end - t0) : 0;
@@ -280,16 +296,8 @@ __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 2 : 3) scan_bwd_kernel(
             gb[c][j] = lo(g2) + hi(g2);
             ga[c][j] = lo(a2) + hi(a2);
           }
-          float v[8] = {lo(db[0]), hi(db[0]), lo(db[1]), hi(db[1]), lo(dc[0]), hi(dc[0]), lo(dc[1]), hi(dc[1])};
-          Sum::run(v, lane);
-          if (Sum::stores(lane)) {
-            const int first = Sum::first(lane);
-#pragma unroll
-            for (int k = 0; k < Sum::kCount; ++k) {
-              const int f = first + k;
-              rt[t * 2 * NP + (f >> 2) * NP + 4 * at.q + (f & 3)] = v[k];
-            }
-          }
+          over.put(t % over.kSteps, db, dc);
+          if (t % over.kSteps == 0) over.add_up(rt + t * 2 * NP);
         }
       }
 #pragma unroll
@@ -559,8 +567,10 @@ int launch_one(const ScanArgs &a, bool adjoint, cudaStream_t stream) {
   if (adjoint) {
     scan_adjoint_kernel<NL><<<grid, kScanThreads, 0, stream>>>(a);
   } else {
-    constexpr int kRed = kWarps * Bwd<NL>::kTile * 8 * NL * 4, kStatic = 4 * Bwd<NL>::kTile * 4 * NL * 4;
-    static_assert(kRed + kStatic <= 48 * 1024, "shared memory that needs no attribute");
+    constexpr int kRed = kWarps * (Bwd<NL>::kTile * 8 * NL + ChannelSum<NL>::kFloats) * 4;
+    constexpr int kStatic = 4 * Bwd<NL>::kTile * 4 * NL * 4;
+    if (kRed + kStatic > 48 * 1024)
+      REMORA_CUDA_TRY(cudaFuncSetAttribute(scan_bwd_kernel<NL>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRed));
     scan_bwd_kernel<NL><<<grid, kScanThreads, kRed, stream>>>(a);
   }
   REMORA_CUDA_TRY(cudaGetLastError());
