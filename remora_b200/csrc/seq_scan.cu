@@ -36,12 +36,13 @@ constexpr int64_t kCutBelow = 148 * 3;
 // MAIN: writes y (and h_last, saved).  Otherwise the first pass of a cut time
 // axis: sum_h and sum_dt.  PADDED: N is not 4 NL; the states past N must stay
 // zero even where s u is not finite.  Four blocks per SM for one lane per channel
-// too (4 x 2000 x 2000 x 4: 67 and 46 us, against 85 and 69 with two).
+// too (4 x 2000 x 2000 x 4: 67 and 46 us, against 85 and 69 with two); three for
+// the main pass of two lanes, which spills otherwise (x 8: 77 against 94 us).
 template <int NL, bool PADDED, bool MAIN>
-__global__ void __launch_bounds__(kScanThreads, 4) scan_fwd_kernel(const ScanArgs a) {
+__global__ void __launch_bounds__(kScanThreads, MAIN && NL == 2 ? 3 : 4) scan_fwd_kernel(const ScanArgs a) {
   constexpr int NP = 4 * NL;
-  constexpr int GROUP = save_every(NL);  // steps whose inputs are loaded together
-  constexpr int PF = GROUP / NL;          // of them, per lane
+  constexpr int GROUP = group_steps(NL), SAVE = save_every(NL);
+  constexpr int PF = GROUP / NL;  // steps of a group whose inputs a lane loads
   __shared__ __align__(16) float bs[2][kTile * NP];
   __shared__ __align__(16) float cs[2][MAIN ? kTile * NP : 4];
   const Place<NL, kChan> at(a);
@@ -121,6 +122,9 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_fwd_kernel(const ScanArg
         if (MAIN) y1[c][i] = skip[c] * ru[c][i], w1[c][i] = gated ? rz[c][i] * sigmoid(rz[c][i]) : 1.0f;
       }
   };
+  const int64_t kept = (a.length + SAVE - 1) / SAVE;
+  // the states kept before every SAVE-th step: [step / SAVE, local channel, q]
+  ulonglong2 *keep = reinterpret_cast<ulonglong2 *>(a.saved) + ((at.b * kept + t0 / SAVE) * a.dim + at.first) * NL;
   // GROUP steps from `base` on, whose b and c rows start at bt and ct.  The
   // inputs of the next group are prepared meanwhile, those of the one after
   // it are on their way.
@@ -152,6 +156,12 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_fwd_kernel(const ScanArg
           part[c][j] = 0.0f;
         }
         if (FULL || base + t < steps) {
+          if (MAIN && t % SAVE == 0 && a.saved) {
+#pragma unroll
+            for (int c = 0; c < kChan; ++c)
+              if (at.live[c]) keep[(unsigned)(at.local[c] * NL + at.q)] = make_ulonglong2(h[c][0], h[c][1]);
+            keep += a.dim * NL;
+          }
           const ulonglong2 b = *reinterpret_cast<const ulonglong2 *>(bt + t * NP + 4 * at.q);
           const ulonglong2 cc = MAIN ? *reinterpret_cast<const ulonglong2 *>(ct + t * NP + 4 * at.q) : b;
 #pragma unroll
@@ -188,9 +198,6 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_fwd_kernel(const ScanArg
     prepare();
     fetch(GROUP);
   }
-  const int64_t kept = (a.length + GROUP - 1) / GROUP;
-  // the states kept at the groups' starts: [group, local channel, q]
-  ulonglong2 *keep = reinterpret_cast<ulonglong2 *>(a.saved) + ((at.b * kept + t0 / GROUP) * a.dim + at.first) * NL;
   int buf = 0;
   for (int tile = 0; tile < steps; tile += kTile, buf ^= 1) {
     if (tile + kTile < steps)
@@ -201,12 +208,6 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_fwd_kernel(const ScanArg
     __syncthreads();
 #pragma unroll 1
     for (int base = tile; base < min(tile + kTile, steps); base += GROUP) {
-      if (MAIN && a.saved) {
-#pragma unroll
-        for (int c = 0; c < kChan; ++c)
-          if (at.live[c]) keep[(unsigned)(at.local[c] * NL + at.q)] = make_ulonglong2(h[c][0], h[c][1]);
-        keep += a.dim * NL;
-      }
       const float *bt = &bs[buf][(base - tile) * NP], *ct = &cs[buf][MAIN ? (base - tile) * NP : 0];
       if (base + GROUP <= steps)
         group(std::true_type{}, base, bt, ct);

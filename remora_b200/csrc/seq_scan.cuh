@@ -22,9 +22,13 @@ namespace remora {
 namespace seq {
 
 constexpr int kScanThreads = 128;
-// Steps between the states that the forward keeps for the backward pass: what
-// fits a thread's registers there.
-constexpr int save_every(int nl) { return nl > 8 ? 16 : nl > 1 ? 8 : 4; }
+// Steps whose inputs are loaded together.
+constexpr int group_steps(int nl) { return nl > 8 ? 16 : nl > 1 ? 8 : 4; }
+// Steps between the states that the forward keeps for the backward pass, whose
+// threads hold as many in registers: a multiple of nl.  Four instead of eight
+// lets three blocks live on an SM instead of two (4 x 2048 x 2048 x 16: 357
+// against 400 us) and costs a write and a read of a state twice as often.
+constexpr int save_every(int nl) { return nl > 8 ? 16 : nl > 4 ? 8 : 4; }
 constexpr int kMaxStates = 64;
 constexpr int64_t kMaxLength = 1 << 30;
 constexpr int kChan = 2;  // channels per thread

@@ -10,15 +10,17 @@
 // recurrence forward once, keeping exp(s a) h_{t-1} of every step in registers,
 // then the adjoint backward (the decay's second exponential costs less there
 // than the registers to keep it).  db and dc sum over the channels of a group:
-// over a thread's channels, over a warp by a transposed shuffle, over a block
+// over a thread's channels, over a warp by way of shared memory, over a block
 // through shared memory, over blocks by partial rows in scratch that a second
 // kernel adds in block order.
 //
-// Bound by issue: some 260 instructions per warp, step and pair of channels (8
-// states per thread), of which the sums over channels and states are a third; 255
-// registers leave 8 warps per SM, which issue every other clock.  Measured on B200
-// for 4 x 2048 x 2048 x 16: 467 us, first pass of the adjoint 95, joins 22; with
-// decays kept instead of recomputed, one channel per thread and spilling 1439.
+// Bound by issue and latency: some 210 instructions per warp, step and pair of
+// channels (8 states per thread), at half of the issue slots or less, since the
+// registers leave 8 to 16 warps per SM.  Measured on B200 for 4 x 2048 x 2048 x 16:
+// 357 us, first pass of the adjoint 90, joins 22.  The sums over channels by
+// shuffles: 414 us, with a state kept every eight steps 400; the steps' s, s u and dp
+// from shared memory instead of shuffles 432; the next step's shuffles ahead of a
+// step, the same time.
 #include <algorithm>
 #include <type_traits>
 
@@ -93,10 +95,13 @@ struct ChannelSum {
   }
 };
 
-// Two blocks per SM, and three for one lane per channel (4 x 2000 x 2000 x 4: 163
-// against 178 us; three for two lanes, 283 against 244).
+// Blocks of an SM that the registers are cut for.  4 x 2048 x 2048 x 16: 357 us with
+// three and 363 with two; 4 x 2000 x 2000: x 8, 172 with four and 189 with three of
+// two channels per thread; x 4, 147 with three and 153 with four.
+constexpr int bwd_blocks(int nl) { return nl > 4 ? 2 : nl == 2 ? 4 : 3; }
+
 template <int NL>
-__global__ void __launch_bounds__(kScanThreads, NL > 1 ? 2 : 3) scan_bwd_kernel(const ScanArgs a) {
+__global__ void __launch_bounds__(kScanThreads, bwd_blocks(NL)) scan_bwd_kernel(const ScanArgs a) {
   constexpr int NP = 4 * NL, C = Bwd<NL>::kChan, T = Bwd<NL>::kPiece, TILE = Bwd<NL>::kTile;
   constexpr int PF = T / NL;
   __shared__ __align__(16) float bs[2][TILE * NP], cs[2][TILE * NP];
@@ -394,7 +399,7 @@ __global__ void __launch_bounds__(kScanThreads, NL > 1 ? 2 : 3) scan_bwd_kernel(
 // start when none enters at its end, and the piece's sum of steps.
 template <int NL>
 __global__ void __launch_bounds__(kScanThreads, 4) scan_adjoint_kernel(const ScanArgs a) {
-  constexpr int NP = 4 * NL, C = Bwd<NL>::kChan, T = Bwd<NL>::kPiece, TILE = Bwd<NL>::kTile;
+  constexpr int NP = 4 * NL, C = Bwd<NL>::kChan, T = group_steps(NL), TILE = Bwd<NL>::kTile;
   constexpr int PF = T / NL;
   __shared__ __align__(16) float cs[2][TILE * NP];
   const Place<NL, C> at(a);
