@@ -9,11 +9,12 @@
 // field for other types than f32, and for a result, as fifth field, what it is
 // made like where it was not given: a tensor whose shape it gets or a tuple of
 // sizes (None: left out).  `results` holds the operands with five fields, given
-// or made (contiguous and unset).  The buffer (bytes, to be kept until the call returns) holds a RemoraMemRefN for
-// each tensor; its address follows in the tuple, None for None.  With table = k
-// > 0 the first k addresses form an argument struct at the buffer's start, whose
-// address stands for them.  None is returned when an operand is not a tensor of
-// its type, rank and device: the caller says which.
+// or made (contiguous and unset).  The buffer (bytes, to be kept until the call
+// returns) holds a RemoraMemRefN for each tensor; its address follows in the
+// tuple, None for None.  With table = k > 0 the first k addresses form an
+// argument struct at the buffer's start, whose address stands for them.  None is returned when an operand is not a tensor of
+// its type, rank and device, or a view whose values are the negatives of what its
+// storage holds: the caller says which.
 #include <ATen/ops/empty.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -87,7 +88,7 @@ PyObject *layout(PyObject *const *args, Py_ssize_t nargs) {
     }
     const at::Tensor &t = make ? results[k] : THPVariable_Unpack(value);
     if (t.scalar_type() != type || t.dim() != rank || rank > kMaxRank || t.get_device() != device ||
-        !t.has_storage())
+        !t.has_storage() || t.is_neg())
       Py_RETURN_NONE;
     tensors[k] = &t;
     starts[k] = t.numel() ? (int64_t)reinterpret_cast<uintptr_t>(t.storage().data()) : 0;

@@ -435,7 +435,8 @@ def _refuse(what: str, device: int, operands) -> None:
             raise RemoraB200Error(f"{what}: {name} is on {t.device}, the first operand on cuda:{device}")
         if t.dim() != rank:
             raise RemoraShapeError(f"{what}: {name} has rank {t.dim()}, not {rank}")
-    raise RemoraUnsupportedError(f"{what}: an operand has no dense storage, or a rank over {L.MAX_RANK}")
+    raise RemoraUnsupportedError(
+        f"{what}: an operand has no dense storage, is a lazily negated view, or has a rank over {L.MAX_RANK}")
 
 
 def _cuda_index(t) -> int:
