@@ -15,18 +15,26 @@
 // argument struct at the buffer's start, whose address stands for them.  None is returned when an operand is not a tensor of
 // its type, rank and device, or a view whose values are the negatives of what its
 // storage holds: the caller says which.
+//
+//   room(device, bytes) -> (uint8 tensor of that many unset bytes, its address)
 #include <ATen/ops/empty.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
 #include <cstring>
-#include <exception>
 
 namespace {
 
 constexpr Py_ssize_t kMaxOperands = 32;
 constexpr int64_t kMaxRank = 10;
+
+// of a negative device: in host memory
+at::Tensor unset(at::IntArrayRef sizes, at::ScalarType type, long device) {
+  const at::Device place = device < 0 ? at::Device(at::kCPU) : at::Device(at::kCUDA, (at::DeviceIndex)device);
+  return at::empty(sizes, at::TensorOptions().dtype(type).device(place));
+}
 
 PyObject *layout(PyObject *const *args, Py_ssize_t nargs) {
   if (nargs != 3 || !PyTuple_Check(args[1])) {
@@ -83,8 +91,7 @@ PyObject *layout(PyObject *const *args, Py_ssize_t nargs) {
         PyErr_SetString(PyExc_TypeError, "describe: the fifth field is a tensor or a tuple of at most 10 sizes");
         return nullptr;
       }
-      const at::Device place = device < 0 ? at::Device(at::kCPU) : at::Device(at::kCUDA, (at::DeviceIndex)device);
-      results[k] = at::empty(of, at::TensorOptions().dtype(type).device(place));
+      results[k] = unset(of, type, device);
     }
     const at::Tensor &t = make ? results[k] : THPVariable_Unpack(value);
     if (t.scalar_type() != type || t.dim() != rank || rank > kMaxRank || t.get_device() != device ||
@@ -152,19 +159,33 @@ PyObject *layout(PyObject *const *args, Py_ssize_t nargs) {
   return result;
 }
 
-// torch throws for tensors without plain strides or storage (nested, wrapped)
+// torch throws without memory for a result, and for tensors without plain strides
+// or storage (nested, wrapped)
 PyObject *describe(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
-  try {
-    return layout(args, nargs);
-  } catch (const std::exception &e) {
-    PyErr_SetString(PyExc_TypeError, e.what());
+  HANDLE_TH_ERRORS
+  return layout(args, nargs);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject *room(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  if (nargs != 2) {
+    PyErr_SetString(PyExc_TypeError, "room(device, bytes)");
     return nullptr;
   }
+  const long device = PyLong_AsLong(args[0]);
+  const int64_t bytes = PyLong_AsLongLong(args[1]);
+  if (PyErr_Occurred()) return nullptr;
+  HANDLE_TH_ERRORS
+  const at::Tensor t = unset({bytes}, at::kByte, device);
+  return Py_BuildValue("NN", THPVariable_Wrap(t), PyLong_FromVoidPtr(t.data_ptr()));
+  END_HANDLE_TH_ERRORS
 }
 
 PyMethodDef methods[] = {
     {"describe", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(describe)), METH_FASTCALL,
      "describe(device, operands, table) -> (buffer, results, address, ...) or None"},
+    {"room", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(room)), METH_FASTCALL,
+     "room(device, bytes) -> (uint8 tensor, its address)"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_binding", "Descriptors of a call's tensors.", -1, methods,

@@ -455,14 +455,13 @@ def _raw_stream(device: int) -> int:
     return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
 
 
-def _scratch(fn, what: str, t, *sizes):
-    """(byte tensor, address, bytes) of the scratch that a _scratch entry point asks for."""
+def _scratch(fn, what: str, device: int, *sizes):
+    """(byte tensor, address, bytes) of the memory that a _scratch or _saved entry point asks for."""
     n = ctypes.c_size_t()
     L.check(fn(*sizes, ctypes.byref(n)), what)
     if not n.value:
         return None, None, 0
-    buf = _torch().empty((n.value,), dtype=_torch().uint8, device=t.device)
-    return buf, buf.data_ptr(), n.value
+    return *_binding().room(device, n.value), n.value
 
 
 # indexed by the flag and by zero_rest: set for results made here, whose rows
@@ -517,7 +516,7 @@ def rms_norm_bwd(s, w, dy, *, dsum=None, eps: float = 1e-6, out=None):
         ("dw", None, 1, f32, w)))
     lib, ctx = L.lib(), context(device).ptr
     dim = s.shape[-1] if rank else 0
-    scratch, at, size = _scratch(lib.remora_b200_rms_norm_bwd_scratch, "rms_norm_bwd", s, ctx,
+    scratch, at, size = _scratch(lib.remora_b200_rms_norm_bwd_scratch, "rms_norm_bwd", device, ctx,
                                  s.numel() // dim if dim else 0, dim)
     spec = L.RemoraNormSpec(eps, 0)
     L.check(lib.remora_b200_rms_norm_bwd(ctx, ctypes.addressof(spec), sd, wd, gd, ed, xd, dwd, rank, at, size,
@@ -554,7 +553,7 @@ def causal_conv_bwd(x, w, dy, bias=None, *, state=None, lengths=None, silu: bool
         ("out", out, 3, f32, x), ("dw", None, 2, f32, w), ("dbias", None, 1, f32, bias),
         ("dstate", None, 3, f32, state), ("lengths", lengths, 1, torch.int32)))
     lib, ctx = L.lib(), context(device).ptr
-    scratch, at, size = _scratch(lib.remora_b200_causal_conv_bwd_scratch, "causal_conv_bwd", x, ctx, *x.shape,
+    scratch, at, size = _scratch(lib.remora_b200_causal_conv_bwd_scratch, "causal_conv_bwd", device, ctx, *x.shape,
                                  w.shape[1])
     L.check(lib.remora_b200_causal_conv_bwd(ctx, _spec(_CONV_SPECS, silu, out is None), xd, wd, bd, sd, ld, gd, ed, dxd,
                                             dwd, dbd, dsd, at, size, _raw_stream(device)), "causal_conv_bwd")
@@ -605,14 +604,12 @@ def selective_scan_fwd(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, so
         ("h_last", h_last, 3, f32, wanted)), table=10)
     lib, ctx = L.lib(), context(device).ptr
     sizes = (*u.shape, A.shape[1])
-    scratch, at, size = _scratch(lib.remora_b200_selective_scan_fwd_scratch, "selective_scan_fwd", u, ctx, *sizes,
+    scratch, at, size = _scratch(lib.remora_b200_selective_scan_fwd_scratch, "selective_scan_fwd", device, ctx, *sizes,
                                  Bg.shape[2])
     saved, kept, kept_size = None, None, 0
     if save:
-        n = ctypes.c_size_t()
-        L.check(lib.remora_b200_selective_scan_saved(*sizes, ctypes.byref(n)), "selective_scan_fwd")
-        saved = torch.empty((n.value // 4,), dtype=torch.float32, device=u.device)
-        kept, kept_size = (saved.data_ptr(), n.value) if n.value else (None, 0)
+        saved, kept, kept_size = _scratch(lib.remora_b200_selective_scan_saved, "selective_scan_fwd", device, *sizes)
+        saved = torch.empty((0,), dtype=f32, device=u.device) if saved is None else saved.view(f32)
     L.check(lib.remora_b200_selective_scan_fwd(ctx, _spec(_SCAN_SPECS, softplus, out is None), args, yd, hd, kept,
                                                kept_size, at, size, _raw_stream(device)), "selective_scan_fwd")
     results = (y,) + ((h_last,) if h_last is not None else ()) + ((saved,) if save else ())
@@ -639,7 +636,7 @@ def selective_scan_bwd(u, delta, A, B, C, dy, saved, D=None, *, z=None, delta_bi
         raise RemoraUnsupportedError("selective_scan_bwd: saved is not what selective_scan_fwd returned")
     to = L.RemoraSelectiveScanGrads(*outs)
     lib, ctx = L.lib(), context(device).ptr
-    scratch, at, size = _scratch(lib.remora_b200_selective_scan_bwd_scratch, "selective_scan_bwd", u, ctx, *u.shape,
+    scratch, at, size = _scratch(lib.remora_b200_selective_scan_bwd_scratch, "selective_scan_bwd", device, ctx, *u.shape,
                                  A.shape[1], Bg.shape[2])
     L.check(lib.remora_b200_selective_scan_bwd(ctx, _spec(_SCAN_SPECS, softplus, True), args, gd, hd, saved.data_ptr(),
                                                4 * saved.numel(), ctypes.addressof(to), at, size, _raw_stream(device)),

@@ -871,3 +871,13 @@ def test_python_refusals(cuda):
     with pytest.raises(RemoraUnsupportedError):
         ops.selective_scan_fwd(y, y, torch.zeros((4, 65), device=cuda), torch.zeros((1, 3, 65), device=cuda),
                                torch.zeros((1, 3, 65), device=cuda))
+
+
+def test_no_memory_for_a_result(cuda):
+    """What torch raises, before any launch."""
+    import torch
+
+    row = torch.ones(1, 1 << 20, device=cuda)
+    with pytest.raises(torch.OutOfMemoryError):
+        ops.rms_norm_fwd(row.expand(1 << 22, -1), row[0])  # 16 TiB
+    np.testing.assert_array_equal(to_host(ops.rms_norm_fwd(row, row[0], eps=0.0)), to_host(row))

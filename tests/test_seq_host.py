@@ -281,6 +281,10 @@ def test_binding_lays_out_descriptors():
     for bad in (("x", one, 3), ("x", one.double(), 2), ("x", one, 2, torch.int32), ("x", 3.0, 0), ("x", one.to_sparse(), 2)):
         assert _binding.describe(-1, (bad,), 0) is None
     assert _binding.describe(0, (("x", one, 2),), 0) is None  # another device
+    room, address = _binding.room(-1, 48)
+    assert room.shape == (48,) and room.dtype == torch.uint8 and room.data_ptr() == address
+    with pytest.raises(RuntimeError):
+        _binding.room(-1, -1)
     negated = torch.zeros(2, 3, dtype=torch.complex64).conj().imag  # its storage holds the negatives
     assert negated.is_neg() and _binding.describe(-1, (("x", negated, 2),), 0) is None
     for wrong in ((-1, [("x", one, 2)], 0), (-1, (("x", one),), 0), (-1, (("x", one, 2, "f32"),), 0), (-1, (("x", one, 2),), 2)):
