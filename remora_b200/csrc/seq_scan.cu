@@ -420,13 +420,19 @@ bool vec_states(const DescView &v) {
 }
 
 // Pieces of the time axis: one when the channels alone give the device enough
-// warps, else as many as do, of at least 64 steps each.
+// warps or when the axis is short, else as many as do, of at least 32 steps each.
+// Cutting costs two more launches: 2 x 96 x 300 x 16 takes 15.4 us a call uncut
+// (13.6 on the device) and 20.2 (14.2) cut, 2 x 192 x 300 x 16 25.4 and 20.1; 2 x 64 x
+// 600 x 4, where a lane has more of a step to itself, 21.5 (19.8) and 25.6 (19.4),
+// 2 x 96 x 600 x 4 29.7 and 25.6.
+constexpr int64_t cut_beyond(int nl) { return nl < 4 ? 64 : 96; }
 void cut_time(int64_t batch, int64_t length, int64_t dim, int states, int groups, int64_t *chunks, int64_t *chunk) {
   const int nl = lanes_for(states);
   const int64_t per_block = block_channels(nl, kChan), per = dim / std::max(groups, 1);
   const int64_t blocks = std::max<int64_t>(1, batch * groups * ((per + per_block - 1) / per_block));
   int64_t n = 1;
-  if (blocks < kCutBelow) n = std::max<int64_t>(1, std::min<int64_t>(kBlocks / blocks, length / 16));
+  if (blocks < kCutBelow && length > cut_beyond(nl))
+    n = std::max<int64_t>(1, std::min<int64_t>(kBlocks / blocks, length / 16));
   *chunk = std::max<int64_t>(kTile, ((length + n - 1) / n + kTile - 1) / kTile * kTile);
   *chunks = std::max<int64_t>(1, (length + *chunk - 1) / *chunk);
 }

@@ -435,6 +435,11 @@ def test_scan_cut_in_time(cuda, T, N):
         within(to_host(state)[0], rlast[0], mlast[0] * tol, "two calls' state")
 
 
+@pytest.mark.parametrize("N", [1, 4, 8, 7, 32, 24, 64, 50])
+def test_scan_cut_in_time_of_other_state_counts(cuda, N):
+    test_scan_cut_in_time(cuda, 203, N)
+
+
 @pytest.mark.parametrize("D,N,G", [(6, 16, 1), (10, 13, 2), (64, 4, 1), (33, 64, 3), (3, 1, 1)])
 def test_scan_steps_continue_a_prompt(cuda, D, N, G):
     rng = np.random.default_rng(D + N)
