@@ -194,7 +194,40 @@ struct Columns {
 // The sum over the rows of part [rows, cols], in a fixed order.
 int reduce_rows(const float *part, int64_t rows, int64_t cols, const Columns &to, cudaStream_t stream);
 
+// More threads down a column where rows are many (592 x 2048: 4.1 us with 32, 6.6
+// with 8; 64 x 20480: 8.5 with 32, 5.1 with 8).
+inline bool tall(int64_t rows) { return rows > 256; }
+
 #ifdef __CUDACC__
+// 32 of those columns by a block of Y rows of 32 threads, x and y its thread.
+template <int Y>
+__device__ __forceinline__ void reduce_columns(const float *__restrict__ part, int64_t rows, int64_t cols,
+                                               const Columns &to, int64_t block, int x, int y, float (&t)[Y][33]) {
+  const int64_t c = block * 32 + x;
+  float v = 0.0f;
+  if (c < cols) {
+    int64_t p = y;
+    for (; p + 3 * Y < rows; p += 4 * Y) {
+      float w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = part[(p + k * Y) * cols + c];
+      v += (w[0] + w[1]) + (w[2] + w[3]);
+    }
+    for (; p < rows; p += Y) v += part[p * cols + c];
+  }
+  t[y][x] = v;
+  __syncthreads();
+  if (y == 0 && c < cols) {
+    float s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < Y; ++k) s += t[k][x];
+    if (c < to.split && to.out != nullptr)
+      to.out[(c / to.inner) * to.outer_stride + (c % to.inner) * to.inner_stride] = s;
+    else if (c >= to.split && to.tail != nullptr)
+      to.tail[(c - to.split) * to.tail_stride] = s;
+  }
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

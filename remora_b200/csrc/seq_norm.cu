@@ -512,29 +512,7 @@ template <int Y>
 __global__ void __launch_bounds__(32 * Y) reduce_rows_kernel(const float *__restrict__ part, int64_t rows, int64_t cols,
                                                              const Columns to) {
   __shared__ float t[Y][33];
-  const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x;
-  float v = 0.0f;
-  if (c < cols) {
-    int64_t p = threadIdx.y;
-    for (; p + 3 * Y < rows; p += 4 * Y) {
-      float x[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) x[k] = part[(p + k * Y) * cols + c];
-      v += (x[0] + x[1]) + (x[2] + x[3]);
-    }
-    for (; p < rows; p += Y) v += part[p * cols + c];
-  }
-  t[threadIdx.y][threadIdx.x] = v;
-  __syncthreads();
-  if (threadIdx.y == 0 && c < cols) {
-    float s = 0.0f;
-#pragma unroll
-    for (int k = 0; k < Y; ++k) s += t[k][threadIdx.x];
-    if (c < to.split && to.out != nullptr)
-      to.out[(c / to.inner) * to.outer_stride + (c % to.inner) * to.inner_stride] = s;
-    else if (c >= to.split && to.tail != nullptr)
-      to.tail[(c - to.split) * to.tail_stride] = s;
-  }
+  reduce_columns<Y>(part, rows, cols, to, blockIdx.x, threadIdx.x, threadIdx.y, t);
 }
 
 // ------------------------------------------------------------------ host --
@@ -819,10 +797,8 @@ int launch_bwd(const NormBwdArgs &a, const Tiling &t, unsigned grid, cudaStream_
 int reduce_rows(const float *part, int64_t rows, int64_t cols, const Columns &to, cudaStream_t stream) {
   if (cols == 0) return REMORA_OK;
   note_launch();
-  // more threads down a column where rows are many (592 x 2048: 4.1 us with 32, 6.6
-  // with 8; 64 x 20480: 8.5 with 32, 5.1 with 8)
   const unsigned grid = (unsigned)((cols + 31) / 32);
-  if (rows > 256)
+  if (tall(rows))
     reduce_rows_kernel<32><<<grid, dim3(32, 32), 0, stream>>>(part, rows, cols, to);
   else
     reduce_rows_kernel<8><<<grid, dim3(32, 8), 0, stream>>>(part, rows, cols, to);

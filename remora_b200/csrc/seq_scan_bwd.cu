@@ -17,7 +17,7 @@
 // Bound by issue and latency: some 210 instructions per warp, step and pair of
 // channels (8 states per thread), at half of the issue slots or less, since the
 // registers leave 8 to 16 warps per SM.  Measured on B200 for 4 x 2048 x 2048 x 16:
-// 357 us, first pass of the adjoint 90, joins 22.  The sums over channels by
+// 357 us, first pass of the adjoint 90, joins 23.  The sums over channels by
 // shuffles: 414 us, with a state kept every eight steps 400; the steps' s, s u and dp
 // from shared memory instead of shuffles 432; the next step's shuffles ahead of a
 // step, the same time.
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kScanThreads, bwd_blocks(NL)) scan_bwd_kernel(
     zero_rows(ldu, at, a, t0, len);
     zero_rows(ldd, at, a, t0, len);
     if (a.dz.p) zero_rows(ldz, at, a, t0, len);
-    if (a.blocks_d == 1) {  // else by join_bc_kernel
+    if (a.blocks_d == 1) {  // else by join_kernel
       const int64_t from = max(t0, len), rows = min(t0 + a.chunk, a.length) - from;
       for (int64_t i = threadIdx.x; i < rows * a.states; i += kScanThreads) {
         const int64_t t = from + i / a.states, n = i % a.states;
@@ -511,9 +511,8 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_adjoint_kernel(const Sca
 }
 
 // db and dc of one position, group and state: the channel blocks' shares.
-__global__ void __launch_bounds__(256) join_bc_kernel(const ScanArgs a) {
+__device__ __forceinline__ void join_bc(const ScanArgs &a, int64_t i) {
   const int64_t plane = a.batch * a.length * a.groups * a.states;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= plane) return;
   const int64_t n = i % a.states, g = i / a.states % a.groups, bt = i / a.states / a.groups;
   const int64_t t = bt % a.length, b = bt / a.length;
@@ -529,6 +528,27 @@ __global__ void __launch_bounds__(256) join_bc_kernel(const ScanArgs a) {
   if (rest) vb = vc = 0.0f;  // their shares were never written
   a.db.p[b * a.db.s0 + t * a.db.s1 + g * a.db.s2 + n * a.db.s3] = vb;
   a.dc.p[b * a.dc.s0 + t * a.dc.s1 + g * a.dc.s2 + n * a.dc.s3] = vc;
+}
+
+// The rows of the partial sums and where their columns go.
+struct Joins {
+  int64_t rows;
+  Columns a, d;
+  unsigned blocks_a, blocks_d;  // the first blocks of the grid; the others join db and dc
+};
+
+// All sums that are left: of da, of dd and ddelta_bias over the pieces of time and
+// the batch, of db and dc over the channel blocks.  In one launch: as three, 3 x 509
+// x 388 x 13 took 6 us more.
+template <int Y>
+__global__ void __launch_bounds__(32 * Y) join_kernel(const ScanArgs a, const Joins j) {
+  __shared__ float t[Y][33];
+  const int x = threadIdx.x % 32, y = threadIdx.x / 32;
+  unsigned block = blockIdx.x;
+  if (block < j.blocks_a) return reduce_columns<Y>(a.part_a, j.rows, a.dim * a.states, j.a, block, x, y, t);
+  block -= j.blocks_a;
+  if (block < j.blocks_d) return reduce_columns<Y>(a.part_d, j.rows, 2 * a.dim, j.d, block, x, y, t);
+  join_bc(a, (int64_t)(block - j.blocks_d) * (32 * Y) + threadIdx.x);
 }
 
 // ------------------------------------------------------------------ host --
@@ -692,17 +712,25 @@ int remora_b200_selective_scan_bwd(RemoraB200Ctx *ctx, const RemoraSelectiveScan
     }
     REMORA_TRY(launch_bwd(a, nl, false, stream));
   }
-  if (B * L > 0 && a.blocks_d != 1) {  // no channels: zeros
-    note_launch();
-    join_bc_kernel<<<(unsigned)((B * L * G * N + 255) / 256), 256, 0, stream>>>(a);
-    REMORA_CUDA_TRY(cudaGetLastError());
-  }
-  const Columns da = {reinterpret_cast<float *>(o[2].data(4)), N, o[2].strides[0], o[2].strides[1], D * N, nullptr, 0};
-  REMORA_TRY(reduce_rows(a.part_a, B * a.chunks, D * N, da, stream));
-  if (!have[5] && !have[7]) return REMORA_OK;
-  const Columns dd = {have[5] ? reinterpret_cast<float *>(o[5].data(4)) : nullptr, D, 0, have[5] ? o[5].strides[0] : 0, D,
-                      have[7] ? reinterpret_cast<float *>(o[7].data(4)) : nullptr, have[7] ? o[7].strides[0] : 0};
-  return reduce_rows(a.part_d, B * a.chunks, 2 * D, dd, stream);
+  Joins j = {B * a.chunks};
+  j.a = {reinterpret_cast<float *>(o[2].data(4)), N, o[2].strides[0], o[2].strides[1], D * N, nullptr, 0};
+  j.d = {have[5] ? reinterpret_cast<float *>(o[5].data(4)) : nullptr, D, 0, have[5] ? o[5].strides[0] : 0, D,
+         have[7] ? reinterpret_cast<float *>(o[7].data(4)) : nullptr, have[7] ? o[7].strides[0] : 0};
+  const bool wide = tall(j.rows);
+  const int threads = wide ? 1024 : 256;
+  j.blocks_a = (unsigned)((D * N + 31) / 32);
+  j.blocks_d = have[5] || have[7] ? (unsigned)((2 * D + 31) / 32) : 0;
+  // without channels db and dc are zeros
+  const unsigned blocks =
+      j.blocks_a + j.blocks_d + (a.blocks_d != 1 ? (unsigned)((B * L * G * N + threads - 1) / threads) : 0);
+  if (blocks == 0) return REMORA_OK;
+  note_launch();
+  if (wide)
+    join_kernel<32><<<blocks, threads, 0, stream>>>(a, j);
+  else
+    join_kernel<8><<<blocks, threads, 0, stream>>>(a, j);
+  REMORA_CUDA_TRY(cudaGetLastError());
+  return REMORA_OK;
 }
 
 }  // extern "C"
