@@ -886,3 +886,66 @@ def test_no_memory_for_a_result(cuda):
     with pytest.raises(torch.OutOfMemoryError):
         ops.rms_norm_fwd(row.expand(1 << 22, -1), row[0])  # 16 TiB
     np.testing.assert_array_equal(to_host(ops.rms_norm_fwd(row, row[0], eps=0.0)), to_host(row))
+
+
+def test_calls_from_two_threads(cuda):
+    """Each on a stream of its own: the results of one thread alone, bit for bit."""
+    import threading
+
+    import torch
+
+    rng = np.random.default_rng(77)
+    v = [scan_inputs(rng, 2, 150, 70, 16, 1, True) for _ in range(2)]
+    given = [scan_own(x, cuda) for x in v]
+
+    def train(i):
+        pos, Dv, kw = given[i]
+        y, saved = ops.selective_scan_fwd(*pos, Dv, softplus=True, save=True, **kw)
+        grads = ops.selective_scan_bwd(*pos, y, saved, Dv, softplus=True, **kw)
+        n, q = ops.rms_norm_fwd(y, Dv), ops.causal_conv_fwd(y, pos[2][:, :4], Dv, silu=True)
+        return [y, n, q, *grads]
+
+    alone = [train(i) for i in range(2)]
+    torch.cuda.synchronize()
+    seen, errors = [[], []], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    seen[i].append(train(i))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not errors
+    for want, runs in zip(alone, seen):
+        for got in runs:
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("N,T", [(64, 140), (16, 40), (8, 140)])
+def test_scan_captured_and_replayed(cuda, N, T):
+    """With new inputs in the captured call's tensors."""
+    import torch
+
+    rng = np.random.default_rng(N + T)
+    v = scan_inputs(rng, 2, T, 40, N, 1, True)
+    pos, Dv, kw = scan_own(v, cuda)
+
+    def train():
+        y, saved = ops.selective_scan_fwd(*pos, Dv, softplus=True, save=True, **kw)
+        return [y, *ops.selective_scan_bwd(*pos, y, saved, Dv, softplus=True, **kw)]
+
+    train()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = train()
+    for _ in range(2):
+        pos[0].copy_(dev(rnd(rng, 2, T, 40), cuda))
+        pos[3].copy_(dev(rnd(rng, 2, T, 1, N), cuda))
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, train()))
