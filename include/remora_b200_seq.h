@@ -54,9 +54,9 @@ int remora_b200_rms_norm_fwd(RemoraB200Ctx *ctx, const RemoraNormSpec *spec,
                              int32_t rank, remora_stream_t stream);
 
 /* The same y in 8 bits: per row or per group of columns
-   scale = max(max|y| / 448, 2^-126), q = y / scale rounded to the nearest
-   e4m3 value (4 exponent and 3 fraction bits, largest 448, ties to even), one
-   byte each.  q has x's shape, scales x's leading axes and one last axis of
+   scale = max(max|y| / 448, 2^-126), q = the f32 quotient y / scale rounded to
+   the nearest e4m3 value (4 exponent and 3 fraction bits, largest 448, ties to
+   even), one byte each.  q has x's shape, scales x's leading axes and one last axis of
    dim / group (1 for group 0).  A NaN in a row gives NaN scales there. */
 int remora_b200_rms_norm_quant(RemoraB200Ctx *ctx, const RemoraNormSpec *spec,
                                const void *x, const void *residual,
