@@ -244,10 +244,11 @@ __device__ __forceinline__ float rcp(float x) {
 // show; within ex2.approx's 2^-22.
 __device__ __forceinline__ float exp_fast(float v) {
   const float t = v * 1.4426950408889634f;
-  // log2(e) is the constant above plus 1.926e-8; inf - inf is kept out
+  // log2(e) is the constant above plus 1.926e-8
   const float r = fmaf(v, 1.4426950408889634f, -t) + v * 1.925963033500e-08f;
   const float e = ex2(t);
-  return fabsf(v) < 3.0e38f ? fmaf(e, r * 0.6931471805599453f, e) : e;
+  // from 2^128 on e is inf, below 2^-128 zero, and r may be inf: nothing to correct
+  return fabsf(t) < 128.0f ? fmaf(e, r * 0.6931471805599453f, e) : e;
 }
 
 // 1 / (1 + exp(-v)): within (6 + |v|) 2^-24; exp(-v) = inf gives 0.

@@ -32,3 +32,37 @@ def test_quant_is_the_quotient_rounded(cuda, rows, D, group):
                                                      np.float32(2.0 ** -126)))
     want = torch.from_numpy(y / scales).to(torch.float8_e4m3fn).float().numpy()
     np.testing.assert_array_equal(to_host(q.float()).reshape(want.shape), want)
+
+
+# ------------------------------------------------------------------- scan
+BIG = [2.3e38, 2.5e38, 3.2e38, 3.4e38]
+
+
+@pytest.mark.parametrize("length", [1, 5, 200])
+def test_softplus_of_the_largest_steps(cuda, length):
+    """softplus(v) is v, and its slope 1, at the top of the f32 range; both are 0
+    at the bottom.  In the long axis, which is cut, such steps stand apart."""
+    D, N = len(BIG), 4
+    delta = np.full((2, length, D), -4.0, np.float32)
+    delta[0, -1], delta[1, -1] = BIG, [-v for v in BIG]
+    u = np.full(delta.shape, 1e-30, np.float32)
+    A, B, C = -np.ones((D, N), np.float32), np.ones((2, length, N), np.float32), np.full((2, length, N), 0.125, np.float32)
+    h0, dy = np.ones((2, D, N), np.float32), np.zeros_like(delta)
+    dy[:, -1] = 1
+    d = lambda v: dev(v, cuda)  # noqa: E731
+    args = d(u), d(delta), d(A), d(B), d(C)
+    y, last, saved = ops.selective_scan_fwd(*args, softplus=True, h0=d(h0), return_state=True, save=True)
+    du, ddelta, dA, *_ = ops.selective_scan_bwd(*args, d(dy), saved, softplus=True, h0=d(h0))
+    s, few = np.array(BIG, np.float32), 16 * 2.0 ** -24
+    # nothing is left of the state ahead of the first row's last step, all of it in the other
+    np.testing.assert_allclose(to_host(last)[0, :, 0], s * u[0, 0, 0], rtol=few)
+    np.testing.assert_allclose(to_host(y)[0, -1], s * u[0, 0, 0] / 2, rtol=few)
+    np.testing.assert_allclose(to_host(du)[0, -1], s / 2, rtol=few)
+    np.testing.assert_allclose(to_host(ddelta)[0, -1], u[0, 0] / 2, rtol=few)
+    decay = np.exp(-np.logaddexp(-4.0, 0) * (length - 1))
+    np.testing.assert_allclose(to_host(y)[1, -1], decay / 2, rtol=6 * length * 2.0 ** -24 + few)
+    assert (to_host(du)[1, -1] == 0).all() and (to_host(ddelta)[1, -1] == 0).all()
+    assert np.isfinite(to_host(dA)).all()
+    y = ops.selective_scan_step(d(h0), d(u[:, -1]), d(delta[:, -1]), d(A), d(B[:, -1]), d(C[:, -1]), softplus=True)
+    np.testing.assert_allclose(to_host(y)[0], s * u[0, 0, 0] / 2, rtol=few)
+    np.testing.assert_allclose(to_host(y)[1], 0.5, rtol=few)
