@@ -251,7 +251,11 @@ __device__ __forceinline__ float exp_fast(float v) {
   return fabsf(t) < 128.0f ? fmaf(e, r * 0.6931471805599453f, e) : e;
 }
 
-// 1 / (1 + exp(-v)): within (6 + |v|) 2^-24; exp(-v) = inf gives 0.
+// 1 / (1 + exp(-v)): within (6 + |v|) 2^-24 of its value for v > -87, within
+// 2^-126 below, where it becomes 0 as soon as it is no normal number.  exp_fast's
+// second part would leave 8 2^-24 of it for every v, but costs a convolution 5 %
+// (1 x 8192 x 4096: 47.2 and 49.5 us); without it the value at v = -80, 2e-35, is
+// off by 5e-6 of itself.
 __device__ __forceinline__ float sigmoid(float v) { return rcp(1.0f + ex2(v * -1.4426950408889634f)); }
 
 // log(1 + exp(v)) = max(v, 0) + log1p(e), e = exp(-|v|) in (0, 1].  With

@@ -7,9 +7,10 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
+import seq_reference as ref
 from conftest import to_host
 from remora_b200 import ops
-from test_gpu_seq import dev, rnd
+from test_gpu_seq import E, dev, rnd, within
 
 pytestmark = pytest.mark.gpu
 
@@ -32,6 +33,34 @@ def test_quant_is_the_quotient_rounded(cuda, rows, D, group):
                                                      np.float32(2.0 ** -126)))
     want = torch.from_numpy(y / scales).to(torch.float8_e4m3fn).float().numpy()
     np.testing.assert_array_equal(to_host(q.float()).reshape(want.shape), want)
+
+
+# ------------------------------------------------------------------- silu
+def test_silu_far_from_zero(cuda):
+    """v / (1 + exp(-v)) within 6 + |v| units (E) of the sigmoid, where exp(-v)
+    counts beside 1, and one of each product.  Below -87 the sigmoid is less than
+    the least normal number, and may be 0.  silu' = s (1 + v (1 - s)) carries the
+    sigmoid's error |v| times."""
+    v = np.concatenate([np.linspace(-87, 88, 3000), [-1e30, -200, -120, -100, -90, -88, 120, 1e30]]).astype(np.float32)
+    want = v.astype(np.float64) * ref.sigmoid(v.astype(np.float64))
+    units = (10 + np.minimum(np.abs(v.astype(np.float64)), 88) * (v < 17)) * E  # exp(-17) is below E
+    bound = np.abs(want) * units + np.where(v < -87, np.minimum(np.abs(want), np.abs(v.astype(np.float64)) * 2.0 ** -126), 0)
+    n = len(v)
+    x, w = dev(v.reshape(1, 1, n), cuda), dev(np.tile(np.float32([0, 1]), (n, 1)), cuda)
+    one = dev(np.ones((1, 1, n), np.float32), cuda)
+    within(ops.causal_conv_fwd(x, w, silu=True)[0, 0], want, bound, "conv")
+    state = dev(np.zeros((1, 1, n), np.float32), cuda)
+    within(ops.causal_conv_step(x[0], state, w, silu=True)[0], want, bound, "conv step")
+    s = ref.sigmoid(v.astype(np.float64))
+    slope = s * (1 + v * (1 - s))
+    tiny = np.where(v < -87, np.abs(slope), 0)
+    steep = np.minimum(np.abs(v.astype(np.float64)), 200)  # behind it s is 0 or 1
+    within(ops.causal_conv_bwd(x, w, one, silu=True)[0][0, 0], slope, s * (1 + steep) * units + tiny, "conv gradient")
+    zero = dev(np.zeros((1, 1, 4), np.float32), cuda)
+    A, D = dev(-np.ones((n, 4), np.float32), cuda), dev(np.ones(n, np.float32), cuda)
+    within(ops.selective_scan_fwd(one, one, A, zero, zero, D, z=x)[0, 0], want, bound, "scan")
+    h = dev(np.zeros((1, n, 4), np.float32), cuda)
+    within(ops.selective_scan_step(h, one[0], one[0], A, zero[0], zero[0], D, z=x[0])[0], want, bound, "scan step")
 
 
 # ------------------------------------------------------------------- scan
