@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(kScanThreads, MAIN && NL == 2 ? 3 : 4) scan_fw
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const bool on = k < nv;
-      av[k] = on ? a.a[at.d[c] * a.a_d + (4 * at.q + k) * a.a_n] * kLog2e : 0.0f;
+      av[k] = on ? a.a[at.d[c] * a.a_d + (4 * at.q + k) * a.a_n] * kLog2e : kPastN;
       hv[k] = 0.0f;
       if (MAIN && on && a.chunks == 1 && a.h0.p)
         hv[k] = a.h0.p[at.b * a.h0.s0 + at.d[c] * a.h0.s1 + (4 * at.q + k) * a.h0.s2];
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(256) scan_combine_kernel(const ScanArgs a, int
   const int64_t used = max((int64_t)1, (len + a.chunk - 1) / a.chunk);
   const Op3 &first = reverse ? a.dh_last : a.h0;
   const bool on = n < a.states;
-  const float A = on ? a.a[d * a.a_d + n * a.a_n] * kLog2e : 0.0f;
+  const float A = on ? a.a[d * a.a_d + n * a.a_n] * kLog2e : kPastN;
   float h = on && first.p ? first.p[b * first.s0 + d * first.s1 + n * first.s2] : 0.0f;
   constexpr int U = 8;  // pieces whose sums are on their way together
   for (int64_t k0 = 0; k0 < used; k0 += U) {

@@ -32,6 +32,9 @@ constexpr int save_every(int nl) { return nl > 8 ? 16 : nl > 4 ? 8 : 4; }
 constexpr int kMaxStates = 64;
 constexpr int64_t kMaxLength = 1 << 30;
 constexpr int kChan = 2;  // channels per thread
+// a of the states past N: their decay is 0 for a step that is inf, where a = 0
+// would make it, and through the sums over the states every output, NaN.
+constexpr float kPastN = -1.0f;
 
 struct Op3 {  // [B, time, D], or [B, D, N]
   float *p;

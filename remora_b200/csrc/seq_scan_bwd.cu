@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kScanThreads, bwd_blocks(NL)) scan_bwd_kernel(
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const bool on = at.live[c] && k < nv;
-      av[k] = on ? a.a[at.d[c] * a.a_d + (4 * at.q + k) * a.a_n] * kLog2e : 0.0f;
+      av[k] = on ? a.a[at.d[c] * a.a_d + (4 * at.q + k) * a.a_n] * kLog2e : kPastN;
       gv[k] = 0.0f;
       if (on && a.chunks == 1 && a.dh_last.p)
         gv[k] = a.dh_last.p[at.b * a.dh_last.s0 + at.d[c] * a.dh_last.s1 + (4 * at.q + k) * a.dh_last.s2];
@@ -417,7 +417,8 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_adjoint_kernel(const Sca
   for (int c = 0; c < C; ++c) {
     float av[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) av[k] = k < nv ? a.a[at.d[c] * a.a_d + (4 * at.q + k) * a.a_n] * kLog2e : 0.0f;
+    for (int k = 0; k < 4; ++k)
+      av[k] = k < nv ? a.a[at.d[c] * a.a_d + (4 * at.q + k) * a.a_n] * kLog2e : kPastN;
 #pragma unroll
     for (int k = 0; k < 2; ++k) A[c][k] = pair(av[2 * k], av[2 * k + 1]), G[c][k] = 0;
     bias[c] = a.bias ? a.bias[at.d[c] * a.bias_s] : 0.0f;

@@ -95,3 +95,33 @@ def test_softplus_of_the_largest_steps(cuda, length):
     y = ops.selective_scan_step(d(h0), d(u[:, -1]), d(delta[:, -1]), d(A), d(B[:, -1]), d(C[:, -1]), softplus=True)
     np.testing.assert_allclose(to_host(y)[0], s * u[0, 0, 0] / 2, rtol=few)
     np.testing.assert_allclose(to_host(y)[1], 0.5, rtol=few)
+
+
+@pytest.mark.parametrize("N", [1, 4, 5, 13, 16, 33, 64])
+@pytest.mark.parametrize("length,at", [(9, 6), (300, 170)])
+def test_an_infinite_step_leaves_what_is_ahead_of_it(cuda, N, length, at):
+    """A step that is inf forgets the state, whatever the number of states: ahead of
+    it everything is as in the sequence cut there, in both directions, and from it
+    on the states of positive inputs are +inf."""
+    rng = np.random.default_rng(N + length)
+    D = 6
+    pos = lambda *shape: rng.uniform(0.5, 1.5, shape).astype(np.float32)  # noqa: E731
+    u, delta, B, C = pos(1, length, D), rnd(rng, 1, length, D) - 3, pos(1, length, N), pos(1, length, N)
+    A, h0, dy = -pos(D, N), pos(1, D, N), rnd(rng, 1, length, D)
+    delta[:, at], dy[:, at:] = np.inf, 0
+    d = lambda v: dev(v, cuda)  # noqa: E731
+    args = [d(v) for v in (u, delta, A, B, C)]
+    cut = d(np.array([at], np.int32))
+    outs, grads = [], []
+    for lengths in (None, cut):
+        y, saved = ops.selective_scan_fwd(*args, softplus=True, h0=d(h0), lengths=lengths, save=True)
+        g = ops.selective_scan_bwd(*args, d(dy), saved, softplus=True, h0=d(h0), lengths=lengths)
+        outs.append(to_host(y))
+        grads.append([to_host(g[k])[:, :at] if k < 8 else to_host(g[k]) for k in (0, 1, 3, 4, 8)])
+    np.testing.assert_array_equal(outs[0][:, :at], outs[1][:, :at])
+    assert np.isfinite(outs[1]).all() and (outs[0][:, at:] == np.inf).all()
+    for a, b in zip(*grads):
+        assert np.isfinite(b).all()
+        np.testing.assert_array_equal(a, b)
+    y = ops.selective_scan_step(d(h0), *(d(v[:, at]) for v in (u, delta)), d(A), d(B[:, at]), d(C[:, at]), softplus=True)
+    assert (to_host(y) == np.inf).all()
