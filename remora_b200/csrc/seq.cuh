@@ -151,17 +151,23 @@ struct Named {
   int esize;
 };
 
-// Refuses outputs that overlap an input or another output.  An output listed
-// in `in_place` may be exactly that input.
+// An output that may be exactly this input.
+struct InPlace {
+  const DescView *out, *in;
+};
+
+// Refuses outputs that overlap an input, but for those of in_place, or another
+// output.
 inline int want_apart(std::initializer_list<Named> outs, std::initializer_list<Named> ins,
-                      std::initializer_list<const DescView *> in_place = {}) {
+                      std::initializer_list<InPlace> in_place = {}) {
   for (const Named &o : outs) {
     if (o.v == nullptr) continue;
     REMORA_TRY(want_own_elements(*o.v, o.name));
     for (const Named &i : ins) {
       if (i.v == nullptr || !may_overlap(*o.v, o.esize, *i.v, i.esize)) continue;
       bool allowed = false;
-      for (const DescView *p : in_place) allowed |= p == i.v && o.esize == i.esize && same_view(*o.v, *i.v);
+      for (const InPlace &p : in_place)
+        allowed |= p.out == o.v && p.in == i.v && o.esize == i.esize && same_view(*o.v, *i.v);
       if (!allowed) return fail(REMORA_ERR_ARG, "%s overlaps %s", o.name, i.name);
     }
     for (const Named &p : outs)

@@ -479,7 +479,8 @@ int remora_b200_causal_conv_fwd(RemoraB200Ctx *ctx, const RemoraCausalConvSpec *
                                           {lp, "lengths", 4}, {has_o ? &ov : nullptr, "state_out", 4}}));
   if (has_o)
     REMORA_TRY(want_apart({{&ov, "state_out", 4}},
-                          {{&xv, "x", 4}, {&wv, "w", 4}, {bp, "bias", 4}, {sp, "state", 4}, {lp, "lengths", 4}}, {sp}));
+                          {{&xv, "x", 4}, {&wv, "w", 4}, {bp, "bias", 4}, {sp, "state", 4}, {lp, "lengths", 4}},
+                          {{&ov, sp}}));
   if (B == 0 || D == 0 || (L == 0 && !has_o)) return REMORA_OK;
   ConvArgs a = {};
   a.x = op3(xv), a.y = op3(yv);
@@ -601,7 +602,7 @@ int remora_b200_causal_conv_step(RemoraB200Ctx *ctx, const RemoraCausalConvSpec 
   if (B > 65535) return fail(REMORA_ERR_LIMIT, "causal_conv_step: more than 65535 rows");
   REMORA_TRY(want_apart({{&yv, "y", 4}, {&ov, "state_out", 4}},
                         {{&xv, "x", 4}, {&sv, "state", 4}, {&wv, "w", 4}, {has_b ? &bv : nullptr, "bias", 4},
-                         {has_l ? &lv : nullptr, "slots", 4}}, {&sv}));
+                         {has_l ? &lv : nullptr, "slots", 4}}, {{&ov, &sv}}));
   if (B == 0 || D == 0) return REMORA_OK;
   StepArgs a = {};
   a.state = op3(sv), a.state_out = op3(ov);

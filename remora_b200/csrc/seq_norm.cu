@@ -720,7 +720,8 @@ int norm_forward(RemoraB200Ctx *ctx, const RemoraNormSpec *spec, const void *x, 
   if (sh.rows > 0x7fffffff) return fail(REMORA_ERR_LIMIT, "%s: more than 2^31 - 1 rows", name);
   const DescView *rp = has_r ? &rv : nullptr, *sp = has_s ? &sv : nullptr, *cp = quant ? &cv : nullptr;
   REMORA_TRY(want_apart({{&yv, "the output", quant ? 1 : 4}, {sp, "sum", 4}, {cp, "scales", 4}},
-                        {{&xv, "x", 4}, {rp, "residual", 4}, {&wv, "w", 4}}, {&xv, rp}));
+                        {{&xv, "x", 4}, {rp, "residual", 4}, {&wv, "w", 4}},
+                        {{&yv, &xv}, {&yv, rp}, {sp, &xv}, {sp, rp}}));
   NormArgs a = {};
   a.x = rows_of(xv, 4);
   a.y = rows_of(yv, quant ? 1 : 4);
@@ -858,7 +859,8 @@ int remora_b200_rms_norm_bwd(RemoraB200Ctx *ctx, const RemoraNormSpec *spec, con
   if (sh.rows > 0x7fffffff) return fail(REMORA_ERR_LIMIT, "rms_norm_bwd: more than 2^31 - 1 rows");
   const DescView *dp = has_ds ? &dv : nullptr;
   REMORA_TRY(want_apart({{&xv, "dx", 4}, {&dwv, "dw", 4}},
-                        {{&sv, "s", 4}, {&wv, "w", 4}, {&gv, "dy", 4}, {dp, "dsum", 4}}, {&sv, &gv, dp}));
+                        {{&sv, "s", 4}, {&wv, "w", 4}, {&gv, "dy", 4}, {dp, "dsum", 4}},
+                        {{&xv, &sv}, {&xv, &gv}, {&xv, dp}}));
   REMORA_TRY(want_scratch(scratch, scratch_bytes, bwd_scratch(sh.rows, sh.dim), "rms_norm_bwd"));
   NormBwdArgs a = {};
   a.s = rows_of(sv, 4), a.dy = rows_of(gv, 4), a.dx = rows_of(xv, 4);
