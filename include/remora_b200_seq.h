@@ -21,8 +21,8 @@
  *    behind a sequence's end are never read; in outputs and gradients they
  *    stay as they were, or become zero where the spec's zero_rest is set.
  *  - Outputs must not overlap inputs or each other, except where an entry
- *    point says so; views that interleave (columns of one wider array) do not
- *    count as overlapping.  Input gradients of one array passed twice are two
+ *    point says so, nor share addresses among their own elements; views that
+ *    interleave (columns of one wider array) do not count as overlapping.  Input gradients of one array passed twice are two
  *    separate outputs.
  *  - Results do not depend on timing: sums run in a fixed order.
  */

@@ -136,13 +136,29 @@ inline bool may_overlap(const DescView &a, int ea, const DescView &b, int eb) {
   return o.hits(0, o.target);
 }
 
-// An output whose own elements share addresses (a stride of 0 over more than
-// one element) cannot hold a result.
-inline int want_own_elements(const DescView &v, const char *what) {
-  for (int d = 0; d < v.rank; ++d)
-    if (v.sizes[d] > 1 && v.strides[d] == 0)
-      return fail(REMORA_ERR_ARG, "%s: an output with stride 0 along axis %d", what, d);
-  return REMORA_OK;
+// Whether two elements of a view share an address: whether two indices differ by
+// steps along its axes that add up to nothing.  Not where each stride is longer
+// than all that the smaller ones span; else the steps along every axis are tried
+// against those along the axes of smaller strides, with the same limit as above.
+inline bool overlaps_itself(const DescView &v) {
+  if (v.numel() == 0) return false;
+  Overlap o;  // its axes have the differences of two indices, -(size - 1) to size - 1
+  for (int d = 0; d < v.rank; ++d) {
+    if (v.sizes[d] <= 1) continue;
+    if (v.strides[d] == 0) return true;
+    const int64_t stride = v.strides[d] < 0 ? -v.strides[d] : v.strides[d];
+    int k = o.count++;
+    for (; k > 0 && o.axes[k - 1].stride < stride; --k) o.axes[k] = o.axes[k - 1];
+    o.axes[k] = {stride, 2 * v.sizes[d] - 1};  // the largest stride first
+  }
+  o.rest[o.count] = 0;
+  for (int i = o.count - 1; i >= 0; --i) {
+    const int64_t stride = o.axes[i].stride, most = o.axes[i].size / 2, span = o.rest[i + 1] / 2;
+    for (int64_t k = 1; k <= most && k * stride <= span; ++k)
+      if (o.hits(i + 1, span - k * stride)) return true;
+    o.rest[i] = o.rest[i + 1] + stride * 2 * most;
+  }
+  return false;
 }
 
 struct Named {
@@ -156,13 +172,20 @@ struct InPlace {
   const DescView *out, *in;
 };
 
+// Refuses outputs that cannot hold a result, since elements share addresses.
+inline int want_own_elements(std::initializer_list<Named> outs) {
+  for (const Named &o : outs)
+    if (o.v != nullptr && overlaps_itself(*o.v))
+      return fail(REMORA_ERR_ARG, "%s: elements of this output share addresses", o.name);
+  return REMORA_OK;
+}
+
 // Refuses outputs that overlap an input, but for those of in_place, or another
 // output.
 inline int want_apart(std::initializer_list<Named> outs, std::initializer_list<Named> ins,
                       std::initializer_list<InPlace> in_place = {}) {
   for (const Named &o : outs) {
     if (o.v == nullptr) continue;
-    REMORA_TRY(want_own_elements(*o.v, o.name));
     for (const Named &i : ins) {
       if (i.v == nullptr || !may_overlap(*o.v, o.esize, *i.v, i.esize)) continue;
       bool allowed = false;

@@ -481,6 +481,7 @@ int remora_b200_causal_conv_fwd(RemoraB200Ctx *ctx, const RemoraCausalConvSpec *
     REMORA_TRY(want_apart({{&ov, "state_out", 4}},
                           {{&xv, "x", 4}, {&wv, "w", 4}, {bp, "bias", 4}, {sp, "state", 4}, {lp, "lengths", 4}},
                           {{&ov, sp}}));
+  REMORA_TRY(want_own_elements({{&yv, "y", 4}, {has_o ? &ov : nullptr, "state_out", 4}}));
   if (B == 0 || D == 0 || (L == 0 && !has_o)) return REMORA_OK;
   ConvArgs a = {};
   a.x = op3(xv), a.y = op3(yv);
@@ -547,6 +548,8 @@ int remora_b200_causal_conv_bwd(RemoraB200Ctx *ctx, const RemoraCausalConvSpec *
                         {{&xv, "x", 4}, {&wv, "w", 4}, {&gv, "dy", 4}, {has_b ? &bv : nullptr, "bias", 4},
                          {has_s ? &sv : nullptr, "state", 4}, {has_l ? &lv : nullptr, "lengths", 4},
                          {has_e ? &ev : nullptr, "dstate_out", 4}}));
+  REMORA_TRY(want_own_elements({{&dxv, "dx", 4}, {&dwv, "dw", 4}, {has_db ? &dbv : nullptr, "dbias", 4},
+                                {has_ds ? &dsv : nullptr, "dstate", 4}}));
   const int64_t parts = bwd_parts(B, L, D);
   REMORA_TRY(want_scratch(scratch, scratch_bytes, (size_t)parts * (size_t)(W + 1) * (size_t)D * 4, "causal_conv_bwd"));
   if (D == 0) return REMORA_OK;
@@ -603,6 +606,7 @@ int remora_b200_causal_conv_step(RemoraB200Ctx *ctx, const RemoraCausalConvSpec 
   REMORA_TRY(want_apart({{&yv, "y", 4}, {&ov, "state_out", 4}},
                         {{&xv, "x", 4}, {&sv, "state", 4}, {&wv, "w", 4}, {has_b ? &bv : nullptr, "bias", 4},
                          {has_l ? &lv : nullptr, "slots", 4}}, {{&ov, &sv}}));
+  REMORA_TRY(want_own_elements({{&yv, "y", 4}, {&ov, "state_out", 4}}));
   if (B == 0 || D == 0) return REMORA_OK;
   StepArgs a = {};
   a.state = op3(sv), a.state_out = op3(ov);

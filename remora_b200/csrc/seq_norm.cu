@@ -722,6 +722,7 @@ int norm_forward(RemoraB200Ctx *ctx, const RemoraNormSpec *spec, const void *x, 
   REMORA_TRY(want_apart({{&yv, "the output", quant ? 1 : 4}, {sp, "sum", 4}, {cp, "scales", 4}},
                         {{&xv, "x", 4}, {rp, "residual", 4}, {&wv, "w", 4}},
                         {{&yv, &xv}, {&yv, rp}, {sp, &xv}, {sp, rp}}));
+  REMORA_TRY(want_own_elements({{&yv, "the output", 1}, {sp, "sum", 4}, {cp, "scales", 4}}));
   NormArgs a = {};
   a.x = rows_of(xv, 4);
   a.y = rows_of(yv, quant ? 1 : 4);
@@ -862,6 +863,7 @@ int remora_b200_rms_norm_bwd(RemoraB200Ctx *ctx, const RemoraNormSpec *spec, con
                         {{&sv, "s", 4}, {&wv, "w", 4}, {&gv, "dy", 4}, {dp, "dsum", 4}},
                         {{&xv, &sv}, {&xv, &gv}, {&xv, dp}}));
   REMORA_TRY(want_scratch(scratch, scratch_bytes, bwd_scratch(sh.rows, sh.dim), "rms_norm_bwd"));
+  REMORA_TRY(want_own_elements({{&xv, "dx", 4}, {&dwv, "dw", 4}}));
   NormBwdArgs a = {};
   a.s = rows_of(sv, 4), a.dy = rows_of(gv, 4), a.dx = rows_of(xv, 4);
   if (has_ds) a.ds = rows_of(dv, 4);

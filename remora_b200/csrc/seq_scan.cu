@@ -576,6 +576,7 @@ int remora_b200_selective_scan_fwd(RemoraB200Ctx *ctx, const RemoraSelectiveScan
                         {{given(0), "u", 4}, {given(1), "delta", 4}, {given(2), "a", 4}, {given(3), "b", 4},
                          {given(4), "c", 4}, {given(5), "d", 4}, {given(6), "z", 4}, {given(7), "delta_bias", 4},
                          {given(8), "h0", 4}, {given(9), "lengths", 4}}, {{&hv, &v[8]}}));
+  REMORA_TRY(want_own_elements({{&yv, "y", 4}, {has_h ? &hv : nullptr, "h_last", 4}}));
   for (int k : {0, 1, 6})
     if (v[k].aligned) REMORA_TRY(check_reach(v[k], nl, kChan, "selective_scan_fwd"));
   REMORA_TRY(check_reach(yv, nl, kChan, "selective_scan_fwd"));
@@ -643,6 +644,7 @@ int remora_b200_selective_scan_step(RemoraB200Ctx *ctx, const RemoraSelectiveSca
                         {{&sv, "state", 4}, {&uv, "u", 4}, {&ev, "delta", 4}, {&av, "a", 4}, {&bv, "b", 4},
                          {&cv, "c", 4}, {has_d ? &dv : nullptr, "d", 4}, {has_z ? &zv : nullptr, "z", 4},
                          {has_i ? &iv : nullptr, "delta_bias", 4}, {has_l ? &lv : nullptr, "slots", 4}}, {{&ov, &sv}}));
+  REMORA_TRY(want_own_elements({{&yv, "y", 4}, {&ov, "state_out", 4}}));
   if (B == 0 || D == 0) return REMORA_OK;
   if (std::max(D, S) > 0x1fffffff)
     return fail(REMORA_ERR_LIMIT, "selective_scan_step: 2^29 channels or rows of state, or more");

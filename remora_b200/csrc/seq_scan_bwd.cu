@@ -681,6 +681,7 @@ int remora_b200_selective_scan_bwd(RemoraB200Ctx *ctx, const RemoraSelectiveScan
                          {given(4), "c", 4}, {given(5), "d", 4}, {given(6), "z", 4}, {given(7), "delta_bias", 4},
                          {given(8), "h0", 4}, {given(9), "lengths", 4}, {&gy, "dy", 4},
                          {has_gh ? &gh : nullptr, "dh_last", 4}}));
+  for (int k = 0; k < 9; ++k) REMORA_TRY(want_own_elements({{out(k), "a gradient", 4}}));
   const Layout l = layout_for(B, L, D, a.states, G);
   size_t need = 0;
   REMORA_TRY(remora_b200_selective_scan_saved(B, L, D, N, &need));

@@ -10,11 +10,26 @@ import numpy as np
 import pytest
 
 from remora_b200 import _lib as L
-from test_seq_host import BASE, FAKE, ad, desc
+from test_seq_host import BASE, FAKE, desc
 
 FAR = [BASE + (k << 24) for k in range(32)]
+KEPT: list = []
+
+
+def ad(d):
+    """A descriptor's address; the descriptor lives as long as the tests."""
+    KEPT.append(d)
+    return ctypes.addressof(d) if d is not None else None
+
+
 # what a call that is refused for want of memory answers: every other check is behind it
 LAST = L.ERR_LIMIT
+
+
+def device_present() -> bool:
+    import torch
+
+    return torch.cuda.is_available()
 
 
 def scan_fwd(y, h_last=None, saved=(BASE, 8), scratch=(None, 0), **members):
@@ -52,3 +67,79 @@ def test_each_output_may_lie_over_its_own_inputs_only():
     quant = lambda scales, s: L.lib().remora_b200_rms_norm_quant(  # noqa: E731
         FAKE, ctypes.addressof(spec), ad(x), ad(r), ad(desc(1, at=FAR[4])), ad(q), ad(scales), ad(s), 2, None)
     assert quant(x, None) == L.ERR_ARG and quant(r, None) == L.ERR_ARG and quant(scales, scales) == L.ERR_ARG
+
+
+def conv_bwd(shape, dx):
+    """A backward of the convolution without scratch, which is refused last."""
+    B, T, D = shape
+    x, w, dy = desc(B, T, D, at=1 << 48), desc(D, 3, at=FAR[1]), desc(B, T, D, at=1 << 49)
+    spec, dw = L.RemoraCausalConvSpec(1, 0), desc(D, 3, at=FAR[3])
+    return L.lib().remora_b200_causal_conv_bwd(FAKE, ctypes.addressof(spec), ad(x), ad(w), None, None, None, ad(dy), None,
+                                               ad(dx), ad(dw), None, None, None, 0, None)
+
+
+def test_outputs_whose_elements_share_addresses_are_refused():
+    """Against enumeration: random small views as dx of a convolution's backward."""
+    rng = np.random.default_rng(1)
+    seen = {False: 0, True: 0}
+    for _ in range(600):
+        shape = [int(rng.integers(1, 5)) for _ in range(3)]
+        strides = [int(rng.choice([-1, 1])) * int(rng.integers(0, 25)) for _ in range(3)]
+        cells = sum(strides[k] * np.arange(shape[k]).reshape([-1 if j == k else 1 for j in range(3)]) for k in range(3))
+        shared = len(np.unique(cells)) < cells.size
+        st = conv_bwd(shape, desc(*shape, at=FAR[5], strides=strides))
+        assert st == (L.ERR_ARG if shared else LAST), (shape, strides, L.last_error())
+        seen[shared] += 1
+    assert min(seen.values()) > 100
+    # large views are decided without trying their elements
+    n = 1 << 10
+    for strides, shared in (((n * n, n, 1), False), ((1, n, n * n), False), ((n * n - 1, n, 1), True),
+                            ((n * n, n - 1, 1), True), ((2 * n * n, 2 * n, 2), False)):
+        assert conv_bwd((n, n, n), desc(n, n, n, at=1 << 44, strides=list(strides))) == (L.ERR_ARG if shared else LAST)
+
+
+def test_every_entry_point_refuses_such_outputs():
+    """Strides 1 and 1 over the last two axes, one output at a time."""
+    def own(*shape):
+        return desc(*shape, at=FAR[20], strides=[*([1000] * (len(shape) - 2)), 1, 1])
+
+    m = scan_operands(2, 5, 4, 3)
+    assert scan_fwd(own(2, 5, 4), **m) == L.ERR_ARG
+    assert scan_fwd(desc(2, 5, 4, at=FAR[6]), own(2, 4, 3), **m) == L.ERR_ARG
+    shapes = [(2, 5, 4), (2, 5, 4), (4, 3), (2, 5, 1, 3), (2, 5, 1, 3), (4,), (2, 5, 4), (4,), (2, 4, 3)]
+    args = L.RemoraSelectiveScanIn(*(ad(m.get(k)) for k, _ in L.RemoraSelectiveScanIn._fields_))
+    args.z = ad(desc(2, 5, 4, at=FAR[7]))
+    spec = L.RemoraSelectiveScanSpec(1, 0)
+    for bad in (None, 0, 1, 2, 6, 8):
+        outs = [own(*s) if k == bad else desc(*s, at=FAR[10 + k]) for k, s in enumerate(shapes)]
+        grads = L.RemoraSelectiveScanGrads(*(ad(v) for v in outs))
+        st = L.lib().remora_b200_selective_scan_bwd(FAKE, ctypes.addressof(spec), ctypes.addressof(args),
+                                                    ad(desc(2, 5, 4, at=FAR[8])), None, None, 0, ctypes.addressof(grads),
+                                                    None, 0, None)
+        assert st == (LAST if bad is None else L.ERR_ARG), L.last_error()
+    # the calls below have no later refusal: without these they would be launched
+    if device_present():
+        return
+    x, w, y = desc(4, 8, at=FAR[0]), desc(8, at=FAR[1]), desc(4, 8, at=FAR[2])
+    norm = L.RemoraNormSpec(1e-6, 0)
+    lib, at = L.lib(), ctypes.addressof
+    r, other = desc(4, 8, at=FAR[3]), desc(4, 8, at=FAR[4])
+    for out, s in ((own(4, 8), other), (y, own(4, 8))):
+        assert lib.remora_b200_rms_norm_fwd(FAKE, at(norm), ad(x), ad(r), ad(w), ad(out), ad(s), 2, None) == L.ERR_ARG
+        q = lib.remora_b200_rms_norm_quant(FAKE, at(norm), ad(x), ad(r), ad(w), ad(out), ad(desc(4, 1, at=FAR[6])), ad(s), 2, None)
+        assert q == L.ERR_ARG
+    assert lib.remora_b200_rms_norm_bwd(FAKE, at(norm), ad(x), ad(w), ad(y), None, ad(own(4, 8)), ad(desc(8, at=FAR[5])),
+                                        2, FAR[9], 1 << 20, None) == L.ERR_ARG
+    conv, taps, state = L.RemoraCausalConvSpec(1, 0), desc(8, 3, at=FAR[7]), desc(4, 2, 8, at=FAR[8])
+    for out, s in ((own(4, 8), state), (y, own(4, 2, 8))):
+        st = lib.remora_b200_causal_conv_step(FAKE, at(conv), ad(x), ad(state), ad(taps), None, None, ad(out), ad(s), None)
+        assert st == L.ERR_ARG
+        three = [desc(4, 1, 8, at=v.aligned, strides=[v.stride0, 8, v.stride1]) for v in (x, out)]
+        if s is not state:
+            st = lib.remora_b200_causal_conv_fwd(FAKE, at(conv), ad(three[0]), ad(taps), None, ad(state), None,
+                                                 ad(three[1]), ad(s), None)
+            assert st == L.ERR_ARG
+    h, a, b = desc(4, 8, 3, at=FAR[8]), desc(8, 3, at=FAR[7]), desc(4, 1, 3, at=FAR[9])
+    step = L.RemoraSelectiveStepIn(ad(h), ad(x), ad(r), ad(a), ad(b), ad(b))
+    for out, s in ((own(4, 8), h), (y, own(4, 8, 3))):
+        assert lib.remora_b200_selective_scan_step(FAKE, at(spec), at(step), ad(out), ad(s), None) == L.ERR_ARG
