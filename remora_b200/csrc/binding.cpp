@@ -9,12 +9,13 @@
 // field for other types than f32, and for a result, as fifth field, what it is
 // made like where it was not given: a tensor whose shape it gets or a tuple of
 // sizes (None: left out).  `results` holds the operands with five fields, given
-// or made (contiguous and unset).  The buffer (bytes, to be kept until the call
+// or made (contiguous and unset); their storage is asked for as what is written,
+// so that one shared with a lazy clone becomes the result's own.  The buffer (bytes, to be kept until the call
 // returns) holds a RemoraMemRefN for each tensor; its address follows in the
 // tuple, None for None.  With table = k > 0 the first k addresses form an
-// argument struct at the buffer's start, whose address stands for them.  None is returned when an operand is not a tensor of
-// its type, rank and device, or a view whose values are the negatives of what its
-// storage holds: the caller says which.
+// argument struct at the buffer's start, whose address stands for them.  None is
+// returned when an operand is not a tensor of its type, rank and device, or a view
+// whose values are the negatives of what its storage holds: the caller says which.
 //
 //   room(device, bytes) -> (uint8 tensor of that many unset bytes, its address)
 #include <ATen/ops/empty.h>
@@ -98,10 +99,16 @@ PyObject *layout(PyObject *const *args, Py_ssize_t nargs) {
         !t.has_storage() || t.is_neg())
       Py_RETURN_NONE;
     tensors[k] = &t;
-    starts[k] = t.numel() ? (int64_t)reinterpret_cast<uintptr_t>(t.storage().data()) : 0;
     t.strides();
     words += 3 + 2 * rank;
   }
+  // results first: an operand may be the same tensor, or a view of it
+  for (Py_ssize_t k = 0; k < n; ++k)
+    if (tensors[k] && tensors[k]->numel() && PyTuple_GET_SIZE(PyTuple_GET_ITEM(operands, k)) == 5)
+      tensors[k]->storage().mutable_data();
+  for (Py_ssize_t k = 0; k < n; ++k)
+    if (tensors[k])
+      starts[k] = tensors[k]->numel() ? (int64_t)reinterpret_cast<uintptr_t>(tensors[k]->storage().data()) : 0;
   PyObject *buffer = PyBytes_FromStringAndSize(nullptr, words * 8);
   if (buffer == nullptr) return nullptr;
   char *base = PyBytes_AS_STRING(buffer);

@@ -569,9 +569,9 @@ def causal_conv_step(x, state, w, bias=None, *, silu: bool = False, slots=None, 
     device = _cuda_index(x)
     if state_out is None:
         state_out = state
-    keep, (y,), xd, sd, wd, bd, yd, od, ld = _describe("causal_conv_step", device, (
+    keep, (y, _), xd, sd, wd, bd, yd, od, ld = _describe("causal_conv_step", device, (
         ("x", x, 2), ("state", state, 3), ("w", w, 2), ("bias", bias, 1), ("out", out, 2, torch.float32, x),
-        ("state_out", state_out, 3), ("slots", slots, 1, torch.int32)))
+        ("state_out", state_out, 3, torch.float32, None), ("slots", slots, 1, torch.int32)))
     L.check(L.lib().remora_b200_causal_conv_step(context(device).ptr, _spec(_CONV_SPECS, silu, out is None), xd, sd, wd,
                                                  bd, ld, yd, od, _raw_stream(device)), "causal_conv_step")
     return y
@@ -657,10 +657,10 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, *, z=None, delta_bias=
     torch = _torch()
     if state_out is None:
         state_out = state
-    keep, (y,), args, yd, od = _describe("selective_scan_step", device, (
+    keep, (y, _), args, yd, od = _describe("selective_scan_step", device, (
         ("state", state, 3), ("u", u, 2), ("delta", delta, 2), ("A", A, 2), ("B", Bg, 3), ("C", Cg, 3), ("D", D, 1),
         ("z", z, 2), ("delta_bias", delta_bias, 1), ("slots", slots, 1, torch.int32), ("out", out, 2, torch.float32, u),
-        ("state_out", state_out, 3)), table=10)
+        ("state_out", state_out, 3, torch.float32, None)), table=10)
     L.check(L.lib().remora_b200_selective_scan_step(context(device).ptr, _spec(_SCAN_SPECS, softplus, out is None), args,
                                                     yd, od, _raw_stream(device)), "selective_scan_step")
     return y

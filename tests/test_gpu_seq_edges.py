@@ -125,3 +125,19 @@ def test_an_infinite_step_leaves_what_is_ahead_of_it(cuda, N, length, at):
         np.testing.assert_array_equal(a, b)
     y = ops.selective_scan_step(d(h0), *(d(v[:, at]) for v in (u, delta)), d(A), d(B[:, at]), d(C[:, at]), softplus=True)
     assert (to_host(y) == np.inf).all()
+
+
+# ------------------------------------------------------------------ results
+def test_in_place_results_leave_a_lazy_clone_alone(cuda):
+    import torch
+
+    rng = np.random.default_rng(0)
+    x, w, state = dev(rnd(rng, 3, 8), cuda), dev(rnd(rng, 8, 4), cuda), dev(rnd(rng, 3, 3, 8), cuda)
+    before, mine = to_host(state), torch._lazy_clone(state)
+    ops.causal_conv_step(x, mine, w)
+    np.testing.assert_array_equal(to_host(mine)[:, -1], to_host(x))
+    np.testing.assert_array_equal(to_host(state), before)
+    y, copy = torch._lazy_clone(x), to_host(x)
+    ops.rms_norm_fwd(y, dev(np.ones(8, np.float32), cuda), out=y)
+    np.testing.assert_array_equal(to_host(x), copy)
+    assert (to_host(y) != copy).any()

@@ -143,3 +143,27 @@ def test_every_entry_point_refuses_such_outputs():
     step = L.RemoraSelectiveStepIn(ad(h), ad(x), ad(r), ad(a), ad(b), ad(b))
     for out, s in ((own(4, 8), h), (y, own(4, 8, 3))):
         assert lib.remora_b200_selective_scan_step(FAKE, at(spec), at(step), ad(out), ad(s), None) == L.ERR_ARG
+
+
+# ------------------------------------------------------------------ binding
+def test_a_result_does_not_share_memory_with_a_lazy_clone():
+    """Storage that a lazy clone shares is made a result's own before its address is
+    taken, in whatever order the operands come; an operand that is only read
+    stays shared."""
+    import torch
+
+    from remora_b200 import _binding
+
+    def aligned(address):
+        return ctypes.cast(address, ctypes.POINTER(ctypes.c_uint64))[1]
+
+    source = torch.arange(6.0)
+    at_first = source.data_ptr()  # asking a clone's source for it would make that one's own, too
+    clone = torch._lazy_clone(source)
+    f32 = torch.float32
+    _, (out,), read, written = _binding.describe(-1, (("state", clone[2:], 1), ("state_out", clone[2:], 1, f32, None)), 0)
+    assert aligned(read) == aligned(written) != at_first
+    shared = torch._lazy_clone(source)
+    keep, _, at = _binding.describe(-1, (("x", shared, 1),), 0)
+    assert aligned(at) == at_first
+    assert source.tolist() == shared.tolist() == list(range(6))
