@@ -18,6 +18,9 @@
 // whose values are the negatives of what its storage holds: the caller says which.
 //
 //   room(device, bytes) -> (uint8 tensor of that many unset bytes, its address)
+//
+//   written(tensor or None, ...): raises the version of what a call has written, by
+//   which autograd notices that a value it kept is gone
 #include <ATen/ops/empty.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
@@ -188,11 +191,28 @@ PyObject *room(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+PyObject *written(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  for (Py_ssize_t k = 0; k < nargs; ++k) {
+    if (args[k] == Py_None) continue;
+    if (!THPVariable_Check(args[k])) {
+      PyErr_SetString(PyExc_TypeError, "written(tensor or None, ...)");
+      return nullptr;
+    }
+    const at::Tensor &t = THPVariable_Unpack(args[k]);
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();  // an inference tensor has none
+  }
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"describe", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(describe)), METH_FASTCALL,
      "describe(device, operands, table) -> (buffer, results, address, ...) or None"},
     {"room", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(room)), METH_FASTCALL,
      "room(device, bytes) -> (uint8 tensor, its address)"},
+    {"written", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(written)), METH_FASTCALL,
+     "written(tensor or None, ...): raises their versions"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_binding", "Descriptors of a call's tensors.", -1, methods,

@@ -387,6 +387,9 @@ def append(a, b, out=None):
 # sequence's end are never read; results made here are zero there, and those
 # rows of a given `out` stay as they were.
 #
+# Arrays that a caller gives to be written count as modified in place: autograd
+# refuses a backward pass that would have needed their old values.
+#
 # A single-token call costs what the host does, so the operands of a call are
 # checked and laid out, and its results made, natively (csrc/binding.cpp).
 def _describe(what: str, device: int, operands, table: int = 0):
@@ -485,6 +488,7 @@ def rms_norm_fwd(x, w, *, residual=None, eps: float = 1e-6, out=None, sum_out=No
     spec = L.RemoraNormSpec(eps, 0)
     L.check(L.lib().remora_b200_rms_norm_fwd(context(device).ptr, ctypes.addressof(spec), xd, rd, wd, yd, sd, rank,
                                              _raw_stream(device)), "rms_norm_fwd")
+    _binding().written(y, s)
     return y if residual is None else (y, s)
 
 
@@ -502,6 +506,7 @@ def rms_norm_quant(x, w, *, residual=None, eps: float = 1e-6, group: int = 0, ou
     spec = L.RemoraNormSpec(eps, group)
     L.check(L.lib().remora_b200_rms_norm_quant(context(device).ptr, ctypes.addressof(spec), xd, rd, wd, qd, cd, sd,
                                                rank, _raw_stream(device)), "rms_norm_quant")
+    _binding().written(q, scales, s)
     return (q, scales) if residual is None else (q, scales, s)
 
 
@@ -521,6 +526,7 @@ def rms_norm_bwd(s, w, dy, *, dsum=None, eps: float = 1e-6, out=None):
     spec = L.RemoraNormSpec(eps, 0)
     L.check(lib.remora_b200_rms_norm_bwd(ctx, ctypes.addressof(spec), sd, wd, gd, ed, xd, dwd, rank, at, size,
                                          _raw_stream(device)), "rms_norm_bwd")
+    _binding().written(dx)
     return dx, dw
 
 
@@ -539,6 +545,7 @@ def causal_conv_fwd(x, w, bias=None, *, state=None, lengths=None, silu: bool = F
         ("state_out", state_out, 3, f32, wanted), ("lengths", lengths, 1, torch.int32)))
     L.check(L.lib().remora_b200_causal_conv_fwd(context(device).ptr, _spec(_CONV_SPECS, silu, out is None), xd, wd, bd,
                                                 sd, ld, yd, od, _raw_stream(device)), "causal_conv_fwd")
+    _binding().written(y, state_out)
     return y if state_out is None else (y, state_out)
 
 
@@ -557,6 +564,7 @@ def causal_conv_bwd(x, w, dy, bias=None, *, state=None, lengths=None, silu: bool
                                  w.shape[1])
     L.check(lib.remora_b200_causal_conv_bwd(ctx, _spec(_CONV_SPECS, silu, out is None), xd, wd, bd, sd, ld, gd, ed, dxd,
                                             dwd, dbd, dsd, at, size, _raw_stream(device)), "causal_conv_bwd")
+    _binding().written(dx)
     return dx, dw, dbias, dstate
 
 
@@ -574,6 +582,7 @@ def causal_conv_step(x, state, w, bias=None, *, silu: bool = False, slots=None, 
         ("state_out", state_out, 3, torch.float32, None), ("slots", slots, 1, torch.int32)))
     L.check(L.lib().remora_b200_causal_conv_step(context(device).ptr, _spec(_CONV_SPECS, silu, out is None), xd, sd, wd,
                                                  bd, ld, yd, od, _raw_stream(device)), "causal_conv_step")
+    _binding().written(y, state_out)
     return y
 
 
@@ -612,6 +621,7 @@ def selective_scan_fwd(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, so
         saved = torch.empty((0,), dtype=f32, device=u.device) if saved is None else saved.view(f32)
     L.check(lib.remora_b200_selective_scan_fwd(ctx, _spec(_SCAN_SPECS, softplus, out is None), args, yd, hd, kept,
                                                kept_size, at, size, _raw_stream(device)), "selective_scan_fwd")
+    _binding().written(y, h_last)
     results = (y,) + ((h_last,) if h_last is not None else ()) + ((saved,) if save else ())
     return results if len(results) > 1 else y
 
@@ -663,4 +673,5 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, *, z=None, delta_bias=
         ("state_out", state_out, 3, torch.float32, None)), table=10)
     L.check(L.lib().remora_b200_selective_scan_step(context(device).ptr, _spec(_SCAN_SPECS, softplus, out is None), args,
                                                     yd, od, _raw_stream(device)), "selective_scan_step")
+    _binding().written(y, state_out)
     return y

@@ -141,3 +141,28 @@ def test_in_place_results_leave_a_lazy_clone_alone(cuda):
     ops.rms_norm_fwd(y, dev(np.ones(8, np.float32), cuda), out=y)
     np.testing.assert_array_equal(to_host(x), copy)
     assert (to_host(y) != copy).any()
+
+
+def test_given_results_count_as_modified(cuda):
+    """A value that autograd keeps is not replaced unnoticed."""
+    import torch
+
+    rng = np.random.default_rng(1)
+    t = lambda *shape: dev(rnd(rng, *shape), cuda)  # noqa: E731
+    x, w, state, pool = t(3, 8), t(8, 4), t(3, 3, 8), t(3, 8, 4)
+    seq, ones, total = t(3, 5, 8), torch.ones(8, device=cuda), t(3, 8)
+    calls = [(lambda o: ops.rms_norm_fwd(x, ones, out=o), x),
+             (lambda o: ops.rms_norm_fwd(x, ones, residual=total, sum_out=o), total),
+             (lambda o: ops.rms_norm_bwd(x, ones, total, out=o), total),
+             (lambda o: ops.causal_conv_fwd(seq, w, state=o, state_out=o), state),
+             (lambda o: ops.causal_conv_bwd(seq, w, seq, out=o), t(3, 5, 8)),
+             (lambda o: ops.causal_conv_step(x, o, w), state),
+             (lambda o: ops.selective_scan_step(o, x, x, -pool[0].abs(), pool[:, 0], pool[:, 1]), pool.clone())]
+    for call, out in calls:
+        leaf = torch.ones_like(out, requires_grad=True)
+        kept = leaf * out  # keeps `out` for its gradient
+        call(out)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            kept.sum().backward()
+    with torch.inference_mode():
+        ops.causal_conv_step(x.clone(), state.clone(), w)

@@ -167,3 +167,17 @@ def test_a_result_does_not_share_memory_with_a_lazy_clone():
     keep, _, at = _binding.describe(-1, (("x", shared, 1),), 0)
     assert aligned(at) == at_first
     assert source.tolist() == shared.tolist() == list(range(6))
+
+
+def test_written_raises_versions():
+    import torch
+
+    from remora_b200 import _binding
+
+    a, b = torch.zeros(3), torch.zeros(4)
+    _binding.written(a, None, b[1:])
+    assert (a._version, b._version) == (1, 1)
+    with torch.inference_mode():
+        _binding.written(torch.zeros(2))
+    with pytest.raises(TypeError):
+        _binding.written(3.0)
