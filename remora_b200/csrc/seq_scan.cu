@@ -578,8 +578,8 @@ int remora_b200_selective_scan_fwd(RemoraB200Ctx *ctx, const RemoraSelectiveScan
                          {given(8), "h0", 4}, {given(9), "lengths", 4}}, {{&hv, &v[8]}}));
   REMORA_TRY(want_own_elements({{&yv, "y", 4}, {has_h ? &hv : nullptr, "h_last", 4}}));
   for (int k : {0, 1, 6})
-    if (v[k].aligned) REMORA_TRY(check_reach(v[k], nl, kChan, "selective_scan_fwd"));
-  REMORA_TRY(check_reach(yv, nl, kChan, "selective_scan_fwd"));
+    if (v[k].aligned) REMORA_TRY(check_reach(v[k], nl, kChan, a.per, "selective_scan_fwd"));
+  REMORA_TRY(check_reach(yv, nl, kChan, a.per, "selective_scan_fwd"));
   a.y = op3(yv);
   if (has_h) a.h_last = op3(hv);
   cut_time(a.batch, a.length, a.dim, a.states, a.groups, &a.chunks, &a.chunk);

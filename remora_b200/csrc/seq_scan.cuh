@@ -74,12 +74,16 @@ struct ScanArgs {
 // Channels of a block whose threads hold `chan` channels each.
 inline int64_t block_channels(int nl, int chan) { return (int64_t)kScanThreads / nl * chan; }
 
-// Lane's 32-bit offsets reach the block's channels and a lane group's steps.
-inline int check_reach(const DescView &v, int nl, int chan, const char *what) {
+// Lane's 32-bit offsets reach the block's channels, of the `per` of a group, and a
+// lane group's steps.
+inline int check_reach(const DescView &v, int nl, int chan, int64_t per, const char *what) {
   const int64_t most = (int64_t)1 << 30;
   const int64_t s1 = stride_of(v, 1) < 0 ? -stride_of(v, 1) : stride_of(v, 1);
   const int64_t s2 = stride_of(v, 2) < 0 ? -stride_of(v, 2) : stride_of(v, 2);
-  if (s1 > most || s2 > most || s2 * (block_channels(nl, chan) - 1) + s1 * (nl - 1) >= most)
+  const int64_t steps = (v.sizes[1] < nl ? v.sizes[1] : nl) - 1;
+  const int64_t channels = (per < block_channels(nl, chan) ? per : block_channels(nl, chan)) - 1;
+  if ((steps > 0 && s1 > most / steps) || (channels > 0 && s2 > most / channels) ||
+      (steps > 0 ? s1 * steps : 0) + (channels > 0 ? s2 * channels : 0) >= most)
     return fail(REMORA_ERR_LIMIT, "%s: time and channel strides of %lld and %lld elements spread a block over 2^30", what,
                 (long long)s1, (long long)s2);
   return REMORA_OK;
@@ -118,6 +122,7 @@ struct Place {
   static constexpr int kChannels = kScanThreads / NL * CHAN;  // of a block
   int64_t bd, g, chunk, b, d[CHAN];
   int64_t first;    // the block's first channel
+  int channels, lanes;  // of a block's channels and a lane group's steps, those that there are anywhere
   int local[CHAN];  // a channel's place in the block
   int q;
   bool live[CHAN], whole;  // whole: the block has no dead channel
@@ -129,6 +134,8 @@ struct Place {
     chunk = i % chunks, b = i / chunks;
     q = threadIdx.x % NL;
     first = g * a.per + bd * kChannels;
+    channels = (int)min(a.per, (int64_t)kChannels);
+    lanes = (int)min(a.length, (int64_t)NL);
     const int64_t left = a.per - bd * kChannels;
     whole = left >= kChannels;
 #pragma unroll
@@ -143,14 +150,15 @@ struct Place {
 
 // A lane's elements of a [B, time, D] operand: a base address that the whole
 // block shares, moved along time, and a 32-bit offset per channel.  The offset
-// counts from the lowest of the block's addresses, so it is never negative.
+// counts from the lowest of the block's addresses, so it is never negative (but for
+// lanes past the axis's end, which use none).
 template <int NL, int CHAN>
 struct Lane {
   char *base;
   int64_t step;  // bytes per time step
   unsigned off[CHAN];
   __device__ __forceinline__ Lane(const Op3 &o, const Place<NL, CHAN> &at, int64_t t0) {
-    const int64_t low = (o.s2 < 0 ? o.s2 * (at.kChannels - 1) : 0) + (o.s1 < 0 ? o.s1 * (NL - 1) : 0);
+    const int64_t low = (o.s2 < 0 ? o.s2 * (at.channels - 1) : 0) + (o.s1 < 0 ? o.s1 * (at.lanes - 1) : 0);
     base = reinterpret_cast<char *>(o.p + (at.b * o.s0 + t0 * o.s1 + at.first * o.s2 + low));
     step = o.s1 * 4;
 #pragma unroll

@@ -689,9 +689,9 @@ int remora_b200_selective_scan_bwd(RemoraB200Ctx *ctx, const RemoraSelectiveScan
   REMORA_TRY(want_scratch(scratch, scratch_bytes, l.total * 4, "selective_scan_bwd"));
   const int chan = bwd_chan(nl);
   for (int k : {0, 1, 6})
-    if (v[k].aligned) REMORA_TRY(check_reach(v[k], nl, chan, "selective_scan_bwd"));
+    if (v[k].aligned) REMORA_TRY(check_reach(v[k], nl, chan, a.per, "selective_scan_bwd"));
   for (const DescView *x : {&gy, &o[0], &o[1], have[6] ? &o[6] : &o[0]})
-    REMORA_TRY(check_reach(*x, nl, chan, "selective_scan_bwd"));
+    REMORA_TRY(check_reach(*x, nl, chan, a.per, "selective_scan_bwd"));
   a.dy = op3(gy);
   if (has_gh) a.dh_last = op3(gh);
   a.du = op3(o[0]), a.ddelta = op3(o[1]);

@@ -166,3 +166,44 @@ def test_given_results_count_as_modified(cuda):
             kept.sum().backward()
     with torch.inference_mode():
         ops.causal_conv_step(x.clone(), state.clone(), w)
+
+
+# ------------------------------------------------------------------ strides
+@pytest.mark.parametrize("N", [4, 16])
+def test_few_channels_far_apart(cuda, N):
+    """Three channels 2^28 elements from one another, upwards and (by descriptors
+    alone) downwards, time likewise."""
+    import ctypes
+
+    import torch
+
+    from remora_b200 import _lib as L
+    from remora_b200.abi import make_memref_descriptor, tensor_descriptor
+    from remora_b200.runtime import context
+
+    rng = np.random.default_rng(N)
+    T, D, far = 21, 3, 1 << 28
+    buf = torch.empty((D - 1) * far + 2 * T, dtype=torch.float32, device=cuda)
+    wide, out = (buf.as_strided((1, T, D), (0, 1, far), at) for at in (0, T))
+    u, dy = dev(rnd(rng, 1, T, D), cuda), dev(rnd(rng, 1, T, D), cuda)
+    A, b, c = dev(-np.abs(rnd(rng, D, N)), cuda), dev(rnd(rng, 1, T, N), cuda), dev(rnd(rng, 1, T, N), cuda)
+    wide.copy_(u)
+    want, saved = ops.selective_scan_fwd(u, u, A, b, c, z=u, softplus=True, save=True)
+    got, kept = ops.selective_scan_fwd(wide, wide, A, b, c, z=wide, softplus=True, save=True, out=out)
+    np.testing.assert_array_equal(to_host(got), to_host(want))
+    for g, r in zip(ops.selective_scan_bwd(wide, wide, A, b, c, dy, kept, z=wide, softplus=True),
+                    ops.selective_scan_bwd(u, u, A, b, c, dy, saved, z=u, softplus=True)):
+        if g is not None:
+            np.testing.assert_array_equal(to_host(g), to_host(r))
+    turned = u.flip(1, 2).contiguous()
+    want = ops.selective_scan_fwd(turned, turned, A, b, c, softplus=True)
+    back = make_memref_descriptor(buf.data_ptr(), (1, T, D), (0, -1, -far), offset=T - 1 + (D - 1) * far)
+    y = torch.empty_like(u)
+    descs = [tensor_descriptor(t) for t in (A, b.unsqueeze(2), c.unsqueeze(2))]
+    args = L.RemoraSelectiveScanIn(ctypes.addressof(back), ctypes.addressof(back), *(ctypes.addressof(x) for x in descs))
+    spec, to = L.RemoraSelectiveScanSpec(1, 0), tensor_descriptor(y)
+    stream = ctypes.c_void_p(torch.cuda.current_stream(cuda).cuda_stream)
+    L.check(L.lib().remora_b200_selective_scan_fwd(context(0).ptr, ctypes.addressof(spec), ctypes.addressof(args),
+                                                   ctypes.addressof(to), None, None, 0, None, 0, stream))
+    np.testing.assert_array_equal(to_host(y), to_host(want))
+    del buf

@@ -181,3 +181,28 @@ def test_written_raises_versions():
         _binding.written(torch.zeros(2))
     with pytest.raises(TypeError):
         _binding.written(3.0)
+
+
+# ------------------------------------------------------------------ strides
+def test_reach_counts_the_channels_and_steps_that_there_are():
+    """A scan's operands may be as far apart as 2^30 elements within a block: of its
+    channels and steps, those that the operand has."""
+    far = 1 << 44
+
+    def call(B, T, D, N, strides, offset=0):
+        m = scan_operands(B, T, D, N)
+        m["u"] = desc(B, T, D, at=far, strides=strides, offset=offset)
+        st = scan_fwd(desc(B, T, D, at=1 << 50), **m)
+        assert st == LAST
+        return "spread" in L.last_error()
+
+    assert not call(1, 5, 2, 4, [0, 1, 1 << 25])
+    assert not call(1, 5, 2, 4, [0, 1, (1 << 30) - 1])
+    assert not call(1, 5, 2, 4, [0, -1, -(1 << 30) + 1], offset=1 << 40)
+    assert not call(1, 2, 2, 64, [0, 1 << 28, 1])
+    assert not call(1, 5, 2, 4, [0, 1 << 40, 1])  # one lane per channel: no two steps share a base
+    assert not call(2, 5, 300, 4, [1 << 40, 1 << 22, 1 << 22])
+    assert call(1, 5, 2, 4, [0, 1, 1 << 30])
+    assert call(1, 5, 3, 4, [0, 1, 1 << 29])
+    assert call(1, 2, 2, 64, [0, (1 << 30) - 1, 1])
+    assert call(1, 5, 300, 4, [0, 1, 1 << 23])  # 256 channels of a block
