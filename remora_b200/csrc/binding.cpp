@@ -220,4 +220,8 @@ PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_binding", "Descriptors of a c
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__binding(void) { return PyModule_Create(&module_def); }
+PyMODINIT_FUNC PyInit__binding(void) {
+  PyObject *module = PyModule_Create(&module_def);
+  if (module && PyModule_AddStringConstant(module, "torch_release", REMORA_TORCH_RELEASE) < 0) Py_CLEAR(module);
+  return module;
+}

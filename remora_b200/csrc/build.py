@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import importlib.util
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -71,14 +72,22 @@ def _build_binding(verbose: bool) -> None:
     Without torch there is nothing that it could bind, and C programs need the
     library alone."""
     src = HERE / "binding.cpp"
-    if BINDING.exists() and BINDING.stat().st_mtime >= src.stat().st_mtime:
-        return
     spec = importlib.util.find_spec("torch")
     if spec is None or not spec.submodule_search_locations:
         print("remora_b200._binding is left out: torch is not installed", file=sys.stderr, flush=True)
         return
     torch_dir = Path(next(iter(spec.submodule_search_locations)))
     cxx = _host_compiler()[1:] or ["g++"]
+    # what it is compiled against: with another torch, Python or compiler its layouts differ
+    release = re.search(r"__version__ = '([^']*)'", (torch_dir / "version.py").read_text())
+    version = release.group(1) if release else "unknown"
+    compiler = subprocess.run([*cxx, "--version"], capture_output=True, text=True, check=True).stdout.splitlines()[0]
+    key = "\n".join([version, str(torch_dir), sysconfig.get_config_var("SOABI") or sys.version, " ".join(cxx), compiler])
+    stamp = BUILD / "binding.key"
+    if (BINDING.exists() and BINDING.stat().st_mtime >= src.stat().st_mtime
+            and stamp.exists() and stamp.read_text() == key):
+        return
+    made = BUILD / BINDING.name
     cmd = [
         *cxx,
         "-O2",
@@ -88,9 +97,10 @@ def _build_binding(verbose: bool) -> None:
         f"-I{torch_dir / 'include'}",
         f"-I{torch_dir / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
         f"-I{sysconfig.get_paths()['include']}",
+        f'-DREMORA_TORCH_RELEASE="{version}"',
         str(src),
         "-o",
-        str(BINDING),
+        str(made),
         f"-L{torch_dir / 'lib'}",
         "-ltorch_python",
         "-ltorch_cpu",
@@ -100,6 +110,10 @@ def _build_binding(verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
+    # put in place as a whole, and named by its key only then
+    stamp.unlink(missing_ok=True)
+    os.replace(made, BINDING)
+    stamp.write_text(key)
 
 
 def build(verbose: bool = False, jobs: int | None = None) -> Path:

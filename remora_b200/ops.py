@@ -409,11 +409,15 @@ def _describe(what: str, device: int, operands, table: int = 0):
 def _binding():
     global _binding_module
     if _binding_module is None:
-        _torch()  # its libraries are the binding's
+        torch = _torch()  # its libraries are the binding's
+        build = "run `python -m remora_b200.csrc.build`"
         try:
             from remora_b200 import _binding as module
         except ImportError as e:
-            raise RemoraB200Error(f"remora_b200._binding is not built; run `python -m remora_b200.csrc.build` ({e})")
+            raise RemoraB200Error(f"remora_b200._binding is not built, or not for the installed torch; {build} ({e})")
+        if module.torch_release != torch.__version__:
+            raise RemoraB200Error(
+                f"remora_b200._binding is built for torch {module.torch_release}, not {torch.__version__}; {build}")
         _binding_module = module
     return _binding_module
 
