@@ -446,6 +446,13 @@ def _refuse(what: str, device: int, operands) -> None:
         f"{what}: an operand has no dense storage, is a lazily negated view, or has a rank over {L.MAX_RANK}")
 
 
+def _want_tensors(what: str, **operands) -> None:
+    """Refuses operands whose shape is needed ahead of _describe."""
+    for name, t in operands.items():
+        if not isinstance(t, _torch().Tensor):
+            raise RemoraB200Error(f"{what}: {name} is a {type(t).__name__}, not a tensor")
+
+
 def _cuda_index(t) -> int:
     if not isinstance(t, _torch().Tensor):
         raise RemoraB200Error(f"the first operand is a {type(t).__name__}, not a tensor")
@@ -543,7 +550,8 @@ def causal_conv_fwd(x, w, bias=None, *, state=None, lengths=None, silu: bool = F
     (y, the state that continues the sequence), else y."""
     torch = _torch()
     device, f32 = _cuda_index(x), torch.float32
-    wanted = (x.shape[0], w.shape[1] - 1, x.shape[2]) if return_state and x.dim() == 3 and w.dim() == 2 else None
+    _want_tensors("causal_conv_fwd", w=w)
+    wanted = (x.shape[0], max(w.shape[1] - 1, 0), x.shape[2]) if return_state and x.dim() == 3 and w.dim() == 2 else None
     keep, (y, state_out), xd, wd, bd, sd, yd, od, ld = _describe("causal_conv_fwd", device, (
         ("x", x, 3), ("w", w, 2), ("bias", bias, 1), ("state", state, 3), ("out", out, 3, f32, x),
         ("state_out", state_out, 3, f32, wanted), ("lengths", lengths, 1, torch.int32)))
@@ -559,6 +567,7 @@ def causal_conv_bwd(x, w, dy, bias=None, *, state=None, lengths=None, silu: bool
     returned state; `out` receives dx."""
     torch = _torch()
     device, f32 = _cuda_index(x), torch.float32
+    _want_tensors("causal_conv_bwd", w=w)
     keep, (dx, dw, dbias, dstate), xd, wd, bd, sd, gd, ed, dxd, dwd, dbd, dsd, ld = _describe("causal_conv_bwd", device, (
         ("x", x, 3), ("w", w, 2), ("bias", bias, 1), ("state", state, 3), ("dy", dy, 3), ("dstate_out", dstate_out, 3),
         ("out", out, 3, f32, x), ("dw", None, 2, f32, w), ("dbias", None, 1, f32, bias),
@@ -592,8 +601,8 @@ def causal_conv_step(x, state, w, bias=None, *, silu: bool = False, slots=None, 
 
 def _groups(what: str, B, C, rank: int):
     """B and C with their group axis: rank - 1 means one group."""
-    if B.dim() != C.dim():
-        raise RemoraShapeError(f"{what}: B has rank {B.dim()} and C rank {C.dim()}")
+    if B.dim() != C.dim() or not rank - 1 <= B.dim() <= rank:
+        raise RemoraShapeError(f"{what}: B has rank {B.dim()} and C rank {C.dim()}, not both {rank - 1} or {rank}")
     return (B, C) if B.dim() == rank else (B.unsqueeze(-2), C.unsqueeze(-2))
 
 
@@ -608,6 +617,7 @@ def selective_scan_fwd(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, so
     may be h0 itself), then with save what selective_scan_bwd needs."""
     torch = _torch()
     device = _cuda_index(u)
+    _want_tensors("selective_scan_fwd", A=A, B=B, C=C)
     Bg, Cg = _groups("selective_scan_fwd", B, C, 4)
     f32 = torch.float32
     wanted = (u.shape[0], u.shape[2], A.shape[1]) if return_state and u.dim() == 3 and A.dim() == 2 else None
@@ -637,6 +647,7 @@ def selective_scan_bwd(u, delta, A, B, C, dy, saved, D=None, *, z=None, delta_bi
     ddelta_bias, dh0), None where the input is None.  dh_last is the gradient
     that reaches the returned state."""
     device = _cuda_index(u)
+    _want_tensors("selective_scan_bwd", A=A, B=B, C=C, saved=saved)
     Bg, Cg = _groups("selective_scan_bwd", B, C, 4)
 
     f32 = _torch().float32
@@ -646,7 +657,7 @@ def selective_scan_bwd(u, delta, A, B, C, dy, saved, D=None, *, z=None, delta_bi
         ("dh_last", dh_last, 3), ("saved", saved, 1), ("du", None, 3, f32, u), ("ddelta", None, 3, f32, delta),
         ("dA", None, 2, f32, A), ("dB", None, 4, f32, Bg), ("dC", None, 4, f32, Cg), ("dD", None, 1, f32, D),
         ("dz", None, 3, f32, z), ("ddelta_bias", None, 1, f32, delta_bias), ("dh0", None, 3, f32, h0)), table=10)
-    if saved is None or not saved.is_contiguous():
+    if not saved.is_contiguous():
         raise RemoraUnsupportedError("selective_scan_bwd: saved is not what selective_scan_fwd returned")
     to = L.RemoraSelectiveScanGrads(*outs)
     lib, ctx = L.lib(), context(device).ptr
@@ -667,6 +678,7 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, *, z=None, delta_bias=
     state row slots[i], or row i without slots; a row whose slot is -1 or was
     named by an earlier row is left out, as in causal_conv_step."""
     device = _cuda_index(u)
+    _want_tensors("selective_scan_step", B=B, C=C)
     Bg, Cg = _groups("selective_scan_step", B, C, 3)
     torch = _torch()
     if state_out is None:

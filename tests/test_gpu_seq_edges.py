@@ -207,3 +207,36 @@ def test_few_channels_far_apart(cuda, N):
                                                    ctypes.addressof(to), None, None, 0, None, 0, stream))
     np.testing.assert_array_equal(to_host(y), to_host(want))
     del buf
+
+
+# ----------------------------------------------------------------- refusals
+def test_operands_that_are_missing_or_no_tensors_are_refused(cuda):
+    """Every operand that a call needs, left out or of another type, and weights
+    without taps: the framework's own errors, before anything is launched."""
+    import torch
+
+    from remora_b200 import _lib as L
+    from remora_b200.errors import RemoraB200Error
+
+    t = lambda *shape: torch.zeros(shape, device=cuda)  # noqa: E731
+    y, saved = ops.selective_scan_fwd(t(2, 5, 8), t(2, 5, 8), t(8, 4), t(2, 5, 4), t(2, 5, 4), save=True)
+    scan = dict(u=t(2, 5, 8), delta=t(2, 5, 8), A=t(8, 4), B=t(2, 5, 4), C=t(2, 5, 4))
+    step = dict(state=t(2, 8, 4), u=t(2, 8), delta=t(2, 8), A=t(8, 4), B=t(2, 4), C=t(2, 4))
+    calls = [(ops.rms_norm_fwd, dict(x=t(2, 8), w=t(8))), (ops.rms_norm_quant, dict(x=t(2, 8), w=t(8))),
+             (ops.rms_norm_bwd, dict(s=t(2, 8), w=t(8), dy=t(2, 8))),
+             (ops.causal_conv_fwd, dict(x=t(2, 5, 8), w=t(8, 3))),
+             (lambda **k: ops.causal_conv_fwd(**k, return_state=True), dict(x=t(2, 5, 8), w=t(8, 3))),
+             (ops.causal_conv_bwd, dict(x=t(2, 5, 8), w=t(8, 3), dy=t(2, 5, 8))),
+             (ops.causal_conv_step, dict(x=t(2, 8), state=t(2, 2, 8), w=t(8, 3))),
+             (ops.selective_scan_fwd, scan), (lambda **k: ops.selective_scan_fwd(**k, return_state=True), scan),
+             (ops.selective_scan_bwd, dict(scan, dy=t(2, 5, 8), saved=saved)), (ops.selective_scan_step, step)]
+    before = L.launch_count()
+    for call, good in calls:
+        for name in good:
+            for bad in (None, 3.0, [1.0], t(), t(3).cpu()):
+                with pytest.raises(RemoraB200Error):
+                    call(**{**good, name: bad})
+        if "w" in good and good["w"].dim() == 2:
+            with pytest.raises(RemoraB200Error):
+                call(**{**good, "w": t(8, 0)})
+    assert L.launch_count() == before
