@@ -8,9 +8,10 @@ import numpy as np
 import pytest
 
 import seq_reference as ref
+import test_gpu_seq as base
 from conftest import to_host
 from remora_b200 import ops
-from test_gpu_seq import E, dev, rnd, within
+from test_gpu_seq import E, dev, norm_tol, rnd, within
 
 pytestmark = pytest.mark.gpu
 
@@ -33,6 +34,50 @@ def test_quant_is_the_quotient_rounded(cuda, rows, D, group):
                                                      np.float32(2.0 ** -126)))
     want = torch.from_numpy(y / scales).to(torch.float8_e4m3fn).float().numpy()
     np.testing.assert_array_equal(to_host(q.float()).reshape(want.shape), want)
+
+
+@pytest.mark.parametrize("rows,D", [(5, 77), (700, 32), (700, 300), (700, 1001), (3, 8191), (700, 8191), (1, 1)])
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm_of_operands_aligned_differently(cuda, rows, D, residual):
+    """Rows whose starts lie differently on 16-byte boundaries are read by single
+    elements, one to eight (backward sixteen) per thread."""
+    rng = np.random.default_rng(rows + D)
+    x, w, dy = rnd(rng, rows, D), rnd(rng, D), rnd(rng, rows, D)
+    r = rnd(rng, rows, D) if residual else None
+    beside = lambda a: dev(np.concatenate([a[:, :1], a], axis=1), cuda)[:, 1:]  # noqa: E731  (rows D + 1 apart)
+    xd, wd, rd = beside(x), dev(w, cuda), dev(r, cuda)
+    y, s = ref.rms_norm(x, w, r, 1e-5)
+    tol = np.abs(y) * (norm_tol(D) + E) + np.abs(w) * np.abs(y / np.where(w == 0, 1, w)) * E
+    got = ops.rms_norm_fwd(xd, wd, residual=rd, eps=1e-5)
+    if residual:
+        got, total = got
+        np.testing.assert_array_equal(to_host(total), x + r)
+    within(got, y, tol, "y")
+    q, scales, *_ = ops.rms_norm_quant(xd, wd, residual=rd, eps=1e-5)
+    want = np.maximum(np.abs(y).max(axis=1, keepdims=True) / 448, 2.0 ** -126)
+    within(scales, want, want * (norm_tol(D) + 4 * E), "scales")
+    # to a level off by half its distance: 2^-4 of the value, or 2^-10 of the scale below 2^-6
+    within(to_host(q.float()) * to_host(scales).astype(np.float64), y, np.abs(y) * 2.0 ** -4 * (1 + 1e-5) + want * 2.0 ** -10)
+    s32 = x if r is None else x + r
+    rx, rw = ref.rms_norm_bwd(s32, w, dy, dy, 1e-5)
+    s6 = s32.astype(np.float64)
+    rstd = 1 / np.sqrt((s6 * s6).mean(axis=1, keepdims=True) + 1e-5)
+    mean = np.abs(s6 * rstd * w * dy).mean(axis=1, keepdims=True)
+    mag = rstd * (np.abs(w * dy) + np.abs(s6 * rstd) * mean) + np.abs(dy)
+    wmag = np.abs(dy * s6 * rstd).sum(axis=0) * (norm_tol(D) + rows * E + 8 * E)
+    sd, gd = beside(s32), dev(dy, cuda)
+    for out in (None, sd):
+        dx, dw = ops.rms_norm_bwd(sd, wd, gd, dsum=gd, eps=1e-5, out=out)
+        within(dx, rx, mag * 4 * norm_tol(D), "dx")
+        within(dw, rw, wmag, "dw")
+    assert dx is sd
+
+
+@pytest.mark.parametrize("rows,D", [(700, 256), (700, 4096), (3, 4096)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("residual", [False, True])
+def test_groups_over_several_vectors_of_a_thread(cuda, rows, D, group, residual):
+    base.test_norm_quant(cuda, rows, D, group, residual)
 
 
 # ------------------------------------------------------------------- silu
@@ -125,6 +170,21 @@ def test_an_infinite_step_leaves_what_is_ahead_of_it(cuda, N, length, at):
         np.testing.assert_array_equal(a, b)
     y = ops.selective_scan_step(d(h0), *(d(v[:, at]) for v in (u, delta)), d(A), d(B[:, at]), d(C[:, at]), softplus=True)
     assert (to_host(y) == np.inf).all()
+
+
+@pytest.mark.parametrize("N", [3, 8, 13, 16, 33, 64])
+@pytest.mark.parametrize("full", [False, True])
+def test_long_axes_that_are_not_cut(cuda, N, full):
+    """444 blocks of channels (here: groups) and more leave the time axis whole in
+    both directions, however long it is."""
+    base.test_scan_forward_backward(cuda, 3, 400, 148, N, 148, full)
+
+
+@pytest.mark.parametrize("B,T,D,N", [(300, 5, 3, 13), (260, 3, 10, 64), (30, 300, 3, 4), (30, 300, 40, 33)])
+def test_sums_over_many_pieces(cuda, B, T, D, N):
+    """More than 256 rows of partial sums of da, dd and ddelta_bias: a batch of more
+    sequences than that, or nine pieces of each of 30; one channel block or two."""
+    base.test_scan_forward_backward(cuda, B, T, D, N, 1, True)
 
 
 # ------------------------------------------------------------------ results
