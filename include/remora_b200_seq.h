@@ -118,7 +118,11 @@ int remora_b200_causal_conv_bwd(
    (exactly state for an update in place) gets the moved window in the same
    row, its other rows stay as they were.  A row whose slot is outside 0..S-1
    (-1 for padding) or was named by an earlier row is left out: all states and,
-   without zero_rest, its y stay as they were. */
+   without zero_rest, its y stay as they were.  B is at most 65535; each block
+   of a row reads the slots ahead of it, so with slots the time has a part that
+   grows with B squared (conv step of 4096 channels, 4 taps: 4096 rows 152 us
+   without slots and 163 with; scan step of 4096 channels, 16 states: 1024 rows
+   130 and 168 us, 4096 rows 504 and 1101). */
 int remora_b200_causal_conv_step(RemoraB200Ctx *ctx,
                                  const RemoraCausalConvSpec *spec,
                                  const RemoraMemRef2 *x,
@@ -161,7 +165,9 @@ typedef struct {
 /* y [B,L,D]; h_last [B,D,N] (may be NULL, may be exactly h0) gets the state
    behind each sequence's last position.  saved (may be NULL): f32 memory of
    remora_b200_selective_scan_saved bytes, 16-byte aligned, that gets the
-   states the backward pass starts from. */
+   states the backward pass starts from: those ahead of every 4th position (8th
+   above 16 states, 16th above 32), N rounded up to a power of two, at least 4.
+   That is N bytes per element of u for 4, 8 and 16 states and 16 bytes for more. */
 int remora_b200_selective_scan_saved(int64_t batch, int64_t length, int64_t dim,
                                      int64_t states, size_t *bytes);
 int remora_b200_selective_scan_fwd_scratch(RemoraB200Ctx *ctx, int64_t batch,

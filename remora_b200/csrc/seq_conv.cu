@@ -10,10 +10,12 @@
 // W rows in registers, so each row is read once but for the W-1 rows ahead of
 // a run, which its neighbour in the block has just brought into L1.
 //
-// Measured on B200 (a copy runs at 6.46 TB/s): forward with SiLU of 8 x 2048 x 4096
-// 83 us, 6.5 TB/s, of 1 x 8192 x 4096 46 us, 5.9 TB/s; backward of 8 x 2048 x 4096
-// 152 us and 5 us for the join of dw and dbias, 5.3 TB/s, where the instructions
-// (recomputed pre-activations, 4 W products per element) begin to count.
+// Measured on B200 over buffers past the L2's 126 MB, back to back (a copy runs at
+// 6.46 TB/s): forward with SiLU of 8 x 2048 x 4096 88 us, 6.1 TB/s, of 1 x 8192 x
+// 4096 47.5 us, 5.7 TB/s; backward of 8 x 2048 x 4096 161 us with the join of dw and
+// dbias, 5.0 TB/s, where the instructions (recomputed pre-activations, 4 W products
+// per element) begin to count.  Times below are of single launches, whose last
+// output is still in the L2.
 #include <algorithm>
 #include <type_traits>
 

@@ -12,10 +12,12 @@
 // allow it, else 4-byte ones.  Rows that are too long for that, or whose elements
 // are not consecutive, are read again from L2.
 //
-// Measured on B200 (a copy runs at 6.46 TB/s): forward with a residual of 16384 x
-// 2048 77 us, 7.0 TB/s; to e4m3 with a scale per 128 columns, 8192 x 4096, 78 us,
-// 5.6 TB/s; backward of 16384 x 2048 with the residual's gradient 90 us and 4 us
-// for the join of dw, 6.0 TB/s.
+// Measured on B200 over buffers past the L2's 126 MB, back to back (a copy runs at
+// 6.46 TB/s): forward with a residual of 16384 x 2048 83 us, 6.5 TB/s; to e4m3 with
+// a scale per 128 columns, 8192 x 4096, 78 us, 5.6 TB/s; backward of 16384 x 2048
+// with the residual's gradient 94 us with the join of dw, 5.7 TB/s.  A launch by
+// itself ends 5 to 15 us earlier, with the last of its output still in the L2.  Rows
+// past the register kernels' backward, 4096 x 16384: 485 us, 1.7 TB/s.
 #include <cuda_fp8.h>
 
 #include <algorithm>

@@ -5,8 +5,8 @@
 //
 // Per position and channel: 16 bytes of HBM (u, delta, z, y), N exponentials
 // and about 6 N other operations.  At N = 16 the exponentials bound it: the
-// special function units give 16 per clock and SM, 4.5e12 a second, and two
-// thirds of that is what the first pass reaches.
+// special function units give 16 per clock and SM, 4.5e12 a second, and three
+// quarters of that is what the first pass reaches.
 //
 // The recurrence is serial in time.  Where batch x channels give too few
 // threads, time is cut into pieces: a first pass gives each piece's end state
@@ -421,6 +421,9 @@ bool vec_states(const DescView &v) {
 
 // Pieces of the time axis: one when the channels alone give the device enough
 // warps or when the axis is short, else as many as do, of at least 32 steps each.
+// 2048 positions of 16 states, whole and in pieces: 128 blocks 266 and 221 us, 256
+// 322 and 400, 320 425 and 504, 384 427 and 575, 448 533 and 684, 512 538 and 690.
+// So the axis should stay whole from some 200 blocks on rather than from kCutBelow.
 // Cutting costs two more launches: 2 x 96 x 300 x 16 takes 15.4 us a call uncut
 // (13.6 on the device) and 20.2 (14.2) cut, 2 x 192 x 300 x 16 25.4 and 20.1; 2 x 64 x
 // 600 x 4, where a lane has more of a step to itself, 21.5 (19.8) and 25.6 (19.4),

@@ -14,9 +14,9 @@
 // through shared memory, over blocks by partial rows in scratch that a second
 // kernel adds in block order.
 //
-// Bound by issue and latency: some 210 instructions per warp, step and pair of
-// channels (8 states per thread), at half of the issue slots or less, since the
-// registers leave 8 to 16 warps per SM.  Measured on B200 for 4 x 2048 x 2048 x 16:
+// Bound by issue and latency: some 220 instructions per warp, step and pair of
+// channels (8 states per thread), at 57 % of the issue slots, since the registers
+// leave 8 to 16 warps per SM.  Measured on B200 for 4 x 2048 x 2048 x 16:
 // 357 us, first pass of the adjoint 90, joins 23.  The sums over channels by
 // shuffles: 414 us, with a state kept every eight steps 400; the steps' s, s u and dp
 // from shared memory instead of shuffles 432; the next step's shuffles ahead of a
@@ -553,7 +553,12 @@ __global__ void __launch_bounds__(32 * Y) join_kernel(const ScanArgs a, const Jo
 }
 
 // ------------------------------------------------------------------ host --
-// As the forward's: pieces only where the channels give too few warps.
+// As the forward's: pieces only where the channels give too few warps.  Training
+// steps of 2048 positions and 16 states with the backward's axis whole and in pieces,
+// the forward alike on both sides: 128 blocks 986 and 717 us, 256 1371 and 1323, 320
+// 1751 and 1649, 384 1828 and 1942, 448 2423 and 2148, 512 2428 and 2289, 768 3268 and
+// 3408, 1024 3970 and 4180.  444 blocks fit the device at once: a whole axis wins
+// where they fill their last round, which kCutBelow alone does not tell.
 void cut_time(int64_t batch, int64_t length, int64_t dim, int nl, int64_t groups, int64_t *chunks, int64_t *chunk) {
   const int64_t per_block = bwd_channels(nl), per = dim / std::max<int64_t>(groups, 1);
   const int64_t blocks = std::max<int64_t>(1, batch * groups * ((per + per_block - 1) / per_block));

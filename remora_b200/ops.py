@@ -585,7 +585,8 @@ def causal_conv_step(x, state, w, bias=None, *, silu: bool = False, slots=None, 
     """One token per row of x [B, D]: y, with the window state [S, W - 1, D]
     moved on in place (or into state_out).  Row i uses state row slots[i], or
     row i without slots; a row whose slot is -1 or was named by an earlier row
-    is left out (its y is zero, or as it was in a given `out`)."""
+    is left out (its y is zero, or as it was in a given `out`).  Finding those
+    takes time that grows with the square of the rows."""
     torch = _torch()
     device = _cuda_index(x)
     if state_out is None:
@@ -614,7 +615,9 @@ def selective_scan_fwd(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, so
     times silu(z) with a gate z.  A is [D, N] (N up to 64), B and C are
     [B, L, N] or, shared by groups of channels, [B, L, G, N].  Returns y, then
     the state behind each sequence's end with return_state (or h_last, which
-    may be h0 itself), then with save what selective_scan_bwd needs."""
+    may be h0 itself), then with save what selective_scan_bwd needs: the states
+    of every fourth position (every eighth above 16 states, sixteenth above 32),
+    with 16 states 16 bytes per element of u, four times u itself."""
     torch = _torch()
     device = _cuda_index(u)
     _want_tensors("selective_scan_fwd", A=A, B=B, C=C)
