@@ -33,8 +33,9 @@ constexpr int kMaxStates = 64;
 constexpr int64_t kMaxLength = 1 << 30;
 constexpr int kChan = 2;  // channels per thread
 // a of the states past N: their decay is 0 for a step that is inf, where a = 0
-// would make it, and through the sums over the states every output, NaN.
-constexpr float kPastN = -1.0f;
+// would make it, and through the sums over the states every output, NaN; and it is
+// finite for every finite step, of either sign.
+constexpr float kPastN = -1.17549435e-38f;
 
 struct Op3 {  // [B, time, D], or [B, D, N]
   float *p;

@@ -172,6 +172,36 @@ def test_an_infinite_step_leaves_what_is_ahead_of_it(cuda, N, length, at):
     assert (to_host(y) == np.inf).all()
 
 
+@pytest.mark.parametrize("N", [1, 4, 5, 13, 16, 33])
+@pytest.mark.parametrize("T", [7, 300])
+def test_large_steps_of_either_sign(cuda, N, T):
+    """Without softplus a step may be negative and large, where the rates are small:
+    the decay is e^2 at most here."""
+    rng = np.random.default_rng(N + T)
+    D, tol = 6, (6 * T + 64) * E
+    delta = (rnd(rng, 2, T, D) * np.float32(0.01)).astype(np.float32)
+    delta[0, T // 2], delta[1, T // 3] = -200, 200
+    v = dict(u=rnd(rng, 2, T, D), delta=delta, A=-rng.uniform(0.001, 0.01, (D, N)).astype(np.float32), B=rnd(rng, 2, T, 1, N),
+             C=rnd(rng, 2, T, 1, N), D=None, z=None, bias=None, h0=rnd(rng, 2, D, N))
+    dy = rnd(rng, 2, T, D)
+    pos, Dv, kw = base.scan_own(v, cuda)
+    y, last, saved = ops.selective_scan_fwd(*pos, Dv, return_state=True, save=True, **kw)
+    args = (*(v[k] for k in ("u", "delta", "A", "B", "C", "D", "z", "bias")), False, v["h0"], None)
+    for got, want, mag in zip((y, last), ref.selective_scan(*args), ref.selective_scan(*args, absolute=True)):
+        within(got, want, mag * tol)
+    got = ops.selective_scan_bwd(*pos, dev(dy, cuda), saved, Dv, **kw)
+    want, mag = (ref.selective_scan_bwd(*args, dy, None, absolute=a) for a in (False, True))
+    for name, g in zip(base.NAMES, got):
+        if g is not None:
+            extra = {"dA": 2 * T, "dB": D, "dC": D}.get(name, 0)
+            within(g, want[name], mag[name] * (2 * tol + extra * E), name)
+    for row, t in ((0, T // 2), (1, T // 3)):
+        one = [dev(v[k][row:row + 1, t], cuda) for k in ("u", "delta", "B", "C")]
+        y = ops.selective_scan_step(dev(v["h0"][row:row + 1], cuda), *one[:2], pos[2], *one[2:])
+        cut = tuple(a if k in (2, 5, 6, 7, 8, 9, 10) else a[:, t:t + 1] for k, a in enumerate(args))
+        within(y[0], ref.selective_scan(*cut)[0][row, 0], ref.selective_scan(*cut, absolute=True)[0][row, 0] * 70 * E)
+
+
 @pytest.mark.parametrize("N", [3, 8, 13, 16, 33, 64])
 @pytest.mark.parametrize("full", [False, True])
 def test_long_axes_that_are_not_cut(cuda, N, full):
