@@ -447,7 +447,8 @@ def _refuse(what: str, device: int, operands) -> None:
 
 
 def _want_tensors(what: str, **operands) -> None:
-    """Refuses operands whose shape is needed ahead of _describe."""
+    """Refuses operands that are no tensors, where a shape is needed ahead of
+    _describe or a missing operand's after it."""
     for name, t in operands.items():
         if not isinstance(t, _torch().Tensor):
             raise RemoraB200Error(f"{what}: {name} is a {type(t).__name__}, not a tensor")
@@ -550,7 +551,8 @@ def causal_conv_fwd(x, w, bias=None, *, state=None, lengths=None, silu: bool = F
     (y, the state that continues the sequence), else y."""
     torch = _torch()
     device, f32 = _cuda_index(x), torch.float32
-    _want_tensors("causal_conv_fwd", w=w)
+    if return_state:
+        _want_tensors("causal_conv_fwd", w=w)
     wanted = (x.shape[0], max(w.shape[1] - 1, 0), x.shape[2]) if return_state and x.dim() == 3 and w.dim() == 2 else None
     keep, (y, state_out), xd, wd, bd, sd, yd, od, ld = _describe("causal_conv_fwd", device, (
         ("x", x, 3), ("w", w, 2), ("bias", bias, 1), ("state", state, 3), ("out", out, 3, f32, x),
@@ -602,9 +604,14 @@ def causal_conv_step(x, state, w, bias=None, *, silu: bool = False, slots=None, 
 
 def _groups(what: str, B, C, rank: int):
     """B and C with their group axis: rank - 1 means one group."""
-    if B.dim() != C.dim() or not rank - 1 <= B.dim() <= rank:
-        raise RemoraShapeError(f"{what}: B has rank {B.dim()} and C rank {C.dim()}, not both {rank - 1} or {rank}")
-    return (B, C) if B.dim() == rank else (B.unsqueeze(-2), C.unsqueeze(-2))
+    try:
+        b, c = B.dim(), C.dim()
+    except AttributeError:
+        _want_tensors(what, B=B, C=C)
+        raise
+    if b != c or not rank - 1 <= b <= rank:
+        raise RemoraShapeError(f"{what}: B has rank {b} and C rank {c}, not both {rank - 1} or {rank}")
+    return (B, C) if b == rank else (B.unsqueeze(-2), C.unsqueeze(-2))
 
 
 def selective_scan_fwd(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, softplus: bool = False, h0=None,
@@ -620,7 +627,7 @@ def selective_scan_fwd(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, so
     with 16 states 16 bytes per element of u, four times u itself."""
     torch = _torch()
     device = _cuda_index(u)
-    _want_tensors("selective_scan_fwd", A=A, B=B, C=C)
+    _want_tensors("selective_scan_fwd", A=A)
     Bg, Cg = _groups("selective_scan_fwd", B, C, 4)
     f32 = torch.float32
     wanted = (u.shape[0], u.shape[2], A.shape[1]) if return_state and u.dim() == 3 and A.dim() == 2 else None
@@ -650,7 +657,7 @@ def selective_scan_bwd(u, delta, A, B, C, dy, saved, D=None, *, z=None, delta_bi
     ddelta_bias, dh0), None where the input is None.  dh_last is the gradient
     that reaches the returned state."""
     device = _cuda_index(u)
-    _want_tensors("selective_scan_bwd", A=A, B=B, C=C, saved=saved)
+    _want_tensors("selective_scan_bwd", A=A, saved=saved)
     Bg, Cg = _groups("selective_scan_bwd", B, C, 4)
 
     f32 = _torch().float32
@@ -681,7 +688,6 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, *, z=None, delta_bias=
     state row slots[i], or row i without slots; a row whose slot is -1 or was
     named by an earlier row is left out, as in causal_conv_step."""
     device = _cuda_index(u)
-    _want_tensors("selective_scan_step", B=B, C=C)
     Bg, Cg = _groups("selective_scan_step", B, C, 3)
     torch = _torch()
     if state_out is None:
